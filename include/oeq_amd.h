@@ -22,7 +22,7 @@
 #include <stdint.h>
 
 /* Changes with every change of a struct, an argument list or an enumerator below. */
-#define OEQ_ABI_VERSION 8
+#define OEQ_ABI_VERSION 9
 
 #ifdef __cplusplus
 extern "C" {
@@ -361,6 +361,86 @@ int oeq_grouped_sum(oeq_kernels* k, int64_t n_segments, int64_t n_items, int64_t
                     const void* src, void* dst, const int64_t* keys,
                     void* workspace, size_t workspace_bytes, void* stream);
 size_t oeq_grouped_sum_workspace_bytes(const oeq_kernels* k, int64_t n_segments, int64_t n_items);
+
+/* ---- operators on the nodes of a batch ------------------------------------ */
+/* Their kernels are part of the library. Strides are in elements; the elements of a head are contiguous, pointers and
+ * the strides of rows and heads are multiples of 16 bytes. The reference has no counterpart of these. */
+typedef enum {
+    OEQ_FLOAT32 = 0,
+    OEQ_FLOAT16 = 1,
+    OEQ_BFLOAT16 = 2,
+    OEQ_FLOAT64 = 3     /* oeq_irrep_dropout only */
+} oeq_element;
+
+/* Attention among the rows of segments. Segment s owns the query rows q_ptr[s] .. q_ptr[s + 1] and of the key rows
+ * from k_ptr[s] on the first k_len[s] (NULL: all up to k_ptr[s + 1]); both pointers ascend, on the device, with
+ * segments + 1 entries. Query head h reads key head h / (q_heads / k_heads). causal: the last query row of a segment
+ * sees all its keys, the one before all but the last, and so on. A row that sees nothing has the result 0. Entries
+ * that point outside the tensors are cut off at their ends. */
+typedef struct {
+    int32_t type;               /* oeq_element of q, k, v, results and gradients */
+    int32_t causal;
+    int32_t segments;
+    int32_t q_heads, k_heads;   /* q_heads is a multiple of k_heads */
+    int32_t head_dim;           /* a multiple of 8 up to 128 */
+    float scale;                /* positive */
+    int32_t reserved;
+    int64_t q_rows, k_rows;
+    int64_t q_row_stride, q_head_stride, k_row_stride, k_head_stride, v_row_stride, v_head_stride;
+    const void *q, *k, *v;
+    const int64_t *q_ptr, *k_ptr, *k_len;
+} oeq_attention;
+
+/* Elements between the heads of the row statistics: a few rows more than q_rows. */
+int64_t oeq_attention_stat_stride(int64_t q_rows);
+size_t oeq_attention_forward_workspace_bytes(const oeq_attention* a);
+/* out: [q_rows, q_heads, head_dim], log2_sum: [q_heads, stat_stride], the base-2 logarithm of each row's sum of
+ * exponentials (-inf where a row sees nothing). out_rest, of out's shape and type, takes what out's rounding took off; it
+ * makes the gradients more exact and may be NULL. */
+int oeq_attention_forward(const oeq_attention* a, void* out, void* out_rest, float* log2_sum, void* workspace,
+                          size_t workspace_bytes, void* stream);
+/* The gradients are contiguous like out; delta is scratch of log2_sum's size. No atomics: the results do not depend on
+ * the order in which blocks run. */
+int oeq_attention_backward(const oeq_attention* a, const void* out, const void* out_rest, const float* log2_sum, const void* out_grad,
+                           int64_t grad_row_stride, int64_t grad_head_stride, void* q_grad, void* k_grad, void* v_grad,
+                           float* delta, void* stream);
+
+/* Norm of each head of queries and keys over its root mean square, times a weight of head_dim elements (NULL: no norm),
+ * and rotation of its first rotary_dim elements by the row of `table` that positions[row] names: rotary_dim / 2 cosines,
+ * then as many sines. A position outside the table gives NaN. */
+typedef struct {
+    int32_t type;
+    int32_t interleaved;        /* pairs are neighbours, else elements i and i + rotary_dim / 2 */
+    int32_t q_heads, k_heads;
+    int32_t head_dim, rotary_dim;   /* multiples of 8, head_dim up to 128 */
+    float eps;
+    int32_t reserved;
+    int64_t rows, table_rows;
+    int64_t q_row_stride, q_head_stride, k_row_stride, k_head_stride;
+    const void *q, *k, *q_weight, *k_weight;
+    const int64_t* positions;
+    const float* table;         /* [table_rows, 2, rotary_dim / 2] */
+} oeq_qk_rotary;
+
+/* q_out, k_out: contiguous [rows, heads, head_dim]. */
+int oeq_qk_norm_rotary(const oeq_qk_rotary* a, void* q_out, void* k_out, void* stream);
+/* The keys, and the values as they are, go to row slots[row] of the caches (rows of the caches: cache_rows); rows whose
+ * slot is outside the caches are not written. */
+int oeq_qk_norm_rotary_append(const oeq_qk_rotary* a, const void* v, int64_t v_row_stride, int64_t v_head_stride,
+                              void* q_out, void* k_cache, int64_t k_cache_row_stride, int64_t k_cache_head_stride,
+                              void* v_cache, int64_t v_cache_row_stride, int64_t v_cache_head_stride,
+                              const int64_t* slots, int64_t cache_rows, void* stream);
+size_t oeq_qk_norm_rotary_backward_workspace_bytes(const oeq_qk_rotary* a);
+int oeq_qk_norm_rotary_backward(const oeq_qk_rotary* a, const void* q_grad, int64_t q_grad_row_stride,
+                                int64_t q_grad_head_stride, const void* k_grad, int64_t k_grad_row_stride,
+                                int64_t k_grad_head_stride, void* q_in_grad, void* k_in_grad, void* q_weight_grad,
+                                void* k_weight_grad, void* workspace, size_t workspace_bytes, void* stream);
+
+/* out = residual + x keep / (1 - p) on contiguous [rows, dim], residual may be NULL. channels[column] is the channel that
+ * a column belongs to; the columns of one channel are kept or dropped together, by 16 random bits that depend on
+ * seed[0], seed[1] (on the device), the row and the channel alone. */
+int oeq_irrep_dropout(int type, int64_t rows, int64_t dim, const void* x, const void* residual, void* out,
+                      const int32_t* channels, const int64_t* seed, double p, void* stream);
 
 /* ---- per-kernel timing --------------------------------------------------- */
 /* Replaces GPUTimer (extension/backend/backend_hip.hpp:67-101). While enabled,

@@ -17,6 +17,7 @@ __version__ = "0.1.0"
 if os.environ.get("OEQ_NOTORCH") != "1":
     import torch
 
+    from ._torch.nodes import (IrrepDropout, packed_attention, qk_norm_rotary, qk_norm_rotary_append, rotary_table)
     from ._torch.tensor_product import TensorProduct
     from ._torch.tensor_product_conv import TensorProductConv
     from ._torch.utils import torch_to_oeq_dtype, transpose_irreps
@@ -36,4 +37,5 @@ def torch_ext_so_path():
 
 
 __all__ = ["TPProblem", "Irrep", "Irreps", "Instruction", "TensorProduct", "TensorProductConv",
+           "IrrepDropout", "packed_attention", "qk_norm_rotary", "qk_norm_rotary_append", "rotary_table",
            "torch_to_oeq_dtype", "transpose_irreps", "torch_ext_so_path"]

@@ -54,18 +54,25 @@ _COTANGENTS = "Tensor L1_dgrad, Tensor L2_dgrad, Tensor W_dgrad"
 _EDGES = "Tensor rows, Tensor cols, Tensor transpose_perm"
 _ID = "int kid, Tensor? spec=None"
 _THREE, _FOUR = "(Tensor, Tensor, Tensor)", "(Tensor, Tensor, Tensor, Tensor)"
+
+
+def define_op(schema: str):
+    """Defines an op of the library; where its kernels could not be loaded, a call says so."""
+    name = _library.define(schema, tags=(torch.Tag.pt2_compliant_tag,))
+    if _native is None:
+        def _unavailable(*_args):
+            raise rt.OeqError(f"the torch ops could not be loaded: {_native_error}") from _native_error
+
+        _library.impl(name, _unavailable, "CUDA")
+
+
 for _schema in (f"tp_forward({_OPERANDS}, {_ID}) -> Tensor",
                 f"tp_backward({_OPERANDS}, Tensor L3_grad, {_ID}) -> {_THREE}",
                 f"tp_double_backward({_OPERANDS}, Tensor L3_grad, {_COTANGENTS}, {_ID}) -> {_FOUR}",
                 f"conv_forward({_OPERANDS}, {_EDGES}, {_ID}) -> Tensor",
                 f"conv_backward({_OPERANDS}, Tensor L3_grad, {_EDGES}, {_ID}) -> {_THREE}",
                 f"conv_double_backward({_OPERANDS}, Tensor L3_grad, {_COTANGENTS}, {_EDGES}, {_ID}) -> {_FOUR}"):
-    _name = _library.define(_schema, tags=(torch.Tag.pt2_compliant_tag,))
-    if _native is None:
-        def _unavailable(*_args):
-            raise rt.OeqError(f"the torch ops could not be loaded: {_native_error}") from _native_error
-
-        _library.impl(_name, _unavailable, "CUDA")
+    define_op(_schema)
 
 
 class _Registry(dict):

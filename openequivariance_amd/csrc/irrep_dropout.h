@@ -1,0 +1,96 @@
+// Device code of dropout of whole irreps.
+//
+// A channel of a node keeps all 2 l + 1 components or none, so that the result turns with its input: out = residual +
+// x keep(row, channel) / (1 - p). keep() is not stored anywhere: it is 16 bits of a random word that a counter-based
+// generator gives for the key (seed[0]) and the counter (channel / 8, row, seed[1]), here and again in the gradient,
+// which is the same operator on the output's gradient. The generator is Philox-4x32 with ten rounds (Salmon, Moraes,
+// Dror, Shaw: Parallel random numbers: as easy as 1, 2, 3, SC 2011): 128 bits a call, enough for eight channels.
+// Sixteen bits make p a multiple of 2^-16, and the kept values are scaled by that p's 1 / (1 - p).
+#ifndef OEQ_IRREP_DROPOUT_H
+#define OEQ_IRREP_DROPOUT_H
+
+#include <hip/hip_runtime.h>
+
+#include <cstdint>
+
+namespace irrep_dropout {
+
+struct Words {
+    uint32_t w[4];
+};
+
+__device__ __forceinline__ Words philox(uint32_t c0, uint32_t c1, uint32_t c2, uint32_t c3, uint32_t k0, uint32_t k1) {
+#pragma unroll
+    for (int i = 0; i < 10; ++i) {
+        const uint64_t a = (uint64_t)c0 * 0xD2511F53u, b = (uint64_t)c2 * 0xCD9E8D57u;
+        c0 = (uint32_t)(b >> 32) ^ c1 ^ k0;
+        c1 = (uint32_t)b;
+        c2 = (uint32_t)(a >> 32) ^ c3 ^ k1;
+        c3 = (uint32_t)a;
+        k0 += 0x9E3779B9u;
+        k1 += 0xBB67AE85u;
+    }
+    return {{c0, c1, c2, c3}};
+}
+
+// 16 bytes (V elements) to a thread of `count` elements in rows of `dim`; rows are numbered from first_row on. The last
+// thread takes what is left.
+template <typename T, typename F, int V>
+__global__ __launch_bounds__(256) void dropout(const T* x, const T* residual, T* out, const int* channels,
+                                               const int64_t* seed, unsigned count, unsigned dim, int64_t first_row,
+                                               unsigned drop, F scale) {
+    typedef T vec __attribute__((ext_vector_type(V)));
+    const unsigned at = (blockIdx.x * 256 + threadIdx.x) * V;
+    if (at >= count) return;
+    const int n = min((unsigned)V, count - at);
+    unsigned row = at / dim, column = at - row * dim;
+    unsigned rows[V];
+    int channel[V];
+#pragma unroll
+    for (int e = 0; e < V; ++e) {
+        rows[e] = row;
+        channel[e] = channels[column];
+        if (++column == dim) column = 0, ++row;
+    }
+    const uint64_t key = (uint64_t)seed[0], step = (uint64_t)seed[1];
+    unsigned open = (1u << n) - 1, kept = 0;
+    while (open) {  // the elements of one row and group of eight channels at a time, most often all
+        const int e0 = __builtin_ctz(open);
+        unsigned r = rows[0];
+        int group = channel[0] >> 3;
+#pragma unroll
+        for (int e = 1; e < V; ++e)
+            if (e == e0) r = rows[e], group = channel[e] >> 3;
+        const Words w = philox(group, (uint32_t)(first_row + r), (uint32_t)step, (uint32_t)(step >> 32), (uint32_t)key,
+                               (uint32_t)(key >> 32));
+#pragma unroll
+        for (int e = 0; e < V; ++e)
+            if ((open >> e & 1) && rows[e] == r && channel[e] >> 3 == group) {
+                const int c = channel[e];
+                const uint32_t word = c & 4 ? (c & 2 ? w.w[3] : w.w[2]) : (c & 2 ? w.w[1] : w.w[0]);
+                open &= ~(1u << e);
+                if (((c & 1 ? word >> 16 : word) & 0xffff) >= drop) kept |= 1u << e;
+            }
+    }
+    if (n == V) {
+        const vec a = *(const vec*)(x + at);
+        vec b = (T)0;
+        if (residual) b = *(const vec*)(residual + at);
+#pragma unroll
+        for (int e = 0; e < V; ++e) {
+            const F y = kept >> e & 1 ? (F)a[e] * scale : (F)0;
+            b[e] = (T)(y + (F)b[e]);
+        }
+        *(vec*)(out + at) = b;
+    } else {
+#pragma unroll
+        for (int e = 0; e < V; ++e)
+            if (e < n) {
+                const F y = kept >> e & 1 ? (F)x[at + e] * scale : (F)0;
+                out[at + e] = (T)(y + (residual ? (F)residual[at + e] : (F)0));
+            }
+    }
+}
+
+}  // namespace irrep_dropout
+#endif

@@ -6,13 +6,13 @@
 // entry point (oeq_conv_forward_static). The kernel argument lists used here are the contract the Python
 // code generator (openequivariance_amd/codegen) emits against.
 #include "oeq_amd.h"
+#include "oeq_error.h"
 
 #include <hip/hip_runtime.h>
 #include <hip/hiprtc.h>
 
 #include <algorithm>
 #include <atomic>
-#include <cstdarg>
 #include <cstdio>
 #include <cstdlib>
 #include <cstring>
@@ -20,26 +20,10 @@
 #include <string>
 #include <vector>
 
+using oeq_internal::fail;
+using oeq_internal::g_error;
+
 namespace {
-
-thread_local std::string g_error;
-
-int fail(int code, const char* fmt, ...) {
-    char buf[2048];
-    va_list ap;
-    va_start(ap, fmt);
-    vsnprintf(buf, sizeof(buf), fmt, ap);
-    va_end(ap);
-    g_error = buf;
-    return code;
-}
-
-#define HIP_TRY(expr)                                                                  \
-    do {                                                                               \
-        hipError_t e_ = (expr);                                                        \
-        if (e_ != hipSuccess)                                                          \
-            return fail(OEQ_ERR_HIP, "%s failed: %s", #expr, hipGetErrorString(e_));   \
-    } while (0)
 
 constexpr int kMaxDevices = 16;
 

@@ -1,0 +1,298 @@
+// The operators on the nodes of a batch behind the C ABI: checks of arguments, choice of kernels, launches. Their device
+// code is in packed_attention.h (compiled per element type from packed_attention.hip), qk_rotary.h and irrep_dropout.h.
+#include "oeq_amd.h"
+#include "oeq_error.h"
+
+#include "irrep_dropout.h"
+#include "packed_attention_launch.h"
+#include "qk_rotary.h"
+
+#include <algorithm>
+#include <climits>
+#include <cmath>
+
+using oeq_internal::fail;
+
+namespace {
+
+int element_bytes(int type) {
+    return type == OEQ_FLOAT32 ? 4 : type == OEQ_FLOAT16 || type == OEQ_BFLOAT16 ? 2 : 0;
+}
+
+bool aligned(const void* p) { return ((uintptr_t)p & 15) == 0; }
+bool aligned(int64_t stride, int type) { return stride * element_bytes(type) % 16 == 0; }
+
+// A tile's rows are addressed by 32-bit offsets from its first.
+constexpr int64_t kMostRowBytes = (int64_t)INT_MAX / 64 - 1024;
+
+int check_attention(const char* who, const oeq_attention* a) {
+    if (!a) return fail(OEQ_ERR_INVALID, "%s: NULL description", who);
+    if (!element_bytes(a->type)) return fail(OEQ_ERR_INVALID, "%s: element type %d", who, a->type);
+    if (a->segments < 0 || a->q_rows < 0 || a->k_rows < 0 || a->q_rows > INT_MAX - 256 || a->k_rows > INT_MAX - 256)
+        return fail(OEQ_ERR_INVALID, "%s: %d segments, %lld query rows, %lld key rows", who, a->segments,
+                    (long long)a->q_rows, (long long)a->k_rows);
+    if (a->k_heads <= 0 || a->q_heads <= 0 || a->q_heads % a->k_heads)
+        return fail(OEQ_ERR_INVALID, "%s: %d query heads for %d key heads", who, a->q_heads, a->k_heads);
+    if (a->head_dim <= 0 || a->head_dim > 128 || a->head_dim % 8)
+        return fail(OEQ_ERR_INVALID, "%s: heads of %d elements (multiples of 8 up to 128)", who, a->head_dim);
+    if (!(a->scale > 0) || !std::isfinite(a->scale)) return fail(OEQ_ERR_INVALID, "%s: scale %g", who, a->scale);
+    for (int64_t s : {a->q_row_stride, a->q_head_stride, a->k_row_stride, a->k_head_stride, a->v_row_stride, a->v_head_stride})
+        if (!aligned(s, a->type)) return fail(OEQ_ERR_INVALID, "%s: a stride of %lld elements", who, (long long)s);
+    for (int64_t s : {a->q_row_stride, a->k_row_stride, a->v_row_stride})
+        if (s < 0 || s * element_bytes(a->type) > kMostRowBytes)
+            return fail(OEQ_ERR_INVALID, "%s: a row stride of %lld elements", who, (long long)s);
+    if (a->q_rows && !a->q) return fail(OEQ_ERR_INVALID, "%s: NULL buffer", who);
+    if (a->k_rows && (!a->k || !a->v)) return fail(OEQ_ERR_INVALID, "%s: NULL buffer", who);
+    if ((a->q_rows || a->k_rows) && (!a->q_ptr || !a->k_ptr)) return fail(OEQ_ERR_INVALID, "%s: NULL buffer", who);
+    if (!aligned(a->q) || !aligned(a->k) || !aligned(a->v)) return fail(OEQ_ERR_INVALID, "%s: unaligned buffer", who);
+    return OEQ_OK;
+}
+
+packed_attention::Args attention_args(const oeq_attention& a) {
+    packed_attention::Args g = {};
+    g.q = a.q, g.k = a.k, g.v = a.v;
+    g.q_ptr = a.q_ptr, g.k_ptr = a.k_ptr, g.k_len = a.k_len;
+    g.q_row = a.q_row_stride, g.q_head = a.q_head_stride;
+    g.k_row = a.k_row_stride, g.k_head = a.k_head_stride;
+    g.v_row = a.v_row_stride, g.v_head = a.v_head_stride;
+    g.stat_stride = oeq_attention_stat_stride(a.q_rows);
+    g.segments = a.segments, g.nq = (int)a.q_rows, g.nk = (int)a.k_rows;
+    g.hq = a.q_heads, g.hk = a.k_heads, g.d = a.head_dim, g.causal = a.causal != 0;
+    g.tiles = (int)((a.q_rows + 127) / 128);
+    g.scale_log2 = a.scale * 1.4426950408889634f;
+    return g;
+}
+
+int check_rotary(const char* who, const oeq_qk_rotary* a) {
+    if (!a) return fail(OEQ_ERR_INVALID, "%s: NULL description", who);
+    if (!element_bytes(a->type)) return fail(OEQ_ERR_INVALID, "%s: element type %d", who, a->type);
+    if (a->rows < 0 || a->table_rows < 0 || a->q_heads < 0 || a->k_heads < 0)
+        return fail(OEQ_ERR_INVALID, "%s: %lld rows, %lld rows of the table, %d and %d heads", who, (long long)a->rows,
+                    (long long)a->table_rows, a->q_heads, a->k_heads);
+    if (a->head_dim <= 0 || a->head_dim > 128 || a->head_dim % 8)
+        return fail(OEQ_ERR_INVALID, "%s: heads of %d elements (multiples of 8 up to 128)", who, a->head_dim);
+    if (a->rotary_dim < 0 || a->rotary_dim > a->head_dim || a->rotary_dim % 8)
+        return fail(OEQ_ERR_INVALID, "%s: %d turned elements of %d (multiples of 8)", who, a->rotary_dim, a->head_dim);
+    if (a->rows > (int64_t)INT_MAX * 8 / (a->q_heads + 2 * a->k_heads + 1))
+        return fail(OEQ_ERR_INVALID, "%s: %lld rows", who, (long long)a->rows);
+    for (int64_t s : {a->q_row_stride, a->q_head_stride, a->k_row_stride, a->k_head_stride})
+        if (!aligned(s, a->type)) return fail(OEQ_ERR_INVALID, "%s: a stride of %lld elements", who, (long long)s);
+    if (a->rows && ((a->q_heads && !a->q) || (a->k_heads && !a->k) || (a->rotary_dim && (!a->positions || !a->table))))
+        return fail(OEQ_ERR_INVALID, "%s: NULL buffer", who);
+    if (!aligned(a->q) || !aligned(a->k) || !aligned(a->q_weight) || !aligned(a->k_weight) || !aligned(a->table))
+        return fail(OEQ_ERR_INVALID, "%s: unaligned buffer", who);
+    return OEQ_OK;
+}
+
+qk_rotary::Args rotary_args(const oeq_qk_rotary& a) {
+    qk_rotary::Args g = {};
+    g.q = a.q, g.k = a.k, g.q_weight = a.q_weight, g.k_weight = a.k_weight;
+    g.positions = a.positions, g.table = a.table, g.table_rows = a.table_rows;
+    g.q_row = a.q_row_stride, g.q_head = a.q_head_stride;
+    g.k_row = a.k_row_stride, g.k_head = a.k_head_stride;
+    g.q_heads = a.q_heads, g.k_heads = a.k_heads, g.d = a.head_dim, g.rotary = a.rotary_dim;
+    g.interleaved = a.interleaved != 0;
+    g.eps = a.eps;
+    g.lanes = 1;
+    while (8 * g.lanes < a.head_dim) g.lanes *= 2;
+    g.units = a.rows * (a.q_heads + a.k_heads);
+    return g;
+}
+
+template <bool APPEND>
+int launch_rotary(int type, const qk_rotary::Args& g, hipStream_t stream) {
+    const unsigned blocks = (unsigned)((g.units * g.lanes + 255) / 256);
+    if (type == OEQ_FLOAT32)
+        qk_rotary::forward<float, APPEND><<<blocks, 256, 0, stream>>>(g);
+    else if (type == OEQ_FLOAT16)
+        qk_rotary::forward<_Float16, APPEND><<<blocks, 256, 0, stream>>>(g);
+    else
+        qk_rotary::forward<__bf16, APPEND><<<blocks, 256, 0, stream>>>(g);
+    HIP_TRY(hipGetLastError());
+    return OEQ_OK;
+}
+
+// Blocks of the gradient: a few for each compute unit, so that the rows of partial sums stay few.
+constexpr int kGradientBlocks = 1024;
+
+unsigned gradient_blocks(const qk_rotary::Args& g) {
+    return (unsigned)std::min<int64_t>(kGradientBlocks, (g.units * g.lanes + 255) / 256);
+}
+
+template <typename T>
+int launch_rotary_gradient(const qk_rotary::Args& g, void* q_weight_grad, void* k_weight_grad, hipStream_t stream) {
+    const unsigned blocks = gradient_blocks(g);
+    if (blocks) {
+        qk_rotary::backward<T><<<blocks, 256, 0, stream>>>(g);
+        HIP_TRY(hipGetLastError());
+    }
+    if (g.partial) {
+        qk_rotary::weight_gradient<T><<<(16 * g.lanes + 63) / 64, 1024, 0, stream>>>(g, (int)blocks, (T*)q_weight_grad,
+                                                                                     (T*)k_weight_grad);
+        HIP_TRY(hipGetLastError());
+    }
+    return OEQ_OK;
+}
+
+template <typename T, typename F>
+int launch_dropout(int64_t rows, int64_t dim, const void* x, const void* residual, void* out, const int32_t* channels,
+                   const int64_t* seed, unsigned drop, hipStream_t stream) {
+    constexpr int V = 16 / (int)sizeof(T);
+    const F scale = drop < 65536 ? (F)(65536.0 / (65536 - drop)) : (F)0;
+    // elements are numbered in 32 bits: longer tensors go in parts of whole rows, a multiple of V of them so that every
+    // part begins at 16 bytes
+    const int64_t part = std::max<int64_t>(V, ((int64_t)1 << 31) / dim / V * V);
+    for (int64_t first = 0; first < rows; first += part) {
+        const int64_t at = first * dim;
+        const unsigned count = (unsigned)(std::min(part, rows - first) * dim);
+        const unsigned threads = (count + V - 1) / V;
+        irrep_dropout::dropout<T, F, V><<<(threads + 255) / 256, 256, 0, stream>>>(
+            (const T*)x + at, residual ? (const T*)residual + at : nullptr, (T*)out + at, channels, seed, count, (unsigned)dim,
+            first, drop, scale);
+        HIP_TRY(hipGetLastError());
+    }
+    return OEQ_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int64_t oeq_attention_stat_stride(int64_t q_rows) { return (q_rows + 63) / 64 * 64 + 64; }
+
+size_t oeq_attention_forward_workspace_bytes(const oeq_attention*) { return 0; }
+
+int oeq_attention_forward(const oeq_attention* a, void* out, void* out_rest, float* log2_sum, void* workspace,
+                          size_t workspace_bytes, void* stream) {
+    const char* who = "oeq_attention_forward";
+    if (int rc = check_attention(who, a)) return rc;
+    if (a->q_rows == 0) return OEQ_OK;
+    if (!out || !log2_sum) return fail(OEQ_ERR_INVALID, "%s: NULL buffer", who);
+    if (!aligned(out) || !aligned(out_rest)) return fail(OEQ_ERR_INVALID, "%s: unaligned buffer", who);
+    if (workspace_bytes < oeq_attention_forward_workspace_bytes(a) || (workspace_bytes && !workspace))
+        return fail(OEQ_ERR_INVALID, "%s: workspace too small", who);
+    packed_attention::Args g = attention_args(*a);
+    g.o = out, g.rest = out_rest, g.lse = log2_sum;
+    const auto s = (hipStream_t)stream;
+    HIP_TRY(a->type == OEQ_FLOAT32 ? packed_attention::Launch<float>::forward(g, s)
+            : a->type == OEQ_FLOAT16 ? packed_attention::Launch<_Float16>::forward(g, s)
+                                     : packed_attention::Launch<__bf16>::forward(g, s));
+    return OEQ_OK;
+}
+
+int oeq_attention_backward(const oeq_attention* a, const void* out, const void* out_rest, const float* log2_sum, const void* out_grad,
+                           int64_t grad_row_stride, int64_t grad_head_stride, void* q_grad, void* k_grad, void* v_grad,
+                           float* delta, void* stream) {
+    const char* who = "oeq_attention_backward";
+    if (int rc = check_attention(who, a)) return rc;
+    if (!aligned(grad_row_stride, a->type) || !aligned(grad_head_stride, a->type) || grad_row_stride < 0 ||
+        grad_row_stride * element_bytes(a->type) > kMostRowBytes)
+        return fail(OEQ_ERR_INVALID, "%s: strides of %lld and %lld elements", who, (long long)grad_row_stride,
+                    (long long)grad_head_stride);
+    if ((a->q_rows && (!out || !log2_sum || !out_grad || !q_grad || !delta)) || (a->k_rows && (!k_grad || !v_grad)))
+        return fail(OEQ_ERR_INVALID, "%s: NULL buffer", who);
+    if (!aligned(out) || !aligned(out_rest) || !aligned(out_grad) || !aligned(q_grad) || !aligned(k_grad) || !aligned(v_grad))
+        return fail(OEQ_ERR_INVALID, "%s: unaligned buffer", who);
+    packed_attention::Args g = attention_args(*a);
+    g.out = out, g.out_rest = out_rest, g.grad = out_grad, g.g_row = grad_row_stride, g.g_head = grad_head_stride;
+    g.dq = q_grad, g.dk = k_grad, g.dv = v_grad, g.lse = (float*)log2_sum, g.delta = delta;
+    const int key_tiles = (int)((a->k_rows + 127) / 128);
+    const auto s = (hipStream_t)stream;
+    HIP_TRY(a->type == OEQ_FLOAT32 ? packed_attention::Launch<float>::backward(g, key_tiles, s)
+            : a->type == OEQ_FLOAT16 ? packed_attention::Launch<_Float16>::backward(g, key_tiles, s)
+                                     : packed_attention::Launch<__bf16>::backward(g, key_tiles, s));
+    return OEQ_OK;
+}
+
+int oeq_qk_norm_rotary(const oeq_qk_rotary* a, void* q_out, void* k_out, void* stream) {
+    const char* who = "oeq_qk_norm_rotary";
+    if (int rc = check_rotary(who, a)) return rc;
+    qk_rotary::Args g = rotary_args(*a);
+    if (g.units == 0) return OEQ_OK;
+    if ((a->q_heads && !q_out) || (a->k_heads && !k_out)) return fail(OEQ_ERR_INVALID, "%s: NULL buffer", who);
+    if (!aligned(q_out) || !aligned(k_out)) return fail(OEQ_ERR_INVALID, "%s: unaligned buffer", who);
+    g.q_out = q_out, g.k_out = k_out;
+    g.ko_head = a->head_dim, g.ko_row = (int64_t)a->k_heads * a->head_dim;
+    return launch_rotary<false>(a->type, g, (hipStream_t)stream);
+}
+
+int oeq_qk_norm_rotary_append(const oeq_qk_rotary* a, const void* v, int64_t v_row_stride, int64_t v_head_stride,
+                              void* q_out, void* k_cache, int64_t k_cache_row_stride, int64_t k_cache_head_stride,
+                              void* v_cache, int64_t v_cache_row_stride, int64_t v_cache_head_stride,
+                              const int64_t* slots, int64_t cache_rows, void* stream) {
+    const char* who = "oeq_qk_norm_rotary_append";
+    if (int rc = check_rotary(who, a)) return rc;
+    for (int64_t s : {v_row_stride, v_head_stride, k_cache_row_stride, k_cache_head_stride, v_cache_row_stride,
+                      v_cache_head_stride})
+        if (!aligned(s, a->type)) return fail(OEQ_ERR_INVALID, "%s: a stride of %lld elements", who, (long long)s);
+    if (cache_rows < 0) return fail(OEQ_ERR_INVALID, "%s: %lld rows of the caches", who, (long long)cache_rows);
+    qk_rotary::Args g = rotary_args(*a);
+    g.units = a->rows * (a->q_heads + 2 * (int64_t)a->k_heads);
+    if (g.units == 0) return OEQ_OK;
+    if ((a->q_heads && !q_out) || (a->k_heads && (!v || !slots || (cache_rows && (!k_cache || !v_cache)))))
+        return fail(OEQ_ERR_INVALID, "%s: NULL buffer", who);
+    if (!aligned(v) || !aligned(q_out) || !aligned(k_cache) || !aligned(v_cache))
+        return fail(OEQ_ERR_INVALID, "%s: unaligned buffer", who);
+    g.v = v, g.v_row = v_row_stride, g.v_head = v_head_stride;
+    g.q_out = q_out, g.k_out = k_cache, g.v_out = v_cache;
+    g.ko_row = k_cache_row_stride, g.ko_head = k_cache_head_stride;
+    g.vo_row = v_cache_row_stride, g.vo_head = v_cache_head_stride;
+    g.slots = slots, g.slots_end = cache_rows;
+    return launch_rotary<true>(a->type, g, (hipStream_t)stream);
+}
+
+size_t oeq_qk_norm_rotary_backward_workspace_bytes(const oeq_qk_rotary* a) {
+    if (!a || (!a->q_weight && !a->k_weight) || a->head_dim <= 0 || a->head_dim > 128) return 0;
+    return (size_t)kGradientBlocks * 2 * 128 * sizeof(float);
+}
+
+int oeq_qk_norm_rotary_backward(const oeq_qk_rotary* a, const void* q_grad, int64_t q_grad_row_stride,
+                                int64_t q_grad_head_stride, const void* k_grad, int64_t k_grad_row_stride,
+                                int64_t k_grad_head_stride, void* q_in_grad, void* k_in_grad, void* q_weight_grad,
+                                void* k_weight_grad, void* workspace, size_t workspace_bytes, void* stream) {
+    const char* who = "oeq_qk_norm_rotary_backward";
+    if (int rc = check_rotary(who, a)) return rc;
+    for (int64_t s : {q_grad_row_stride, q_grad_head_stride, k_grad_row_stride, k_grad_head_stride})
+        if (!aligned(s, a->type)) return fail(OEQ_ERR_INVALID, "%s: a stride of %lld elements", who, (long long)s);
+    qk_rotary::Args g = rotary_args(*a);
+    if (g.units && ((a->q_heads && (!q_grad || !q_in_grad)) || (a->k_heads && (!k_grad || !k_in_grad))))
+        return fail(OEQ_ERR_INVALID, "%s: NULL buffer", who);
+    if ((a->q_weight && !q_weight_grad) || (a->k_weight && !k_weight_grad))
+        return fail(OEQ_ERR_INVALID, "%s: NULL buffer", who);
+    const size_t need = oeq_qk_norm_rotary_backward_workspace_bytes(a);
+    if (need && (workspace_bytes < need || !workspace)) return fail(OEQ_ERR_INVALID, "%s: workspace too small", who);
+    if (!aligned(q_grad) || !aligned(k_grad) || !aligned(q_in_grad) || !aligned(k_in_grad))
+        return fail(OEQ_ERR_INVALID, "%s: unaligned buffer", who);
+    g.q_grad = q_grad, g.gq_row = q_grad_row_stride, g.gq_head = q_grad_head_stride;
+    g.k_grad = k_grad, g.gk_row = k_grad_row_stride, g.gk_head = k_grad_head_stride;
+    g.q_out = q_in_grad, g.k_out = k_in_grad;
+    g.partial = need ? (float*)workspace : nullptr;
+    if (!a->q_weight) q_weight_grad = nullptr;
+    if (!a->k_weight) k_weight_grad = nullptr;
+    const auto s = (hipStream_t)stream;
+    if (a->type == OEQ_FLOAT32) return launch_rotary_gradient<float>(g, q_weight_grad, k_weight_grad, s);
+    if (a->type == OEQ_FLOAT16) return launch_rotary_gradient<_Float16>(g, q_weight_grad, k_weight_grad, s);
+    return launch_rotary_gradient<__bf16>(g, q_weight_grad, k_weight_grad, s);
+}
+
+int oeq_irrep_dropout(int type, int64_t rows, int64_t dim, const void* x, const void* residual, void* out,
+                      const int32_t* channels, const int64_t* seed, double p, void* stream) {
+    const char* who = "oeq_irrep_dropout";
+    if (rows < 0 || dim < 0 || rows > INT_MAX || dim > (1 << 27))
+        return fail(OEQ_ERR_INVALID, "%s: %lld rows of %lld", who, (long long)rows, (long long)dim);
+    if (!(p >= 0.0 && p <= 1.0)) return fail(OEQ_ERR_INVALID, "%s: p = %g", who, p);
+    if (type != OEQ_FLOAT64 && !element_bytes(type)) return fail(OEQ_ERR_INVALID, "%s: element type %d", who, type);
+    if (rows == 0 || dim == 0) return OEQ_OK;
+    if (!x || !out || !channels || !seed) return fail(OEQ_ERR_INVALID, "%s: NULL buffer", who);
+    if (!aligned(x) || !aligned(residual) || !aligned(out)) return fail(OEQ_ERR_INVALID, "%s: unaligned buffer", who);
+    const unsigned drop = (unsigned)std::nearbyint(p * 65536);
+    const auto s = (hipStream_t)stream;
+    switch (type) {
+        case OEQ_FLOAT32: return launch_dropout<float, float>(rows, dim, x, residual, out, channels, seed, drop, s);
+        case OEQ_FLOAT16: return launch_dropout<_Float16, float>(rows, dim, x, residual, out, channels, seed, drop, s);
+        case OEQ_BFLOAT16: return launch_dropout<__bf16, float>(rows, dim, x, residual, out, channels, seed, drop, s);
+        default: return launch_dropout<double, double>(rows, dim, x, residual, out, channels, seed, drop, s);
+    }
+}
+
+}  // extern "C"

@@ -12,13 +12,11 @@
 // most: it runs in the autograd engine's thread, where Python code finds neither its interpreter state nor its data in
 // the caches. Looking up the kept index and choosing the second-order route in Python cost, per pass, before / now:
 // MACE-medium, 192 nodes, new edges, forward and backward 157 / 96 us; 16 molecules with second order 281 / 192.
-#include "oeq_amd.h"
+#include "oeq_torch.h"
 
 #include <ATen/ATen.h>
 #include <ATen/Context.h>
 #include <ATen/core/dispatch/Dispatcher.h>
-#include <ATen/hip/impl/HIPGuardImplMasqueradingAsCUDA.h>
-#include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/grad_mode.h>
@@ -41,6 +39,7 @@ using at::Tensor;
 using OptTensor = std::optional<Tensor>;
 using Tensor3 = std::tuple<Tensor, Tensor, Tensor>;
 using Tensor4 = std::tuple<Tensor, Tensor, Tensor, Tensor>;
+using namespace oeq_torch;
 
 namespace {
 
@@ -71,6 +70,18 @@ struct Callbacks {
 };
 Callbacks* g_py = nullptr;
 
+}  // namespace
+
+void oeq_torch::raise(const std::string& text) {
+    py::gil_scoped_acquire gil;
+    PyErr_SetString(g_py->error_type.ptr(), text.c_str());
+    python_error err;
+    err.persist();
+    throw err;
+}
+
+namespace {
+
 EntryRef entry_of(int64_t kid, const OptTensor& spec) {
     for (int attempt = 0; attempt < 2; ++attempt) {
         {
@@ -91,40 +102,6 @@ int64_t without_terms(int64_t kid) {
     return g_py->without_terms(kid).cast<int64_t>();
 }
 
-void check(int rc, const char* what) {
-    if (rc == OEQ_OK) return;
-    const char* msg = oeq_last_error();
-    const std::string text = std::string(what) + " failed (" + std::to_string(rc) + "): " + (msg ? msg : "");
-    py::gil_scoped_acquire gil;
-    PyErr_SetString(g_py->error_type.ptr(), text.c_str());
-    python_error err;
-    err.persist();
-    throw err;
-}
-
-int dtype_code(at::ScalarType t) {  // the reference's codes
-    switch (t) {
-        case at::kFloat: return 1;
-        case at::kDouble: return 2;
-        case at::kInt: return 3;
-        case at::kLong: return 4;
-        case at::kByte: return 5;
-        default: return 0;
-    }
-}
-
-std::string dtype_text(at::ScalarType t) {
-    const int code = dtype_code(t);
-    return code ? std::to_string(code) : std::string(at::toString(t));
-}
-
-void check_tensor(const Tensor& t, at::IntArrayRef shape, at::ScalarType dtype, const char* name) {
-    TORCH_CHECK(t.sizes() == shape, "Shape mismatch for tensor '", name, "'. Expected: ", shape, ". Got: ", t.sizes());
-    TORCH_CHECK(t.is_cuda(), "Tensor '", name, "' is not on the GPU.");
-    TORCH_CHECK(t.scalar_type() == dtype, "Dtype mismatch for tensor '", name, "'. Expected: ", dtype_text(dtype),
-                ". Got: ", dtype_text(t.scalar_type()));
-}
-
 void check_weights(const Entry& e, const Tensor& w, int64_t rows, const char* name) {
     if (e.shared)
         check_tensor(w, {e.WN}, e.dtype, name);
@@ -133,19 +110,6 @@ void check_weights(const Entry& e, const Tensor& w, int64_t rows, const char* na
 }
 
 int64_t rows_of(const Tensor& t) { return t.dim() > 0 ? t.size(0) : -1; }
-
-// The device of a call's operands made current, and torch's stream on it.
-struct OnDevice {
-    c10::hip::OptionalHIPGuardMasqueradingAsCUDA guard;
-    void* stream;
-    explicit OnDevice(const Tensor& t) : guard(t.device()) {
-        stream = (void*)(hipStream_t)c10::hip::getCurrentHIPStreamMasqueradingAsCUDA(t.device().index());
-    }
-};
-
-Tensor scratch(const Tensor& like, size_t bytes) {
-    return at::empty({(int64_t)(bytes ? bytes : 1)}, like.options().dtype(at::kByte));
-}
 
 // An operand as the kernels read it: its rows one after the other and, where they are brought into LDS 16 bytes at a time,
 // from a multiple of 16 on. A view into a larger tensor can begin anywhere (plain loads of any width want no more than
@@ -669,11 +633,6 @@ struct NotDifferentiated : public torch::autograd::Function<NotDifferentiated<Si
 
 const char* const kTpDoubleBackward = "oeq_amd::tp_double_backward";
 const char* const kConvDoubleBackward = "oeq_amd::conv_double_backward";
-
-template <typename... Ts>
-bool records(const Ts&... ts) {
-    return at::GradMode::is_enabled() && (ts.requires_grad() || ...);
-}
 
 Tensor tp_forward_autograd(const Tensor& x, const Tensor& y, const Tensor& w, int64_t kid, const OptTensor& spec) {
     if (records(x, y, w)) return TpForward::apply(x, y, w, kid, spec);

@@ -1,0 +1,829 @@
+// Device code of attention among the rows of segments (packed_attention.hip has the launches).
+//
+// Row i of a query segment sees the keys lo(i) <= j < hi(i) of its key segment; with scores s_ij = c q_i.k_j it returns
+//
+//   o_i = sum_j p_ij v_j,  p_ij = exp(s_ij - lse_i),  lse_i = log sum_j exp(s_ij)
+//
+// and, for a gradient g of o,  dv_j = sum_i p_ij g_i,  ds_ij = p_ij (g_i.v_j - delta_i) with delta_i = g_i.o_i,
+// dq_i = c sum_j ds_ij k_j,  dk_j = c sum_i ds_ij q_i, the last two sums over the query heads that share a key head too.
+// Scores, p, ds and all sums are held in 32 bits; where operands have 16, p and ds are rounded to their type as
+// operands of the second products (the products themselves are exact in 32 bits), which costs an error of the size of
+// the output's own rounding. delta would add a third such error where rows see few keys, were it taken from the rounded
+// output: a pass that will be differentiated keeps what the rounding took off beside it (`rest`, 16 bits).
+//
+// Layout of the products. All of them run on the 32x32 matrix instructions with the *transposed* result in registers:
+// S^T = K Q^T puts query i in lane i of either half of a wave and 16 keys in its registers (row 8 (r / 4) + 4 half +
+// r % 4 of the tile in register r), so that a row's maximum and sum are sums over a lane's own registers and one
+// exchange between the halves. The order in which a product sums over keys is free, so registers of P^T serve as they
+// are as the second operand of O^T = V^T P^T if V's rows are read in the order of the registers: no lane ever needs
+// another lane's p. V^T comes from LDS through the transposing reads (16 bit) or four-byte reads (32 bit).
+// dQ^T = K^T dS^T works the same way, and so do dV^T = G^T P and dK^T = Q^T dS with the keys in the lanes.
+//
+// Rows are packed without regard to segments: a block takes 128 consecutive rows, reads the keys from the first that its
+// first row sees to the last that its last row sees, and masks by each row's own bounds. Small segments (molecules)
+// share a tile that way instead of leaving most of it idle: 512 molecules of 9 to 61 atoms fill 110 tiles.
+//
+// What a mask hides has no influence, whatever it holds: hidden scores are replaced before the maximum, hidden p and ds
+// are set to zero. A product still multiplies that zero with the hidden row, which is no zero if that row holds an
+// infinity or NaN; such a product leaves NaN in the sums. So a wave that finds its result not finite computes those rows
+// again one by one from the visible rows alone. Nothing is paid for that where results are finite.
+#ifndef OEQ_PACKED_ATTENTION_H
+#define OEQ_PACKED_ATTENTION_H
+
+#include <hip/hip_runtime.h>
+
+#include <climits>
+#include <cstdint>
+
+namespace packed_attention {
+
+// Rows and heads are strided, a head's elements are contiguous; strides in elements. Gradients and outputs are
+// contiguous [rows, heads, d]. lse (log2 of the sum, see below) and delta are [q_heads, stat_stride].
+struct Args {
+    const void *q, *k, *v, *out, *out_rest, *grad;
+    void *o, *rest, *dq, *dk, *dv;
+    float *lse, *delta;
+    const int64_t *q_ptr, *k_ptr, *k_len;
+    int64_t q_row, q_head, k_row, k_head, v_row, v_head, g_row, g_head, stat_stride;
+    int segments, nq, nk, hq, hk, d, causal, tiles;
+    float scale_log2;  // c * log2(e): the kernels work with powers of two
+    // the form for few queries: keys per part, parts, partial results
+    int part, parts;
+    float* partial;
+};
+
+typedef float float4_t __attribute__((ext_vector_type(4)));
+typedef float float8_t __attribute__((ext_vector_type(8)));
+typedef float float16_t __attribute__((ext_vector_type(16)));
+typedef _Float16 half4_t __attribute__((ext_vector_type(4)));
+typedef _Float16 half8_t __attribute__((ext_vector_type(8)));
+typedef __bf16 bf4_t __attribute__((ext_vector_type(4)));
+typedef __bf16 bf8_t __attribute__((ext_vector_type(8)));
+typedef short short4_t __attribute__((ext_vector_type(4)));
+typedef unsigned uint4_t __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(1))) const void* gptr_t;
+typedef __attribute__((address_space(3))) void* lptr_t;
+typedef __attribute__((address_space(3))) short4_t* ltr_t;
+
+// A fragment is 16 bytes of a row: E elements, the operand of a product over 2 E elements (E in either half of a wave).
+// Powers of two that p and ds carry while they are operands, so that small ones keep their bits (v_exp_f32 knows no
+// numbers below 2^-126, and 16-bit floats of eleven bits end at 2^-24, a weight among 10^7 equal ones); they leave the
+// sums at the end. In the forward pass p reaches 2^8 before that (its maximum is an older one), in the gradients 1.
+// ds of eleven bits is left as it is: its size is that of the output's gradient, whose scale is the caller's choice.
+template <typename T>
+struct Types;
+template <>
+struct Types<float> {
+    typedef float4_t frag;
+    typedef float4_t quad;
+    static constexpr int kForward = 0, kP = 40, kDs = 40;
+};
+template <>
+struct Types<_Float16> {
+    typedef half8_t frag;
+    typedef half4_t quad;
+    static constexpr int kForward = 7, kP = 12, kDs = 0;
+};
+template <>
+struct Types<__bf16> {
+    typedef bf8_t frag;
+    typedef bf4_t quad;
+    static constexpr int kForward = 0, kP = 40, kDs = 40;
+};
+template <int N>
+constexpr float power = N > 0 ? (float)(1ull << (N > 0 ? N : 0)) : 1.0f / (float)(1ull << (N < 0 ? -N : 0));
+
+// 2^(x + N). Where results keep 24 bits the sum would cost some of x's: x is raised only where it is large enough not to
+// lose any, else the result is.
+template <typename T, int N>
+__device__ __forceinline__ float raised(float x) {
+    if constexpr (sizeof(T) == 2 || N == 0) return __builtin_amdgcn_exp2f(x + N);
+    const bool low = x < -100.0f;
+    return __builtin_amdgcn_exp2f(low ? x + N : x) * (low ? 1.0f : power<N>);
+}
+
+__device__ __forceinline__ float16_t mma(float4_t a, float4_t b, float16_t c) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) c = __builtin_amdgcn_mfma_f32_32x32x2f32(a[j], b[j], c, 0, 0, 0);
+    return c;
+}
+__device__ __forceinline__ float16_t mma(half8_t a, half8_t b, float16_t c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
+}
+__device__ __forceinline__ float16_t mma(bf8_t a, bf8_t b, float16_t c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+}
+
+// The same quantity of both halves of a wave: lanes l and l + 32.
+__device__ __forceinline__ float max_halves(float x) {
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ __forceinline__ float sum_halves(float x) {
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+__device__ __forceinline__ float wave_sum(float x) {
+#pragma unroll
+    for (int m = 1; m < 32; m <<= 1) x += __shfl_xor(x, m);
+    return sum_halves(x);
+}
+__device__ __forceinline__ int wave_min(int x) {
+#pragma unroll
+    for (int m = 1; m < 64; m <<= 1) x = min(x, __shfl_xor(x, m));
+    return x;
+}
+__device__ __forceinline__ int wave_max(int x) {
+#pragma unroll
+    for (int m = 1; m < 64; m <<= 1) x = max(x, __shfl_xor(x, m));
+    return x;
+}
+__device__ __forceinline__ bool finite(float x) { return fabsf(x) < INFINITY; }
+
+// ---------------------------------------------------------------------------
+// tiles in LDS
+// ---------------------------------------------------------------------------
+
+// BK rows of DP elements; 16-byte chunk c of row r lies at place c ^ swizzle(r) of the row, so that the eight lanes
+// that a 16-byte read serves in one clock, with the same chunk of eight consecutive rows, touch all banks once.
+template <typename T, int DP, int ROWS, int WAVES = 4>
+struct Tile {
+    static constexpr int kRowBytes = DP * (int)sizeof(T);
+    static constexpr int kChunks = kRowBytes / 16;
+    static constexpr int kBytes = ROWS * kRowBytes;
+    static constexpr int kFrags = kChunks / 2;
+    typedef typename Types<T>::frag frag;
+
+    static __device__ __forceinline__ int swizzle(int r) {
+        return kChunks >= 16 ? (r & 15) : kChunks == 8 ? (r & 7) : ((r >> 1) & 3);
+    }
+
+    // Where the lanes of a wave find their part of a tile, relative to its first row: 1 KB an instruction. Chunks past
+    // the head's end are placed where the reads' own bounds leave them out.
+    static constexpr int kRowsPer = 64 / kChunks, kEach = kBytes / 1024 / WAVES;
+    struct Places {
+        int at[kEach];
+        __device__ __forceinline__ Places(int row_bytes, int chunks, int wave, int lane) {
+            static_assert(kBytes % (1024 * WAVES) == 0, "the waves share a tile");
+#pragma unroll
+            for (int i = 0; i < kEach; ++i) {
+                const int r = (wave * kEach + i) * kRowsPer + lane / kChunks, c = (lane % kChunks) ^ swizzle(r);
+                at[i] = c < chunks ? r * row_bytes + c * 16 : INT_MAX;
+            }
+        }
+    };
+
+    // Requests the tile from row `first` on, straight into LDS. `base` is the head's first row. Nothing is read past the
+    // last row: bounds go with the request, and what lies outside them arrives as zeros.
+    static __device__ __forceinline__ void request(char* lds, const char* base, int row_bytes, const Places& places, int first,
+                                                   int rows, int chunks, int wave) {
+        const int64_t left = (int64_t)(rows - 1 - first) * row_bytes + chunks * 16;
+        const auto from = __builtin_amdgcn_make_buffer_rsrc((void*)(base + (int64_t)first * row_bytes), 0,
+                                                            (int)min(left, (int64_t)INT_MAX - 16), 0x00020000);
+#pragma unroll
+        for (int i = 0; i < kEach; ++i)
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(from, (lptr_t)(lds + (wave * kEach + i) * 1024), 16, places.at[i], 0, 0, 0);
+    }
+
+    // Fragment f of row r: elements (2 f + half) E ... of it.
+    static __device__ __forceinline__ frag row(const char* lds, int r, int f, int half) {
+        return *(const frag*)(lds + r * kRowBytes + (((2 * f + half) ^ swizzle(r)) << 4));
+    }
+};
+
+// Fragment of the transposed tile for the summation over its rows: lane l holds column 32 t + l % 32 of the rows that
+// registers [E f, E f + E) of a result with these rows belong to; `first` is the result's first row in the tile.
+template <typename T, int DP, int ROWS>
+__device__ __forceinline__ typename Types<T>::frag column(const char* lds, int first, int f, int t, int lane) {
+    typedef Tile<T, DP, ROWS> L;
+    typename Types<T>::frag x;
+    if constexpr (sizeof(T) == 2) {
+        // a transposing read gives each of 16 lanes four rows of its column out of the 4 x 16 block whose rows the lanes
+        // address by quarters
+        const int l = lane & 15, c = 4 * t + 2 * ((lane >> 4) & 1) + ((l & 3) >> 1);
+        union {
+            short4_t q[2];
+            typename Types<T>::frag f;
+        } u;
+#pragma unroll
+        for (int g = 0; g < 2; ++g) {
+            const int r = first + 16 * f + 8 * g + 4 * (lane >> 5) + (l >> 2);
+            u.q[g] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                (ltr_t)(lds + r * L::kRowBytes + ((c ^ L::swizzle(r)) << 4) + ((l & 1) << 3)));
+        }
+        x = u.f;
+    } else {
+        const int d = 32 * t + (lane & 31);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const int r = first + 8 * f + 4 * (lane >> 5) + j;
+            x[j] = *(const float*)(lds + r * L::kRowBytes + (((d >> 2) ^ L::swizzle(r)) << 4) + ((d & 3) << 2));
+        }
+    }
+    return x;
+}
+
+// Registers [E f, E f + E) of a result as an operand.
+template <typename T>
+__device__ __forceinline__ typename Types<T>::frag operand(const float16_t& s, int f) {
+    typename Types<T>::frag x;
+    if constexpr (sizeof(T) == 2) {
+        float8_t w;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) w[j] = s[8 * f + j];
+        x = __builtin_convertvector(w, typename Types<T>::frag);
+    } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) x[j] = s[4 * f + j];
+    }
+    return x;
+}
+
+// Fragments of a lane's row straight from memory; `chunks` of 16 bytes exist.
+template <typename T, int FRAGS>
+__device__ __forceinline__ void load_row(typename Types<T>::frag (&x)[FRAGS], const char* row, int chunks, int half) {
+#pragma unroll
+    for (int f = 0; f < FRAGS; ++f) {
+        x[f] = 0;
+        if (2 * f + half < chunks) x[f] = *(const typename Types<T>::frag*)(row + (2 * f + half) * 16);
+    }
+}
+
+// A lane's column of a result (the elements 32 t + 8 (r / 4) + 4 half + r % 4 of its row) times `by` to memory, and to
+// `rest`, if there is one, what rounding takes off.
+template <typename T, int DT>
+__device__ __forceinline__ void store_row(T* row, const float16_t (&acc)[DT], float by, int d, int half, T* rest = nullptr) {
+#pragma unroll
+    for (int t = 0; t < DT; ++t)
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+            const int at = 32 * t + 8 * g + 4 * half;
+            float4_t w;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) w[j] = acc[t][4 * g + j] * by;
+            const auto x = __builtin_convertvector(w, typename Types<T>::quad);
+            if (at < d) *(typename Types<T>::quad*)(row + at) = x;
+            if (rest && at < d)
+                *(typename Types<T>::quad*)(rest + at) =
+                    __builtin_convertvector(w - __builtin_convertvector(x, float4_t), typename Types<T>::quad);
+        }
+}
+
+// ---------------------------------------------------------------------------
+// bounds
+// ---------------------------------------------------------------------------
+
+struct Bounds {
+    int lo, hi;  // what a row sees: lo <= other < hi
+};
+
+__device__ __forceinline__ int clamped(int64_t x, int most) { return (int)(x < 0 ? 0 : x > most ? most : x); }
+
+// The last segment that begins at or before a lane's row (-1: none), out of ascending starts ptr[0 .. segments]. Rows of
+// a wave's lanes are near each other: the wave narrows the range for its least row by 64 pivots at a time, then every
+// lane looks for its own among the next 64 starts (two or three dependent reads for any number of segments up to 4096).
+__device__ __forceinline__ int find_segment(const int64_t* ptr, int segments, int row, int lane) {
+    const int least = wave_min(row);
+    int base = 0, n = segments + 1;
+    while (n > 64) {
+        const int step = (n + 63) / 64;
+        const bool le = lane * step < n && ptr[base + min(lane * step, n - 1)] <= least;
+        const int count = __popcll(__ballot(le));
+        const int skip = max(count - 1, 0) * step;
+        n = min(step, n - skip);
+        base += skip;
+    }
+    int seg = base - 1;
+    for (;;) {
+        const int64_t start = ptr[min(base + lane, segments)];
+        const int window = min(64, segments + 1 - base);
+        const int mine = start > (int64_t)INT_MAX ? INT_MAX : start < (int64_t)INT_MIN ? INT_MIN : (int)start;
+        int count = 0;  // how many of the window's starts are at or before the row
+#pragma unroll
+        for (int step = 32; step >= 1; step >>= 1) {
+            const int v = __shfl(mine, count + step - 1);
+            if (count + step <= window && v <= row) count += step;
+        }
+        const int last = __shfl(mine, min(63, window - 1));
+        if (count == 63 && window == 64 && last <= row) count = 64;
+        if (count > 0) seg = base + count - 1;
+        if (window < 64 || !__any(count == 64)) break;
+        base += 63;
+    }
+    return seg;
+}
+
+// Keys that query row i sees. Causal: the segments' last rows stand side by side, and a row sees up to its own place.
+__device__ __forceinline__ Bounds keys_of(const Args& a, int i, int lane) {
+    const int s = find_segment(a.q_ptr, a.segments, i, lane);
+    Bounds b = {0, 0};
+    if (s >= 0 && s < a.segments) {
+        const int64_t q0 = a.q_ptr[s], q1 = a.q_ptr[s + 1];
+        const int k0 = clamped(a.k_ptr[s], a.nk), k1 = clamped(a.k_ptr[s + 1], a.nk);
+        int len = max(k1 - k0, 0);
+        if (a.k_len) len = min(len, clamped(a.k_len[s], INT_MAX));
+        if (a.causal) len = min((int64_t)len, max((int64_t)0, len - (q1 - q0) + (i - q0) + 1));
+        if (i < q1 && len > 0) b = {k0, k0 + len};
+    }
+    return b;
+}
+
+// Query rows that see key j.
+__device__ __forceinline__ Bounds queries_of(const Args& a, int j, int lane) {
+    const int s = find_segment(a.k_ptr, a.segments, j, lane);
+    Bounds b = {0, 0};
+    if (s >= 0 && s < a.segments) {
+        const int k0 = clamped(a.k_ptr[s], a.nk), k1 = clamped(a.k_ptr[s + 1], a.nk);
+        int len = max(k1 - k0, 0);
+        if (a.k_len) len = min(len, clamped(a.k_len[s], INT_MAX));
+        const int q0 = clamped(a.q_ptr[s], a.nq), q1 = clamped(a.q_ptr[s + 1], a.nq);
+        int first = q0;
+        if (a.causal) first = max(q0, q1 - len + (j - k0));
+        if (j >= k0 && j < k0 + len && first < q1) b = {first, q1};
+    }
+    return b;
+}
+
+// What a wave needs of its lanes' bounds: the union it walks and the intersection in which nothing is hidden.
+struct Walk {
+    int lo, hi, full_lo, full_hi;
+    __device__ __forceinline__ explicit Walk(Bounds b) {
+        const bool any = b.lo < b.hi;
+        lo = __builtin_amdgcn_readfirstlane(wave_min(any ? b.lo : INT_MAX));
+        hi = __builtin_amdgcn_readfirstlane(wave_max(any ? b.hi : 0));
+        full_lo = __builtin_amdgcn_readfirstlane(wave_max(any ? b.lo : INT_MAX));
+        full_hi = __builtin_amdgcn_readfirstlane(wave_min(any ? b.hi : 0));
+    }
+    __device__ __forceinline__ bool needs(int first, int n) const { return first < hi && first + n > lo; }
+    __device__ __forceinline__ bool whole(int first, int n) const { return first >= full_lo && first + n <= full_hi; }
+};
+
+// The union over the block's four waves.
+__device__ __forceinline__ Bounds block_range(const Walk& w, int (&shared)[8], int wave, int lane) {
+    if (lane == 0) {
+        shared[2 * wave] = w.lo;
+        shared[2 * wave + 1] = w.hi;
+    }
+    __syncthreads();
+    Bounds b = {shared[0], shared[1]};
+#pragma unroll
+    for (int i = 1; i < 4; ++i) {
+        b.lo = min(b.lo, shared[2 * i]);
+        b.hi = max(b.hi, shared[2 * i + 1]);
+    }
+    b.lo = __builtin_amdgcn_readfirstlane(b.lo);
+    b.hi = __builtin_amdgcn_readfirstlane(b.hi);
+    return b;
+}
+
+// Block -> (tile, head): blocks that an XCD runs (every eighth) share key heads, so that its L2 holds few of them at a
+// time; causal tiles run from the last on, whose walks are the longest.
+__device__ __forceinline__ void place(const Args& a, int heads, int& tile, int& head) {
+    const int id = blockIdx.x, at = id % heads;
+    tile = id / heads;
+    if (a.causal) tile = a.tiles - 1 - tile;
+    head = heads % 8 == 0 ? (at % 8) * (heads / 8) + at / 8 : at;
+}
+
+// Blocks of four waves on a compute unit: 256 registers a lane for two, 512 where a head of 128 four-byte elements needs
+// more for its row alone.
+template <typename T, int DP>
+constexpr int blocks_per_unit() { return sizeof(T) * DP > 256 ? 1 : 2; }
+
+template <typename T>
+constexpr int tile_rows() { return sizeof(T) == 2 ? 64 : 32; }
+
+__device__ __forceinline__ void arrived() {
+    // what this wave requested is in LDS; then the same for the others, and all are done with the other buffer
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+}
+
+template <int BYTES>
+__device__ __forceinline__ void clear(char* lds) {
+    for (int i = threadIdx.x * 16; i < BYTES; i += 256 * 16) *(uint4_t*)(lds + i) = 0;
+}
+
+// ---------------------------------------------------------------------------
+// rows one by one (see the beginning: results that are not finite)
+// ---------------------------------------------------------------------------
+
+template <typename T>
+__device__ __forceinline__ float dot_row(const T* x, const T* y, int d, int lane) {
+    float s = 0;
+    for (int e = lane; e < d; e += 64) s += (float)x[e] * (float)y[e];
+    return wave_sum(s);
+}
+
+template <typename T>
+__device__ __forceinline__ void forward_row(const Args& a, int i, int h, int lo, int hi, int lane) {
+    const int kh = h / (a.hq / a.hk);
+    const T* q = (const T*)a.q + i * a.q_row + h * a.q_head;
+    const T *k = (const T*)a.k + kh * a.k_head, *v = (const T*)a.v + kh * a.v_head;
+    float m = -INFINITY, l = 0, o0 = 0, o1 = 0;
+    const int e0 = lane, e1 = lane + 64;
+    for (int j = lo; j < hi; ++j) {
+        const float s = dot_row(q, k + j * a.k_row, a.d, lane) * a.scale_log2;
+        const float top = fmaxf(m, s);
+        if (top == -INFINITY && !(s != s)) continue;  // exp(-inf) of nothing yet
+        const float keep = m == -INFINITY ? 0.0f : exp2f(m - top), p = exp2f(s - top);
+        m = top;
+        l = l * keep + p;
+        if (e0 < a.d) o0 = o0 * keep + p * (float)v[j * a.v_row + e0];
+        if (e1 < a.d) o1 = o1 * keep + p * (float)v[j * a.v_row + e1];
+    }
+    const int64_t at = ((int64_t)i * a.hq + h) * a.d;
+    const float by = hi > lo ? 1.0f / l : 0.0f;
+    const auto put = [&](int e, float x) {
+        const T y = (T)x;
+        ((T*)a.o)[at + e] = y;
+        if (a.rest) ((T*)a.rest)[at + e] = (T)(x - (float)y);
+    };
+    if (e0 < a.d) put(e0, hi > lo ? o0 * by : 0.0f);
+    if (e1 < a.d) put(e1, hi > lo ? o1 * by : 0.0f);
+    if (lane == 0) a.lse[h * a.stat_stride + i] = hi > lo ? m + log2f(l) : -INFINITY;
+}
+
+template <typename T>
+__device__ __forceinline__ void query_gradient_row(const Args& a, int i, int h, int lo, int hi, int lane) {
+    const int kh = h / (a.hq / a.hk);
+    const T *q = (const T*)a.q + i * a.q_row + h * a.q_head, *g = (const T*)a.grad + i * a.g_row + h * a.g_head;
+    const T *k = (const T*)a.k + kh * a.k_head, *v = (const T*)a.v + kh * a.v_head;
+    const float lse = a.lse[h * a.stat_stride + i], delta = a.delta[h * a.stat_stride + i];
+    float x0 = 0, x1 = 0;
+    const int e0 = lane, e1 = lane + 64;
+    for (int j = lo; j < hi; ++j) {
+        const float p = exp2f(dot_row(q, k + j * a.k_row, a.d, lane) * a.scale_log2 - lse);
+        const float ds = p * (dot_row(g, v + j * a.v_row, a.d, lane) - delta);
+        if (e0 < a.d) x0 += ds * (float)k[j * a.k_row + e0];
+        if (e1 < a.d) x1 += ds * (float)k[j * a.k_row + e1];
+    }
+    const float by = a.scale_log2 * 0.6931471805599453f;
+    T* dq = (T*)a.dq + ((int64_t)i * a.hq + h) * a.d;
+    if (e0 < a.d) dq[e0] = (T)(x0 * by);
+    if (e1 < a.d) dq[e1] = (T)(x1 * by);
+}
+
+template <typename T>
+__device__ __forceinline__ void key_gradient_row(const Args& a, int j, int kh, int lo, int hi, int lane) {
+    const int group = a.hq / a.hk;
+    const T *k = (const T*)a.k + j * a.k_row + kh * a.k_head, *v = (const T*)a.v + j * a.v_row + kh * a.v_head;
+    float k0 = 0, k1 = 0, v0 = 0, v1 = 0;
+    const int e0 = lane, e1 = lane + 64;
+    for (int h = kh * group; h < (kh + 1) * group; ++h)
+        for (int i = lo; i < hi; ++i) {
+            const T *q = (const T*)a.q + i * a.q_row + h * a.q_head, *g = (const T*)a.grad + i * a.g_row + h * a.g_head;
+            const float p = exp2f(dot_row(q, k, a.d, lane) * a.scale_log2 - a.lse[h * a.stat_stride + i]);
+            const float ds = p * (dot_row(g, v, a.d, lane) - a.delta[h * a.stat_stride + i]);
+            if (e0 < a.d) v0 += p * (float)g[e0], k0 += ds * (float)q[e0];
+            if (e1 < a.d) v1 += p * (float)g[e1], k1 += ds * (float)q[e1];
+        }
+    const float by = a.scale_log2 * 0.6931471805599453f;
+    const int64_t at = ((int64_t)j * a.hk + kh) * a.d;
+    if (e0 < a.d) ((T*)a.dk)[at + e0] = (T)(k0 * by), ((T*)a.dv)[at + e0] = (T)v0;
+    if (e1 < a.d) ((T*)a.dk)[at + e1] = (T)(k1 * by), ((T*)a.dv)[at + e1] = (T)v1;
+}
+
+template <int DT>
+__device__ __forceinline__ bool all_finite(const float16_t (&acc)[DT]) {
+    float z = 0;  // 0 x is NaN where x is not finite
+#pragma unroll
+    for (int t = 0; t < DT; ++t)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) z = fmaf(acc[t][r], 0.0f, z);
+    return z == 0.0f;
+}
+
+// ---------------------------------------------------------------------------
+// forward
+// ---------------------------------------------------------------------------
+
+template <typename T, int DP>
+__global__ __launch_bounds__(256, (blocks_per_unit<T, DP>())) void forward(Args a) {
+    constexpr int BK = tile_rows<T>(), SUB = BK / 32, DT = DP / 32;
+    constexpr int PF = sizeof(T) == 2 ? 2 : 4;  // fragments of 32 keys
+    typedef Tile<T, DP, BK> L;
+    __shared__ __align__(1024) char key0[L::kBytes], key1[L::kBytes], val0[L::kBytes], val1[L::kBytes];
+    __shared__ int shared[8];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5;
+    int tile, h;
+    place(a, a.hq, tile, h);
+    const int kh = h / (a.hq / a.hk), chunks = a.d * (int)sizeof(T) / 16;
+    const int row = (tile * 4 + wave) * 32 + (lane & 31), i = min(row, a.nq - 1);
+    if (chunks < L::kChunks) {
+        clear<L::kBytes>(key0), clear<L::kBytes>(key1), clear<L::kBytes>(val0), clear<L::kBytes>(val1);
+    }
+    const Bounds b = keys_of(a, i, lane);
+    const Walk walk(b);
+    const Bounds all = block_range(walk, shared, wave, lane);
+    const char* kbase = (const char*)((const T*)a.k + kh * a.k_head);
+    const char* vbase = (const char*)((const T*)a.v + kh * a.v_head);
+    const int krow = (int)a.k_row * (int)sizeof(T), vrow = (int)a.v_row * (int)sizeof(T);
+    const typename L::Places kplaces(krow, chunks, wave, lane), vplaces(vrow, chunks, wave, lane);
+    typename L::frag q[L::kFrags];
+    load_row<T, L::kFrags>(q, (const char*)((const T*)a.q + i * a.q_row + h * a.q_head), chunks, half);
+    float16_t acc[DT];
+#pragma unroll
+    for (int t = 0; t < DT; ++t) acc[t] = 0.0f;
+    float m = -INFINITY, l = 0;
+    const float c = a.scale_log2;
+
+    auto products = [&](const char* kt, const char* vt, int first) {
+        float16_t s[SUB];
+#pragma unroll
+        for (int u = 0; u < SUB; ++u) {
+            s[u] = 0.0f;
+#pragma unroll
+            for (int f = 0; f < L::kFrags; ++f) s[u] = mma(L::row(kt, 32 * u + (lane & 31), f, half), q[f], s[u]);
+        }
+        if (!walk.whole(first, BK)) {
+            const int shift = first + 4 * half - b.lo;
+            const unsigned n = b.hi - b.lo;
+#pragma unroll
+            for (int u = 0; u < SUB; ++u)
+#pragma unroll
+                for (int r = 0; r < 16; ++r)
+                    if ((unsigned)(shift + 32 * u + 8 * (r / 4) + r % 4) >= n) s[u][r] = -INFINITY;
+        }
+        float top = s[0][0];
+#pragma unroll
+        for (int u = 0; u < SUB; ++u)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) top = fmaxf(top, s[u][r]);
+        top = max_halves(top);
+        // sums are scaled to another maximum only where it grew by a factor of 2^8: up to there p fits every type
+        if (__any((top - m) * c > 8.0f)) {
+            const float now = fmaxf(m, top);
+            const float by = now == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f((m - now) * c);
+            m = now;
+            l *= by;
+#pragma unroll
+            for (int t = 0; t < DT; ++t) acc[t] *= by;
+        }
+        const float mc = m == -INFINITY ? 0.0f : m * c - Types<T>::kForward;
+#pragma unroll
+        for (int u = 0; u < SUB; ++u) {
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                s[u][r] = __builtin_amdgcn_exp2f(fmaf(s[u][r], c, -mc));
+                l += s[u][r];
+            }
+#pragma unroll
+            for (int f = 0; f < PF; ++f) {
+                const auto p = operand<T>(s[u], f);
+#pragma unroll
+                for (int t = 0; t < DT; ++t) acc[t] = mma(column<T, DP, BK>(vt, 32 * u, f, t, lane), p, acc[t]);
+            }
+        }
+    };
+    auto step = [&](char* kt, char* vt, char* kn, char* vn, int first) {
+        arrived();
+        if (first + BK < all.hi) {
+            L::request(kn, kbase, krow, kplaces, first + BK, a.nk, chunks, wave);
+            L::request(vn, vbase, vrow, vplaces, first + BK, a.nk, chunks, wave);
+        }
+        if (walk.needs(first, BK)) products(kt, vt, first);
+    };
+    if (all.lo < all.hi) {
+        L::request(key0, kbase, krow, kplaces, all.lo, a.nk, chunks, wave);
+        L::request(val0, vbase, vrow, vplaces, all.lo, a.nk, chunks, wave);
+    }
+    for (int first = all.lo; first < all.hi; first += 2 * BK) {
+        step(key0, val0, key1, val1, first);
+        if (first + BK < all.hi) step(key1, val1, key0, val0, first + BK);
+    }
+    l = sum_halves(l);
+    const bool seen = b.lo < b.hi, mine = row < a.nq;
+    const float by = seen ? 1.0f / l : 0.0f;
+    if (mine) {
+        const int64_t at = ((int64_t)i * a.hq + h) * a.d;
+        store_row<T, DT>((T*)a.o + at, acc, by, a.d, half, a.rest ? (T*)a.rest + at : nullptr);
+        if (half == 0) a.lse[h * a.stat_stride + i] = seen ? m * c + (__builtin_amdgcn_logf(l) - Types<T>::kForward) : -INFINITY;
+    }
+    uint64_t bad = __ballot(mine && !(all_finite<DT>(acc) && finite(by)));
+    bad = (bad | bad >> 32) & 0xffffffffu;
+    while (bad) {
+        const int at = __builtin_ctzll(bad);
+        bad &= bad - 1;
+        forward_row<T>(a, (tile * 4 + wave) * 32 + at, h, __shfl(b.lo, at), __shfl(b.hi, at), lane);
+    }
+}
+
+// ---------------------------------------------------------------------------
+// gradient of the queries; delta on the way
+// ---------------------------------------------------------------------------
+
+template <typename T, int DP>
+__global__ __launch_bounds__(256, (blocks_per_unit<T, DP>())) void query_gradient(Args a) {
+    constexpr int BK = tile_rows<T>(), SUB = BK / 32, DT = DP / 32;
+    constexpr int PF = sizeof(T) == 2 ? 2 : 4;
+    typedef Tile<T, DP, BK> L;
+    __shared__ __align__(1024) char key0[L::kBytes], key1[L::kBytes], val0[L::kBytes], val1[L::kBytes];
+    __shared__ int shared[8];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5;
+    int tile, h;
+    place(a, a.hq, tile, h);
+    const int kh = h / (a.hq / a.hk), chunks = a.d * (int)sizeof(T) / 16;
+    const int row = (tile * 4 + wave) * 32 + (lane & 31), i = min(row, a.nq - 1);
+    if (chunks < L::kChunks) {
+        clear<L::kBytes>(key0), clear<L::kBytes>(key1), clear<L::kBytes>(val0), clear<L::kBytes>(val1);
+    }
+    const Bounds b = keys_of(a, i, lane);
+    const Walk walk(b);
+    const Bounds all = block_range(walk, shared, wave, lane);
+    const char* kbase = (const char*)((const T*)a.k + kh * a.k_head);
+    const char* vbase = (const char*)((const T*)a.v + kh * a.v_head);
+    const int krow = (int)a.k_row * (int)sizeof(T), vrow = (int)a.v_row * (int)sizeof(T);
+    const typename L::Places kplaces(krow, chunks, wave, lane), vplaces(vrow, chunks, wave, lane);
+    if (all.lo < all.hi) {
+        L::request(key0, kbase, krow, kplaces, all.lo, a.nk, chunks, wave);
+        L::request(val0, vbase, vrow, vplaces, all.lo, a.nk, chunks, wave);
+    }
+    typename L::frag q[L::kFrags], g[L::kFrags];
+    load_row<T, L::kFrags>(q, (const char*)((const T*)a.q + i * a.q_row + h * a.q_head), chunks, half);
+    load_row<T, L::kFrags>(g, (const char*)((const T*)a.grad + i * a.g_row + h * a.g_head), chunks, half);
+    float delta = 0;
+    {
+        const int64_t at = ((int64_t)i * a.hq + h) * a.d;
+        const char *o = (const char*)((const T*)a.out + at), *rest = (const char*)((const T*)a.out_rest + at);
+#pragma unroll
+        for (int f = 0; f < L::kFrags; ++f) {
+            typename L::frag x = 0, y = 0;
+            if (2 * f + half < chunks) {
+                x = *(const typename L::frag*)(o + (2 * f + half) * 16);
+                if (a.out_rest) y = *(const typename L::frag*)(rest + (2 * f + half) * 16);
+            }
+#pragma unroll
+            for (int e = 0; e < 16 / (int)sizeof(T); ++e) delta = fmaf((float)x[e] + (float)y[e], (float)g[f][e], delta);
+        }
+        delta = sum_halves(delta);
+    }
+    const bool mine = row < a.nq;
+    if (mine && half == 0) a.delta[h * a.stat_stride + i] = delta;
+    const float lse = a.lse[h * a.stat_stride + i], c = a.scale_log2;
+    float16_t acc[DT];
+#pragma unroll
+    for (int t = 0; t < DT; ++t) acc[t] = 0.0f;
+
+    auto products = [&](const char* kt, const char* vt, int first) {
+#pragma unroll
+        for (int u = 0; u < SUB; ++u) {
+            float16_t s = 0.0f, x = 0.0f;
+#pragma unroll
+            for (int f = 0; f < L::kFrags; ++f) s = mma(L::row(kt, 32 * u + (lane & 31), f, half), q[f], s);
+#pragma unroll
+            for (int f = 0; f < L::kFrags; ++f) x = mma(L::row(vt, 32 * u + (lane & 31), f, half), g[f], x);
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                const float p = raised<T, Types<T>::kDs>(fmaf(s[r], c, -lse));
+                x[r] = p * (x[r] - delta);
+            }
+            if (!walk.whole(first, BK)) {
+                const int shift = first + 32 * u + 4 * half - b.lo;
+                const unsigned n = b.hi - b.lo;
+#pragma unroll
+                for (int r = 0; r < 16; ++r)
+                    if ((unsigned)(shift + 8 * (r / 4) + r % 4) >= n) x[r] = 0.0f;
+            }
+#pragma unroll
+            for (int f = 0; f < PF; ++f) {
+                const auto p = operand<T>(x, f);
+#pragma unroll
+                for (int t = 0; t < DT; ++t) acc[t] = mma(column<T, DP, BK>(kt, 32 * u, f, t, lane), p, acc[t]);
+            }
+        }
+    };
+    auto step = [&](char* kt, char* vt, char* kn, char* vn, int first) {
+        arrived();
+        if (first + BK < all.hi) {
+            L::request(kn, kbase, krow, kplaces, first + BK, a.nk, chunks, wave);
+            L::request(vn, vbase, vrow, vplaces, first + BK, a.nk, chunks, wave);
+        }
+        if (walk.needs(first, BK)) products(kt, vt, first);
+    };
+    for (int first = all.lo; first < all.hi; first += 2 * BK) {
+        step(key0, val0, key1, val1, first);
+        if (first + BK < all.hi) step(key1, val1, key0, val0, first + BK);
+    }
+    if (mine)
+        store_row<T, DT>((T*)a.dq + ((int64_t)i * a.hq + h) * a.d, acc, c * (0.6931471805599453f * power<-Types<T>::kDs>), a.d, half);
+    uint64_t bad = __ballot(mine && !all_finite<DT>(acc));
+    bad = (bad | bad >> 32) & 0xffffffffu;
+    while (bad) {
+        const int at = __builtin_ctzll(bad);
+        bad &= bad - 1;
+        query_gradient_row<T>(a, (tile * 4 + wave) * 32 + at, h, __shfl(b.lo, at), __shfl(b.hi, at), lane);
+    }
+}
+
+// ---------------------------------------------------------------------------
+// gradients of keys and values
+// ---------------------------------------------------------------------------
+
+template <typename T, int DP>
+__global__ __launch_bounds__(256, 1) void key_gradient(Args a) {
+    constexpr int BQ = tile_rows<T>(), SUB = BQ / 32, DT = DP / 32;
+    constexpr int PF = sizeof(T) == 2 ? 2 : 4;
+    typedef Tile<T, DP, BQ> L;
+    __shared__ __align__(1024) char que0[L::kBytes], que1[L::kBytes], gra0[L::kBytes], gra1[L::kBytes];
+    __shared__ __align__(1024) float sta0[128], sta1[128];  // lse, then delta, of the tile's rows
+    __shared__ int shared[8];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5;
+    int tile, kh;
+    place(a, a.hk, tile, kh);
+    if (a.causal) tile = a.tiles - 1 - tile;  // the first keys have the longest walks
+    const int group = a.hq / a.hk, chunks = a.d * (int)sizeof(T) / 16;
+    const int row = (tile * 4 + wave) * 32 + (lane & 31), j = min(row, a.nk - 1);
+    if (chunks < L::kChunks) {
+        clear<L::kBytes>(que0), clear<L::kBytes>(que1), clear<L::kBytes>(gra0), clear<L::kBytes>(gra1);
+    }
+    const Bounds b = queries_of(a, j, lane);
+    const Walk walk(b);
+    const Bounds all = block_range(walk, shared, wave, lane);
+    const int qrow = (int)a.q_row * (int)sizeof(T), grow = (int)a.g_row * (int)sizeof(T);
+    const typename L::Places qplaces(qrow, chunks, wave, lane), gplaces(grow, chunks, wave, lane);
+    const int steps = all.lo < all.hi ? (all.hi - all.lo + BQ - 1) / BQ : 0, total = steps * group;
+
+    auto request = [&](char* qt, char* gt, float* st, int n) {
+        const int h = kh * group + n / steps, first = all.lo + (n % steps) * BQ;
+        L::request(qt, (const char*)((const T*)a.q + h * a.q_head), qrow, qplaces, first, a.nq, chunks, wave);
+        L::request(gt, (const char*)((const T*)a.grad + h * a.g_head), grow, gplaces, first, a.nq, chunks, wave);
+        // (a row of statistics is longer than the queries by more than a tile)
+        if (wave < 2)
+            __builtin_amdgcn_global_load_lds((gptr_t)((wave ? a.delta : a.lse) + h * a.stat_stride + first + lane),
+                                             (lptr_t)(st + 64 * wave), 4, 0, 0);
+    };
+    if (total) request(que0, gra0, sta0, 0);
+    typename L::frag k[L::kFrags], v[L::kFrags];
+    load_row<T, L::kFrags>(k, (const char*)((const T*)a.k + j * a.k_row + kh * a.k_head), chunks, half);
+    load_row<T, L::kFrags>(v, (const char*)((const T*)a.v + j * a.v_row + kh * a.v_head), chunks, half);
+    const float c = a.scale_log2;
+    float16_t dk[DT], dv[DT];
+#pragma unroll
+    for (int t = 0; t < DT; ++t) dk[t] = 0.0f, dv[t] = 0.0f;
+
+    constexpr float kRatio = power<Types<T>::kDs - Types<T>::kP>;
+    auto products = [&](const char* qt, const char* gt, const float* st, int first) {
+#pragma unroll
+        for (int u = 0; u < SUB; ++u) {
+            float16_t s = 0.0f, x = 0.0f;
+#pragma unroll
+            for (int f = 0; f < L::kFrags; ++f) s = mma(L::row(qt, 32 * u + (lane & 31), f, half), k[f], s);
+#pragma unroll
+            for (int f = 0; f < L::kFrags; ++f) x = mma(L::row(gt, 32 * u + (lane & 31), f, half), v[f], x);
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+                const float4_t lse = *(const float4_t*)(st + 32 * u + 8 * g + 4 * half);
+                const float4_t delta = *(const float4_t*)(st + 64 + 32 * u + 8 * g + 4 * half);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const int r = 4 * g + e;
+                    s[r] = raised<T, Types<T>::kP>(fmaf(s[r], c, -lse[e]));
+                    x[r] = s[r] * fmaf(x[r], kRatio, -delta[e] * kRatio);
+                }
+            }
+            if (!walk.whole(first, BQ)) {
+                const int shift = first + 32 * u + 4 * half - b.lo;
+                const unsigned n = b.hi - b.lo;
+#pragma unroll
+                for (int r = 0; r < 16; ++r)
+                    if ((unsigned)(shift + 8 * (r / 4) + r % 4) >= n) s[r] = 0.0f, x[r] = 0.0f;
+            }
+#pragma unroll
+            for (int f = 0; f < PF; ++f) {
+                const auto p = operand<T>(s, f);
+#pragma unroll
+                for (int t = 0; t < DT; ++t) dv[t] = mma(column<T, DP, BQ>(gt, 32 * u, f, t, lane), p, dv[t]);
+                const auto d = operand<T>(x, f);
+#pragma unroll
+                for (int t = 0; t < DT; ++t) dk[t] = mma(column<T, DP, BQ>(qt, 32 * u, f, t, lane), d, dk[t]);
+            }
+        }
+    };
+    auto step = [&](char* qt, char* gt, float* st, char* qn, char* gn, float* sn, int n) {
+        arrived();
+        if (n + 1 < total) request(qn, gn, sn, n + 1);
+        const int first = all.lo + (n % steps) * BQ;
+        if (walk.needs(first, BQ)) products(qt, gt, st, first);
+    };
+    for (int n = 0; n < total; n += 2) {
+        step(que0, gra0, sta0, que1, gra1, sta1, n);
+        if (n + 1 < total) step(que1, gra1, sta1, que0, gra0, sta0, n + 1);
+    }
+    const bool mine = row < a.nk;
+    if (mine) {
+        const int64_t at = ((int64_t)j * a.hk + kh) * a.d;
+        store_row<T, DT>((T*)a.dk + at, dk, c * (0.6931471805599453f * power<-Types<T>::kDs>), a.d, half);
+        store_row<T, DT>((T*)a.dv + at, dv, power<-Types<T>::kP>, a.d, half);
+    }
+    uint64_t bad = __ballot(mine && !(all_finite<DT>(dk) && all_finite<DT>(dv)));
+    bad = (bad | bad >> 32) & 0xffffffffu;
+    while (bad) {
+        const int at = __builtin_ctzll(bad);
+        bad &= bad - 1;
+        key_gradient_row<T>(a, (tile * 4 + wave) * 32 + at, kh, __shfl(b.lo, at), __shfl(b.hi, at), lane);
+    }
+}
+
+}  // namespace packed_attention
+#endif

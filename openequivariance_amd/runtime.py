@@ -20,7 +20,7 @@ from typing import Dict, List, Optional, Sequence, Tuple
 _PKG_DIR = Path(__file__).resolve().parent
 _REPO_DIR = _PKG_DIR.parent
 _LIB_PATH = _PKG_DIR / "liboeq_amd.so"
-_SRC_PATH = _PKG_DIR / "csrc" / "oeq_amd.cpp"
+_CSRC_DIR = _PKG_DIR / "csrc"
 _INCLUDE_DIR = _REPO_DIR / "include"
 
 DEFAULT_ARCH = "gfx950"
@@ -62,7 +62,7 @@ ROLE_SLICE_PLACE = 24
 
 CONV_ATOMIC, CONV_SORTED, CONV_GROUPED = 0, 1, 2
 DX_TERMS, DX_ATOMIC, DX_ARRIVAL, DX_SENDER_WALK = 0, 1, 2, 3
-ABI_VERSION = 8
+ABI_VERSION = 9
 
 
 class OeqError(RuntimeError):
@@ -114,25 +114,72 @@ class _ProblemDims(ctypes.Structure):
     ]
 
 
+class _Attention(ctypes.Structure):
+    _fields_ = ([(n, ctypes.c_int32) for n in ("type", "causal", "segments", "q_heads", "k_heads", "head_dim")]
+                + [("scale", ctypes.c_float), ("reserved", ctypes.c_int32)]
+                + [(n, ctypes.c_int64) for n in ("q_rows", "k_rows", "q_row_stride", "q_head_stride", "k_row_stride",
+                                                 "k_head_stride", "v_row_stride", "v_head_stride")]
+                + [(n, ctypes.c_void_p) for n in ("q", "k", "v", "q_ptr", "k_ptr", "k_len")])
+
+
+class _QkRotary(ctypes.Structure):
+    _fields_ = ([(n, ctypes.c_int32) for n in ("type", "interleaved", "q_heads", "k_heads", "head_dim", "rotary_dim")]
+                + [("eps", ctypes.c_float), ("reserved", ctypes.c_int32)]
+                + [(n, ctypes.c_int64) for n in ("rows", "table_rows", "q_row_stride", "q_head_stride", "k_row_stride",
+                                                 "k_head_stride")]
+                + [(n, ctypes.c_void_p) for n in ("q", "k", "q_weight", "k_weight", "positions", "table")])
+
+
+# What liboeq_amd.so is compiled from, with the macros of each object: the runtime and the operators on nodes, whose
+# attention kernels make one object per element type (they take the longest: compiled side by side).
+_OBJECTS = [("oeq_amd.cpp", []), ("oeq_nodes.hip", [])] + [
+    ("packed_attention.hip", [f"-DOEQ_ATTENTION_TYPE={t}"]) for t in ("float", "_Float16", "__bf16")]
+
+
+def _sources() -> List[Path]:
+    headers = sorted(_CSRC_DIR.glob("*.h"))
+    return [_CSRC_DIR / name for name in sorted({o[0] for o in _OBJECTS})] + headers + [_INCLUDE_DIR / "oeq_amd.h"]
+
+
 def build_library(verbose: bool = False) -> Path:
-    """Compile csrc/oeq_amd.cpp into liboeq_amd.so next to this file."""
-    # the library carries one device-side object (the scratch array of oeq_conv_forward_static), so it is
-    # compiled for the target architecture, with the device flags every kernel here is compiled with
+    """Compile csrc into liboeq_amd.so next to this file."""
+    import tempfile
+    # the library carries device code of its own (the kernels of the operators on nodes and the scratch array of
+    # oeq_conv_forward_static), so it is compiled for the target architecture, with the device flags every kernel
+    # here is compiled with
     # built under a temporary name and moved into place, so that a process loading the library while
     # another one rebuilds it never maps a half-written file
     tmp = _LIB_PATH.with_name(f"{_LIB_PATH.name}.tmp{os.getpid()}")
-    cmd = [
-        "hipcc", "-O2", "-std=c++17", "-shared", "-fPIC", f"--offload-arch={DEFAULT_ARCH}",
-        "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops", f"-I{_INCLUDE_DIR}",
-        str(_SRC_PATH), "-o", str(tmp), "-lhiprtc",
-    ]
-    res = subprocess.run(cmd, capture_output=True, text=True)
+    with tempfile.TemporaryDirectory(prefix="oeq_build_") as objects:
+        cmds, procs = [], []
+        for n, (name, macros) in enumerate(_OBJECTS):
+            cmds.append(["hipcc", "-O3" if name.endswith(".hip") else "-O2", "-std=c++17", "-fPIC",
+                         f"--offload-arch={DEFAULT_ARCH}", "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
+                         f"-I{_INCLUDE_DIR}", *macros, "-c", str(_CSRC_DIR / name), "-o", f"{objects}/{n}.o"])
+        cmds.append(["hipcc", "-shared", "-fPIC", f"--offload-arch={DEFAULT_ARCH}",
+                     *[f"{objects}/{n}.o" for n in range(len(_OBJECTS))], "-o", str(tmp), "-lhiprtc"])
+        logs = []
+        try:
+            for n, cmd in enumerate(cmds[:-1]):
+                logs.append(open(f"{objects}/{n}.log", "w+"))
+                procs.append(subprocess.Popen(cmd, stdout=logs[-1], stderr=subprocess.STDOUT))
+        finally:
+            status = [p.wait() for p in procs]  # (every child is waited for)
+            texts = []
+            for log in logs:
+                log.seek(0)
+                texts.append(log.read())
+                log.close()
+        if any(status):
+            raise OeqError("building liboeq_amd.so failed:\n" + "\n".join(t for t, rc in zip(texts, status) if rc))
+        res = subprocess.run(cmds[-1], capture_output=True, text=True)
     if res.returncode != 0:
         tmp.unlink(missing_ok=True)
         raise OeqError(f"building liboeq_amd.so failed:\n{res.stdout}\n{res.stderr}")
     os.replace(tmp, _LIB_PATH)
     if verbose:
-        print(" ".join(cmd).replace(str(tmp), str(_LIB_PATH)))
+        for cmd in cmds:
+            print(" ".join(cmd).replace(str(tmp), str(_LIB_PATH)))
     return _LIB_PATH
 
 
@@ -183,6 +230,17 @@ EXPORTS = {
     "oeq_kernel_timing_enable": (ctypes.c_int, [_P, ctypes.c_int]),
     "oeq_kernel_timing_collect": (ctypes.c_int, [_P, ctypes.c_int, ctypes.POINTER(ctypes.c_double),
                                                  ctypes.POINTER(_I64)]),
+    "oeq_attention_stat_stride": (_I64, [_I64]),
+    "oeq_attention_forward_workspace_bytes": (_SZ, [ctypes.POINTER(_Attention)]),
+    "oeq_attention_forward": (ctypes.c_int, [ctypes.POINTER(_Attention), _P, _P, _P, _P, _SZ, _P]),
+    "oeq_attention_backward": (ctypes.c_int, [ctypes.POINTER(_Attention), _P, _P, _P, _P, _I64, _I64] + [_P] * 5),
+    "oeq_qk_norm_rotary": (ctypes.c_int, [ctypes.POINTER(_QkRotary), _P, _P, _P]),
+    "oeq_qk_norm_rotary_append": (ctypes.c_int, [ctypes.POINTER(_QkRotary), _P, _I64, _I64, _P, _P, _I64, _I64, _P, _I64,
+                                                 _I64, _P, _I64, _P]),
+    "oeq_qk_norm_rotary_backward_workspace_bytes": (_SZ, [ctypes.POINTER(_QkRotary)]),
+    "oeq_qk_norm_rotary_backward": (ctypes.c_int, [ctypes.POINTER(_QkRotary), _P, _I64, _I64, _P, _I64, _I64, _P, _P, _P,
+                                                   _P, _P, _SZ, _P]),
+    "oeq_irrep_dropout": (ctypes.c_int, [ctypes.c_int, _I64, _I64, _P, _P, _P, _P, _P, ctypes.c_double, _P]),
     "oeq_last_error": (ctypes.c_char_p, []),
     "oeq_abi_version": (ctypes.c_int, []),
 }
@@ -195,7 +253,7 @@ def lib_path() -> Path:
 def _stale() -> bool:
     """The built library is older than the sources it is made from."""
     built = _LIB_PATH.stat().st_mtime
-    return any(src.exists() and src.stat().st_mtime > built for src in (_SRC_PATH, _INCLUDE_DIR / "oeq_amd.h"))
+    return any(src.exists() and src.stat().st_mtime > built for src in _sources())
 
 
 def load_library():
