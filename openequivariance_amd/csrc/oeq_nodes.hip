@@ -10,6 +10,7 @@
 #include <algorithm>
 #include <climits>
 #include <cmath>
+#include <cstdlib>
 
 using oeq_internal::fail;
 
@@ -62,6 +63,23 @@ packed_attention::Args attention_args(const oeq_attention& a) {
     g.scale_log2 = a.scale * 1.4426950408889634f;
     return g;
 }
+
+// How many shares the form for few queries cuts a row's keys into; 0: the form for tiles of rows.
+//
+// Lengths are on the device, so the rule goes by means over the segments. Tiles are for rows that share keys with their
+// neighbours; with few rows to a segment and many keys to a row nearly all of a tile's scores are hidden ones.
+int parts_of(const oeq_attention& a) {
+    { const char* e = getenv("OEQ_TRY_FORM"); if (e && atoi(e) == 0) return 0; if (!e && (a.q_rows > 8 * (int64_t)a.segments || a.k_rows < 16 * a.q_rows)) return 0; }
+    const int64_t blocks = a.q_rows * a.k_heads * ((a.q_heads / a.k_heads + 31) / 32);
+    const int64_t keys = (a.k_rows + a.segments - 1) / a.segments;  // to a row
+    static const int target = [] { const char* e = getenv("OEQ_TRY_BLOCKS"); return e ? atoi(e) : 1024; }();
+    static const int least = [] { const char* e = getenv("OEQ_TRY_LEAST"); return e ? atoi(e) : 256; }();
+    const int64_t parts = std::min({target / blocks, (keys + least - 1) / least, (int64_t)packed_attention::kMostParts});
+    if (blocks > INT_MAX / packed_attention::kMostParts) return 0;
+    return (int)std::max<int64_t>(parts, 1);
+}
+
+int head_tile(int d) { return d <= 32 ? 32 : d <= 64 ? 64 : 128; }
 
 int check_rotary(const char* who, const oeq_qk_rotary* a) {
     if (!a) return fail(OEQ_ERR_INVALID, "%s: NULL description", who);
@@ -160,7 +178,11 @@ extern "C" {
 
 int64_t oeq_attention_stat_stride(int64_t q_rows) { return (q_rows + 63) / 64 * 64 + 64; }
 
-size_t oeq_attention_forward_workspace_bytes(const oeq_attention*) { return 0; }
+size_t oeq_attention_forward_workspace_bytes(const oeq_attention* a) {
+    if (!a || a->k_heads <= 0 || a->q_heads <= 0 || a->segments < 0 || a->q_rows <= 0) return 0;
+    const int parts = parts_of(*a);
+    return parts > 1 ? (size_t)a->q_rows * a->q_heads * parts * (head_tile(a->head_dim) + 4) * sizeof(float) : 0;
+}
 
 int oeq_attention_forward(const oeq_attention* a, void* out, void* out_rest, float* log2_sum, void* workspace,
                           size_t workspace_bytes, void* stream) {
@@ -173,6 +195,7 @@ int oeq_attention_forward(const oeq_attention* a, void* out, void* out_rest, flo
         return fail(OEQ_ERR_INVALID, "%s: workspace too small", who);
     packed_attention::Args g = attention_args(*a);
     g.o = out, g.rest = out_rest, g.lse = log2_sum;
+    g.parts = parts_of(*a), g.partial = (float*)workspace;
     const auto s = (hipStream_t)stream;
     HIP_TRY(a->type == OEQ_FLOAT32 ? packed_attention::Launch<float>::forward(g, s)
             : a->type == OEQ_FLOAT16 ? packed_attention::Launch<_Float16>::forward(g, s)

@@ -47,8 +47,7 @@ struct Args {
     int64_t q_row, q_head, k_row, k_head, v_row, v_head, g_row, g_head, stat_stride;
     int segments, nq, nk, hq, hk, d, causal, tiles;
     float scale_log2;  // c * log2(e): the kernels work with powers of two
-    // the form for few queries: keys per part, parts, partial results
-    int part, parts;
+    int parts;  // the form for few queries: shares of a row's keys, and their results
     float* partial;
 };
 
@@ -194,7 +193,7 @@ struct Tile {
 // Fragment of the transposed tile for the summation over its rows: lane l holds column 32 t + l % 32 of the rows that
 // registers [E f, E f + E) of a result with these rows belong to; `first` is the result's first row in the tile.
 template <typename T, int DP, int ROWS>
-__device__ __forceinline__ typename Types<T>::frag column(const char* lds, int first, int f, int t, int lane) {
+__device__ __forceinline__ typename Types<T>::frag column_of(const char* lds, int first, int f, int t, int lane) {
     typedef Tile<T, DP, ROWS> L;
     typename Types<T>::frag x;
     if constexpr (sizeof(T) == 2) {
@@ -572,21 +571,21 @@ __global__ __launch_bounds__(256, (blocks_per_unit<T, DP>())) void forward(Args 
             for (int f = 0; f < PF; ++f) {
                 const auto p = operand<T>(s[u], f);
 #pragma unroll
-                for (int t = 0; t < DT; ++t) acc[t] = mma(column<T, DP, BK>(vt, 32 * u, f, t, lane), p, acc[t]);
+                for (int t = 0; t < DT; ++t) acc[t] = mma(column_of<T, DP, BK>(vt, 32 * u, f, t, lane), p, acc[t]);
             }
         }
     };
     auto step = [&](char* kt, char* vt, char* kn, char* vn, int first) {
         arrived();
         if (first + BK < all.hi) {
-            L::request(kn, kbase, krow, kplaces, first + BK, a.nk, chunks, wave);
-            L::request(vn, vbase, vrow, vplaces, first + BK, a.nk, chunks, wave);
+            L::request(kn, kbase, krow, kplaces, first + BK, all.hi, chunks, wave);
+            L::request(vn, vbase, vrow, vplaces, first + BK, all.hi, chunks, wave);
         }
         if (walk.needs(first, BK)) products(kt, vt, first);
     };
     if (all.lo < all.hi) {
-        L::request(key0, kbase, krow, kplaces, all.lo, a.nk, chunks, wave);
-        L::request(val0, vbase, vrow, vplaces, all.lo, a.nk, chunks, wave);
+        L::request(key0, kbase, krow, kplaces, all.lo, all.hi, chunks, wave);
+        L::request(val0, vbase, vrow, vplaces, all.lo, all.hi, chunks, wave);
     }
     for (int first = all.lo; first < all.hi; first += 2 * BK) {
         step(key0, val0, key1, val1, first);
@@ -607,6 +606,253 @@ __global__ __launch_bounds__(256, (blocks_per_unit<T, DP>())) void forward(Args 
         bad &= bad - 1;
         forward_row<T>(a, (tile * 4 + wave) * 32 + at, h, __shfl(b.lo, at), __shfl(b.hi, at), lane);
     }
+}
+
+// ---------------------------------------------------------------------------
+// forward, few queries to many keys
+// ---------------------------------------------------------------------------
+//
+// A new token against its cache reads every key and value once and computes next to nothing: the work is to keep reads in
+// flight on all compute units. A block has one query row, one key head and one of `parts` equal shares of the row's keys;
+// the query heads that share the key head (up to 32) are the columns of the products, so that keys and values are read
+// once for all of them. Each wave walks tiles of 32 keys of its own through LDS, the next one always on its way, and
+// meets the others only at the end. Rows past the share's end are cut off by the reads' bounds and arrive as zeros. Shares
+// of more than one block's row meet in `join`, in the order of the keys.
+
+template <typename T, int DP>
+struct Few {
+    typedef Tile<T, DP, 32, 1> L;
+    static constexpr int kWaves = 4 * L::kBytes >= 32768 ? 2 : 4;  // (two tiles each of keys and values to a wave)
+    static constexpr int kRow = DP + 4;  // floats of a partial result: sums, then the maximum (log2) and the sum of p
+    // Where four sums of a wave's column lie once the tiles in LDS are done with: in the first key buffer, the upper half
+    // of a 16-bit head in the first value buffer; quads are permuted by column so that columns begin in different banks.
+    static __device__ __forceinline__ float4_t* sums(char* key, char* val, int wave, int column, int d) {
+        constexpr int kIn = sizeof(T) == 4 ? DP : DP / 2, kQuads = kIn / 4, kMask = kQuads < 8 ? kQuads - 1 : 7;
+        char* buffer = d < kIn ? key : val;
+        return (float4_t*)(buffer + (((wave * 32 + column) * kQuads + ((d % kIn / 4) ^ (column & kMask))) << 4));
+    }
+};
+
+constexpr int kMostParts = 256;
+
+struct Share {
+    int first, last, count;  // keys of this part; parts that have any
+    __device__ __forceinline__ Share(Bounds b, int parts, int part, int grain) {
+        const int n = b.hi - b.lo, each = (((n + parts - 1) / parts + grain - 1) / grain) * grain;
+        count = n > 0 ? (n + each - 1) / each : 0;
+        first = b.lo + (int)min((int64_t)part * each, (int64_t)n);
+        last = min(first + each, b.hi);
+    }
+};
+
+template <typename T, int DP>
+__global__ __launch_bounds__((64 * Few<T, DP>::kWaves), 1) void forward_few(Args a) {
+    constexpr int W = Few<T, DP>::kWaves, DT = DP / 32, PF = sizeof(T) == 2 ? 2 : 4, ROW = Few<T, DP>::kRow;
+    typedef typename Few<T, DP>::L L;
+    __shared__ __align__(1024) char key0[W * L::kBytes], key1[W * L::kBytes], val0[W * L::kBytes], val1[W * L::kBytes];
+    __shared__ float top_of[W][32], sum_of[W][32];
+    __shared__ int bad;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5;
+    const int group = a.hq / a.hk, stacks = (group + 31) / 32;
+    int id = blockIdx.x;
+    const int part = id % a.parts;
+    id /= a.parts;
+    const int stack = id % stacks;
+    id /= stacks;
+    const int kh = id % a.hk, i = id / a.hk;
+    const int heads = min(32, group - 32 * stack), h0 = kh * group + 32 * stack, column = lane & 31;
+    const int chunks = a.d * (int)sizeof(T) / 16;
+    const Bounds b = keys_of(a, i, lane);
+    const Share mine(Bounds{__builtin_amdgcn_readfirstlane(b.lo), __builtin_amdgcn_readfirstlane(b.hi)}, a.parts, part, 32 * W);
+    if (part && mine.first >= mine.last) return;
+    char *kt0 = key0 + wave * L::kBytes, *kt1 = key1 + wave * L::kBytes;
+    char *vt0 = val0 + wave * L::kBytes, *vt1 = val1 + wave * L::kBytes;
+    if (chunks < L::kChunks) {  // (a wave's own part of the buffers: no barrier)
+        for (int n = lane * 16; n < L::kBytes; n += 1024)
+            *(uint4_t*)(kt0 + n) = 0, *(uint4_t*)(kt1 + n) = 0, *(uint4_t*)(vt0 + n) = 0, *(uint4_t*)(vt1 + n) = 0;
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    }
+    const char* kbase = (const char*)((const T*)a.k + kh * a.k_head);
+    const char* vbase = (const char*)((const T*)a.v + kh * a.v_head);
+    const int krow = (int)a.k_row * (int)sizeof(T), vrow = (int)a.v_row * (int)sizeof(T);
+    const typename L::Places kplaces(krow, chunks, 0, lane), vplaces(vrow, chunks, 0, lane);
+    auto request = [&](char* kt, char* vt, int first) {
+        L::request(kt, kbase, krow, kplaces, first, mine.last, chunks, 0);
+        L::request(vt, vbase, vrow, vplaces, first, mine.last, chunks, 0);
+    };
+    constexpr int kStep = 32 * W, kAhead = 2 * L::kEach;  // (requests of a tile's keys and values)
+    const int start = mine.first + 32 * wave;
+    if (start < mine.last) request(kt0, vt0, start);
+    typename L::frag q[L::kFrags];
+    const bool live = column < heads;
+    load_row<T, L::kFrags>(q, (const char*)((const T*)a.q + i * a.q_row + (h0 + (live ? column : 0)) * a.q_head),
+                           live ? chunks : 0, half);
+    float16_t acc[DT];
+#pragma unroll
+    for (int t = 0; t < DT; ++t) acc[t] = 0.0f;
+    float m = -INFINITY, l = 0;
+    const float c = a.scale_log2;
+
+    auto step = [&](char* kt, char* vt, char* kn, char* vn, int first) {
+        if (first + kStep < mine.last) {
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // what was read from there has come
+            request(kn, vn, first + kStep);
+            asm volatile("s_waitcnt vmcnt(%0)" ::"n"(kAhead) : "memory");
+        } else {
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        }
+        float16_t s = 0.0f;
+#pragma unroll
+        for (int f = 0; f < L::kFrags; ++f) s = mma(L::row(kt, lane & 31, f, half), q[f], s);
+        if (first + 32 > mine.last) {
+#pragma unroll
+            for (int r = 0; r < 16; ++r)
+                if (first + 4 * half + 8 * (r / 4) + r % 4 >= mine.last) s[r] = -INFINITY;
+        }
+        float top = s[0];
+#pragma unroll
+        for (int r = 1; r < 16; ++r) top = fmaxf(top, s[r]);
+        top = max_halves(top);
+        if (__any((top - m) * c > 8.0f)) {
+            const float now = fmaxf(m, top);
+            const float by = now == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f((m - now) * c);
+            m = now;
+            l *= by;
+#pragma unroll
+            for (int t = 0; t < DT; ++t) acc[t] *= by;
+        }
+        const float mc = m == -INFINITY ? 0.0f : m * c - Types<T>::kForward;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+            s[r] = __builtin_amdgcn_exp2f(fmaf(s[r], c, -mc));
+            l += s[r];
+        }
+#pragma unroll
+        for (int f = 0; f < PF; ++f) {
+            const auto p = operand<T>(s, f);
+#pragma unroll
+            for (int t = 0; t < DT; ++t) acc[t] = mma(column_of<T, DP, 32>(vt, 0, f, t, lane), p, acc[t]);
+        }
+    };
+    for (int first = start; first < mine.last; first += 2 * kStep) {
+        step(kt0, vt0, kt1, vt1, first);
+        if (first + kStep < mine.last) step(kt1, vt1, kt0, vt0, first + kStep);
+    }
+    // the waves' results: sums under the largest maximum, added in order
+    l = sum_halves(l);
+    if (half == 0) top_of[wave][column] = m, sum_of[wave][column] = l;
+    if (threadIdx.x == 0) bad = 0;
+    __syncthreads();
+    float top = top_of[0][column];
+#pragma unroll
+    for (int w = 1; w < W; ++w) top = fmaxf(top, top_of[w][column]);
+    {
+        const float by = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((m - top) * c);
+        if (live)
+#pragma unroll
+            for (int t = 0; t < DT; ++t)
+#pragma unroll
+                for (int g = 0; g < 4; ++g) {
+                    float4_t x;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) x[e] = acc[t][4 * g + e] * by;
+                    *Few<T, DP>::sums(key0, val0, wave, column, 32 * t + 8 * g + 4 * half) = x;
+                }
+    }
+    __syncthreads();
+    const bool seen = mine.count > 0;
+    bool finite_all = true;
+    for (int at = threadIdx.x; at < heads * (DP / 4); at += 64 * W) {
+        const int col = at / (DP / 4), e = at % (DP / 4) * 4, h = h0 + col;
+        if (e >= a.d) continue;
+        float high = top_of[0][col], total = 0;
+        float4_t x = 0.0f;
+#pragma unroll
+        for (int w = 1; w < W; ++w) high = fmaxf(high, top_of[w][col]);
+#pragma unroll
+        for (int w = 0; w < W; ++w) {
+            const float one = top_of[w][col];
+            total += one == -INFINITY ? 0.0f * sum_of[w][col] : sum_of[w][col] * __builtin_amdgcn_exp2f((one - high) * c);
+            x += *Few<T, DP>::sums(key0, val0, w, col, e);
+        }
+        const float log2_top = high == -INFINITY ? high : high * c - Types<T>::kForward;
+        if (mine.count > 1) {
+            float* to = a.partial + (((int64_t)i * a.hq + h) * a.parts + part) * ROW;
+            *(float4_t*)(to + e) = x;
+            if (e == 0) to[DP] = log2_top, to[DP + 1] = total;
+            continue;
+        }
+        const int64_t out = ((int64_t)i * a.hq + h) * a.d + e;
+        const float by = seen ? 1.0f / total : 0.0f;
+        x *= by;
+        const auto y = __builtin_convertvector(x, typename Types<T>::quad);
+        *(typename Types<T>::quad*)((T*)a.o + out) = y;
+        if (a.rest)
+            *(typename Types<T>::quad*)((T*)a.rest + out) =
+                __builtin_convertvector(x - __builtin_convertvector(y, float4_t), typename Types<T>::quad);
+        if (e == 0) a.lse[h * a.stat_stride + i] = seen ? log2_top + __builtin_amdgcn_logf(total) : -INFINITY;
+        finite_all = finite_all && finite(x[0] + x[1] + x[2] + x[3]) && finite(by);
+    }
+    if (mine.count > 1) return;
+    if (!finite_all) bad = 1;
+    __syncthreads();
+    if (!bad) return;
+    for (int n = wave; n < heads; n += W) forward_row<T>(a, i, h0 + n, b.lo, b.hi, lane);
+}
+
+// Adds up the shares of one row's head: eight groups of 32 lanes take every eighth share, then in order.
+template <typename T, int DP>
+__global__ __launch_bounds__(256) void join(Args a) {
+    constexpr int ROW = Few<T, DP>::kRow;
+    __shared__ float weight[kMostParts], tops[4], totals[4];
+    __shared__ __align__(16) float sums[8][DP];
+    __shared__ int bad;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int h = blockIdx.x % a.hq, i = blockIdx.x / a.hq;
+    const Bounds b = keys_of(a, i, lane);
+    const int count = Share(b, a.parts, 0, 32 * Few<T, DP>::kWaves).count;
+    if (count <= 1) return;
+    const float* from = a.partial + ((int64_t)i * a.hq + h) * a.parts * ROW;
+    const bool mine = (int)threadIdx.x < count;
+    const float m = mine ? from[(int64_t)threadIdx.x * ROW + DP] : -INFINITY;
+    const float l = mine ? from[(int64_t)threadIdx.x * ROW + DP + 1] : 0.0f;
+    float top = m;
+#pragma unroll
+    for (int n = 1; n < 64; n <<= 1) top = fmaxf(top, __shfl_xor(top, n));
+    if (lane == 0) tops[wave] = top;
+    if (threadIdx.x == 0) bad = 0;
+    __syncthreads();
+    top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
+    const float by = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - top);
+    weight[threadIdx.x] = by;
+    const float total = wave_sum(l * by);
+    if (lane == 0) totals[wave] = total;
+    __syncthreads();
+    const int e = (threadIdx.x & 31) * 4, n0 = threadIdx.x >> 5;
+    if (e < DP) {
+        float4_t x = 0.0f;
+        if (e < a.d) {
+#pragma unroll 8
+            for (int n = n0; n < count; n += 8) x += weight[n] * *(const float4_t*)(from + (int64_t)n * ROW + e);
+        }
+        *(float4_t*)&sums[n0][e] = x;
+    }
+    __syncthreads();
+    const float all = totals[0] + totals[1] + totals[2] + totals[3];
+    if ((int)threadIdx.x < a.d) {
+        float x = 0;
+#pragma unroll
+        for (int n = 0; n < 8; ++n) x += sums[n][threadIdx.x];
+        x /= all;
+        const int64_t out = ((int64_t)i * a.hq + h) * a.d + threadIdx.x;
+        const T y = (T)x;
+        ((T*)a.o)[out] = y;
+        if (a.rest) ((T*)a.rest)[out] = (T)(x - (float)y);
+        if (threadIdx.x == 0) a.lse[h * a.stat_stride + i] = top + __builtin_amdgcn_logf(all);
+        if (!finite(x)) bad = 1;
+    }
+    __syncthreads();
+    if (bad && wave == 0) forward_row<T>(a, i, h, b.lo, b.hi, lane);
 }
 
 // ---------------------------------------------------------------------------
@@ -636,8 +882,8 @@ __global__ __launch_bounds__(256, (blocks_per_unit<T, DP>())) void query_gradien
     const int krow = (int)a.k_row * (int)sizeof(T), vrow = (int)a.v_row * (int)sizeof(T);
     const typename L::Places kplaces(krow, chunks, wave, lane), vplaces(vrow, chunks, wave, lane);
     if (all.lo < all.hi) {
-        L::request(key0, kbase, krow, kplaces, all.lo, a.nk, chunks, wave);
-        L::request(val0, vbase, vrow, vplaces, all.lo, a.nk, chunks, wave);
+        L::request(key0, kbase, krow, kplaces, all.lo, all.hi, chunks, wave);
+        L::request(val0, vbase, vrow, vplaces, all.lo, all.hi, chunks, wave);
     }
     typename L::frag q[L::kFrags], g[L::kFrags];
     load_row<T, L::kFrags>(q, (const char*)((const T*)a.q + i * a.q_row + h * a.q_head), chunks, half);
@@ -689,15 +935,15 @@ __global__ __launch_bounds__(256, (blocks_per_unit<T, DP>())) void query_gradien
             for (int f = 0; f < PF; ++f) {
                 const auto p = operand<T>(x, f);
 #pragma unroll
-                for (int t = 0; t < DT; ++t) acc[t] = mma(column<T, DP, BK>(kt, 32 * u, f, t, lane), p, acc[t]);
+                for (int t = 0; t < DT; ++t) acc[t] = mma(column_of<T, DP, BK>(kt, 32 * u, f, t, lane), p, acc[t]);
             }
         }
     };
     auto step = [&](char* kt, char* vt, char* kn, char* vn, int first) {
         arrived();
         if (first + BK < all.hi) {
-            L::request(kn, kbase, krow, kplaces, first + BK, a.nk, chunks, wave);
-            L::request(vn, vbase, vrow, vplaces, first + BK, a.nk, chunks, wave);
+            L::request(kn, kbase, krow, kplaces, first + BK, all.hi, chunks, wave);
+            L::request(vn, vbase, vrow, vplaces, first + BK, all.hi, chunks, wave);
         }
         if (walk.needs(first, BK)) products(kt, vt, first);
     };
@@ -746,8 +992,8 @@ __global__ __launch_bounds__(256, 1) void key_gradient(Args a) {
 
     auto request = [&](char* qt, char* gt, float* st, int n) {
         const int h = kh * group + n / steps, first = all.lo + (n % steps) * BQ;
-        L::request(qt, (const char*)((const T*)a.q + h * a.q_head), qrow, qplaces, first, a.nq, chunks, wave);
-        L::request(gt, (const char*)((const T*)a.grad + h * a.g_head), grow, gplaces, first, a.nq, chunks, wave);
+        L::request(qt, (const char*)((const T*)a.q + h * a.q_head), qrow, qplaces, first, all.hi, chunks, wave);
+        L::request(gt, (const char*)((const T*)a.grad + h * a.g_head), grow, gplaces, first, all.hi, chunks, wave);
         // (a row of statistics is longer than the queries by more than a tile)
         if (wave < 2)
             __builtin_amdgcn_global_load_lds((gptr_t)((wave ? a.delta : a.lse) + h * a.stat_stride + first + lane),
@@ -793,10 +1039,10 @@ __global__ __launch_bounds__(256, 1) void key_gradient(Args a) {
             for (int f = 0; f < PF; ++f) {
                 const auto p = operand<T>(s, f);
 #pragma unroll
-                for (int t = 0; t < DT; ++t) dv[t] = mma(column<T, DP, BQ>(gt, 32 * u, f, t, lane), p, dv[t]);
+                for (int t = 0; t < DT; ++t) dv[t] = mma(column_of<T, DP, BQ>(gt, 32 * u, f, t, lane), p, dv[t]);
                 const auto d = operand<T>(x, f);
 #pragma unroll
-                for (int t = 0; t < DT; ++t) dk[t] = mma(column<T, DP, BQ>(qt, 32 * u, f, t, lane), d, dk[t]);
+                for (int t = 0; t < DT; ++t) dk[t] = mma(column_of<T, DP, BQ>(qt, 32 * u, f, t, lane), d, dk[t]);
             }
         }
     };

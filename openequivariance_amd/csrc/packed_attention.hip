@@ -13,6 +13,12 @@ struct Kernels {
         forward<T, DP><<<(unsigned)(a.tiles * a.hq), 256, 0, stream>>>(a);
         return hipGetLastError();
     }
+    static hipError_t forward_shares(const Args& a, hipStream_t stream) {
+        const unsigned stacks = (unsigned)(a.hq / a.hk + 31) / 32;
+        forward_few<T, DP><<<(unsigned)a.nq * a.hk * stacks * a.parts, 64 * Few<T, DP>::kWaves, 0, stream>>>(a);
+        if (a.parts > 1) join<T, DP><<<(unsigned)a.nq * a.hq, 256, 0, stream>>>(a);
+        return hipGetLastError();
+    }
     static hipError_t gradients(const Args& a, int key_tiles, hipStream_t stream) {
         if (a.tiles) query_gradient<T, DP><<<(unsigned)(a.tiles * a.hq), 256, 0, stream>>>(a);
         Args b = a;
@@ -28,7 +34,7 @@ struct Kernels {
 
 template <>
 hipError_t Launch<OEQ_ATTENTION_TYPE>::forward(const Args& a, hipStream_t stream) {
-    return OEQ_BY_HEAD(forward_rows(a, stream));
+    return a.parts ? OEQ_BY_HEAD(forward_shares(a, stream)) : OEQ_BY_HEAD(forward_rows(a, stream));
 }
 
 template <>
