@@ -10,7 +10,6 @@
 #include <algorithm>
 #include <climits>
 #include <cmath>
-#include <cstdlib>
 
 using oeq_internal::fail;
 
@@ -66,17 +65,25 @@ packed_attention::Args attention_args(const oeq_attention& a) {
 
 // How many shares the form for few queries cuts a row's keys into; 0: the form for tiles of rows.
 //
-// Lengths are on the device, so the rule goes by means over the segments. Tiles are for rows that share keys with their
-// neighbours; with few rows to a segment and many keys to a row nearly all of a tile's scores are hidden ones.
+// Lengths are on the device, so the rule goes by their means over the segments and takes the smaller of two estimates, in
+// steps of about a microsecond. Tiles: blocks of 128 rows walk the keys of all segments that their rows belong to, 64 a
+// step. Few: blocks of a row and a key head walk that row's keys alone, 80 a step after some 5 steps of latency (a block's
+// bounds, first reads and end). Either way two blocks a compute unit run at a time. Measured with 8 heads of 64, bf16,
+// tiles / few in us: 128 segments of 1 row, 512 keys 1 023 / 26, of 2 rows, 16 keys 22 / 21, of 4 rows, 64 keys 39 / 39, of 8 rows,
+// 64 keys 22 / 74, 512 keys 132 / 122; 1 024 segments of 1 row, 32 keys 72 / 73; a segment of 16 rows, 4 096 keys 57 / 22.
 int parts_of(const oeq_attention& a) {
-    { const char* e = getenv("OEQ_TRY_FORM"); if (e && atoi(e) == 0) return 0; if (!e && (a.q_rows > 8 * (int64_t)a.segments || a.k_rows < 16 * a.q_rows)) return 0; }
-    const int64_t blocks = a.q_rows * a.k_heads * ((a.q_heads / a.k_heads + 31) / 32);
-    const int64_t keys = (a.k_rows + a.segments - 1) / a.segments;  // to a row
-    static const int target = [] { const char* e = getenv("OEQ_TRY_BLOCKS"); return e ? atoi(e) : 1024; }();
-    static const int least = [] { const char* e = getenv("OEQ_TRY_LEAST"); return e ? atoi(e) : 256; }();
-    const int64_t parts = std::min({target / blocks, (keys + least - 1) / least, (int64_t)packed_attention::kMostParts});
+    constexpr int64_t kBlocks = 1024;   // (one token against 65 537 keys: 512 and 1 024 blocks 62 us, 2 048 blocks 73)
+    constexpr int64_t kLeastKeys = 256;  // a share is worth its block and its row of the join
+    const int64_t segments = std::max(a.segments, 1), group = a.q_heads / a.k_heads;
+    const int64_t blocks = a.q_rows * a.k_heads * ((group + 31) / 32);
     if (blocks > INT_MAX / packed_attention::kMostParts) return 0;
-    return (int)std::max<int64_t>(parts, 1);
+    const double keys = std::ceil((double)a.k_rows / segments), rows = std::max(1.0, (double)a.q_rows / segments);
+    const int64_t parts = std::max<int64_t>(
+        1, std::min({kBlocks / blocks, (int64_t)keys / kLeastKeys, (int64_t)packed_attention::kMostParts}));
+    const double walk = std::min((double)a.k_rows, (127 / rows + 1) * keys);
+    const double tiles = std::max(1.0, (a.q_rows + 127) / 128 * a.q_heads / 512.0) * std::ceil(walk / 64);
+    const double few = std::max(1.0, blocks * parts / 512.0) * (5 + keys / parts / 80);
+    return few < tiles ? (int)parts : 0;
 }
 
 int head_tile(int d) { return d <= 32 ? 32 : d <= 64 ? 64 : 128; }

@@ -143,8 +143,12 @@ __device__ __forceinline__ bool finite(float x) { return fabsf(x) < INFINITY; }
 // tiles in LDS
 // ---------------------------------------------------------------------------
 
-// BK rows of DP elements; 16-byte chunk c of row r lies at place c ^ swizzle(r) of the row, so that the eight lanes
-// that a 16-byte read serves in one clock, with the same chunk of eight consecutive rows, touch all banks once.
+// Rows of DP elements; 16-byte chunk c of row r lies at place c ^ swizzle(r) of the row. LDS has 64 banks, 256 bytes: a
+// 16-byte read meets them with the same chunk of 16 consecutive rows, a transposing read with four neighbouring chunks of
+// four rows that begin at a multiple of four. Either way the 16 chunks have to lie in different places modulo 16, so the
+// rows that share 256 bytes need no swizzle among them, the next bits of the row choose among the groups of four chunks
+// and the ones after that within a group. (With the row's bits in order, good for the first kind alone, the forward kernel
+// spent 59 % of its clocks in LDS on conflicts.)
 template <typename T, int DP, int ROWS, int WAVES = 4>
 struct Tile {
     static constexpr int kRowBytes = DP * (int)sizeof(T);
@@ -154,7 +158,7 @@ struct Tile {
     typedef typename Types<T>::frag frag;
 
     static __device__ __forceinline__ int swizzle(int r) {
-        return kChunks >= 16 ? (r & 15) : kChunks == 8 ? (r & 7) : ((r >> 1) & 3);
+        return kChunks >= 16 ? ((r & 3) << 2 | (r >> 2 & 3)) : kChunks == 8 ? ((r >> 1 & 1) << 2 | (r >> 2 & 3)) : (r >> 2 & 3);
     }
 
     // Where the lanes of a wave find their part of a tile, relative to its first row: 1 KB an instruction. Chunks past
@@ -388,6 +392,9 @@ __device__ __forceinline__ void place(const Args& a, int heads, int& tile, int& 
 // more for its row alone.
 template <typename T, int DP>
 constexpr int blocks_per_unit() { return sizeof(T) * DP > 256 ? 1 : 2; }
+
+template <typename T, int DP>
+constexpr int key_blocks_per_unit() { return sizeof(T) * DP >= 256 ? 1 : 2; }
 
 template <typename T>
 constexpr int tile_rows() { return sizeof(T) == 2 ? 64 : 32; }
@@ -937,6 +944,7 @@ __global__ __launch_bounds__(256, (blocks_per_unit<T, DP>())) void query_gradien
 #pragma unroll
                 for (int t = 0; t < DT; ++t) acc[t] = mma(column_of<T, DP, BK>(kt, 32 * u, f, t, lane), p, acc[t]);
             }
+            __builtin_amdgcn_sched_barrier(0);  // (reads of the next 32 keys this early would take registers that are not there)
         }
     };
     auto step = [&](char* kt, char* vt, char* kn, char* vn, int first) {
@@ -966,20 +974,21 @@ __global__ __launch_bounds__(256, (blocks_per_unit<T, DP>())) void query_gradien
 // gradients of keys and values
 // ---------------------------------------------------------------------------
 
-template <typename T, int DP>
-__global__ __launch_bounds__(256, 1) void key_gradient(Args a) {
-    constexpr int BQ = tile_rows<T>(), SUB = BQ / 32, DT = DP / 32;
+template <typename T, int DP, int KEYS>
+__global__ __launch_bounds__(256, (key_blocks_per_unit<T, DP>())) void key_gradient(Args a) {
+    constexpr int BQ = 64, QW = 4 / KEYS, SUB = 2 / QW, DT = DP / 32;
     constexpr int PF = sizeof(T) == 2 ? 2 : 4;
     typedef Tile<T, DP, BQ> L;
     __shared__ __align__(1024) char que0[L::kBytes], que1[L::kBytes], gra0[L::kBytes], gra1[L::kBytes];
     __shared__ __align__(1024) float sta0[128], sta1[128];  // lse, then delta, of the tile's rows
     __shared__ int shared[8];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5;
+    const int keys = wave % KEYS, rows = wave / KEYS;  // which 32 keys and which part of a tile's rows the wave has
     int tile, kh;
     place(a, a.hk, tile, kh);
     if (a.causal) tile = a.tiles - 1 - tile;  // the first keys have the longest walks
     const int group = a.hq / a.hk, chunks = a.d * (int)sizeof(T) / 16;
-    const int row = (tile * 4 + wave) * 32 + (lane & 31), j = min(row, a.nk - 1);
+    const int row = (tile * KEYS + keys) * 32 + (lane & 31), j = min(row, a.nk - 1);
     if (chunks < L::kChunks) {
         clear<L::kBytes>(que0), clear<L::kBytes>(que1), clear<L::kBytes>(gra0), clear<L::kBytes>(gra1);
     }
@@ -988,10 +997,8 @@ __global__ __launch_bounds__(256, 1) void key_gradient(Args a) {
     const Bounds all = block_range(walk, shared, wave, lane);
     const int qrow = (int)a.q_row * (int)sizeof(T), grow = (int)a.g_row * (int)sizeof(T);
     const typename L::Places qplaces(qrow, chunks, wave, lane), gplaces(grow, chunks, wave, lane);
-    const int steps = all.lo < all.hi ? (all.hi - all.lo + BQ - 1) / BQ : 0, total = steps * group;
 
-    auto request = [&](char* qt, char* gt, float* st, int n) {
-        const int h = kh * group + n / steps, first = all.lo + (n % steps) * BQ;
+    auto request = [&](char* qt, char* gt, float* st, int h, int first) {
         L::request(qt, (const char*)((const T*)a.q + h * a.q_head), qrow, qplaces, first, all.hi, chunks, wave);
         L::request(gt, (const char*)((const T*)a.grad + h * a.g_head), grow, gplaces, first, all.hi, chunks, wave);
         // (a row of statistics is longer than the queries by more than a tile)
@@ -999,7 +1006,11 @@ __global__ __launch_bounds__(256, 1) void key_gradient(Args a) {
             __builtin_amdgcn_global_load_lds((gptr_t)((wave ? a.delta : a.lse) + h * a.stat_stride + first + lane),
                                              (lptr_t)(st + 64 * wave), 4, 0, 0);
     };
-    if (total) request(que0, gra0, sta0, 0);
+    const int last_head = (kh + 1) * group;
+    // Tiles of rows are walked from the last on. Causal: blocks of neighbouring keys, which run at the same time on an XCD,
+    // see the same last rows and differ in their first, and this way they read the same tiles at the same time.
+    const int top = all.lo < all.hi ? all.lo + (all.hi - all.lo - 1) / BQ * BQ : 0;
+    if (all.lo < all.hi) request(que0, gra0, sta0, kh * group, top);
     typename L::frag k[L::kFrags], v[L::kFrags];
     load_row<T, L::kFrags>(k, (const char*)((const T*)a.k + j * a.k_row + kh * a.k_head), chunks, half);
     load_row<T, L::kFrags>(v, (const char*)((const T*)a.v + j * a.v_row + kh * a.v_head), chunks, half);
@@ -1009,18 +1020,19 @@ __global__ __launch_bounds__(256, 1) void key_gradient(Args a) {
     for (int t = 0; t < DT; ++t) dk[t] = 0.0f, dv[t] = 0.0f;
 
     constexpr float kRatio = power<Types<T>::kDs - Types<T>::kP>;
-    auto products = [&](const char* qt, const char* gt, const float* st, int first) {
+    auto products = [&](const char* qt, const char* gt, const float* st, int first, bool whole) {
 #pragma unroll
         for (int u = 0; u < SUB; ++u) {
+            const int r0 = 32 * (rows * SUB + u);
             float16_t s = 0.0f, x = 0.0f;
 #pragma unroll
-            for (int f = 0; f < L::kFrags; ++f) s = mma(L::row(qt, 32 * u + (lane & 31), f, half), k[f], s);
+            for (int f = 0; f < L::kFrags; ++f) s = mma(L::row(qt, r0 + (lane & 31), f, half), k[f], s);
 #pragma unroll
-            for (int f = 0; f < L::kFrags; ++f) x = mma(L::row(gt, 32 * u + (lane & 31), f, half), v[f], x);
+            for (int f = 0; f < L::kFrags; ++f) x = mma(L::row(gt, r0 + (lane & 31), f, half), v[f], x);
 #pragma unroll
             for (int g = 0; g < 4; ++g) {
-                const float4_t lse = *(const float4_t*)(st + 32 * u + 8 * g + 4 * half);
-                const float4_t delta = *(const float4_t*)(st + 64 + 32 * u + 8 * g + 4 * half);
+                const float4_t lse = *(const float4_t*)(st + r0 + 8 * g + 4 * half);
+                const float4_t delta = *(const float4_t*)(st + 64 + r0 + 8 * g + 4 * half);
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                     const int r = 4 * g + e;
@@ -1028,8 +1040,8 @@ __global__ __launch_bounds__(256, 1) void key_gradient(Args a) {
                     x[r] = s[r] * fmaf(x[r], kRatio, -delta[e] * kRatio);
                 }
             }
-            if (!walk.whole(first, BQ)) {
-                const int shift = first + 32 * u + 4 * half - b.lo;
+            if (!whole) {
+                const int shift = first + r0 + 4 * half - b.lo;
                 const unsigned n = b.hi - b.lo;
 #pragma unroll
                 for (int r = 0; r < 16; ++r)
@@ -1039,22 +1051,47 @@ __global__ __launch_bounds__(256, 1) void key_gradient(Args a) {
             for (int f = 0; f < PF; ++f) {
                 const auto p = operand<T>(s, f);
 #pragma unroll
-                for (int t = 0; t < DT; ++t) dv[t] = mma(column_of<T, DP, BQ>(gt, 32 * u, f, t, lane), p, dv[t]);
+                for (int t = 0; t < DT; ++t) dv[t] = mma(column_of<T, DP, BQ>(gt, r0, f, t, lane), p, dv[t]);
                 const auto d = operand<T>(x, f);
 #pragma unroll
-                for (int t = 0; t < DT; ++t) dk[t] = mma(column_of<T, DP, BQ>(qt, 32 * u, f, t, lane), d, dk[t]);
+                for (int t = 0; t < DT; ++t) dk[t] = mma(column_of<T, DP, BQ>(qt, r0, f, t, lane), d, dk[t]);
             }
         }
     };
-    auto step = [&](char* qt, char* gt, float* st, char* qn, char* gn, float* sn, int n) {
+    int h = kh * group, first = top;
+    auto step = [&](char* qt, char* gt, float* st, char* qn, char* gn, float* sn) {
         arrived();
-        if (n + 1 < total) request(qn, gn, sn, n + 1);
-        const int first = all.lo + (n % steps) * BQ;
-        if (walk.needs(first, BQ)) products(qt, gt, st, first);
+        const int now = first;
+        first -= BQ;
+        if (first < all.lo) first = top, ++h;
+        if (h < last_head) request(qn, gn, sn, h, first);
+        const int mine = now + 32 * rows * SUB;
+        products(qt, gt, st, now, walk.whole(mine, 32 * SUB));
     };
-    for (int n = 0; n < total; n += 2) {
-        step(que0, gra0, sta0, que1, gra1, sta1, n);
-        if (n + 1 < total) step(que1, gra1, sta1, que0, gra0, sta0, n + 1);
+    if (all.lo < all.hi)
+        while (h < last_head) {
+            step(que0, gra0, sta0, que1, gra1, sta1);
+            if (h < last_head) step(que1, gra1, sta1, que0, gra0, sta0);
+        }
+    if constexpr (QW == 2) {
+        // the waves with the second half of the rows hand their sums to those with the first, 32 columns of the head at a
+        // time through LDS (4 KB a wave)
+        __shared__ __align__(16) float4_t swap[2][4][64];
+#pragma unroll
+        for (int t = 0; t < 2 * DT; ++t) {
+            float16_t& x = t < DT ? dk[t] : dv[t - DT];
+            __syncthreads();
+            if (rows == 1)
+#pragma unroll
+                for (int g = 0; g < 4; ++g) swap[keys][g][lane] = float4_t{x[4 * g], x[4 * g + 1], x[4 * g + 2], x[4 * g + 3]};
+            __syncthreads();
+            if (rows == 0)
+#pragma unroll
+                for (int g = 0; g < 4; ++g)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) x[4 * g + e] += swap[keys][g][lane][e];
+        }
+        if (rows == 1) return;
     }
     const bool mine = row < a.nk;
     if (mine) {
@@ -1067,7 +1104,7 @@ __global__ __launch_bounds__(256, 1) void key_gradient(Args a) {
     while (bad) {
         const int at = __builtin_ctzll(bad);
         bad &= bad - 1;
-        key_gradient_row<T>(a, (tile * 4 + wave) * 32 + at, kh, __shfl(b.lo, at), __shfl(b.hi, at), lane);
+        key_gradient_row<T>(a, (tile * KEYS + keys) * 32 + at, kh, __shfl(b.lo, at), __shfl(b.hi, at), lane);
     }
 }
 
