@@ -226,7 +226,7 @@ int oeq_attention_backward(const oeq_attention* a, const void* out, const void* 
     packed_attention::Args g = attention_args(*a);
     g.out = out, g.out_rest = out_rest, g.grad = out_grad, g.g_row = grad_row_stride, g.g_head = grad_head_stride;
     g.dq = q_grad, g.dk = k_grad, g.dv = v_grad, g.lse = (float*)log2_sum, g.delta = delta;
-    const int key_tiles = (int)((a->k_rows + 127) / 128);
+    const int key_tiles = (int)((a->k_rows + 63) / 64);
     const auto s = (hipStream_t)stream;
     HIP_TRY(a->type == OEQ_FLOAT32 ? packed_attention::Launch<float>::backward(g, key_tiles, s)
             : a->type == OEQ_FLOAT16 ? packed_attention::Launch<_Float16>::backward(g, key_tiles, s)

@@ -161,16 +161,19 @@ struct Tile {
         return kChunks >= 16 ? ((r & 3) << 2 | (r >> 2 & 3)) : kChunks == 8 ? ((r >> 1 & 1) << 2 | (r >> 2 & 3)) : (r >> 2 & 3);
     }
 
-    // Where the lanes of a wave find their part of a tile, relative to its first row: 1 KB an instruction. Chunks past
-    // the head's end are placed where the reads' own bounds leave them out.
+    // Where the lanes of a wave find their part of a tile, relative to its first row: 1 KB an instruction. Instructions whose
+    // rows lie 16 apart have the same swizzle and are a stride apart (which is added where they are issued: kept in
+    // registers, the sums take what the products need). Chunks past the head's end are placed where the reads' own bounds
+    // leave them out.
     static constexpr int kRowsPer = 64 / kChunks, kEach = kBytes / 1024 / WAVES;
+    static constexpr int kApart = WAVES * kRowsPer, kPlaces = kApart >= 16 ? 1 : kEach < 16 / kApart ? kEach : 16 / kApart;
     struct Places {
-        int at[kEach];
+        int at[kPlaces];
         __device__ __forceinline__ Places(int row_bytes, int chunks, int wave, int lane) {
             static_assert(kBytes % (1024 * WAVES) == 0, "the waves share a tile");
 #pragma unroll
-            for (int i = 0; i < kEach; ++i) {
-                const int r = (wave * kEach + i) * kRowsPer + lane / kChunks, c = (lane % kChunks) ^ swizzle(r);
+            for (int i = 0; i < kPlaces; ++i) {
+                const int r = (i * WAVES + wave) * kRowsPer + lane / kChunks, c = (lane % kChunks) ^ swizzle(r);
                 at[i] = c < chunks ? r * row_bytes + c * 16 : INT_MAX;
             }
         }
@@ -183,9 +186,12 @@ struct Tile {
         const int64_t left = (int64_t)(rows - 1 - first) * row_bytes + chunks * 16;
         const auto from = __builtin_amdgcn_make_buffer_rsrc((void*)(base + (int64_t)first * row_bytes), 0,
                                                             (int)min(left, (int64_t)INT_MAX - 16), 0x00020000);
+        int stride = kPlaces * kApart * row_bytes;
+        asm volatile("" : "+s"(stride));  // (not to be added up outside the loop)
 #pragma unroll
         for (int i = 0; i < kEach; ++i)
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(from, (lptr_t)(lds + (wave * kEach + i) * 1024), 16, places.at[i], 0, 0, 0);
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(from, (lptr_t)(lds + (i * WAVES + wave) * 1024), 16,
+                                                     places.at[i % kPlaces] + i / kPlaces * stride, 0, 0, 0);
     }
 
     // Fragment f of row r: elements (2 f + half) E ... of it.
@@ -394,10 +400,17 @@ template <typename T, int DP>
 constexpr int blocks_per_unit() { return sizeof(T) * DP > 256 ? 1 : 2; }
 
 template <typename T, int DP>
+constexpr bool kFenced = sizeof(T) == 2 && DP == 128;  // key_gradient: one wave to a SIMD, see there
+
+template <typename T, int DP>
 constexpr int key_blocks_per_unit() { return sizeof(T) * DP >= 256 ? 1 : 2; }
 
 template <typename T>
 constexpr int tile_rows() { return sizeof(T) == 2 ? 64 : 32; }
+
+// Everything that was requested so far has come, and the compiler knows: a row that is loaded before a loop would else be
+// waited for inside it, at its first use, together with what the loop has requested since.
+__device__ __forceinline__ void settle() { __builtin_amdgcn_s_waitcnt(0x0f70); }  // vmcnt(0)
 
 __device__ __forceinline__ void arrived() {
     // what this wave requested is in LDS; then the same for the others, and all are done with the other buffer
@@ -533,6 +546,7 @@ __global__ __launch_bounds__(256, (blocks_per_unit<T, DP>())) void forward(Args 
     for (int t = 0; t < DT; ++t) acc[t] = 0.0f;
     float m = -INFINITY, l = 0;
     const float c = a.scale_log2;
+    settle();
 
     auto products = [&](const char* kt, const char* vt, int first) {
         float16_t s[SUB];
@@ -914,6 +928,7 @@ __global__ __launch_bounds__(256, (blocks_per_unit<T, DP>())) void query_gradien
     const bool mine = row < a.nq;
     if (mine && half == 0) a.delta[h * a.stat_stride + i] = delta;
     const float lse = a.lse[h * a.stat_stride + i], c = a.scale_log2;
+    settle();
     float16_t acc[DT];
 #pragma unroll
     for (int t = 0; t < DT; ++t) acc[t] = 0.0f;
@@ -974,21 +989,28 @@ __global__ __launch_bounds__(256, (blocks_per_unit<T, DP>())) void query_gradien
 // gradients of keys and values
 // ---------------------------------------------------------------------------
 
-template <typename T, int DP, int KEYS>
+// A block has 64 keys in two pairs of waves; of a tile of 64 query rows one wave of a pair takes the first half, the other
+// the second, and at the end they add up. (With 128 keys a block, one wave for both halves, long walks of few blocks
+// decide: a training step on 9 packed sequences took 696 us here, not 480.) At a head of 128 a lane holds 128 sums and 64
+// elements of its key and value, so there is one wave to a SIMD and nothing else runs while it waits: reads from LDS go
+// ahead of their products in batches, with a fence behind each. (Left to itself the compiler puts every read right before
+// its product, and the wave waited for 45 % of its clocks.)
+template <typename T, int DP>
 __global__ __launch_bounds__(256, (key_blocks_per_unit<T, DP>())) void key_gradient(Args a) {
-    constexpr int BQ = 64, QW = 4 / KEYS, SUB = 2 / QW, DT = DP / 32;
-    constexpr int PF = sizeof(T) == 2 ? 2 : 4;
+    constexpr int BQ = 64, DT = DP / 32, PF = sizeof(T) == 2 ? 2 : 4;
     typedef Tile<T, DP, BQ> L;
-    __shared__ __align__(1024) char que0[L::kBytes], que1[L::kBytes], gra0[L::kBytes], gra1[L::kBytes];
+    __shared__ __align__(1024) char que0[L::kBytes], que1[L::kBytes];
+    __shared__ __align__(1024) char gra0[L::kBytes], gra1[L::kBytes];
     __shared__ __align__(1024) float sta0[128], sta1[128];  // lse, then delta, of the tile's rows
+    __shared__ __align__(16) float4_t swap[2][4][64];
     __shared__ int shared[8];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5;
-    const int keys = wave % KEYS, rows = wave / KEYS;  // which 32 keys and which part of a tile's rows the wave has
+    const int keys = wave & 1, r0 = 32 * (wave >> 1);  // which 32 keys, and the first row of the wave's half of a tile
     int tile, kh;
     place(a, a.hk, tile, kh);
     if (a.causal) tile = a.tiles - 1 - tile;  // the first keys have the longest walks
     const int group = a.hq / a.hk, chunks = a.d * (int)sizeof(T) / 16;
-    const int row = (tile * KEYS + keys) * 32 + (lane & 31), j = min(row, a.nk - 1);
+    const int row = (tile * 2 + keys) * 32 + (lane & 31), j = min(row, a.nk - 1);
     if (chunks < L::kChunks) {
         clear<L::kBytes>(que0), clear<L::kBytes>(que1), clear<L::kBytes>(gra0), clear<L::kBytes>(gra1);
     }
@@ -998,19 +1020,22 @@ __global__ __launch_bounds__(256, (key_blocks_per_unit<T, DP>())) void key_gradi
     const int qrow = (int)a.q_row * (int)sizeof(T), grow = (int)a.g_row * (int)sizeof(T);
     const typename L::Places qplaces(qrow, chunks, wave, lane), gplaces(grow, chunks, wave, lane);
 
-    auto request = [&](char* qt, char* gt, float* st, int h, int first) {
-        L::request(qt, (const char*)((const T*)a.q + h * a.q_head), qrow, qplaces, first, all.hi, chunks, wave);
-        L::request(gt, (const char*)((const T*)a.grad + h * a.g_head), grow, gplaces, first, all.hi, chunks, wave);
-        // (a row of statistics is longer than the queries by more than a tile)
-        if (wave < 2)
-            __builtin_amdgcn_global_load_lds((gptr_t)((wave ? a.delta : a.lse) + h * a.stat_stride + first + lane),
-                                             (lptr_t)(st + 64 * wave), 4, 0, 0);
-    };
-    const int last_head = (kh + 1) * group;
     // Tiles of rows are walked from the last on. Causal: blocks of neighbouring keys, which run at the same time on an XCD,
     // see the same last rows and differ in their first, and this way they read the same tiles at the same time.
-    const int top = all.lo < all.hi ? all.lo + (all.hi - all.lo - 1) / BQ * BQ : 0;
-    if (all.lo < all.hi) request(que0, gra0, sta0, kh * group, top);
+    const int top = all.lo < all.hi ? all.lo + (all.hi - all.lo - 1) / BQ * BQ : 0, last_head = (kh + 1) * group;
+    int next_h = all.lo < all.hi ? kh * group : last_head, next_first = top;  // the tile to be requested
+    auto request = [&](char* qt, char* gt, float* st) {
+        if (next_h == last_head) return;
+        L::request(qt, (const char*)((const T*)a.q + next_h * a.q_head), qrow, qplaces, next_first, all.hi, chunks, wave);
+        L::request(gt, (const char*)((const T*)a.grad + next_h * a.g_head), grow, gplaces, next_first, all.hi, chunks, wave);
+        // (a row of statistics is longer than the queries by more than a tile)
+        if (wave < 2)
+            __builtin_amdgcn_global_load_lds((gptr_t)((wave ? a.delta : a.lse) + next_h * a.stat_stride + next_first + lane),
+                                             (lptr_t)(st + 64 * wave), 4, 0, 0);
+        next_first -= BQ;
+        if (next_first < all.lo) next_first = top, ++next_h;
+    };
+    request(que0, gra0, sta0);
     typename L::frag k[L::kFrags], v[L::kFrags];
     load_row<T, L::kFrags>(k, (const char*)((const T*)a.k + j * a.k_row + kh * a.k_head), chunks, half);
     load_row<T, L::kFrags>(v, (const char*)((const T*)a.v + j * a.v_row + kh * a.v_head), chunks, half);
@@ -1018,37 +1043,90 @@ __global__ __launch_bounds__(256, (key_blocks_per_unit<T, DP>())) void key_gradi
     float16_t dk[DT], dv[DT];
 #pragma unroll
     for (int t = 0; t < DT; ++t) dk[t] = 0.0f, dv[t] = 0.0f;
+    settle();
 
     constexpr float kRatio = power<Types<T>::kDs - Types<T>::kP>;
-    auto products = [&](const char* qt, const char* gt, const float* st, int first, bool whole) {
+    // p and ds from the scores and g.v
+    auto weigh = [&](float16_t& s, float16_t& x, const float* st) {
 #pragma unroll
-        for (int u = 0; u < SUB; ++u) {
-            const int r0 = 32 * (rows * SUB + u);
-            float16_t s = 0.0f, x = 0.0f;
+        for (int g = 0; g < 4; ++g) {
+            const float4_t lse = *(const float4_t*)(st + r0 + 8 * g + 4 * half);
+            const float4_t delta = *(const float4_t*)(st + 64 + r0 + 8 * g + 4 * half);
 #pragma unroll
-            for (int f = 0; f < L::kFrags; ++f) s = mma(L::row(qt, r0 + (lane & 31), f, half), k[f], s);
+            for (int e = 0; e < 4; ++e) {
+                const int r = 4 * g + e;
+                s[r] = raised<T, Types<T>::kP>(fmaf(s[r], c, -lse[e]));
+                x[r] = s[r] * fmaf(x[r], kRatio, -delta[e] * kRatio);
+            }
+        }
+    };
+    auto hide = [&](float16_t& s, float16_t& x, int first) {
+        if (walk.whole(first + r0, 32)) return;
+        const int shift = first + r0 + 4 * half - b.lo;
+        const unsigned n = b.hi - b.lo;
 #pragma unroll
-            for (int f = 0; f < L::kFrags; ++f) x = mma(L::row(gt, r0 + (lane & 31), f, half), v[f], x);
+        for (int r = 0; r < 16; ++r)
+            if ((unsigned)(shift + 8 * (r / 4) + r % 4) >= n) s[r] = 0.0f, x[r] = 0.0f;
+    };
+    const int steps = all.lo < all.hi ? ((all.hi - all.lo - 1) / BQ + 1) * group : 0;
+    int first = top;
+    auto step = [&](char* qt, char* gt, float* st, char* qn, char* gn, float* sn) {
+        arrived();
+        request(qn, gn, sn);
+        float16_t s = 0.0f, x = 0.0f;
+        if constexpr (kFenced<T, DP>) {
+            typename L::frag rows[2][8], columns[2][2 * DT];
+            auto load_rows = [&](int n) {
 #pragma unroll
-            for (int g = 0; g < 4; ++g) {
-                const float4_t lse = *(const float4_t*)(st + r0 + 8 * g + 4 * half);
-                const float4_t delta = *(const float4_t*)(st + 64 + r0 + 8 * g + 4 * half);
+                for (int f = 0; f < 4; ++f) {
+                    rows[n][2 * f] = L::row(qt, r0 + (lane & 31), 4 * n + f, half);
+                    rows[n][2 * f + 1] = L::row(gt, r0 + (lane & 31), 4 * n + f, half);
+                }
+                __builtin_amdgcn_sched_barrier(0);
+            };
+            auto load_columns = [&](int f) {
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const int r = 4 * g + e;
-                    s[r] = raised<T, Types<T>::kP>(fmaf(s[r], c, -lse[e]));
-                    x[r] = s[r] * fmaf(x[r], kRatio, -delta[e] * kRatio);
+                for (int t = 0; t < DT; ++t) {
+                    columns[f][2 * t] = column_of<T, DP, BQ>(gt, r0, f, t, lane);
+                    columns[f][2 * t + 1] = column_of<T, DP, BQ>(qt, r0, f, t, lane);
+                }
+                __builtin_amdgcn_sched_barrier(0);
+            };
+            load_rows(0);
+            load_rows(1);
+#pragma unroll
+            for (int f = 0; f < 8; ++f) {
+                s = mma(rows[f / 4][2 * (f % 4)], k[f], s);
+                x = mma(rows[f / 4][2 * (f % 4) + 1], v[f], x);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+            load_columns(0);
+            weigh(s, x, st);
+            hide(s, x, first);
+            load_columns(1);
+#pragma unroll
+            for (int f = 0; f < 2; ++f) {
+                const auto p = operand<T>(s, f), d = operand<T>(x, f);
+#pragma unroll
+                for (int t = 0; t < DT; ++t) {
+                    dv[t] = mma(columns[f][2 * t], p, dv[t]);
+                    dk[t] = mma(columns[f][2 * t + 1], d, dk[t]);
                 }
             }
-            if (!whole) {
-                const int shift = first + r0 + 4 * half - b.lo;
-                const unsigned n = b.hi - b.lo;
+        } else {
+            // (512-byte rows: with all reads ahead of all products the 512 registers do not do)
+            const auto fence = [](int f) {
+                if (L::kFrags > 8 && f % 4 == 3) __builtin_amdgcn_sched_barrier(0);
+            };
 #pragma unroll
-                for (int r = 0; r < 16; ++r)
-                    if ((unsigned)(shift + 8 * (r / 4) + r % 4) >= n) s[r] = 0.0f, x[r] = 0.0f;
-            }
+            for (int f = 0; f < L::kFrags; ++f) s = mma(L::row(qt, r0 + (lane & 31), f, half), k[f], s), fence(f);
+#pragma unroll
+            for (int f = 0; f < L::kFrags; ++f) x = mma(L::row(gt, r0 + (lane & 31), f, half), v[f], x), fence(f);
+            weigh(s, x, st);
+            hide(s, x, first);
 #pragma unroll
             for (int f = 0; f < PF; ++f) {
+                fence(3);
                 const auto p = operand<T>(s, f);
 #pragma unroll
                 for (int t = 0; t < DT; ++t) dv[t] = mma(column_of<T, DP, BQ>(gt, r0, f, t, lane), p, dv[t]);
@@ -1057,42 +1135,29 @@ __global__ __launch_bounds__(256, (key_blocks_per_unit<T, DP>())) void key_gradi
                 for (int t = 0; t < DT; ++t) dk[t] = mma(column_of<T, DP, BQ>(qt, r0, f, t, lane), d, dk[t]);
             }
         }
-    };
-    int h = kh * group, first = top;
-    auto step = [&](char* qt, char* gt, float* st, char* qn, char* gn, float* sn) {
-        arrived();
-        const int now = first;
         first -= BQ;
-        if (first < all.lo) first = top, ++h;
-        if (h < last_head) request(qn, gn, sn, h, first);
-        const int mine = now + 32 * rows * SUB;
-        products(qt, gt, st, now, walk.whole(mine, 32 * SUB));
+        if (first < all.lo) first = top;
     };
-    if (all.lo < all.hi)
-        while (h < last_head) {
-            step(que0, gra0, sta0, que1, gra1, sta1);
-            if (h < last_head) step(que1, gra1, sta1, que0, gra0, sta0);
-        }
-    if constexpr (QW == 2) {
-        // the waves with the second half of the rows hand their sums to those with the first, 32 columns of the head at a
-        // time through LDS (4 KB a wave)
-        __shared__ __align__(16) float4_t swap[2][4][64];
-#pragma unroll
-        for (int t = 0; t < 2 * DT; ++t) {
-            float16_t& x = t < DT ? dk[t] : dv[t - DT];
-            __syncthreads();
-            if (rows == 1)
-#pragma unroll
-                for (int g = 0; g < 4; ++g) swap[keys][g][lane] = float4_t{x[4 * g], x[4 * g + 1], x[4 * g + 2], x[4 * g + 3]};
-            __syncthreads();
-            if (rows == 0)
-#pragma unroll
-                for (int g = 0; g < 4; ++g)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) x[4 * g + e] += swap[keys][g][lane][e];
-        }
-        if (rows == 1) return;
+    for (int n = 0; n < steps; n += 2) {
+        step(que0, gra0, sta0, que1, gra1, sta1);
+        if (n + 1 < steps) step(que1, gra1, sta1, que0, gra0, sta0);
     }
+    // the second halves of the rows add to the first, 32 columns of the head at a time
+#pragma unroll
+    for (int t = 0; t < 2 * DT; ++t) {
+        float16_t& x = t < DT ? dk[t] : dv[t - DT];
+        __syncthreads();
+        if (r0)
+#pragma unroll
+            for (int g = 0; g < 4; ++g) swap[keys][g][lane] = float4_t{x[4 * g], x[4 * g + 1], x[4 * g + 2], x[4 * g + 3]};
+        __syncthreads();
+        if (!r0)
+#pragma unroll
+            for (int g = 0; g < 4; ++g)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) x[4 * g + e] += swap[keys][g][lane][e];
+    }
+    if (r0) return;
     const bool mine = row < a.nk;
     if (mine) {
         const int64_t at = ((int64_t)j * a.hk + kh) * a.d;
@@ -1104,7 +1169,7 @@ __global__ __launch_bounds__(256, (key_blocks_per_unit<T, DP>())) void key_gradi
     while (bad) {
         const int at = __builtin_ctzll(bad);
         bad &= bad - 1;
-        key_gradient_row<T>(a, (tile * KEYS + keys) * 32 + at, kh, __shfl(b.lo, at), __shfl(b.hi, at), lane);
+        key_gradient_row<T>(a, (tile * 2 + keys) * 32 + at, kh, __shfl(b.lo, at), __shfl(b.hi, at), lane);
     }
 }
 

@@ -2,7 +2,6 @@
 // their launches.
 #include "packed_attention.h"
 #include "packed_attention_launch.h"
-#include <cstdlib>
 
 namespace packed_attention {
 namespace {
@@ -23,14 +22,8 @@ struct Kernels {
     static hipError_t gradients(const Args& a, int key_tiles, hipStream_t stream) {
         if (a.tiles) query_gradient<T, DP><<<(unsigned)(a.tiles * a.hq), 256, 0, stream>>>(a);
         Args b = a;
-        const int keys = getenv("OEQ_TRY_KEYS") ? atoi(getenv("OEQ_TRY_KEYS")) : 2;
-        b.tiles = (a.nk + 32 * keys - 1) / (32 * keys);
-        if (b.tiles) {
-            if (keys == 2)
-                key_gradient<T, DP, 2><<<(unsigned)(b.tiles * a.hk), 256, 0, stream>>>(b);
-            else
-                key_gradient<T, DP, 4><<<(unsigned)(b.tiles * a.hk), 256, 0, stream>>>(b);
-        }
+        b.tiles = key_tiles;
+        if (key_tiles) key_gradient<T, DP><<<(unsigned)(key_tiles * a.hk), 256, 0, stream>>>(b);
         return hipGetLastError();
     }
 };
