@@ -399,11 +399,11 @@ size_t oeq_attention_forward_workspace_bytes(const oeq_attention* a);
  * makes the gradients more exact and may be NULL. */
 int oeq_attention_forward(const oeq_attention* a, void* out, void* out_rest, float* log2_sum, void* workspace,
                           size_t workspace_bytes, void* stream);
-/* The gradients are contiguous like out; delta is scratch of log2_sum's size. No atomics: the results do not depend on
- * the order in which blocks run. */
-int oeq_attention_backward(const oeq_attention* a, const void* out, const void* out_rest, const float* log2_sum, const void* out_grad,
-                           int64_t grad_row_stride, int64_t grad_head_stride, void* q_grad, void* k_grad, void* v_grad,
-                           float* delta, void* stream);
+size_t oeq_attention_backward_workspace_bytes(const oeq_attention* a);
+/* The gradients are contiguous like out. No atomics: the results do not depend on the order in which blocks run. */
+int oeq_attention_backward(const oeq_attention* a, const void* out, const void* out_rest, const float* log2_sum,
+                           const void* out_grad, int64_t grad_row_stride, int64_t grad_head_stride, void* q_grad,
+                           void* k_grad, void* v_grad, void* workspace, size_t workspace_bytes, void* stream);
 
 /* Norm of each head of queries and keys over its root mean square, times a weight of head_dim elements (NULL: no norm),
  * and rotation of its first rotary_dim elements by the row of `table` that positions[row] names: rotary_dim / 2 cosines,

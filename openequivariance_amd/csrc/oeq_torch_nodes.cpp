@@ -141,10 +141,11 @@ Tensor3 packed_attention_backward_gpu(const Tensor& grad, const Tensor& q, const
     const Rows g(grad);
     const Tensor o = whole(out), sums = log2_sum.contiguous(), r = whole(rest);
     Tensor dq = at::empty(q.sizes(), q.options()), dk = at::empty(k.sizes(), k.options()), dv = at::empty(v.sizes(), v.options());
-    Tensor delta = at::empty_like(sums);
+    const size_t nb = oeq_attention_backward_workspace_bytes(&call.a);
+    const Tensor ws = scratch(q, nb);
     check(oeq_attention_backward(&call.a, o.data_ptr(), r.numel() ? r.data_ptr() : nullptr, sums.data_ptr<float>(),
                                  g.t.data_ptr(), g.row, g.head, dq.data_ptr(), dk.data_ptr(), dv.data_ptr(),
-                                 delta.data_ptr<float>(), dev.stream),
+                                 ws.data_ptr(), nb, dev.stream),
           "oeq_attention_backward");
     return {dq, dk, dv};
 }

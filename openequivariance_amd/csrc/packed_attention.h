@@ -47,6 +47,7 @@ struct Args {
     int64_t q_row, q_head, k_row, k_head, v_row, v_head, g_row, g_head, stat_stride;
     int segments, nq, nk, hq, hk, d, causal, tiles;
     float scale_log2;  // c * log2(e): the kernels work with powers of two
+    const int *q_order, *k_order;  // tiles by the length of their walks, or NULL
     int parts;  // the form for few queries: shares of a row's keys, and their results
     float* partial;
 };
@@ -386,12 +387,62 @@ __device__ __forceinline__ Bounds block_range(const Walk& w, int (&shared)[8], i
 }
 
 // Block -> (tile, head): blocks that an XCD runs (every eighth) share key heads, so that its L2 holds few of them at a
-// time; causal tiles run from the last on, whose walks are the longest.
-__device__ __forceinline__ void place(const Args& a, int heads, int& tile, int& head) {
+// time; tiles run in the order of `order` (by the length of their walks), or where there is none as they are, causal query
+// tiles from the last on.
+__device__ __forceinline__ void place(const Args& a, int heads, const int* order, bool reversed, int& tile, int& head) {
     const int id = blockIdx.x, at = id % heads;
     tile = id / heads;
-    if (a.causal) tile = a.tiles - 1 - tile;
+    if (order)
+        tile = __builtin_amdgcn_readfirstlane(order[tile]);
+    else if (reversed)
+        tile = a.tiles - 1 - tile;
     head = heads % 8 == 0 ? (at % 8) * (heads / 8) + at / 8 : at;
+}
+
+// Tiles of rows by falling length of their walks: the longest first, so that a launch does not end with a few compute
+// units at work on them. Lengths are
+// those between the first and the last row's bounds; tiles of about the same length come in any order, on which no
+// result depends. One block for query tiles, one for key tiles; order[tiles ..] is scratch.
+[[maybe_unused]] static __global__ __launch_bounds__(1024) void order_tiles(Args a, int* q_order, int q_tiles, int* k_order, int k_tiles) {
+    __shared__ int count[256], longest;
+    const bool keys = blockIdx.x == 1;
+    int* order = keys ? k_order : q_order;
+    const int tiles = keys ? k_tiles : q_tiles, rows = keys ? a.nk : a.nq, each = keys ? 64 : 128;
+    const int lane = threadIdx.x & 63;
+    if (threadIdx.x < 256) count[threadIdx.x] = 0;
+    if (threadIdx.x == 0) longest = 1;
+    __syncthreads();
+    for (int base = 0; base < tiles; base += 1024) {
+        const int t = base + threadIdx.x, first = min(t * each, rows - 1), last = min(first + each - 1, rows - 1);
+        const Bounds x = keys ? queries_of(a, first, lane) : keys_of(a, first, lane);
+        const Bounds y = keys ? queries_of(a, last, lane) : keys_of(a, last, lane);
+        const int n = x.lo < x.hi && y.lo < y.hi ? y.hi - x.lo : max(x.hi - x.lo, y.hi - y.lo);
+        if (t < tiles) {
+            order[tiles + t] = max(n, 0);
+            atomicMax(&longest, n);
+        }
+    }
+    __syncthreads();
+    const float by = 255.0f / longest;
+    for (int t = threadIdx.x; t < tiles; t += 1024) atomicAdd(&count[255 - min(255, (int)(order[tiles + t] * by))], 1);
+    __syncthreads();
+    if (threadIdx.x < 64) {  // where each class begins
+        int c[4], sum = 0;
+#pragma unroll
+        for (int n = 0; n < 4; ++n) c[n] = count[4 * lane + n], sum += c[n];
+        int before = sum;
+#pragma unroll
+        for (int n = 1; n < 64; n <<= 1) {
+            const int x = __shfl_up(before, n);
+            if (lane >= n) before += x;
+        }
+        before -= sum;
+#pragma unroll
+        for (int n = 0; n < 4; ++n) count[4 * lane + n] = before, before += c[n];
+    }
+    __syncthreads();
+    for (int t = threadIdx.x; t < tiles; t += 1024)
+        order[atomicAdd(&count[255 - min(255, (int)(order[tiles + t] * by))], 1)] = t;
 }
 
 // Blocks of four waves on a compute unit: 256 registers a lane for two, 512 where a head of 128 four-byte elements needs
@@ -405,8 +456,14 @@ constexpr bool kFenced = sizeof(T) == 2 && DP == 128;  // key_gradient: one wave
 template <typename T, int DP>
 constexpr int key_blocks_per_unit() { return sizeof(T) * DP >= 256 ? 1 : 2; }
 
-template <typename T>
-constexpr int tile_rows() { return sizeof(T) == 2 ? 64 : 32; }
+// Keys of a tile: 16 KB, or 8 KB where a block's walk over small segments should have few steps (each waits for its tile).
+template <typename T, int DP>
+constexpr int tile_rows() { return sizeof(T) == 2 || DP == 32 ? 64 : 32; }
+
+// Small heads go with small segments: there each wave leaves out the groups of 32 keys that none of its rows sees. (512
+// molecules of 9 to 61 atoms: a wave's 32 rows see some 90 keys, their block's 128 rows 180.)
+template <typename T, int DP>
+constexpr bool kSparse = sizeof(T) == 4 && DP == 32;
 
 // Everything that was requested so far has come, and the compiler knows: a row that is loaded before a loop would else be
 // waited for inside it, at its first use, together with what the loop has requested since.
@@ -519,16 +576,18 @@ __device__ __forceinline__ bool all_finite(const float16_t (&acc)[DT]) {
 
 template <typename T, int DP>
 __global__ __launch_bounds__(256, (blocks_per_unit<T, DP>())) void forward(Args a) {
-    constexpr int BK = tile_rows<T>(), SUB = BK / 32, DT = DP / 32;
+    constexpr int BK = tile_rows<T, DP>(), SUB = kSparse<T, DP> ? 1 : BK / 32, DT = DP / 32;
     constexpr int PF = sizeof(T) == 2 ? 2 : 4;  // fragments of 32 keys
     typedef Tile<T, DP, BK> L;
     __shared__ __align__(1024) char key0[L::kBytes], key1[L::kBytes], val0[L::kBytes], val1[L::kBytes];
     __shared__ int shared[8];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5;
     int tile, h;
-    place(a, a.hq, tile, h);
+    place(a, a.hq, a.q_order, a.causal, tile, h);
     const int kh = h / (a.hq / a.hk), chunks = a.d * (int)sizeof(T) / 16;
     const int row = (tile * 4 + wave) * 32 + (lane & 31), i = min(row, a.nq - 1);
+    typename L::frag q[L::kFrags];
+    load_row<T, L::kFrags>(q, (const char*)((const T*)a.q + i * a.q_row + h * a.q_head), chunks, half);
     if (chunks < L::kChunks) {
         clear<L::kBytes>(key0), clear<L::kBytes>(key1), clear<L::kBytes>(val0), clear<L::kBytes>(val1);
     }
@@ -539,8 +598,6 @@ __global__ __launch_bounds__(256, (blocks_per_unit<T, DP>())) void forward(Args 
     const char* vbase = (const char*)((const T*)a.v + kh * a.v_head);
     const int krow = (int)a.k_row * (int)sizeof(T), vrow = (int)a.v_row * (int)sizeof(T);
     const typename L::Places kplaces(krow, chunks, wave, lane), vplaces(vrow, chunks, wave, lane);
-    typename L::frag q[L::kFrags];
-    load_row<T, L::kFrags>(q, (const char*)((const T*)a.q + i * a.q_row + h * a.q_head), chunks, half);
     float16_t acc[DT];
 #pragma unroll
     for (int t = 0; t < DT; ++t) acc[t] = 0.0f;
@@ -548,16 +605,16 @@ __global__ __launch_bounds__(256, (blocks_per_unit<T, DP>())) void forward(Args 
     const float c = a.scale_log2;
     settle();
 
-    auto products = [&](const char* kt, const char* vt, int first) {
+    auto products = [&](const char* kt, const char* vt, int first, int r0) {
         float16_t s[SUB];
 #pragma unroll
         for (int u = 0; u < SUB; ++u) {
             s[u] = 0.0f;
 #pragma unroll
-            for (int f = 0; f < L::kFrags; ++f) s[u] = mma(L::row(kt, 32 * u + (lane & 31), f, half), q[f], s[u]);
+            for (int f = 0; f < L::kFrags; ++f) s[u] = mma(L::row(kt, r0 + 32 * u + (lane & 31), f, half), q[f], s[u]);
         }
-        if (!walk.whole(first, BK)) {
-            const int shift = first + 4 * half - b.lo;
+        if (!walk.whole(first + r0, 32 * SUB)) {
+            const int shift = first + r0 + 4 * half - b.lo;
             const unsigned n = b.hi - b.lo;
 #pragma unroll
             for (int u = 0; u < SUB; ++u)
@@ -592,7 +649,7 @@ __global__ __launch_bounds__(256, (blocks_per_unit<T, DP>())) void forward(Args 
             for (int f = 0; f < PF; ++f) {
                 const auto p = operand<T>(s[u], f);
 #pragma unroll
-                for (int t = 0; t < DT; ++t) acc[t] = mma(column_of<T, DP, BK>(vt, 32 * u, f, t, lane), p, acc[t]);
+                for (int t = 0; t < DT; ++t) acc[t] = mma(column_of<T, DP, BK>(vt, r0 + 32 * u, f, t, lane), p, acc[t]);
             }
         }
     };
@@ -602,7 +659,9 @@ __global__ __launch_bounds__(256, (blocks_per_unit<T, DP>())) void forward(Args 
             L::request(kn, kbase, krow, kplaces, first + BK, all.hi, chunks, wave);
             L::request(vn, vbase, vrow, vplaces, first + BK, all.hi, chunks, wave);
         }
-        if (walk.needs(first, BK)) products(kt, vt, first);
+#pragma unroll
+        for (int r0 = 0; r0 < BK; r0 += 32 * SUB)
+            if (walk.needs(first + r0, 32 * SUB)) products(kt, vt, first, r0);
     };
     if (all.lo < all.hi) {
         L::request(key0, kbase, krow, kplaces, all.lo, all.hi, chunks, wave);
@@ -882,30 +941,17 @@ __global__ __launch_bounds__(256) void join(Args a) {
 
 template <typename T, int DP>
 __global__ __launch_bounds__(256, (blocks_per_unit<T, DP>())) void query_gradient(Args a) {
-    constexpr int BK = tile_rows<T>(), SUB = BK / 32, DT = DP / 32;
+    constexpr int BK = tile_rows<T, DP>(), SUB = BK / 32, DT = DP / 32;
     constexpr int PF = sizeof(T) == 2 ? 2 : 4;
     typedef Tile<T, DP, BK> L;
     __shared__ __align__(1024) char key0[L::kBytes], key1[L::kBytes], val0[L::kBytes], val1[L::kBytes];
     __shared__ int shared[8];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5;
     int tile, h;
-    place(a, a.hq, tile, h);
+    place(a, a.hq, a.q_order, a.causal, tile, h);
     const int kh = h / (a.hq / a.hk), chunks = a.d * (int)sizeof(T) / 16;
     const int row = (tile * 4 + wave) * 32 + (lane & 31), i = min(row, a.nq - 1);
-    if (chunks < L::kChunks) {
-        clear<L::kBytes>(key0), clear<L::kBytes>(key1), clear<L::kBytes>(val0), clear<L::kBytes>(val1);
-    }
-    const Bounds b = keys_of(a, i, lane);
-    const Walk walk(b);
-    const Bounds all = block_range(walk, shared, wave, lane);
-    const char* kbase = (const char*)((const T*)a.k + kh * a.k_head);
-    const char* vbase = (const char*)((const T*)a.v + kh * a.v_head);
-    const int krow = (int)a.k_row * (int)sizeof(T), vrow = (int)a.v_row * (int)sizeof(T);
-    const typename L::Places kplaces(krow, chunks, wave, lane), vplaces(vrow, chunks, wave, lane);
-    if (all.lo < all.hi) {
-        L::request(key0, kbase, krow, kplaces, all.lo, all.hi, chunks, wave);
-        L::request(val0, vbase, vrow, vplaces, all.lo, all.hi, chunks, wave);
-    }
+    const bool mine = row < a.nq;
     typename L::frag q[L::kFrags], g[L::kFrags];
     load_row<T, L::kFrags>(q, (const char*)((const T*)a.q + i * a.q_row + h * a.q_head), chunks, half);
     load_row<T, L::kFrags>(g, (const char*)((const T*)a.grad + i * a.g_row + h * a.g_head), chunks, half);
@@ -925,8 +971,21 @@ __global__ __launch_bounds__(256, (blocks_per_unit<T, DP>())) void query_gradien
         }
         delta = sum_halves(delta);
     }
-    const bool mine = row < a.nq;
     if (mine && half == 0) a.delta[h * a.stat_stride + i] = delta;
+    if (chunks < L::kChunks) {
+        clear<L::kBytes>(key0), clear<L::kBytes>(key1), clear<L::kBytes>(val0), clear<L::kBytes>(val1);
+    }
+    const Bounds b = keys_of(a, i, lane);
+    const Walk walk(b);
+    const Bounds all = block_range(walk, shared, wave, lane);
+    const char* kbase = (const char*)((const T*)a.k + kh * a.k_head);
+    const char* vbase = (const char*)((const T*)a.v + kh * a.v_head);
+    const int krow = (int)a.k_row * (int)sizeof(T), vrow = (int)a.v_row * (int)sizeof(T);
+    const typename L::Places kplaces(krow, chunks, wave, lane), vplaces(vrow, chunks, wave, lane);
+    if (all.lo < all.hi) {
+        L::request(key0, kbase, krow, kplaces, all.lo, all.hi, chunks, wave);
+        L::request(val0, vbase, vrow, vplaces, all.lo, all.hi, chunks, wave);
+    }
     const float lse = a.lse[h * a.stat_stride + i], c = a.scale_log2;
     settle();
     float16_t acc[DT];
@@ -936,6 +995,7 @@ __global__ __launch_bounds__(256, (blocks_per_unit<T, DP>())) void query_gradien
     auto products = [&](const char* kt, const char* vt, int first) {
 #pragma unroll
         for (int u = 0; u < SUB; ++u) {
+            if (kSparse<T, DP> && !walk.needs(first + 32 * u, 32)) continue;
             float16_t s = 0.0f, x = 0.0f;
 #pragma unroll
             for (int f = 0; f < L::kFrags; ++f) s = mma(L::row(kt, 32 * u + (lane & 31), f, half), q[f], s);
@@ -946,7 +1006,7 @@ __global__ __launch_bounds__(256, (blocks_per_unit<T, DP>())) void query_gradien
                 const float p = raised<T, Types<T>::kDs>(fmaf(s[r], c, -lse));
                 x[r] = p * (x[r] - delta);
             }
-            if (!walk.whole(first, BK)) {
+            if (!(kSparse<T, DP> ? walk.whole(first + 32 * u, 32) : walk.whole(first, BK))) {
                 const int shift = first + 32 * u + 4 * half - b.lo;
                 const unsigned n = b.hi - b.lo;
 #pragma unroll
@@ -1007,10 +1067,12 @@ __global__ __launch_bounds__(256, (key_blocks_per_unit<T, DP>())) void key_gradi
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5;
     const int keys = wave & 1, r0 = 32 * (wave >> 1);  // which 32 keys, and the first row of the wave's half of a tile
     int tile, kh;
-    place(a, a.hk, tile, kh);
-    if (a.causal) tile = a.tiles - 1 - tile;  // the first keys have the longest walks
+    place(a, a.hk, a.k_order, false, tile, kh);  // (causal: the first keys have the longest walks)
     const int group = a.hq / a.hk, chunks = a.d * (int)sizeof(T) / 16;
     const int row = (tile * 2 + keys) * 32 + (lane & 31), j = min(row, a.nk - 1);
+    typename L::frag k[L::kFrags], v[L::kFrags];
+    load_row<T, L::kFrags>(k, (const char*)((const T*)a.k + j * a.k_row + kh * a.k_head), chunks, half);
+    load_row<T, L::kFrags>(v, (const char*)((const T*)a.v + j * a.v_row + kh * a.v_head), chunks, half);
     if (chunks < L::kChunks) {
         clear<L::kBytes>(que0), clear<L::kBytes>(que1), clear<L::kBytes>(gra0), clear<L::kBytes>(gra1);
     }
@@ -1036,9 +1098,6 @@ __global__ __launch_bounds__(256, (key_blocks_per_unit<T, DP>())) void key_gradi
         if (next_first < all.lo) next_first = top, ++next_h;
     };
     request(que0, gra0, sta0);
-    typename L::frag k[L::kFrags], v[L::kFrags];
-    load_row<T, L::kFrags>(k, (const char*)((const T*)a.k + j * a.k_row + kh * a.k_head), chunks, half);
-    load_row<T, L::kFrags>(v, (const char*)((const T*)a.v + j * a.v_row + kh * a.v_head), chunks, half);
     const float c = a.scale_log2;
     float16_t dk[DT], dv[DT];
 #pragma unroll
@@ -1073,6 +1132,10 @@ __global__ __launch_bounds__(256, (key_blocks_per_unit<T, DP>())) void key_gradi
     auto step = [&](char* qt, char* gt, float* st, char* qn, char* gn, float* sn) {
         arrived();
         request(qn, gn, sn);
+        const int now = first;
+        first -= BQ;
+        if (first < all.lo) first = top;
+        if (kSparse<T, DP> && !walk.needs(now + r0, 32)) return;
         float16_t s = 0.0f, x = 0.0f;
         if constexpr (kFenced<T, DP>) {
             typename L::frag rows[2][8], columns[2][2 * DT];
@@ -1102,7 +1165,7 @@ __global__ __launch_bounds__(256, (key_blocks_per_unit<T, DP>())) void key_gradi
             __builtin_amdgcn_sched_barrier(0);
             load_columns(0);
             weigh(s, x, st);
-            hide(s, x, first);
+            hide(s, x, now);
             load_columns(1);
 #pragma unroll
             for (int f = 0; f < 2; ++f) {
@@ -1123,7 +1186,7 @@ __global__ __launch_bounds__(256, (key_blocks_per_unit<T, DP>())) void key_gradi
 #pragma unroll
             for (int f = 0; f < L::kFrags; ++f) x = mma(L::row(gt, r0 + (lane & 31), f, half), v[f], x), fence(f);
             weigh(s, x, st);
-            hide(s, x, first);
+            hide(s, x, now);
 #pragma unroll
             for (int f = 0; f < PF; ++f) {
                 fence(3);
@@ -1135,8 +1198,6 @@ __global__ __launch_bounds__(256, (key_blocks_per_unit<T, DP>())) void key_gradi
                 for (int t = 0; t < DT; ++t) dk[t] = mma(column_of<T, DP, BQ>(qt, r0, f, t, lane), d, dk[t]);
             }
         }
-        first -= BQ;
-        if (first < all.lo) first = top;
     };
     for (int n = 0; n < steps; n += 2) {
         step(que0, gra0, sta0, que1, gra1, sta1);

@@ -12,5 +12,8 @@ struct Launch {
     static hipError_t backward(const Args& a, int key_tiles, hipStream_t stream);
 };
 
+// Rows of a tile of queries and of keys.
+constexpr int kQueryTile = 128, kKeyTile = 64;
+
 }  // namespace packed_attention
 #endif

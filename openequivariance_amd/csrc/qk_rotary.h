@@ -6,8 +6,9 @@
 //
 // A head belongs to 8 (a power of two up to 16) neighbouring lanes with eight elements each, chosen so that both partners
 // of a pair are in one lane: two quads that lie r / 2 apart, or one behind the other where pairs are neighbours or past
-// the r turned elements. So the only thing that passes between lanes is the sum of squares. The kernels are bound by
-// memory: every head is read once and written once, the table's rows come from L2.
+// the r turned elements. So the only thing that passes between lanes is the sum of squares. A block has one row or several
+// and its groups of lanes walk the row's heads, kHeads of them requested at a time, with the row's cosines and sines in
+// registers. The kernels are bound by memory: every head is read once and written once.
 #ifndef OEQ_QK_ROTARY_H
 #define OEQ_QK_ROTARY_H
 
@@ -23,13 +24,14 @@ struct Args {
     const int64_t *positions, *slots;
     const float* table;
     float* partial;  // sums of the weights' gradients: [blocks, 2, 8 lanes]
+    int groups;      // groups of lanes to a row: a power of two
     int64_t q_row, q_head, k_row, k_head, v_row, v_head;
     int64_t gq_row, gq_head, gk_row, gk_head;       // strides of the outputs' gradients
     int64_t ko_row, ko_head, vo_row, vo_head;       // strides of k_out, v_out
     int64_t table_rows, slots_end;
-    int64_t units;  // heads of all rows
-    int q_heads, k_heads, d, rotary, interleaved, lanes;
-    float eps;
+    int64_t rows;
+    int q_heads, k_heads, d, rotary, interleaved;
+    float eps, per_d;  // and 1 / d
 };
 
 template <typename T>
@@ -54,14 +56,20 @@ struct Eight {
     float u[4], v[4];  // the two quads
 };
 
+// As they are in memory: the conversion waits for the load, so it comes when others have been requested.
 template <typename T>
-__device__ __forceinline__ Eight load(const T* row, Where w) {
-    const auto a = *(const typename Quad<T>::type*)(row + w.a), b = *(const typename Quad<T>::type*)(row + w.b);
-    Eight x;
+struct Raw {
+    typename Quad<T>::type a, b;
+    __device__ __forceinline__ Raw() {}
+    __device__ __forceinline__ Raw(const T* row, Where w)
+        : a(*(const typename Quad<T>::type*)(row + w.a)), b(*(const typename Quad<T>::type*)(row + w.b)) {}
+    __device__ __forceinline__ Eight wide() const {
+        Eight x;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) x.u[j] = (float)a[j], x.v[j] = (float)b[j];
-    return x;
-}
+        for (int j = 0; j < 4; ++j) x.u[j] = (float)a[j], x.v[j] = (float)b[j];
+        return x;
+    }
+};
 
 template <typename T>
 __device__ __forceinline__ void store(T* row, Where w, const Eight& x) {
@@ -72,20 +80,34 @@ __device__ __forceinline__ void store(T* row, Where w, const Eight& x) {
     *(typename Quad<T>::type*)(row + w.b) = __builtin_convertvector(b, typename Quad<T>::type);
 }
 
-// Turns the lane's four pairs by the angles of the row, or back.
-__device__ __forceinline__ void turn(Eight& x, const Args& g, const float* table, int i, bool inside, float sign) {
-    float4_t c = NAN, s = NAN;  // (a position that the table does not have)
-    if (inside) {
-        c = *(const float4_t*)(table + 4 * i);
-        s = *(const float4_t*)(table + g.rotary / 2 + 4 * i);
+// The angles of a lane's pairs in a row. (A position that the table does not have gives NaN.)
+struct Angle {
+    float4_t c, s;
+    __device__ __forceinline__ Angle(const Args& g, int64_t row, int i, bool turned) {
+        c = 1.0f, s = 0.0f;
+        if (!turned) return;
+        const int64_t at = g.positions[row];
+        const bool known = at >= 0 && at < g.table_rows;
+        if (known) {
+            c = *(const float4_t*)(g.table + at * g.rotary + 4 * i);
+            s = *(const float4_t*)(g.table + at * g.rotary + g.rotary / 2 + 4 * i);
+        } else {
+            c = NAN, s = NAN;
+        }
     }
+};
+
+// Turns the lane's four pairs, or back.
+__device__ __forceinline__ void turn(Eight& x, const Args& g, const Angle& angle, float sign) {
+    const float4_t &c = angle.c, &s = angle.s;
     if (g.interleaved) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            float* p = j < 2 ? x.u + 2 * j : x.v + 2 * j - 4;
-            const float a = p[0], b = p[1];
-            p[0] = a * c[j] - sign * b * s[j];
-            p[1] = b * c[j] + sign * a * s[j];
+        for (int j = 0; j < 2; ++j) {
+            const float a = x.u[2 * j], b = x.u[2 * j + 1], p = x.v[2 * j], q = x.v[2 * j + 1];
+            x.u[2 * j] = a * c[j] - sign * b * s[j];
+            x.u[2 * j + 1] = b * c[j] + sign * a * s[j];
+            x.v[2 * j] = p * c[2 + j] - sign * q * s[2 + j];
+            x.v[2 * j + 1] = q * c[2 + j] + sign * p * s[2 + j];
         }
     } else {
 #pragma unroll
@@ -97,9 +119,17 @@ __device__ __forceinline__ void turn(Eight& x, const Args& g, const float* table
     }
 }
 
-// The sum over the lanes of a head.
-__device__ __forceinline__ float head_sum(float x, int lanes) {
-    for (int m = 1; m < lanes; m <<= 1) x += __shfl_xor(x, m);
+// The sum over the lanes of a head, in the vector unit: with the neighbour, the next pair, and by mirrors of eight and of
+// sixteen lanes the other quad and the other eight.
+template <int LANES>
+__device__ __forceinline__ float head_sum(float x) {
+#define OEQ_ADD_DPP(control) \
+    x += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), control, 0xf, 0xf, true))
+    if (LANES > 1) OEQ_ADD_DPP(0xb1);    // quad_perm 1 0 3 2
+    if (LANES > 2) OEQ_ADD_DPP(0x4e);    // quad_perm 2 3 0 1
+    if (LANES > 4) OEQ_ADD_DPP(0x141);   // row_half_mirror
+    if (LANES > 8) OEQ_ADD_DPP(0x140);   // row_mirror
+#undef OEQ_ADD_DPP
     return x;
 }
 
@@ -110,99 +140,141 @@ __device__ __forceinline__ float squares(const Eight& x) {
     return s;
 }
 
-// One head to a group of lanes. APPEND: keys go to the row of the cache that slots[] names, values as they are beside
-// them; rows that the cache does not have are left out.
-template <typename T, bool APPEND>
-__global__ __launch_bounds__(256) void forward(Args g) {
-    const int64_t unit = ((int64_t)blockIdx.x * 256 + threadIdx.x) / g.lanes;
-    const int i = threadIdx.x & (g.lanes - 1), heads = g.q_heads + (APPEND ? 2 : 1) * g.k_heads;
-    const bool live = unit < g.units && 8 * i < g.d;
-    const int64_t row = min(unit, g.units - 1) / heads;
-    const int h = (int)(min(unit, g.units - 1) - row * heads);
-    const bool is_q = h < g.q_heads, is_v = h >= g.q_heads + g.k_heads;
-    const int kh = is_q ? 0 : h - g.q_heads - (is_v ? g.k_heads : 0);
-    const T* from = is_q ? (const T*)g.q + row * g.q_row + h * g.q_head
-                         : is_v ? (const T*)g.v + row * g.v_row + kh * g.v_head : (const T*)g.k + row * g.k_row + kh * g.k_head;
-    const T* weight = (const T*)(is_q ? g.q_weight : is_v ? nullptr : g.k_weight);
-    Where w(g, i);
-    Eight x = {};
-    if (live) x = load<T>(from, w);
-    const float mean = head_sum(squares(x), g.lanes) / g.d;
-    if (!live) return;
-    if (weight) {
-        const float by = 1.0f / sqrtf(mean + g.eps);
-        const Eight y = load<T>(weight, w);
+constexpr int kHeads = 2;  // requested at a time
+
+// Which part of a block's rows and heads a thread has. Lanes without elements, heads and rows past the last read what the
+// last ones do and store nothing.
+template <int LANES>
+struct Place {
+    int64_t mine, row;
+    int i, first;
+    bool holds, live;
+    __device__ __forceinline__ Place(const Args& g, int64_t top) {
+        const int lane = threadIdx.x & (LANES - 1);
+        first = threadIdx.x / LANES & (g.groups - 1);
+        mine = top + threadIdx.x / (LANES * g.groups);
+        row = min(mine, g.rows - 1);
+        holds = 8 * lane < g.d;
+        live = holds && mine < g.rows;
+        i = holds ? lane : 0;
+    }
+};
+
+// The heads of one kind in a row: normed by `weight` (if there is one), turned, stored.
+template <typename T, int LANES, bool TURNS>
+__device__ __forceinline__ void heads_forward(const Args& g, const Place<LANES>& at, Where w, const Angle& angle, const T* from,
+                                              int64_t from_head, T* to, int64_t to_head, int heads, const T* weight, bool live) {
+    Eight y;
+    if (weight) y = Raw<T>(weight, w).wide();
+    for (int base = at.first; base < heads; base += kHeads * g.groups) {
+        Raw<T> raw[kHeads];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) x.u[j] *= by * y.u[j], x.v[j] *= by * y.v[j];
+        for (int n = 0; n < kHeads; ++n) raw[n] = Raw<T>(from + min(base + n * g.groups, heads - 1) * from_head, w);
+#pragma unroll
+        for (int n = 0; n < kHeads; ++n) {
+            const int h = base + n * g.groups;
+            Eight x = raw[n].wide();
+            if (weight) {
+                const float by = __builtin_amdgcn_rsqf(head_sum<LANES>(at.holds ? squares(x) : 0.0f) * g.per_d + g.eps);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) x.u[j] *= by * y.u[j], x.v[j] *= by * y.v[j];
+            }
+            if (TURNS && w.turned) turn(x, g, angle, 1.0f);
+            if (live && h < heads) store<T>(to + h * to_head, w, x);
+        }
     }
-    if (w.turned && !is_v) {
-        const int64_t at = g.positions[row];
-        turn(x, g, g.table + at * g.rotary, i, at >= 0 && at < g.table_rows, 1.0f);
-    }
-    if (is_q) {
-        store<T>((T*)g.q_out + (row * g.q_heads + h) * g.d, w, x);
-        return;
-    }
-    int64_t to = row;
-    if (APPEND) {
-        to = g.slots[row];
-        if (to < 0 || to >= g.slots_end) return;
-    }
-    store<T>(is_v ? (T*)g.v_out + to * g.vo_row + kh * g.vo_head : (T*)g.k_out + to * g.ko_row + kh * g.ko_head, w, x);
 }
 
-// Gradients: turned back, gy = w-weighted; with n = x / rms, dx = (gy w - n mean(gy w n)) / rms, dw = sum gy n. A group of
-// lanes walks heads at the distance of the grid; its sums of dw go, per block, to a row of `partial`, which
-// weight_gradient adds up in order.
-template <typename T>
+// APPEND: keys go to the row of the cache that slots[] names, values as they are beside them; rows that the cache does not
+// have are left out.
+template <typename T, int LANES, bool APPEND>
+__global__ __launch_bounds__(256) void forward(Args g) {
+    const Place<LANES> at(g, (int64_t)blockIdx.x * (256 / (LANES * g.groups)));
+    const Where w(g, at.i);
+    const Angle angle(g, at.row, at.i, w.turned);
+    int64_t to = at.row;
+    bool live = at.live;
+    if (APPEND) {
+        to = g.slots[at.row];
+        live = live && to >= 0 && to < g.slots_end;
+    }
+    heads_forward<T, LANES, true>(g, at, w, angle, (const T*)g.q + at.row * g.q_row, g.q_head,
+                                  (T*)g.q_out + at.row * g.q_heads * g.d, g.d, g.q_heads, (const T*)g.q_weight, at.live);
+    heads_forward<T, LANES, true>(g, at, w, angle, (const T*)g.k + at.row * g.k_row, g.k_head, (T*)g.k_out + to * g.ko_row,
+                                  g.ko_head, g.k_heads, (const T*)g.k_weight, live);
+    if (APPEND)
+        heads_forward<T, LANES, false>(g, at, w, angle, (const T*)g.v + at.row * g.v_row, g.v_head, (T*)g.v_out + to * g.vo_row,
+                                       g.vo_head, g.k_heads, nullptr, live);
+}
+
+// The gradients of one kind of heads in a row: gradients turned back, gy; with n = x / rms, dx = (gy w - n mean(gy w n)) / rms
+// and dw = sum gy n.
+template <typename T, int LANES>
+__device__ __forceinline__ void heads_backward(const Args& g, const Place<LANES>& at, Where w, const Angle& angle, const T* grad,
+                                               int64_t grad_head, const T* from, int64_t from_head, T* to, int heads,
+                                               const T* weight, const Eight& wt, Eight& dw) {
+    for (int base = at.first; base < heads; base += kHeads * g.groups) {
+        Raw<T> rx[kHeads], ry[kHeads];
+#pragma unroll
+        for (int n = 0; n < kHeads; ++n) {
+            const int h = min(base + n * g.groups, heads - 1);
+            ry[n] = Raw<T>(grad + h * grad_head, w);
+            if (weight) rx[n] = Raw<T>(from + h * from_head, w);
+        }
+#pragma unroll
+        for (int n = 0; n < kHeads; ++n) {
+            const int h = base + n * g.groups;
+            const bool live = at.live && h < heads;
+            Eight y = ry[n].wide();
+            if (w.turned) turn(y, g, angle, -1.0f);
+            if (weight) {
+                Eight x = rx[n].wide(), z;
+                const float by = __builtin_amdgcn_rsqf(head_sum<LANES>(at.holds ? squares(x) : 0.0f) * g.per_d + g.eps);
+                float along = 0;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    x.u[j] *= by, x.v[j] *= by;
+                    z.u[j] = y.u[j] * wt.u[j], z.v[j] = y.v[j] * wt.v[j];
+                    along = fmaf(z.u[j], x.u[j], fmaf(z.v[j], x.v[j], along));
+                }
+                along = head_sum<LANES>(at.holds ? along : 0.0f) * g.per_d;
+                if (live) {
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        dw.u[j] = fmaf(y.u[j], x.u[j], dw.u[j]), dw.v[j] = fmaf(y.v[j], x.v[j], dw.v[j]);
+                        y.u[j] = by * (z.u[j] - x.u[j] * along);
+                        y.v[j] = by * (z.v[j] - x.v[j] * along);
+                    }
+                }
+            }
+            if (live) store<T>(to + h * g.d, w, y);
+        }
+    }
+}
+
+// Blocks walk rows at the distance of the grid; their sums of dw go, one row a block, to `partial`, which weight_gradient adds
+// up in order.
+template <typename T, int LANES>
 __global__ __launch_bounds__(256) void backward(Args g) {
     __shared__ float sums[2][256][8];
-    const int i = threadIdx.x & (g.lanes - 1), heads = g.q_heads + g.k_heads;
-    const bool holds = 8 * i < g.d;
-    Where w(g, i);
+    const int each = 256 / (LANES * g.groups);
     Eight dq = {}, dk = {}, wq = {}, wk = {};
-    if (holds && g.q_weight) wq = load<T>((const T*)g.q_weight, w);
-    if (holds && g.k_weight) wk = load<T>((const T*)g.k_weight, w);
-    const int64_t first = ((int64_t)blockIdx.x * 256 + threadIdx.x) / g.lanes, step = (int64_t)gridDim.x * 256 / g.lanes;
-    for (int64_t base = first - threadIdx.x / g.lanes; base < g.units; base += step) {
-        const int64_t unit = base + threadIdx.x / g.lanes, row = min(unit, g.units - 1) / heads;
-        const bool live = holds && unit < g.units;
-        const int h = (int)(min(unit, g.units - 1) - row * heads);
-        const bool is_q = h < g.q_heads, normed = is_q ? g.q_weight != nullptr : g.k_weight != nullptr;
-        const int kh = h - g.q_heads;
-        Eight x = {}, y = {};
-        if (live) {
-            y = load<T>(is_q ? (const T*)g.q_grad + row * g.gq_row + h * g.gq_head
-                             : (const T*)g.k_grad + row * g.gk_row + kh * g.gk_head, w);
-            if (normed)
-                x = load<T>(is_q ? (const T*)g.q + row * g.q_row + h * g.q_head
-                                 : (const T*)g.k + row * g.k_row + kh * g.k_head, w);
-            if (w.turned) {
-                const int64_t at = g.positions[row];
-                turn(y, g, g.table + at * g.rotary, i, at >= 0 && at < g.table_rows, -1.0f);
-            }
-        }
-        const float by = 1.0f / sqrtf(head_sum(squares(x), g.lanes) / g.d + g.eps);
-        float along = 0;
-        const Eight& wt = is_q ? wq : wk;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            x.u[j] *= by, x.v[j] *= by;
-            along = fmaf(y.u[j] * wt.u[j], x.u[j], fmaf(y.v[j] * wt.v[j], x.v[j], along));
-        }
-        along = head_sum(along, g.lanes) / g.d;
-        if (!live) continue;
-        if (normed) {
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const float du = y.u[j] * x.u[j], dv = y.v[j] * x.v[j];
-                if (is_q) dq.u[j] += du, dq.v[j] += dv;
-                else dk.u[j] += du, dk.v[j] += dv;
-                y.u[j] = by * (y.u[j] * wt.u[j] - x.u[j] * along);
-                y.v[j] = by * (y.v[j] * wt.v[j] - x.v[j] * along);
-            }
-        }
-        store<T>(is_q ? (T*)g.q_out + (row * g.q_heads + h) * g.d : (T*)g.k_out + (row * g.k_heads + kh) * g.d, w, y);
+    {
+        const Place<LANES> at(g, 0);
+        const Where w(g, at.i);
+        if (g.q_weight) wq = Raw<T>((const T*)g.q_weight, w).wide();
+        if (g.k_weight) wk = Raw<T>((const T*)g.k_weight, w).wide();
+    }
+    for (int64_t top = (int64_t)blockIdx.x * each; top < g.rows; top += (int64_t)gridDim.x * each) {
+        const Place<LANES> at(g, top);
+        const Where w(g, at.i);
+        const Angle angle(g, at.row, at.i, w.turned);
+        heads_backward<T, LANES>(g, at, w, angle, (const T*)g.q_grad + at.row * g.gq_row, g.gq_head,
+                                 (const T*)g.q + at.row * g.q_row, g.q_head, (T*)g.q_out + at.row * g.q_heads * g.d, g.q_heads,
+                                 (const T*)g.q_weight, wq, dq);
+        heads_backward<T, LANES>(g, at, w, angle, (const T*)g.k_grad + at.row * g.gk_row, g.gk_head,
+                                 (const T*)g.k + at.row * g.k_row, g.k_head, (T*)g.k_out + at.row * g.k_heads * g.d, g.k_heads,
+                                 (const T*)g.k_weight, wk, dk);
     }
     if (!g.partial) return;
 #pragma unroll
@@ -211,28 +283,29 @@ __global__ __launch_bounds__(256) void backward(Args g) {
         sums[1][threadIdx.x][j] = dk.u[j], sums[1][threadIdx.x][4 + j] = dk.v[j];
     }
     __syncthreads();
-    const int columns = 8 * g.lanes;  // (up to 128: with both weights one column to a thread)
-    for (int at = threadIdx.x; at < 2 * columns; at += 256) {
-        const int which = at / columns, column = at % columns;
+    constexpr int kColumns = 8 * LANES;  // (up to 128: with both weights one column to a thread)
+    for (int at = threadIdx.x; at < 2 * kColumns; at += 256) {
+        const int which = at / kColumns, column = at % kColumns;
         float s = 0;
-        for (int n = 0; n < 256 / g.lanes; ++n) s += sums[which][n * g.lanes + column / 8][column % 8];
-        g.partial[((int64_t)blockIdx.x * 2 + which) * columns + column] = s;
+        for (int n = 0; n < 256 / LANES; ++n) s += sums[which][n * LANES + column / 8][column % 8];
+        g.partial[((int64_t)blockIdx.x * 2 + which) * kColumns + column] = s;
     }
 }
 
-// Adds up the blocks' rows, in order within each of 16 parts and then over the parts.
+// Adds up the blocks' rows for 16 columns, in order within each of 64 parts and then over the parts.
 template <typename T>
-__global__ __launch_bounds__(1024) void weight_gradient(Args g, int blocks, T* dq, T* dk) {
-    __shared__ float sums[16][64];
-    const int columns = 8 * g.lanes, at = blockIdx.x * 64 + (threadIdx.x & 63), part = threadIdx.x >> 6;
+__global__ __launch_bounds__(1024) void weight_gradient(Args g, int lanes, int blocks, T* dq, T* dk) {
+    __shared__ float sums[64][16];
+    const int columns = 8 * lanes, at = blockIdx.x * 16 + (threadIdx.x & 15), part = threadIdx.x >> 4;
     float s = 0;
-    if (at < 2 * columns)
-        for (int n = part; n < blocks; n += 16) s += g.partial[(int64_t)n * 2 * columns + at];
-    sums[part][threadIdx.x & 63] = s;
+#pragma unroll 8
+    for (int n = part; n < blocks; n += 64) s += g.partial[(int64_t)n * 2 * columns + at];
+    sums[part][threadIdx.x & 15] = s;
     __syncthreads();
-    if (part || at >= 2 * columns) return;
+    if (part) return;
     s = 0;
-    for (int n = 0; n < 16; ++n) s += sums[n][threadIdx.x];
+#pragma unroll
+    for (int n = 0; n < 64; ++n) s += sums[n][threadIdx.x];
     const int which = at / columns, column = at % columns;
     T* out = which ? dk : dq;
     if (!out || 8 * (column / 8) >= g.d) return;

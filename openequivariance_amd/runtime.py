@@ -233,7 +233,8 @@ EXPORTS = {
     "oeq_attention_stat_stride": (_I64, [_I64]),
     "oeq_attention_forward_workspace_bytes": (_SZ, [ctypes.POINTER(_Attention)]),
     "oeq_attention_forward": (ctypes.c_int, [ctypes.POINTER(_Attention), _P, _P, _P, _P, _SZ, _P]),
-    "oeq_attention_backward": (ctypes.c_int, [ctypes.POINTER(_Attention), _P, _P, _P, _P, _I64, _I64] + [_P] * 5),
+    "oeq_attention_backward_workspace_bytes": (_SZ, [ctypes.POINTER(_Attention)]),
+    "oeq_attention_backward": (ctypes.c_int, [ctypes.POINTER(_Attention), _P, _P, _P, _P, _I64, _I64, _P, _P, _P, _P, _SZ, _P]),
     "oeq_qk_norm_rotary": (ctypes.c_int, [ctypes.POINTER(_QkRotary), _P, _P, _P]),
     "oeq_qk_norm_rotary_append": (ctypes.c_int, [ctypes.POINTER(_QkRotary), _P, _I64, _I64, _P, _P, _I64, _I64, _P, _I64,
                                                  _I64, _P, _I64, _P]),
