@@ -34,6 +34,11 @@ for _schema in (
         "irrep_dropout(Tensor x, Tensor? residual, Tensor channels, Tensor seed, float p) -> Tensor"):
     ops.define_op(_schema)
 
+_packed_attention = torch.ops.oeq_amd.packed_attention.default
+_qk_norm_rotary = torch.ops.oeq_amd.qk_norm_rotary.default
+_qk_norm_rotary_append = torch.ops.oeq_amd.qk_norm_rotary_append.default
+_irrep_dropout = torch.ops.oeq_amd.irrep_dropout.default
+
 
 def _stat_stride(rows):
     return (rows + 63) // 64 * 64 + 64
@@ -95,8 +100,7 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_ptr: t
     """
     if scale is None:
         scale = q.shape[-1] ** -0.5
-    out, log2_sum, _rest = torch.ops.oeq_amd.packed_attention(q, k, v, q_ptr, q_ptr if k_ptr is None else k_ptr, k_len, causal,
-                                                       scale)
+    out, log2_sum, _rest = _packed_attention(q, k, v, q_ptr, q_ptr if k_ptr is None else k_ptr, k_len, causal, scale)
     if return_lse:
         return out, (log2_sum[:, :q.shape[0]] * math.log(2.0)).t()
     return out
@@ -139,7 +143,7 @@ def qk_norm_rotary(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, ta
     :param q_weight, k_weight: ``[head_dim]``: ``x -> weight x / sqrt(mean(x^2) + eps)``; no norm where left out.
     :param interleaved: pairs are neighbours ``2 i, 2 i + 1`` instead of ``i, i + rotary_dim / 2``.
     """
-    return torch.ops.oeq_amd.qk_norm_rotary(q, k, positions, table, q_weight, k_weight, eps, interleaved)
+    return _qk_norm_rotary(q, k, positions, table, q_weight, k_weight, eps, interleaved)
 
 
 def qk_norm_rotary_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positions: torch.Tensor, table: torch.Tensor,
@@ -153,8 +157,7 @@ def qk_norm_rotary_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, pos
     :param slots: ``[rows]``, int64; rows whose slot is not one of the caches' (-1, say) are not written. Slots are
         different from each other.
     """
-    return torch.ops.oeq_amd.qk_norm_rotary_append(q, k, v, positions, table, k_cache, v_cache, slots, q_weight, k_weight,
-                                                   eps, interleaved)
+    return _qk_norm_rotary_append(q, k, v, positions, table, k_cache, v_cache, slots, q_weight, k_weight, eps, interleaved)
 
 
 class IrrepDropout(torch.nn.Module):
@@ -198,5 +201,9 @@ class IrrepDropout(torch.nn.Module):
             return x if residual is None else x + residual
         if seed is None:
             seed = torch.empty(2, dtype=torch.int64, device=x.device).random_()
-        channels = self.channels if self.channels.device == x.device else self.channels.to(x.device)
-        return torch.ops.oeq_amd.irrep_dropout(x, residual, channels, seed, self.p)
+        channels = self.channels
+        if channels.device != x.device:  # (a module that was not moved: its table moves with the first call)
+            channels = channels.to(x.device)
+            if not torch.compiler.is_compiling():
+                self.channels = channels
+        return _irrep_dropout(x, residual, channels, seed, self.p)

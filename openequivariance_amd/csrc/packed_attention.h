@@ -453,8 +453,8 @@ constexpr int blocks_per_unit() { return sizeof(T) * DP > 256 ? 1 : 2; }
 template <typename T, int DP>
 constexpr bool kFenced = sizeof(T) == 2 && DP == 128;  // key_gradient: one wave to a SIMD, see there
 
-template <typename T, int DP>
-constexpr int key_blocks_per_unit() { return sizeof(T) * DP >= 256 ? 1 : 2; }
+template <typename T, int DP, int WHAT>
+constexpr int key_blocks_per_unit() { return sizeof(T) * DP >= (WHAT == 3 ? 256 : 512) ? 1 : 2; }
 
 // Keys of a tile: 16 KB, or 8 KB where a block's walk over small segments should have few steps (each waits for its tile).
 template <typename T, int DP>
@@ -951,6 +951,20 @@ __global__ __launch_bounds__(256, (blocks_per_unit<T, DP>())) void query_gradien
     place(a, a.hq, a.q_order, a.causal, tile, h);
     const int kh = h / (a.hq / a.hk), chunks = a.d * (int)sizeof(T) / 16;
     const int row = (tile * 4 + wave) * 32 + (lane & 31), i = min(row, a.nq - 1);
+    if (chunks < L::kChunks) {
+        clear<L::kBytes>(key0), clear<L::kBytes>(key1), clear<L::kBytes>(val0), clear<L::kBytes>(val1);
+    }
+    const Bounds b = keys_of(a, i, lane);
+    const Walk walk(b);
+    const Bounds all = block_range(walk, shared, wave, lane);
+    const char* kbase = (const char*)((const T*)a.k + kh * a.k_head);
+    const char* vbase = (const char*)((const T*)a.v + kh * a.v_head);
+    const int krow = (int)a.k_row * (int)sizeof(T), vrow = (int)a.v_row * (int)sizeof(T);
+    const typename L::Places kplaces(krow, chunks, wave, lane), vplaces(vrow, chunks, wave, lane);
+    if (all.lo < all.hi) {
+        L::request(key0, kbase, krow, kplaces, all.lo, all.hi, chunks, wave);
+        L::request(val0, vbase, vrow, vplaces, all.lo, all.hi, chunks, wave);
+    }
     const bool mine = row < a.nq;
     typename L::frag q[L::kFrags], g[L::kFrags];
     load_row<T, L::kFrags>(q, (const char*)((const T*)a.q + i * a.q_row + h * a.q_head), chunks, half);
@@ -972,20 +986,6 @@ __global__ __launch_bounds__(256, (blocks_per_unit<T, DP>())) void query_gradien
         delta = sum_halves(delta);
     }
     if (mine && half == 0) a.delta[h * a.stat_stride + i] = delta;
-    if (chunks < L::kChunks) {
-        clear<L::kBytes>(key0), clear<L::kBytes>(key1), clear<L::kBytes>(val0), clear<L::kBytes>(val1);
-    }
-    const Bounds b = keys_of(a, i, lane);
-    const Walk walk(b);
-    const Bounds all = block_range(walk, shared, wave, lane);
-    const char* kbase = (const char*)((const T*)a.k + kh * a.k_head);
-    const char* vbase = (const char*)((const T*)a.v + kh * a.v_head);
-    const int krow = (int)a.k_row * (int)sizeof(T), vrow = (int)a.v_row * (int)sizeof(T);
-    const typename L::Places kplaces(krow, chunks, wave, lane), vplaces(vrow, chunks, wave, lane);
-    if (all.lo < all.hi) {
-        L::request(key0, kbase, krow, kplaces, all.lo, all.hi, chunks, wave);
-        L::request(val0, vbase, vrow, vplaces, all.lo, all.hi, chunks, wave);
-    }
     const float lse = a.lse[h * a.stat_stride + i], c = a.scale_log2;
     settle();
     float16_t acc[DT];
@@ -1054,9 +1054,10 @@ __global__ __launch_bounds__(256, (blocks_per_unit<T, DP>())) void query_gradien
 // decide: a training step on 9 packed sequences took 696 us here, not 480.) At a head of 128 a lane holds 128 sums and 64
 // elements of its key and value, so there is one wave to a SIMD and nothing else runs while it waits: reads from LDS go
 // ahead of their products in batches, with a fence behind each. (Left to itself the compiler puts every read right before
-// its product, and the wave waited for 45 % of its clocks.)
-template <typename T, int DP>
-__global__ __launch_bounds__(256, (key_blocks_per_unit<T, DP>())) void key_gradient(Args a) {
+// its product, and the wave waited for 45 % of its clocks.) WHAT: 1 the keys' gradient, 2 the values', 3 both.
+template <typename T, int DP, int WHAT>
+__global__ __launch_bounds__(256, (key_blocks_per_unit<T, DP, WHAT>())) void key_gradient(Args a) {
+    constexpr bool DK = WHAT & 1, DV = WHAT & 2;
     constexpr int BQ = 64, DT = DP / 32, PF = sizeof(T) == 2 ? 2 : 4;
     typedef Tile<T, DP, BQ> L;
     __shared__ __align__(1024) char que0[L::kBytes], que1[L::kBytes];
@@ -1072,7 +1073,7 @@ __global__ __launch_bounds__(256, (key_blocks_per_unit<T, DP>())) void key_gradi
     const int row = (tile * 2 + keys) * 32 + (lane & 31), j = min(row, a.nk - 1);
     typename L::frag k[L::kFrags], v[L::kFrags];
     load_row<T, L::kFrags>(k, (const char*)((const T*)a.k + j * a.k_row + kh * a.k_head), chunks, half);
-    load_row<T, L::kFrags>(v, (const char*)((const T*)a.v + j * a.v_row + kh * a.v_head), chunks, half);
+    if (DK) load_row<T, L::kFrags>(v, (const char*)((const T*)a.v + j * a.v_row + kh * a.v_head), chunks, half);
     if (chunks < L::kChunks) {
         clear<L::kBytes>(que0), clear<L::kBytes>(que1), clear<L::kBytes>(gra0), clear<L::kBytes>(gra1);
     }
@@ -1115,7 +1116,7 @@ __global__ __launch_bounds__(256, (key_blocks_per_unit<T, DP>())) void key_gradi
             for (int e = 0; e < 4; ++e) {
                 const int r = 4 * g + e;
                 s[r] = raised<T, Types<T>::kP>(fmaf(s[r], c, -lse[e]));
-                x[r] = s[r] * fmaf(x[r], kRatio, -delta[e] * kRatio);
+                if (DK) x[r] = s[r] * fmaf(x[r], kRatio, -delta[e] * kRatio);
             }
         }
     };
@@ -1137,7 +1138,7 @@ __global__ __launch_bounds__(256, (key_blocks_per_unit<T, DP>())) void key_gradi
         if (first < all.lo) first = top;
         if (kSparse<T, DP> && !walk.needs(now + r0, 32)) return;
         float16_t s = 0.0f, x = 0.0f;
-        if constexpr (kFenced<T, DP>) {
+        if constexpr (kFenced<T, DP> && WHAT == 3) {
             typename L::frag rows[2][8], columns[2][2 * DT];
             auto load_rows = [&](int n) {
 #pragma unroll
@@ -1177,25 +1178,25 @@ __global__ __launch_bounds__(256, (key_blocks_per_unit<T, DP>())) void key_gradi
                 }
             }
         } else {
-            // (512-byte rows: with all reads ahead of all products the 512 registers do not do)
-            const auto fence = [](int f) {
-                if (L::kFrags > 8 && f % 4 == 3) __builtin_amdgcn_sched_barrier(0);
-            };
 #pragma unroll
-            for (int f = 0; f < L::kFrags; ++f) s = mma(L::row(qt, r0 + (lane & 31), f, half), k[f], s), fence(f);
+            for (int f = 0; f < L::kFrags; ++f) s = mma(L::row(qt, r0 + (lane & 31), f, half), k[f], s);
 #pragma unroll
-            for (int f = 0; f < L::kFrags; ++f) x = mma(L::row(gt, r0 + (lane & 31), f, half), v[f], x), fence(f);
+            for (int f = 0; f < L::kFrags; ++f)
+                if (DK) x = mma(L::row(gt, r0 + (lane & 31), f, half), v[f], x);
             weigh(s, x, st);
             hide(s, x, now);
 #pragma unroll
             for (int f = 0; f < PF; ++f) {
-                fence(3);
-                const auto p = operand<T>(s, f);
+                if (DV) {
+                    const auto p = operand<T>(s, f);
 #pragma unroll
-                for (int t = 0; t < DT; ++t) dv[t] = mma(column_of<T, DP, BQ>(gt, r0, f, t, lane), p, dv[t]);
-                const auto d = operand<T>(x, f);
+                    for (int t = 0; t < DT; ++t) dv[t] = mma(column_of<T, DP, BQ>(gt, r0, f, t, lane), p, dv[t]);
+                }
+                if (DK) {
+                    const auto d = operand<T>(x, f);
 #pragma unroll
-                for (int t = 0; t < DT; ++t) dk[t] = mma(column_of<T, DP, BQ>(qt, r0, f, t, lane), d, dk[t]);
+                    for (int t = 0; t < DT; ++t) dk[t] = mma(column_of<T, DP, BQ>(qt, r0, f, t, lane), d, dk[t]);
+                }
             }
         }
     };
@@ -1205,7 +1206,7 @@ __global__ __launch_bounds__(256, (key_blocks_per_unit<T, DP>())) void key_gradi
     }
     // the second halves of the rows add to the first, 32 columns of the head at a time
 #pragma unroll
-    for (int t = 0; t < 2 * DT; ++t) {
+    for (int t = DK ? 0 : DT; t < (DV ? 2 * DT : DT); ++t) {
         float16_t& x = t < DT ? dk[t] : dv[t - DT];
         __syncthreads();
         if (r0)
@@ -1222,10 +1223,10 @@ __global__ __launch_bounds__(256, (key_blocks_per_unit<T, DP>())) void key_gradi
     const bool mine = row < a.nk;
     if (mine) {
         const int64_t at = ((int64_t)j * a.hk + kh) * a.d;
-        store_row<T, DT>((T*)a.dk + at, dk, c * (0.6931471805599453f * power<-Types<T>::kDs>), a.d, half);
-        store_row<T, DT>((T*)a.dv + at, dv, power<-Types<T>::kP>, a.d, half);
+        if (DK) store_row<T, DT>((T*)a.dk + at, dk, c * (0.6931471805599453f * power<-Types<T>::kDs>), a.d, half);
+        if (DV) store_row<T, DT>((T*)a.dv + at, dv, power<-Types<T>::kP>, a.d, half);
     }
-    uint64_t bad = __ballot(mine && !(all_finite<DT>(dk) && all_finite<DT>(dv)));
+    uint64_t bad = __ballot(mine && !((!DK || all_finite<DT>(dk)) && (!DV || all_finite<DT>(dv))));
     bad = (bad | bad >> 32) & 0xffffffffu;
     while (bad) {
         const int at = __builtin_ctzll(bad);

@@ -23,7 +23,18 @@ struct Kernels {
         if (a.tiles) query_gradient<T, DP><<<(unsigned)(a.tiles * a.hq), 256, 0, stream>>>(a);
         Args b = a;
         b.tiles = key_tiles;
-        if (key_tiles) key_gradient<T, DP><<<(unsigned)(key_tiles * a.hk), 256, 0, stream>>>(b);
+        const unsigned blocks = (unsigned)(key_tiles * a.hk);
+        if (!blocks) return hipGetLastError();
+        if constexpr (sizeof(T) * DP > 256) {
+            // Sums of values' and keys' gradients together do not fit the registers beside rows of 512 bytes (580 bytes of
+            // scratch memory a lane): one after the other, with the scores computed twice. 8 segments of 1 000 rows, 8 / 2
+            // heads of 128, causal: gradients 1 893 us together, 1 183 apart; elsewhere together is faster (heads of 64: 737
+            // and 859, bf16 of 128 in 9 packed sequences: 393 and 580).
+            key_gradient<T, DP, 2><<<blocks, 256, 0, stream>>>(b);
+            key_gradient<T, DP, 1><<<blocks, 256, 0, stream>>>(b);
+        } else {
+            key_gradient<T, DP, 3><<<blocks, 256, 0, stream>>>(b);
+        }
         return hipGetLastError();
     }
 };
