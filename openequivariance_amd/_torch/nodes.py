@@ -130,6 +130,13 @@ def rotary_table(length: int, rotary_dim: int, *, base: float = 10000.0, scaling
     return torch.stack([angle.cos(), angle.sin()], dim=1).float()
 
 
+def _weights(q, *weights):
+    """Weights of a norm in the queries' type: under autocast projections come in 16 bits and parameters in 32."""
+    if torch.is_autocast_enabled("cuda"):
+        return [w if w is None else w.to(q.dtype) for w in weights]
+    return weights
+
+
 def qk_norm_rotary(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, table: torch.Tensor,
                    q_weight: Optional[torch.Tensor] = None, k_weight: Optional[torch.Tensor] = None, *, eps: float = 1e-6,
                    interleaved: bool = False) -> Tuple[torch.Tensor, torch.Tensor]:
@@ -143,6 +150,7 @@ def qk_norm_rotary(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, ta
     :param q_weight, k_weight: ``[head_dim]``: ``x -> weight x / sqrt(mean(x^2) + eps)``; no norm where left out.
     :param interleaved: pairs are neighbours ``2 i, 2 i + 1`` instead of ``i, i + rotary_dim / 2``.
     """
+    q_weight, k_weight = _weights(q, q_weight, k_weight)
     return _qk_norm_rotary(q, k, positions, table, q_weight, k_weight, eps, interleaved)
 
 
@@ -157,6 +165,7 @@ def qk_norm_rotary_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, pos
     :param slots: ``[rows]``, int64; rows whose slot is not one of the caches' (-1, say) are not written. Slots are
         different from each other.
     """
+    q_weight, k_weight = _weights(q, q_weight, k_weight)
     return _qk_norm_rotary_append(q, k, v, positions, table, k_cache, v_cache, slots, q_weight, k_weight, eps, interleaved)
 
 
@@ -206,4 +215,6 @@ class IrrepDropout(torch.nn.Module):
             channels = channels.to(x.device)
             if not torch.compiler.is_compiling():
                 self.channels = channels
+        if residual is not None and torch.is_autocast_enabled("cuda"):
+            x = x.to(residual.dtype)  # (a projection in 16 bits on its way into a stream in 32)
         return _irrep_dropout(x, residual, channels, seed, self.p)

@@ -572,3 +572,18 @@ def test_compiled_calls_keep_their_results():
         if f is layer:
             want = out, grad
     assert torch.equal(out, want[0]) and torch.equal(grad, want[1])
+
+
+def test_autocast():
+    """Projections in 16 bits beside parameters and a residual stream in 32."""
+    n, ptr, positions = 40, on_gpu([0, 15, 40]), torch.arange(40, device="cuda")
+    linear = torch.nn.Linear(64, 3 * 64, bias=False).cuda()
+    w, table = torch.ones(32, device="cuda", requires_grad=True), oeq.rotary_table(40, 32, device="cuda")
+    x, dropout = normal(n, 64), oeq.IrrepDropout("64x0e", 0.1).cuda()
+    with torch.autocast("cuda", dtype=BF16):
+        q, k, v = (t.view(n, 2, 32) for t in linear(x).split(64, 1))
+        q, k = oeq.qk_norm_rotary(q, k, positions, table, w, w)
+        out = dropout(oeq.packed_attention(q, k, v, ptr).flatten(1), x)
+    assert q.dtype == BF16 and out.dtype == F32
+    out.sum().backward()
+    assert w.grad.dtype == F32 and linear.weight.grad.dtype == F32 and torch.isfinite(linear.weight.grad).all()
