@@ -23,6 +23,9 @@ int element_bytes(int type) {
 bool aligned(const void* p) { return ((uintptr_t)p & 15) == 0; }
 bool aligned(int64_t stride, int type) { return stride * element_bytes(type) % 16 == 0; }
 
+// Blocks of 256 threads in a launch: threads are counted in 32 bits.
+constexpr int64_t kMostBlocks = (1 << 24) - 1;
+
 // A tile's rows are addressed by 32-bit offsets from its first.
 constexpr int64_t kMostRowBytes = (int64_t)INT_MAX / 64 - 1024;
 
@@ -34,6 +37,8 @@ int check_attention(const char* who, const oeq_attention* a) {
                     (long long)a->q_rows, (long long)a->k_rows);
     if (a->k_heads <= 0 || a->q_heads <= 0 || a->q_heads % a->k_heads)
         return fail(OEQ_ERR_INVALID, "%s: %d query heads for %d key heads", who, a->q_heads, a->k_heads);
+    if ((a->q_rows + 63) / 64 > kMostBlocks / a->q_heads || (a->k_rows + 63) / 64 > kMostBlocks / a->k_heads)
+        return fail(OEQ_ERR_INVALID, "%s: %lld query rows, %lld key rows", who, (long long)a->q_rows, (long long)a->k_rows);
     if (a->head_dim <= 0 || a->head_dim > 128 || a->head_dim % 8)
         return fail(OEQ_ERR_INVALID, "%s: heads of %d elements (multiples of 8 up to 128)", who, a->head_dim);
     if (!(a->scale > 0) || !std::isfinite(a->scale)) return fail(OEQ_ERR_INVALID, "%s: scale %g", who, a->scale);
@@ -62,7 +67,12 @@ packed_attention::Args attention_args(const oeq_attention& a) {
     g.stat_stride = oeq_attention_stat_stride(a.q_rows);
     g.segments = a.segments, g.nq = (int)a.q_rows, g.nk = (int)a.k_rows;
     g.hq = a.q_heads, g.hk = a.k_heads, g.d = a.head_dim, g.causal = a.causal != 0;
-    g.tiles = (int)query_tiles(a);
+    // Below two blocks a compute unit a block has half as many rows, each shared by two waves that take every other group of
+    // 32 keys. Forward, us, shared / not: 64 blocks of 128 rows, bf16 heads of 128 18 / 24, 150, fp16 of 72 25 / 33, 376, bf16 of 64
+    // 29 / 35, 504, float32 of 128 240 / 296, 512, bf16 of 128 41 / 40, 1 008 80 / 60.
+    g.split = query_tiles(a) * a.q_heads < 512 ? 2 : 1;
+    const int rows = packed_attention::kQueryTile / g.split;
+    g.tiles = (int)((a.q_rows + rows - 1) / rows);
     g.scale_log2 = a.scale * 1.4426950408889634f;
     return g;
 }
@@ -157,7 +167,7 @@ void by_lanes(const qk_rotary::Args& g, F launch) {
 
 template <bool APPEND>
 int launch_rotary(int type, const qk_rotary::Args& g, hipStream_t stream) {
-    const unsigned blocks = (unsigned)rotary_blocks(g);
+    const unsigned blocks = (unsigned)std::min<int64_t>(rotary_blocks(g), kMostBlocks);  // (the blocks walk the rest)
     by_lanes(g, [&](auto lanes) {
         constexpr int kLanes = decltype(lanes)::value;
         if (type == OEQ_FLOAT32)

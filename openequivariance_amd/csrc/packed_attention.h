@@ -19,7 +19,8 @@
 // another lane's p. V^T comes from LDS through the transposing reads (16 bit) or four-byte reads (32 bit).
 // dQ^T = K^T dS^T works the same way, and so do dV^T = G^T P and dK^T = Q^T dS with the keys in the lanes.
 //
-// Rows are packed without regard to segments: a block takes 128 consecutive rows, reads the keys from the first that its
+// Rows are packed without regard to segments: a block takes 128 consecutive rows (64 where there are few blocks, SPLIT: two
+// waves to 32 rows, with every other group of 32 keys each), reads the keys from the first that its
 // first row sees to the last that its last row sees, and masks by each row's own bounds. Small segments (molecules)
 // share a tile that way instead of leaving most of it idle: 512 molecules of 9 to 61 atoms fill 110 tiles.
 //
@@ -45,7 +46,7 @@ struct Args {
     float *lse, *delta;
     const int64_t *q_ptr, *k_ptr, *k_len;
     int64_t q_row, q_head, k_row, k_head, v_row, v_head, g_row, g_head, stat_stride;
-    int segments, nq, nk, hq, hk, d, causal, tiles;
+    int segments, nq, nk, hq, hk, d, causal, tiles, split;
     float scale_log2;  // c * log2(e): the kernels work with powers of two
     const int *q_order, *k_order;  // tiles by the length of their walks, or NULL
     int parts;  // the form for few queries: shares of a row's keys, and their results
@@ -574,18 +575,21 @@ __device__ __forceinline__ bool all_finite(const float16_t (&acc)[DT]) {
 // forward
 // ---------------------------------------------------------------------------
 
-template <typename T, int DP>
+template <typename T, int DP, int SPLIT>
 __global__ __launch_bounds__(256, (blocks_per_unit<T, DP>())) void forward(Args a) {
-    constexpr int BK = tile_rows<T, DP>(), SUB = kSparse<T, DP> ? 1 : BK / 32, DT = DP / 32;
+    constexpr int BK = SPLIT == 2 ? 64 : tile_rows<T, DP>(), SUB = SPLIT == 2 || kSparse<T, DP> ? 1 : BK / 32, DT = DP / 32;
     constexpr int PF = sizeof(T) == 2 ? 2 : 4;  // fragments of 32 keys
     typedef Tile<T, DP, BK> L;
     __shared__ __align__(1024) char key0[L::kBytes], key1[L::kBytes], val0[L::kBytes], val1[L::kBytes];
     __shared__ int shared[8];
+    __shared__ __align__(16) float4_t swap[SPLIT == 2 ? 512 : 1];
+    __shared__ float swap_m[SPLIT == 2 ? 64 : 1], swap_l[SPLIT == 2 ? 64 : 1];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5;
     int tile, h;
     place(a, a.hq, a.q_order, a.causal, tile, h);
     const int kh = h / (a.hq / a.hk), chunks = a.d * (int)sizeof(T) / 16;
-    const int row = (tile * 4 + wave) * 32 + (lane & 31), i = min(row, a.nq - 1);
+    const int rows = wave % (4 / SPLIT), part = wave / (4 / SPLIT);  // which 32 rows, and which of the groups of keys
+    const int row = (tile * (4 / SPLIT) + rows) * 32 + (lane & 31), i = min(row, a.nq - 1);
     typename L::frag q[L::kFrags];
     load_row<T, L::kFrags>(q, (const char*)((const T*)a.q + i * a.q_row + h * a.q_head), chunks, half);
     if (chunks < L::kChunks) {
@@ -659,9 +663,13 @@ __global__ __launch_bounds__(256, (blocks_per_unit<T, DP>())) void forward(Args 
             L::request(kn, kbase, krow, kplaces, first + BK, all.hi, chunks, wave);
             L::request(vn, vbase, vrow, vplaces, first + BK, all.hi, chunks, wave);
         }
+        if constexpr (SPLIT == 2) {
+            if (walk.needs(first + 32 * part, 32)) products(kt, vt, first, 32 * part);
+        } else {
 #pragma unroll
-        for (int r0 = 0; r0 < BK; r0 += 32 * SUB)
-            if (walk.needs(first + r0, 32 * SUB)) products(kt, vt, first, r0);
+            for (int r0 = 0; r0 < BK; r0 += 32 * SUB)
+                if (walk.needs(first + r0, 32 * SUB)) products(kt, vt, first, r0);
+        }
     };
     if (all.lo < all.hi) {
         L::request(key0, kbase, krow, kplaces, all.lo, all.hi, chunks, wave);
@@ -672,6 +680,31 @@ __global__ __launch_bounds__(256, (blocks_per_unit<T, DP>())) void forward(Args 
         if (first + BK < all.hi) step(key1, val1, key0, val0, first + BK);
     }
     l = sum_halves(l);
+    if constexpr (SPLIT == 2) {
+        // the wave with the second groups of keys hands its sums to the one with the first, 32 columns of the head at a time
+        if (part && half == 0) swap_m[32 * rows + lane] = m, swap_l[32 * rows + lane] = l;
+        __syncthreads();
+        const float other = swap_m[32 * rows + (lane & 31)], top = fmaxf(m, other);
+        const float by = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((m - top) * c);
+        const float others = other == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((other - top) * c);
+        if (!part) l = l * by + swap_l[32 * rows + (lane & 31)] * others, m = top;
+#pragma unroll
+        for (int t = 0; t < DT; ++t) {
+            if (part)
+#pragma unroll
+                for (int g = 0; g < 4; ++g)
+                    swap[(rows * 4 + g) * 64 + lane] = float4_t{acc[t][4 * g], acc[t][4 * g + 1], acc[t][4 * g + 2], acc[t][4 * g + 3]};
+            __syncthreads();
+            if (!part)
+#pragma unroll
+                for (int g = 0; g < 4; ++g)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        acc[t][4 * g + e] = acc[t][4 * g + e] * by + swap[(rows * 4 + g) * 64 + lane][e] * others;
+            __syncthreads();
+        }
+        if (part) return;
+    }
     const bool seen = b.lo < b.hi, mine = row < a.nq;
     const float by = seen ? 1.0f / l : 0.0f;
     if (mine) {
@@ -684,7 +717,7 @@ __global__ __launch_bounds__(256, (blocks_per_unit<T, DP>())) void forward(Args 
     while (bad) {
         const int at = __builtin_ctzll(bad);
         bad &= bad - 1;
-        forward_row<T>(a, (tile * 4 + wave) * 32 + at, h, __shfl(b.lo, at), __shfl(b.hi, at), lane);
+        forward_row<T>(a, (tile * (4 / SPLIT) + rows) * 32 + at, h, __shfl(b.lo, at), __shfl(b.hi, at), lane);
     }
 }
 
@@ -939,18 +972,20 @@ __global__ __launch_bounds__(256) void join(Args a) {
 // gradient of the queries; delta on the way
 // ---------------------------------------------------------------------------
 
-template <typename T, int DP>
+template <typename T, int DP, int SPLIT>
 __global__ __launch_bounds__(256, (blocks_per_unit<T, DP>())) void query_gradient(Args a) {
-    constexpr int BK = tile_rows<T, DP>(), SUB = BK / 32, DT = DP / 32;
+    constexpr int BK = SPLIT == 2 ? 64 : tile_rows<T, DP>(), SUB = SPLIT == 2 ? 1 : BK / 32, DT = DP / 32;
     constexpr int PF = sizeof(T) == 2 ? 2 : 4;
     typedef Tile<T, DP, BK> L;
     __shared__ __align__(1024) char key0[L::kBytes], key1[L::kBytes], val0[L::kBytes], val1[L::kBytes];
     __shared__ int shared[8];
+    __shared__ __align__(16) float4_t swap[SPLIT == 2 ? 512 : 1];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5;
     int tile, h;
     place(a, a.hq, a.q_order, a.causal, tile, h);
     const int kh = h / (a.hq / a.hk), chunks = a.d * (int)sizeof(T) / 16;
-    const int row = (tile * 4 + wave) * 32 + (lane & 31), i = min(row, a.nq - 1);
+    const int rows = wave % (4 / SPLIT), part = wave / (4 / SPLIT);  // which 32 rows, and which of the groups of keys
+    const int row = (tile * (4 / SPLIT) + rows) * 32 + (lane & 31), i = min(row, a.nq - 1);
     if (chunks < L::kChunks) {
         clear<L::kBytes>(key0), clear<L::kBytes>(key1), clear<L::kBytes>(val0), clear<L::kBytes>(val1);
     }
@@ -994,8 +1029,9 @@ __global__ __launch_bounds__(256, (blocks_per_unit<T, DP>())) void query_gradien
 
     auto products = [&](const char* kt, const char* vt, int first) {
 #pragma unroll
-        for (int u = 0; u < SUB; ++u) {
-            if (kSparse<T, DP> && !walk.needs(first + 32 * u, 32)) continue;
+        for (int n = 0; n < SUB; ++n) {
+            const int u = SPLIT == 2 ? part : n;
+            if ((SPLIT == 2 || kSparse<T, DP>) && !walk.needs(first + 32 * u, 32)) continue;
             float16_t s = 0.0f, x = 0.0f;
 #pragma unroll
             for (int f = 0; f < L::kFrags; ++f) s = mma(L::row(kt, 32 * u + (lane & 31), f, half), q[f], s);
@@ -1006,7 +1042,7 @@ __global__ __launch_bounds__(256, (blocks_per_unit<T, DP>())) void query_gradien
                 const float p = raised<T, Types<T>::kDs>(fmaf(s[r], c, -lse));
                 x[r] = p * (x[r] - delta);
             }
-            if (!(kSparse<T, DP> ? walk.whole(first + 32 * u, 32) : walk.whole(first, BK))) {
+            if (!(SPLIT == 2 || kSparse<T, DP> ? walk.whole(first + 32 * u, 32) : walk.whole(first, BK))) {
                 const int shift = first + 32 * u + 4 * half - b.lo;
                 const unsigned n = b.hi - b.lo;
 #pragma unroll
@@ -1034,6 +1070,24 @@ __global__ __launch_bounds__(256, (blocks_per_unit<T, DP>())) void query_gradien
         step(key0, val0, key1, val1, first);
         if (first + BK < all.hi) step(key1, val1, key0, val0, first + BK);
     }
+    if constexpr (SPLIT == 2) {
+        // the wave with the second groups of keys hands its sums to the one with the first, 32 columns of the head at a time
+#pragma unroll
+        for (int t = 0; t < DT; ++t) {
+            __syncthreads();
+            if (part)
+#pragma unroll
+                for (int g = 0; g < 4; ++g)
+                    swap[(rows * 4 + g) * 64 + lane] = float4_t{acc[t][4 * g], acc[t][4 * g + 1], acc[t][4 * g + 2], acc[t][4 * g + 3]};
+            __syncthreads();
+            if (!part)
+#pragma unroll
+                for (int g = 0; g < 4; ++g)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) acc[t][4 * g + e] += swap[(rows * 4 + g) * 64 + lane][e];
+        }
+        if (part) return;
+    }
     if (mine)
         store_row<T, DT>((T*)a.dq + ((int64_t)i * a.hq + h) * a.d, acc, c * (0.6931471805599453f * power<-Types<T>::kDs>), a.d, half);
     uint64_t bad = __ballot(mine && !all_finite<DT>(acc));
@@ -1041,7 +1095,7 @@ __global__ __launch_bounds__(256, (blocks_per_unit<T, DP>())) void query_gradien
     while (bad) {
         const int at = __builtin_ctzll(bad);
         bad &= bad - 1;
-        query_gradient_row<T>(a, (tile * 4 + wave) * 32 + at, h, __shfl(b.lo, at), __shfl(b.hi, at), lane);
+        query_gradient_row<T>(a, (tile * (4 / SPLIT) + rows) * 32 + at, h, __shfl(b.lo, at), __shfl(b.hi, at), lane);
     }
 }
 
@@ -1049,28 +1103,29 @@ __global__ __launch_bounds__(256, (blocks_per_unit<T, DP>())) void query_gradien
 // gradients of keys and values
 // ---------------------------------------------------------------------------
 
-// A block has 64 keys in two pairs of waves; of a tile of 64 query rows one wave of a pair takes the first half, the other
-// the second, and at the end they add up. (With 128 keys a block, one wave for both halves, long walks of few blocks
-// decide: a training step on 9 packed sequences took 696 us here, not 480.) At a head of 128 a lane holds 128 sums and 64
+// A block has 64 keys (KEYS = 2 waves' worth) and walks tiles of 64 query rows: of 32 keys one wave takes a tile's first
+// half, another the second, and at the end they add up. (With 128 keys a block, one wave for both halves, long walks of
+// few blocks decide: a training step on 9 packed sequences took 696 us here, not 480.) Where blocks are too few for the
+// compute units they have 32 keys and walk tiles of 128 rows, a wave for each quarter. At a head of 128 a lane holds 128 sums and 64
 // elements of its key and value, so there is one wave to a SIMD and nothing else runs while it waits: reads from LDS go
 // ahead of their products in batches, with a fence behind each. (Left to itself the compiler puts every read right before
 // its product, and the wave waited for 45 % of its clocks.) WHAT: 1 the keys' gradient, 2 the values', 3 both.
-template <typename T, int DP, int WHAT>
+template <typename T, int DP, int WHAT, int KEYS>
 __global__ __launch_bounds__(256, (key_blocks_per_unit<T, DP, WHAT>())) void key_gradient(Args a) {
     constexpr bool DK = WHAT & 1, DV = WHAT & 2;
-    constexpr int BQ = 64, DT = DP / 32, PF = sizeof(T) == 2 ? 2 : 4;
+    constexpr int GROUPS = 4 / KEYS, BQ = 32 * GROUPS, DT = DP / 32, PF = sizeof(T) == 2 ? 2 : 4;
     typedef Tile<T, DP, BQ> L;
     __shared__ __align__(1024) char que0[L::kBytes], que1[L::kBytes];
     __shared__ __align__(1024) char gra0[L::kBytes], gra1[L::kBytes];
-    __shared__ __align__(1024) float sta0[128], sta1[128];  // lse, then delta, of the tile's rows
-    __shared__ __align__(16) float4_t swap[2][4][64];
+    __shared__ __align__(1024) float sta0[2 * BQ], sta1[2 * BQ];  // lse, then delta, of the tile's rows
+    __shared__ __align__(16) float4_t swap[4 - KEYS][4][64];
     __shared__ int shared[8];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5;
-    const int keys = wave & 1, r0 = 32 * (wave >> 1);  // which 32 keys, and the first row of the wave's half of a tile
+    const int keys = wave % KEYS, r0 = 32 * (wave / KEYS);  // which 32 keys, and the wave's first row of a tile
     int tile, kh;
     place(a, a.hk, a.k_order, false, tile, kh);  // (causal: the first keys have the longest walks)
     const int group = a.hq / a.hk, chunks = a.d * (int)sizeof(T) / 16;
-    const int row = (tile * 2 + keys) * 32 + (lane & 31), j = min(row, a.nk - 1);
+    const int row = (tile * KEYS + keys) * 32 + (lane & 31), j = min(row, a.nk - 1);
     typename L::frag k[L::kFrags], v[L::kFrags];
     load_row<T, L::kFrags>(k, (const char*)((const T*)a.k + j * a.k_row + kh * a.k_head), chunks, half);
     if (DK) load_row<T, L::kFrags>(v, (const char*)((const T*)a.v + j * a.v_row + kh * a.v_head), chunks, half);
@@ -1091,10 +1146,11 @@ __global__ __launch_bounds__(256, (key_blocks_per_unit<T, DP, WHAT>())) void key
         if (next_h == last_head) return;
         L::request(qt, (const char*)((const T*)a.q + next_h * a.q_head), qrow, qplaces, next_first, all.hi, chunks, wave);
         L::request(gt, (const char*)((const T*)a.grad + next_h * a.g_head), grow, gplaces, next_first, all.hi, chunks, wave);
-        // (a row of statistics is longer than the queries by more than a tile)
-        if (wave < 2)
-            __builtin_amdgcn_global_load_lds((gptr_t)((wave ? a.delta : a.lse) + next_h * a.stat_stride + next_first + lane),
-                                             (lptr_t)(st + 64 * wave), 4, 0, 0);
+        if (wave < BQ / 32) {
+            const int64_t at = min((int64_t)(next_first + 64 * (wave >> 1) + lane), a.stat_stride - 1);
+            __builtin_amdgcn_global_load_lds((gptr_t)((wave & 1 ? a.delta : a.lse) + next_h * a.stat_stride + at),
+                                             (lptr_t)(st + BQ * (wave & 1) + 64 * (wave >> 1)), 4, 0, 0);
+        }
         next_first -= BQ;
         if (next_first < all.lo) next_first = top, ++next_h;
     };
@@ -1111,7 +1167,7 @@ __global__ __launch_bounds__(256, (key_blocks_per_unit<T, DP, WHAT>())) void key
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
             const float4_t lse = *(const float4_t*)(st + r0 + 8 * g + 4 * half);
-            const float4_t delta = *(const float4_t*)(st + 64 + r0 + 8 * g + 4 * half);
+            const float4_t delta = *(const float4_t*)(st + BQ + r0 + 8 * g + 4 * half);
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
                 const int r = 4 * g + e;
@@ -1204,20 +1260,23 @@ __global__ __launch_bounds__(256, (key_blocks_per_unit<T, DP, WHAT>())) void key
         step(que0, gra0, sta0, que1, gra1, sta1);
         if (n + 1 < steps) step(que1, gra1, sta1, que0, gra0, sta0);
     }
-    // the second halves of the rows add to the first, 32 columns of the head at a time
+    // the waves with a tile's later rows hand their sums to those with the first ones, 32 columns of the head at a time
 #pragma unroll
     for (int t = DK ? 0 : DT; t < (DV ? 2 * DT : DT); ++t) {
         float16_t& x = t < DT ? dk[t] : dv[t - DT];
         __syncthreads();
         if (r0)
 #pragma unroll
-            for (int g = 0; g < 4; ++g) swap[keys][g][lane] = float4_t{x[4 * g], x[4 * g + 1], x[4 * g + 2], x[4 * g + 3]};
+            for (int g = 0; g < 4; ++g)
+                swap[wave - KEYS][g][lane] = float4_t{x[4 * g], x[4 * g + 1], x[4 * g + 2], x[4 * g + 3]};
         __syncthreads();
         if (!r0)
 #pragma unroll
-            for (int g = 0; g < 4; ++g)
+            for (int n = 0; n < GROUPS - 1; ++n)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) x[4 * g + e] += swap[keys][g][lane][e];
+                for (int g = 0; g < 4; ++g)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) x[4 * g + e] += swap[n * KEYS + keys][g][lane][e];
     }
     if (r0) return;
     const bool mine = row < a.nk;
@@ -1231,7 +1290,7 @@ __global__ __launch_bounds__(256, (key_blocks_per_unit<T, DP, WHAT>())) void key
     while (bad) {
         const int at = __builtin_ctzll(bad);
         bad &= bad - 1;
-        key_gradient_row<T>(a, (tile * 2 + keys) * 32 + at, kh, __shfl(b.lo, at), __shfl(b.hi, at), lane);
+        key_gradient_row<T>(a, (tile * KEYS + keys) * 32 + at, kh, __shfl(b.lo, at), __shfl(b.hi, at), lane);
     }
 }
 

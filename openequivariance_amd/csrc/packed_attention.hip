@@ -10,7 +10,10 @@ template <int DP>
 struct Kernels {
     typedef OEQ_ATTENTION_TYPE T;
     static hipError_t forward_rows(const Args& a, hipStream_t stream) {
-        forward<T, DP><<<(unsigned)(a.tiles * a.hq), 256, 0, stream>>>(a);
+        if (a.split == 2)
+            forward<T, DP, 2><<<(unsigned)(a.tiles * a.hq), 256, 0, stream>>>(a);
+        else
+            forward<T, DP, 1><<<(unsigned)(a.tiles * a.hq), 256, 0, stream>>>(a);
         return hipGetLastError();
     }
     static hipError_t forward_shares(const Args& a, hipStream_t stream) {
@@ -20,7 +23,10 @@ struct Kernels {
         return hipGetLastError();
     }
     static hipError_t gradients(const Args& a, int key_tiles, hipStream_t stream) {
-        if (a.tiles) query_gradient<T, DP><<<(unsigned)(a.tiles * a.hq), 256, 0, stream>>>(a);
+        if (a.tiles && a.split == 2)
+            query_gradient<T, DP, 2><<<(unsigned)(a.tiles * a.hq), 256, 0, stream>>>(a);
+        else if (a.tiles)
+            query_gradient<T, DP, 1><<<(unsigned)(a.tiles * a.hq), 256, 0, stream>>>(a);
         Args b = a;
         b.tiles = key_tiles;
         const unsigned blocks = (unsigned)(key_tiles * a.hk);
@@ -30,10 +36,16 @@ struct Kernels {
             // scratch memory a lane): one after the other, with the scores computed twice. 8 segments of 1 000 rows, 8 / 2
             // heads of 128, causal: gradients 1 893 us together, 1 183 apart; elsewhere together is faster (heads of 64: 737
             // and 859, bf16 of 128 in 9 packed sequences: 393 and 580).
-            key_gradient<T, DP, 2><<<blocks, 256, 0, stream>>>(b);
-            key_gradient<T, DP, 1><<<blocks, 256, 0, stream>>>(b);
+            key_gradient<T, DP, 2, 2><<<blocks, 256, 0, stream>>>(b);
+            key_gradient<T, DP, 1, 2><<<blocks, 256, 0, stream>>>(b);
+        } else if (blocks < 256) {
+            // Fewer blocks than compute units: half as many keys to a block and half as long a walk. Gradients together, us, with
+            // 64 / 32 keys: 56 blocks, float32 heads of 64 226 / 145; 112, fp16 of 72 121 / 74; 126, float32 of 64 416 / 268; 252, bf16
+            // of 128 159 / 161; 504 217 / 278. All of them run at once, so they need no order (which is of tiles of 64 keys).
+            b.tiles = (a.nk + 31) / 32, b.k_order = nullptr;
+            key_gradient<T, DP, 3, 1><<<(unsigned)(b.tiles * a.hk), 256, 0, stream>>>(b);
         } else {
-            key_gradient<T, DP, 3><<<blocks, 256, 0, stream>>>(b);
+            key_gradient<T, DP, 3, 2><<<blocks, 256, 0, stream>>>(b);
         }
         return hipGetLastError();
     }

@@ -189,22 +189,25 @@ __device__ __forceinline__ void heads_forward(const Args& g, const Place<LANES>&
 // have are left out.
 template <typename T, int LANES, bool APPEND>
 __global__ __launch_bounds__(256) void forward(Args g) {
-    const Place<LANES> at(g, (int64_t)blockIdx.x * (256 / (LANES * g.groups)));
-    const Where w(g, at.i);
-    const Angle angle(g, at.row, at.i, w.turned);
-    int64_t to = at.row;
-    bool live = at.live;
-    if (APPEND) {
-        to = g.slots[at.row];
-        live = live && to >= 0 && to < g.slots_end;
+    const int each = 256 / (LANES * g.groups);
+    for (int64_t top = (int64_t)blockIdx.x * each; top < g.rows; top += (int64_t)gridDim.x * each) {
+        const Place<LANES> at(g, top);
+        const Where w(g, at.i);
+        const Angle angle(g, at.row, at.i, w.turned);
+        int64_t to = at.row;
+        bool live = at.live;
+        if (APPEND) {
+            to = g.slots[at.row];
+            live = live && to >= 0 && to < g.slots_end;
+        }
+        heads_forward<T, LANES, true>(g, at, w, angle, (const T*)g.q + at.row * g.q_row, g.q_head,
+                                      (T*)g.q_out + at.row * g.q_heads * g.d, g.d, g.q_heads, (const T*)g.q_weight, at.live);
+        heads_forward<T, LANES, true>(g, at, w, angle, (const T*)g.k + at.row * g.k_row, g.k_head, (T*)g.k_out + to * g.ko_row,
+                                      g.ko_head, g.k_heads, (const T*)g.k_weight, live);
+        if (APPEND)
+            heads_forward<T, LANES, false>(g, at, w, angle, (const T*)g.v + at.row * g.v_row, g.v_head, (T*)g.v_out + to * g.vo_row,
+                                           g.vo_head, g.k_heads, nullptr, live);
     }
-    heads_forward<T, LANES, true>(g, at, w, angle, (const T*)g.q + at.row * g.q_row, g.q_head,
-                                  (T*)g.q_out + at.row * g.q_heads * g.d, g.d, g.q_heads, (const T*)g.q_weight, at.live);
-    heads_forward<T, LANES, true>(g, at, w, angle, (const T*)g.k + at.row * g.k_row, g.k_head, (T*)g.k_out + to * g.ko_row,
-                                  g.ko_head, g.k_heads, (const T*)g.k_weight, live);
-    if (APPEND)
-        heads_forward<T, LANES, false>(g, at, w, angle, (const T*)g.v + at.row * g.v_row, g.v_head, (T*)g.v_out + to * g.vo_row,
-                                       g.vo_head, g.k_heads, nullptr, live);
 }
 
 // The gradients of one kind of heads in a row: gradients turned back, gy; with n = x / rms, dx = (gy w - n mean(gy w n)) / rms

@@ -108,6 +108,13 @@ def test_attention_of_few_rows_with_few_or_uneven_segments():
     attention_case(F16, [1, 2], [40, 2000], None, 3, 2048, 16, 4, 96, False, gradients=False)
 
 
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+def test_attention_of_long_segments_with_one_key_head(dtype):
+    """Many tiles of queries, which are put in order, to few of keys, which are not."""
+    ptr = starts([900, 0, 700])
+    attention_case(dtype, ptr, ptr, None, ptr[-1], ptr[-1], 48, 1, 8, True)
+
+
 def test_large_scores():
     """Scores of some hundreds, where every row's weight is on a few keys, and one large common part."""
     ptr = starts([200, 31])
