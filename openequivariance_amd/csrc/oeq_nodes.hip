@@ -26,8 +26,8 @@ bool aligned(int64_t stride, int type) { return stride * element_bytes(type) % 1
 // Blocks of 256 threads in a launch: threads are counted in 32 bits.
 constexpr int64_t kMostBlocks = (1 << 24) - 1;
 
-// A tile's rows are addressed by 32-bit offsets from its first.
-constexpr int64_t kMostRowBytes = (int64_t)INT_MAX / 64 - 1024;
+// A tile's rows, up to 128, are addressed by 32-bit offsets from its first: 127 strides and a head stay below 2^31.
+constexpr int64_t kMostRowBytes = (1 << 24) - 1;
 
 int check_attention(const char* who, const oeq_attention* a) {
     if (!a) return fail(OEQ_ERR_INVALID, "%s: NULL description", who);

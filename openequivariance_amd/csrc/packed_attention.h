@@ -145,7 +145,8 @@ __device__ __forceinline__ bool finite(float x) { return fabsf(x) < INFINITY; }
 // tiles in LDS
 // ---------------------------------------------------------------------------
 
-// Rows of DP elements; 16-byte chunk c of row r lies at place c ^ swizzle(r) of the row. LDS has 64 banks, 256 bytes: a
+// Rows of DP elements (96: in places of 128, of which the products leave out the last quarter); 16-byte chunk c of row r
+// lies at place c ^ swizzle(r) of the row. LDS has 64 banks, 256 bytes: a
 // 16-byte read meets them with the same chunk of 16 consecutive rows, a transposing read with four neighbouring chunks of
 // four rows that begin at a multiple of four. Either way the 16 chunks have to lie in different places modulo 16, so the
 // rows that share 256 bytes need no swizzle among them, the next bits of the row choose among the groups of four chunks
@@ -153,10 +154,10 @@ __device__ __forceinline__ bool finite(float x) { return fabsf(x) < INFINITY; }
 // spent 59 % of its clocks in LDS on conflicts.)
 template <typename T, int DP, int ROWS, int WAVES = 4>
 struct Tile {
-    static constexpr int kRowBytes = DP * (int)sizeof(T);
+    static constexpr int kRowBytes = (DP == 96 ? 128 : DP) * (int)sizeof(T);
     static constexpr int kChunks = kRowBytes / 16;
     static constexpr int kBytes = ROWS * kRowBytes;
-    static constexpr int kFrags = kChunks / 2;
+    static constexpr int kFrags = DP * (int)sizeof(T) / 32;
     typedef typename Types<T>::frag frag;
 
     static __device__ __forceinline__ int swizzle(int r) {
@@ -193,7 +194,7 @@ struct Tile {
 #pragma unroll
         for (int i = 0; i < kEach; ++i)
             __builtin_amdgcn_raw_ptr_buffer_load_lds(from, (lptr_t)(lds + (i * WAVES + wave) * 1024), 16,
-                                                     places.at[i % kPlaces] + i / kPlaces * stride, 0, 0, 0);
+                                                     (int)((unsigned)places.at[i % kPlaces] + i / kPlaces * (unsigned)stride), 0, 0, 0);
     }
 
     // Fragment f of row r: elements (2 f + half) E ... of it.
@@ -452,10 +453,10 @@ template <typename T, int DP>
 constexpr int blocks_per_unit() { return sizeof(T) * DP > 256 ? 1 : 2; }
 
 template <typename T, int DP>
-constexpr bool kFenced = sizeof(T) == 2 && DP == 128;  // key_gradient: one wave to a SIMD, see there
+constexpr bool kFenced = sizeof(T) == 2 && DP >= 96;  // key_gradient: one wave to a SIMD, or nearly, see there
 
 template <typename T, int DP, int WHAT>
-constexpr int key_blocks_per_unit() { return sizeof(T) * DP >= (WHAT == 3 ? 256 : 512) ? 1 : 2; }
+constexpr int key_blocks_per_unit() { return sizeof(T) * DP >= (WHAT == 3 ? 256 : 384) ? 1 : 2; }
 
 // Keys of a tile: 16 KB, or 8 KB where a block's walk over small segments should have few steps (each waits for its tile).
 template <typename T, int DP>
@@ -592,7 +593,7 @@ __global__ __launch_bounds__(256, (blocks_per_unit<T, DP>())) void forward(Args 
     const int row = (tile * (4 / SPLIT) + rows) * 32 + (lane & 31), i = min(row, a.nq - 1);
     typename L::frag q[L::kFrags];
     load_row<T, L::kFrags>(q, (const char*)((const T*)a.q + i * a.q_row + h * a.q_head), chunks, half);
-    if (chunks < L::kChunks) {
+    if (chunks < 2 * L::kFrags) {
         clear<L::kBytes>(key0), clear<L::kBytes>(key1), clear<L::kBytes>(val0), clear<L::kBytes>(val1);
     }
     const Bounds b = keys_of(a, i, lane);
@@ -986,7 +987,7 @@ __global__ __launch_bounds__(256, (blocks_per_unit<T, DP>())) void query_gradien
     const int kh = h / (a.hq / a.hk), chunks = a.d * (int)sizeof(T) / 16;
     const int rows = wave % (4 / SPLIT), part = wave / (4 / SPLIT);  // which 32 rows, and which of the groups of keys
     const int row = (tile * (4 / SPLIT) + rows) * 32 + (lane & 31), i = min(row, a.nq - 1);
-    if (chunks < L::kChunks) {
+    if (chunks < 2 * L::kFrags) {
         clear<L::kBytes>(key0), clear<L::kBytes>(key1), clear<L::kBytes>(val0), clear<L::kBytes>(val1);
     }
     const Bounds b = keys_of(a, i, lane);
@@ -1110,8 +1111,8 @@ __global__ __launch_bounds__(256, (blocks_per_unit<T, DP>())) void query_gradien
 // elements of its key and value, so there is one wave to a SIMD and nothing else runs while it waits: reads from LDS go
 // ahead of their products in batches, with a fence behind each. (Left to itself the compiler puts every read right before
 // its product, and the wave waited for 45 % of its clocks.) WHAT: 1 the keys' gradient, 2 the values', 3 both.
-template <typename T, int DP, int WHAT, int KEYS>
-__global__ __launch_bounds__(256, (key_blocks_per_unit<T, DP, WHAT>())) void key_gradient(Args a) {
+template <typename T, int DP, int WHAT, int KEYS, int UNIT = key_blocks_per_unit<T, DP, WHAT>()>
+__global__ __launch_bounds__(256, UNIT) void key_gradient(Args a) {
     constexpr bool DK = WHAT & 1, DV = WHAT & 2;
     constexpr int GROUPS = 4 / KEYS, BQ = 32 * GROUPS, DT = DP / 32, PF = sizeof(T) == 2 ? 2 : 4;
     typedef Tile<T, DP, BQ> L;
@@ -1129,7 +1130,7 @@ __global__ __launch_bounds__(256, (key_blocks_per_unit<T, DP, WHAT>())) void key
     typename L::frag k[L::kFrags], v[L::kFrags];
     load_row<T, L::kFrags>(k, (const char*)((const T*)a.k + j * a.k_row + kh * a.k_head), chunks, half);
     if (DK) load_row<T, L::kFrags>(v, (const char*)((const T*)a.v + j * a.v_row + kh * a.v_head), chunks, half);
-    if (chunks < L::kChunks) {
+    if (chunks < 2 * L::kFrags) {
         clear<L::kBytes>(que0), clear<L::kBytes>(que1), clear<L::kBytes>(gra0), clear<L::kBytes>(gra1);
     }
     const Bounds b = queries_of(a, j, lane);
@@ -1195,29 +1196,32 @@ __global__ __launch_bounds__(256, (key_blocks_per_unit<T, DP, WHAT>())) void key
         if (kSparse<T, DP> && !walk.needs(now + r0, 32)) return;
         float16_t s = 0.0f, x = 0.0f;
         if constexpr (kFenced<T, DP> && WHAT == 3) {
-            typename L::frag rows[2][8], columns[2][2 * DT];
+            int at = lane;
+            if constexpr (UNIT == 2) asm volatile("" : "+v"(at));  // (places in LDS computed anew: kept, they would take registers)
+            constexpr int kBatch = L::kFrags / 2;
+            typename L::frag rows[2][2 * kBatch], columns[2][2 * DT];
             auto load_rows = [&](int n) {
 #pragma unroll
-                for (int f = 0; f < 4; ++f) {
-                    rows[n][2 * f] = L::row(qt, r0 + (lane & 31), 4 * n + f, half);
-                    rows[n][2 * f + 1] = L::row(gt, r0 + (lane & 31), 4 * n + f, half);
+                for (int f = 0; f < kBatch; ++f) {
+                    rows[n][2 * f] = L::row(qt, r0 + (at & 31), kBatch * n + f, at >> 5);
+                    rows[n][2 * f + 1] = L::row(gt, r0 + (at & 31), kBatch * n + f, at >> 5);
                 }
                 __builtin_amdgcn_sched_barrier(0);
             };
             auto load_columns = [&](int f) {
 #pragma unroll
                 for (int t = 0; t < DT; ++t) {
-                    columns[f][2 * t] = column_of<T, DP, BQ>(gt, r0, f, t, lane);
-                    columns[f][2 * t + 1] = column_of<T, DP, BQ>(qt, r0, f, t, lane);
+                    columns[f][2 * t] = column_of<T, DP, BQ>(gt, r0, f, t, at);
+                    columns[f][2 * t + 1] = column_of<T, DP, BQ>(qt, r0, f, t, at);
                 }
                 __builtin_amdgcn_sched_barrier(0);
             };
             load_rows(0);
             load_rows(1);
 #pragma unroll
-            for (int f = 0; f < 8; ++f) {
-                s = mma(rows[f / 4][2 * (f % 4)], k[f], s);
-                x = mma(rows[f / 4][2 * (f % 4) + 1], v[f], x);
+            for (int f = 0; f < L::kFrags; ++f) {
+                s = mma(rows[f / kBatch][2 * (f % kBatch)], k[f], s);
+                x = mma(rows[f / kBatch][2 * (f % kBatch) + 1], v[f], x);
             }
             __builtin_amdgcn_sched_barrier(0);
             load_columns(0);
@@ -1253,7 +1257,7 @@ __global__ __launch_bounds__(256, (key_blocks_per_unit<T, DP, WHAT>())) void key
 #pragma unroll
                     for (int t = 0; t < DT; ++t) dk[t] = mma(column_of<T, DP, BQ>(qt, r0, f, t, lane), d, dk[t]);
                 }
-            }
+                }
         }
     };
     for (int n = 0; n < steps; n += 2) {

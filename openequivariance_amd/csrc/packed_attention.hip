@@ -22,6 +22,8 @@ struct Kernels {
         if (a.parts > 1) join<T, DP><<<(unsigned)a.nq * a.hq, 256, 0, stream>>>(a);
         return hipGetLastError();
     }
+    // Whether blocks of keys' gradients fit a compute unit twice, but are faster alone: 249 registers a lane, or 400.
+    static constexpr bool kAlone = sizeof(T) == 2 && DP == 96;
     static hipError_t gradients(const Args& a, int key_tiles, hipStream_t stream) {
         if (a.tiles && a.split == 2)
             query_gradient<T, DP, 2><<<(unsigned)(a.tiles * a.hq), 256, 0, stream>>>(a);
@@ -40,10 +42,15 @@ struct Kernels {
             key_gradient<T, DP, 1, 2><<<blocks, 256, 0, stream>>>(b);
         } else if (blocks < 256) {
             // Fewer blocks than compute units: half as many keys to a block and half as long a walk. Gradients together, us, with
-            // 64 / 32 keys: 56 blocks, float32 heads of 64 226 / 145; 112, fp16 of 72 121 / 74; 126, float32 of 64 416 / 268; 252, bf16
+            // 64 / 32 keys: 56 blocks, float32 heads of 64 226 / 145; 126, float32 of 64 416 / 268; 252, bf16
             // of 128 159 / 161; 504 217 / 278. All of them run at once, so they need no order (which is of tiles of 64 keys).
             b.tiles = (a.nk + 31) / 32, b.k_order = nullptr;
-            key_gradient<T, DP, 3, 1><<<(unsigned)(b.tiles * a.hk), 256, 0, stream>>>(b);
+            key_gradient<T, DP, 3, 1, kAlone ? 1 : key_blocks_per_unit<T, DP, 3>()><<<(unsigned)(b.tiles * a.hk), 256, 0, stream>>>(b);
+        } else if (kAlone && a.causal && blocks <= 512) {
+            // Two blocks share a compute unit, or one has it alone and all registers, where the longest of few uneven walks
+            // decides. bf16, 16 heads of 96, gradients, shared / alone: causal, 284 blocks 485 / 431 us, 376 169 / 155, 500 556 / 492, 628
+            // 1 372 / 1 431, 2 000 170 / 215; not causal, 500 blocks 1 524 / 1 687.
+            key_gradient<T, DP, 3, 2, 1><<<blocks, 256, 0, stream>>>(b);
         } else {
             key_gradient<T, DP, 3, 2><<<blocks, 256, 0, stream>>>(b);
         }
@@ -53,11 +60,20 @@ struct Kernels {
 
 }  // namespace
 
-#define OEQ_BY_HEAD(call) (a.d <= 32 ? Kernels<32>::call : a.d <= 64 ? Kernels<64>::call : Kernels<128>::call)
+// Heads of 72 to 96 elements leave out a quarter of the products of 128: bf16, 16 / 4 heads of 96, two segments of 4 000
+// rows, causal, forward 134 us, not 152, gradients 490, not 559; float32, 8 heads of 96, 4 000 rows 249 and 949, not 309 and 1 196.
+#define OEQ_BY_HEAD(call) \
+    (a.d <= 32   ? Kernels<32>::call \
+     : a.d <= 64 ? Kernels<64>::call \
+     : a.d <= 96 ? Kernels<96>::call : Kernels<128>::call)
 
 template <>
 hipError_t Launch<OEQ_ATTENTION_TYPE>::forward(const Args& a, hipStream_t stream) {
-    return a.parts ? OEQ_BY_HEAD(forward_shares(a, stream)) : OEQ_BY_HEAD(forward_rows(a, stream));
+    if (a.parts)
+        return a.d <= 32   ? Kernels<32>::forward_shares(a, stream)
+               : a.d <= 64 ? Kernels<64>::forward_shares(a, stream)
+                           : Kernels<128>::forward_shares(a, stream);
+    return OEQ_BY_HEAD(forward_rows(a, stream));
 }
 
 template <>

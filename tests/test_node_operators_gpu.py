@@ -115,6 +115,34 @@ def test_attention_of_long_segments_with_one_key_head(dtype):
     attention_case(dtype, ptr, ptr, None, ptr[-1], ptr[-1], 48, 1, 8, True)
 
 
+@pytest.mark.parametrize("d", [32, 64, 88, 128])
+@pytest.mark.parametrize("k_heads", [2, 4])
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+def test_attention_of_many_tiles(dtype, k_heads, d):
+    """More blocks than the compute units run at once, and (two key heads) a little more than they have units."""
+    ptr = starts([i % 60 for i in range(305)])
+    assert ptr[-1] > 8 * 1024
+    attention_case(dtype, ptr, ptr, None, ptr[-1], ptr[-1], 8, k_heads, d, k_heads == 2)
+
+
+def test_rows_far_apart():
+    """140 rows 16 MiB apart: a tile of 128 spans nearly 2^31 bytes."""
+    rows, apart = 140, (1 << 23) - 8
+    if torch.cuda.mem_get_info()[0] < 9 << 30:
+        pytest.skip("needs 9 GB")
+    q, k, v = (torch.empty(rows * apart, dtype=BF16, device="cuda").as_strided((rows, 2, 16), (apart, 16, 1)) for _ in range(3))
+    for n, t in enumerate((q, k, v)):
+        t.copy_(normal(rows, 2, 16, dtype=BF16, seed=n))
+        t.requires_grad_()
+    g = normal(rows, 2, 16, dtype=BF16, seed=4)
+    ptr = [0, rows]
+    val, err = N.attention(q, k, v, N.segment_views(ptr, ptr, None, rows, False), 0.25, g)
+    out = oeq.packed_attention(q, k, v, on_gpu(ptr))
+    N.check(out, val["out"], err["out"], "out")
+    for name, x in zip(("dq", "dk", "dv"), torch.autograd.grad(out, (q, k, v), g)):
+        N.check(x, val[name], err[name], name)
+
+
 def test_large_scores():
     """Scores of some hundreds, where every row's weight is on a few keys, and one large common part."""
     ptr = starts([200, 31])
