@@ -452,6 +452,24 @@ __device__ __forceinline__ void place(const Args& a, int heads, const int* order
 template <typename T, int DP>
 constexpr int blocks_per_unit() { return sizeof(T) * DP > 256 ? 1 : 2; }
 
+// Small heads go with small segments: there each wave leaves out the groups of 32 keys that none of its rows sees. (512
+// molecules of 9 to 61 atoms: a wave's 32 rows see some 90 keys, their block's 128 rows 180.)
+template <typename T, int DP>
+constexpr bool kSparse = sizeof(T) == 4 && DP == 32;
+
+// A lane's number, or the same hidden from the compiler, which then computes places in LDS anew instead of keeping them in
+// registers. In key_gradient: kSparse, 192 registers a lane or 138, a wave more to a SIMD: 512 molecules, float32, all
+// gradients 139 / 132 us, 2 048 460 / 424, but a segment of 3 000 rows 260 / 266. (bf16 heads of 32, whose products are 8 times as
+// fast: 2 048 molecules 185 / 177, a segment of 3 000 rows 64 / 73, so they keep them.)
+struct Lane {
+    int at, half;
+    template <bool ANEW>
+    static __device__ __forceinline__ Lane of(int lane, int half) {
+        if constexpr (ANEW) asm volatile("" : "+v"(lane));
+        return {lane, ANEW ? lane >> 5 : half};
+    }
+};
+
 template <typename T, int DP>
 constexpr bool kFenced = sizeof(T) == 2 && DP >= 96;  // key_gradient: one wave to a SIMD, or nearly, see there
 
@@ -461,11 +479,6 @@ constexpr int key_blocks_per_unit() { return sizeof(T) * DP >= (WHAT == 3 ? 256 
 // Keys of a tile: 16 KB, or 8 KB where a block's walk over small segments should have few steps (each waits for its tile).
 template <typename T, int DP>
 constexpr int tile_rows() { return sizeof(T) == 2 || DP == 32 ? 64 : 32; }
-
-// Small heads go with small segments: there each wave leaves out the groups of 32 keys that none of its rows sees. (512
-// molecules of 9 to 61 atoms: a wave's 32 rows see some 90 keys, their block's 128 rows 180.)
-template <typename T, int DP>
-constexpr bool kSparse = sizeof(T) == 4 && DP == 32;
 
 // Everything that was requested so far has come, and the compiler knows: a row that is loaded before a loop would else be
 // waited for inside it, at its first use, together with what the loop has requested since.
@@ -1196,23 +1209,22 @@ __global__ __launch_bounds__(256, UNIT) void key_gradient(Args a) {
         if (kSparse<T, DP> && !walk.needs(now + r0, 32)) return;
         float16_t s = 0.0f, x = 0.0f;
         if constexpr (kFenced<T, DP> && WHAT == 3) {
-            int at = lane;
-            if constexpr (UNIT == 2) asm volatile("" : "+v"(at));  // (places in LDS computed anew: kept, they would take registers)
+            const Lane l = Lane::of<UNIT == 2>(lane, half);  // (kept, the places would take registers that are not there)
             constexpr int kBatch = L::kFrags / 2;
             typename L::frag rows[2][2 * kBatch], columns[2][2 * DT];
             auto load_rows = [&](int n) {
 #pragma unroll
                 for (int f = 0; f < kBatch; ++f) {
-                    rows[n][2 * f] = L::row(qt, r0 + (at & 31), kBatch * n + f, at >> 5);
-                    rows[n][2 * f + 1] = L::row(gt, r0 + (at & 31), kBatch * n + f, at >> 5);
+                    rows[n][2 * f] = L::row(qt, r0 + (l.at & 31), kBatch * n + f, l.half);
+                    rows[n][2 * f + 1] = L::row(gt, r0 + (l.at & 31), kBatch * n + f, l.half);
                 }
                 __builtin_amdgcn_sched_barrier(0);
             };
             auto load_columns = [&](int f) {
 #pragma unroll
                 for (int t = 0; t < DT; ++t) {
-                    columns[f][2 * t] = column_of<T, DP, BQ>(gt, r0, f, t, at);
-                    columns[f][2 * t + 1] = column_of<T, DP, BQ>(qt, r0, f, t, at);
+                    columns[f][2 * t] = column_of<T, DP, BQ>(gt, r0, f, t, l.at);
+                    columns[f][2 * t + 1] = column_of<T, DP, BQ>(qt, r0, f, t, l.at);
                 }
                 __builtin_amdgcn_sched_barrier(0);
             };
@@ -1238,11 +1250,12 @@ __global__ __launch_bounds__(256, UNIT) void key_gradient(Args a) {
                 }
             }
         } else {
+            const Lane l = Lane::of<kSparse<T, DP>>(lane, half);
 #pragma unroll
-            for (int f = 0; f < L::kFrags; ++f) s = mma(L::row(qt, r0 + (lane & 31), f, half), k[f], s);
+            for (int f = 0; f < L::kFrags; ++f) s = mma(L::row(qt, r0 + (l.at & 31), f, l.half), k[f], s);
 #pragma unroll
             for (int f = 0; f < L::kFrags; ++f)
-                if (DK) x = mma(L::row(gt, r0 + (lane & 31), f, half), v[f], x);
+                if (DK) x = mma(L::row(gt, r0 + (l.at & 31), f, l.half), v[f], x);
             weigh(s, x, st);
             hide(s, x, now);
 #pragma unroll
@@ -1250,12 +1263,12 @@ __global__ __launch_bounds__(256, UNIT) void key_gradient(Args a) {
                 if (DV) {
                     const auto p = operand<T>(s, f);
 #pragma unroll
-                    for (int t = 0; t < DT; ++t) dv[t] = mma(column_of<T, DP, BQ>(gt, r0, f, t, lane), p, dv[t]);
+                    for (int t = 0; t < DT; ++t) dv[t] = mma(column_of<T, DP, BQ>(gt, r0, f, t, l.at), p, dv[t]);
                 }
                 if (DK) {
                     const auto d = operand<T>(x, f);
 #pragma unroll
-                    for (int t = 0; t < DT; ++t) dk[t] = mma(column_of<T, DP, BQ>(qt, r0, f, t, lane), d, dk[t]);
+                    for (int t = 0; t < DT; ++t) dk[t] = mma(column_of<T, DP, BQ>(qt, r0, f, t, l.at), d, dk[t]);
                 }
                 }
         }
