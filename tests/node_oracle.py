@@ -3,8 +3,8 @@ arithmetic allows.
 
 With u the half unit of the tensors' type (2^-24, 2^-11, 2^-8 for 24, 11 and 8 bits) the kernels round an output once,
 u |out|, and where operands have 16 bits they round p and ds to operands of a product, u p and u |ds| in every term of a
-sum; delta = g.o uses the rounded output, u sum |g o|. What is left are errors in 32 bits: a dot product of d terms,
-a sum of n, one of exp and log each, in all (d + n + 32) 2^-24 of the sums of absolute values, times 1 + S where a
+sum; delta = g.o of the rounded output (where its remainder is not kept), u sum |g o|. What is left are errors in 32
+bits: a dot product of d terms, a sum of n, one of exp and log each, in all (d + n + 32) 2^-24 of the sums of absolute values, times 1 + S where a
 score of absolute sum S stands in an exponent.
 """
 
