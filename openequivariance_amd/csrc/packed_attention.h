@@ -330,11 +330,11 @@ __device__ __forceinline__ Bounds keys_of(const Args& a, int i, int lane) {
     const int s = find_segment(a.q_ptr, a.segments, i, lane);
     Bounds b = {0, 0};
     if (s >= 0 && s < a.segments) {
-        const int64_t q0 = a.q_ptr[s], q1 = a.q_ptr[s + 1];
+        const int q1 = clamped(a.q_ptr[s + 1], a.nq);  // (cut off at the tensor's end, for the diagonal too)
         const int k0 = clamped(a.k_ptr[s], a.nk), k1 = clamped(a.k_ptr[s + 1], a.nk);
         int len = max(k1 - k0, 0);
         if (a.k_len) len = min(len, clamped(a.k_len[s], INT_MAX));
-        if (a.causal) len = min((int64_t)len, max((int64_t)0, len - (q1 - q0) + (i - q0) + 1));
+        if (a.causal) len = min(len, max(0, len - (q1 - 1 - i)));
         if (i < q1 && len > 0) b = {k0, k0 + len};
     }
     return b;

@@ -622,3 +622,26 @@ def test_autocast():
     assert q.dtype == BF16 and out.dtype == F32
     out.sum().backward()
     assert w.grad.dtype == F32 and linear.weight.grad.dtype == F32 and torch.isfinite(linear.weight.grad).all()
+
+
+# ---------------------------------------------------------------------------
+# ends of segments
+# ---------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("end", [12, 1 << 40])
+@pytest.mark.parametrize("rows,keys", [(8, 8), (8, 5), (150, 190)])
+def test_causal_ends_past_the_tensors_have_one_diagonal(dtype, end, rows, keys):
+    """A segment that is said to go on behind the tensors is the one that is cut off there: its last row sees every key,
+    in the output and in all gradients."""
+    end += rows
+    leaves = [normal(n, h, 32, dtype=dtype, seed=s).requires_grad_() for s, (n, h) in enumerate(((rows, 4), (keys, 2), (keys, 2)))]
+    g = normal(rows, 4, 32, dtype=dtype, seed=5)
+    results = []
+    for q_ptr, k_ptr in (([0, 3, rows], [0, 2, keys]), ([0, 3, end], [0, 2, end]), ([0, 3, end], [0, 2, keys])):
+        out, lse = oeq.packed_attention(*leaves, on_gpu(q_ptr), on_gpu(k_ptr), causal=True, return_lse=True)
+        results.append((out, lse) + torch.autograd.grad(out, leaves, g))
+    for other in results[1:]:
+        for name, a, b in zip(("out", "lse", "dq", "dk", "dv"), results[0], other):
+            assert torch.equal(a, b), name
