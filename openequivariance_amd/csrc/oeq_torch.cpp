@@ -36,7 +36,6 @@
 
 namespace py = pybind11;
 using at::Tensor;
-using OptTensor = std::optional<Tensor>;
 using Tensor3 = std::tuple<Tensor, Tensor, Tensor>;
 using Tensor4 = std::tuple<Tensor, Tensor, Tensor, Tensor>;
 using namespace oeq_torch;
@@ -635,12 +634,14 @@ const char* const kTpDoubleBackward = "oeq_amd::tp_double_backward";
 const char* const kConvDoubleBackward = "oeq_amd::conv_double_backward";
 
 Tensor tp_forward_autograd(const Tensor& x, const Tensor& y, const Tensor& w, int64_t kid, const OptTensor& spec) {
+    refuse_tangents("oeq_amd::tp_forward", x, y, w);
     if (records(x, y, w)) return TpForward::apply(x, y, w, kid, spec);
     at::AutoDispatchBelowADInplaceOrView below;
     return call_tp_forward(x, y, w, kid, spec);
 }
 Tensor3 tp_backward_autograd(const Tensor& x, const Tensor& y, const Tensor& w, const Tensor& g, int64_t kid,
                              const OptTensor& spec) {
+    refuse_tangents("oeq_amd::tp_backward", x, y, w, g);
     if (records(x, y, w, g)) {
         const auto out = TpBackward::apply(x, y, w, g, kid, spec);
         return {out[0], out[1], out[2]};
@@ -650,12 +651,14 @@ Tensor3 tp_backward_autograd(const Tensor& x, const Tensor& y, const Tensor& w, 
 }
 Tensor conv_forward_autograd(const Tensor& x, const Tensor& y, const Tensor& w, const Tensor& r, const Tensor& c,
                              const Tensor& p, int64_t kid, const OptTensor& spec) {
+    refuse_tangents("oeq_amd::conv_forward", x, y, w);
     if (records(x, y, w)) return ConvForward::apply(x, y, w, r, c, p, kid, spec);
     at::AutoDispatchBelowADInplaceOrView below;
     return call_conv_forward(x, y, w, r, c, p, kid, spec);
 }
 Tensor3 conv_backward_autograd(const Tensor& x, const Tensor& y, const Tensor& w, const Tensor& g, const Tensor& r,
                                const Tensor& c, const Tensor& p, int64_t kid, const OptTensor& spec) {
+    refuse_tangents("oeq_amd::conv_backward", x, y, w, g);
     if (records(x, y, w, g)) {
         const auto out = ConvBackward::apply(x, y, w, g, r, c, p, kid, spec);
         return {out[0], out[1], out[2]};
@@ -667,6 +670,7 @@ Tensor3 conv_backward_autograd(const Tensor& x, const Tensor& y, const Tensor& w
 Tensor4 tp_double_backward_autograd(const Tensor& x, const Tensor& y, const Tensor& w, const Tensor& g,
                                     const Tensor& a, const Tensor& b, const Tensor& c, int64_t kid,
                                     const OptTensor& spec) {
+    refuse_tangents("oeq_amd::tp_double_backward", x, y, w, g, a, b, c);
     if (records(x, y, w, g, a, b, c)) {
         const auto out =
             NotDifferentiated<decltype(tp_double_backward_gpu), kTpDoubleBackward>::apply(x, y, w, g, a, b, c, kid, spec);
@@ -678,6 +682,7 @@ Tensor4 tp_double_backward_autograd(const Tensor& x, const Tensor& y, const Tens
 Tensor4 conv_double_backward_autograd(const Tensor& x, const Tensor& y, const Tensor& w, const Tensor& g,
                                       const Tensor& a, const Tensor& b, const Tensor& c, const Tensor& rows,
                                       const Tensor& cols, const Tensor& p, int64_t kid, const OptTensor& spec) {
+    refuse_tangents("oeq_amd::conv_double_backward", x, y, w, g, a, b, c);
     if (records(x, y, w, g, a, b, c)) {
         const auto out = NotDifferentiated<decltype(conv_double_backward_gpu), kConvDoubleBackward>::apply(
             x, y, w, g, a, b, c, rows, cols, p, kid, spec);

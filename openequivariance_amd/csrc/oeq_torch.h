@@ -10,6 +10,7 @@
 #include <ATen/hip/impl/HIPGuardImplMasqueradingAsCUDA.h>
 #include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
 
+#include <optional>
 #include <string>
 
 namespace oeq_torch {
@@ -61,9 +62,28 @@ inline Tensor scratch(const Tensor& like, size_t bytes) {
     return at::empty({(int64_t)(bytes ? bytes : 1)}, like.options().dtype(at::kByte));
 }
 
+using OptTensor = std::optional<Tensor>;
+
+inline bool wants_grad(const Tensor& t) { return t.requires_grad(); }
+inline bool wants_grad(const OptTensor& t) { return t.has_value() && t->requires_grad(); }
+inline Tensor tangent_of(const Tensor& t) { return t.defined() ? Tensor(t._fw_grad(0)) : Tensor(); }
+inline Tensor tangent_of(const OptTensor& t) { return t.has_value() ? tangent_of(*t) : Tensor(); }
+
+// Whether a call of differentiable operands is recorded for a backward pass.
 template <typename... Ts>
 bool records(const Ts&... ts) {
-    return at::GradMode::is_enabled() && (ts.requires_grad() || ...);
+    return at::GradMode::is_enabled() && (wants_grad(ts) || ...);
+}
+
+// Whether an operand is a dual tensor of forward-mode differentiation. Such a tensor need not require a gradient: below
+// autograd its tangent would be lost and the derivative come out as zero.
+template <typename... Ts>
+bool has_tangent(const Ts&... ts) {
+    return (tangent_of(ts).defined() || ...);
+}
+template <typename... Ts>
+void refuse_tangents(const char* op, const Ts&... ts) {
+    TORCH_CHECK(!has_tangent(ts...), op, " has no forward-mode derivative: differentiate it backward");
 }
 
 }  // namespace oeq_torch

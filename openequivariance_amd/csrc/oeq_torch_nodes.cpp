@@ -12,7 +12,6 @@
 #include <tuple>
 
 using namespace oeq_torch;
-using OptTensor = std::optional<Tensor>;
 using Tensor2 = std::tuple<Tensor, Tensor>;
 using Tensor3 = std::tuple<Tensor, Tensor, Tensor>;
 using Tensor4 = std::tuple<Tensor, Tensor, Tensor, Tensor>;
@@ -284,13 +283,6 @@ auto find_op(const char* name) {
 OptTensor optional_of(const Tensor& t) { return t.defined() ? OptTensor(t) : OptTensor(); }
 Tensor tensor_of(const OptTensor& t) { return t.has_value() ? *t : Tensor(); }
 
-bool wants(const Tensor& t) { return t.requires_grad(); }
-bool wants(const OptTensor& t) { return t.has_value() && t->requires_grad(); }
-template <typename... Ts>
-bool recording(const Ts&... ts) {
-    return at::GradMode::is_enabled() && (wants(ts) || ...);
-}
-
 Tensor or_zeros(const Tensor& g, const Tensor& like) { return g.defined() ? g : at::zeros_like(like); }
 
 struct PackedAttention : public torch::autograd::Function<PackedAttention> {
@@ -367,7 +359,8 @@ struct IrrepDropout : public torch::autograd::Function<IrrepDropout> {
 
 Tensor3 packed_attention_autograd(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& q_ptr, const Tensor& k_ptr,
                                   const OptTensor& k_len, bool causal, double scale, bool keep_rest) {
-    if (recording(q, k, v)) {
+    refuse_tangents("oeq_amd::packed_attention", q, k, v);
+    if (records(q, k, v)) {
         const auto out = PackedAttention::apply(q, k, v, q_ptr, k_ptr, k_len, causal, scale);
         return {out[0], out[1], out[2]};
     }
@@ -393,7 +386,8 @@ struct PackedAttentionGradient : public torch::autograd::Function<PackedAttentio
 Tensor3 packed_attention_backward_autograd(const Tensor& grad, const Tensor& q, const Tensor& k, const Tensor& v,
                                            const Tensor& out, const Tensor& log2_sum, const Tensor& rest, const Tensor& q_ptr,
                                            const Tensor& k_ptr, const OptTensor& k_len, bool causal, double scale) {
-    if (recording(grad, q, k, v)) {
+    refuse_tangents("oeq_amd::packed_attention_backward", grad, q, k, v, out, log2_sum, rest);
+    if (records(grad, q, k, v)) {
         const auto g = PackedAttentionGradient::apply(grad, q, k, v, out, log2_sum, rest, q_ptr, k_ptr, k_len, causal, scale);
         return {g[0], g[1], g[2]};
     }
@@ -403,7 +397,8 @@ Tensor3 packed_attention_backward_autograd(const Tensor& grad, const Tensor& q, 
 
 Tensor2 qk_norm_rotary_autograd(const Tensor& q, const Tensor& k, const Tensor& positions, const Tensor& table,
                                 const OptTensor& q_weight, const OptTensor& k_weight, double eps, bool interleaved) {
-    if (recording(q, k, q_weight, k_weight)) {
+    refuse_tangents("oeq_amd::qk_norm_rotary", q, k, table, q_weight, k_weight);
+    if (records(q, k, q_weight, k_weight)) {
         const auto out = QkNormRotary::apply(q, k, positions, table, q_weight, k_weight, eps, interleaved);
         return {out[0], out[1]};
     }
@@ -429,7 +424,8 @@ struct QkNormRotaryGradient : public torch::autograd::Function<QkNormRotaryGradi
 Tensor4 qk_norm_rotary_backward_autograd(const Tensor& q_grad, const Tensor& k_grad, const Tensor& q, const Tensor& k,
                                          const Tensor& positions, const Tensor& table, const OptTensor& q_weight,
                                          const OptTensor& k_weight, double eps, bool interleaved) {
-    if (recording(q_grad, k_grad, q, k, q_weight, k_weight)) {
+    refuse_tangents("oeq_amd::qk_norm_rotary_backward", q_grad, k_grad, q, k, table, q_weight, k_weight);
+    if (records(q_grad, k_grad, q, k, q_weight, k_weight)) {
         const auto g = QkNormRotaryGradient::apply(q_grad, k_grad, q, k, positions, table, q_weight, k_weight, eps, interleaved);
         return {g[0], g[1], g[2], g[3]};
     }
@@ -442,7 +438,8 @@ Tensor4 qk_norm_rotary_backward_autograd(const Tensor& q_grad, const Tensor& k_g
 Tensor qk_norm_rotary_append_autograd(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& positions,
                                       const Tensor& table, const Tensor& k_cache, const Tensor& v_cache, const Tensor& slots,
                                       const OptTensor& q_weight, const OptTensor& k_weight, double eps, bool interleaved) {
-    TORCH_CHECK(!recording(q, k, v, k_cache, v_cache, q_weight, k_weight),
+    refuse_tangents("oeq_amd::qk_norm_rotary_append", q, k, v, table, k_cache, v_cache, q_weight, k_weight);
+    TORCH_CHECK(!records(q, k, v, k_cache, v_cache, q_weight, k_weight),
                 "qk_norm_rotary_append writes into the caches and has no gradient: call it under torch.no_grad(), or ",
                 "qk_norm_rotary where gradients are needed");
     at::AutoDispatchBelowADInplaceOrView below;
@@ -454,7 +451,13 @@ Tensor qk_norm_rotary_append_autograd(const Tensor& q, const Tensor& k, const Te
 }
 
 Tensor irrep_dropout_autograd(const Tensor& x, const OptTensor& residual, const Tensor& channels, const Tensor& seed, double p) {
-    if (recording(x, residual)) return IrrepDropout::apply(x, residual, channels, seed, p);
+    if (has_tangent(x, residual)) {  // linear in x and the residual, and so is what a tangent becomes
+        const Tensor tx = tangent_of(x), tr = tangent_of(residual);
+        const OptTensor base = residual.has_value() ? OptTensor(residual->_fw_primal(0)) : OptTensor();
+        const Tensor out = OEQ_OP(irrep_dropout).call(x._fw_primal(0), base, channels, seed, p);
+        return at::_make_dual(out, tx.defined() ? OEQ_OP(irrep_dropout).call(tx, optional_of(tr), channels, seed, p) : tr, 0);
+    }
+    if (records(x, residual)) return IrrepDropout::apply(x, residual, channels, seed, p);
     at::AutoDispatchBelowADInplaceOrView below;
     return OEQ_OP(irrep_dropout).call(x, residual, channels, seed, p);
 }

@@ -198,3 +198,33 @@ def test_no_kernel_of_the_library_has_scratch_memory():
     attention = {n: r for n, r in names.items() if "packed_attention" in n}
     assert len(attention) >= 30
     assert not {n: r for n, r in attention.items() if r[1] > 0}
+
+
+def test_forward_mode_derivatives_are_right_or_refused():
+    """A dual tensor need not require a gradient; its tangent must not get lost on the way."""
+    import torch.autograd.forward_ad as forward_ad
+    q, k = torch.empty(7, 4, 32, device="meta"), torch.empty(7, 2, 32, device="meta")
+    ptr, at, seed = (torch.empty(n, device="meta", dtype=torch.int64) for n in (3, 7, 2))
+    table, w, x = torch.empty(5, 2, 8, device="meta"), torch.empty(32, device="meta"), torch.empty(6, 8, device="meta")
+    module = oeq.IrrepDropout("2x0e+2x1o", 0.1).to("meta")
+    with forward_ad.dual_level():
+        def dual(t):
+            return forward_ad.make_dual(t, torch.empty_like(t))
+
+        for call in (lambda: oeq.packed_attention(dual(q), k, k, ptr), lambda: oeq.packed_attention(q, dual(k), k, ptr),
+                     lambda: oeq.packed_attention(q, k, dual(k), ptr), lambda: oeq.qk_norm_rotary(dual(q), k, at, table),
+                     lambda: oeq.qk_norm_rotary(q, dual(k), at, table, w),
+                     lambda: oeq.qk_norm_rotary(q, k, at, table, None, dual(w)),
+                     lambda: oeq.qk_norm_rotary(q, k, at, dual(table)),
+                     lambda: oeq.qk_norm_rotary_append(dual(q), k, k, at, table, k.clone(), k.clone(), at),
+                     lambda: torch.ops.oeq_amd.qk_norm_rotary_backward(dual(q), k, q, k, at, table, w, None, 1e-6, False)):
+            with pytest.raises(RuntimeError, match="no forward-mode derivative"):
+                call()
+        for args in ((dual(x), None), (dual(x), x), (x, dual(x)), (dual(x), dual(x)), (dual(x).requires_grad_(), x)):
+            out = module(*args, seed=seed)
+            tangent = forward_ad.unpack_dual(out).tangent
+            assert tangent is not None and tangent.shape == x.shape
+            assert out.requires_grad == args[0].requires_grad
+        assert forward_ad.unpack_dual(module(x, x, seed=seed)).tangent is None
+    value, tangent = torch.func.jvp(lambda t: module(t, seed=seed), (x,), (x,))
+    assert value.shape == tangent.shape == x.shape

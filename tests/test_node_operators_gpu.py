@@ -645,3 +645,21 @@ def test_causal_ends_past_the_tensors_have_one_diagonal(dtype, end, rows, keys):
     for other in results[1:]:
         for name, a, b in zip(("out", "lse", "dq", "dk", "dv"), results[0], other):
             assert torch.equal(a, b), name
+
+
+def test_forward_mode_derivative_of_dropout():
+    module, seed = oeq.IrrepDropout("5x0e+2x1o", 0.4).cuda(), on_gpu([7, 8])
+    x, base, tx, tb = (normal(30, 11, seed=s) for s in range(4))
+    want = module(tx, tb, seed=seed)
+    value, tangent = torch.func.jvp(lambda a, b: module(a, b, seed=seed), (x, base), (tx, tb))
+    assert torch.equal(value, module(x, base, seed=seed)) and torch.equal(tangent, want) and tangent.any()
+    _, tangent = torch.func.jvp(lambda a: module(a, base, seed=seed), (x,), (tx,))
+    assert torch.equal(tangent, module(tx, seed=seed))
+    _, tangent = torch.func.jvp(lambda b: module(x, b, seed=seed), (base,), (tb,))
+    assert torch.equal(tangent, tb)
+    q, ptr = normal(11, 2, 32), on_gpu([0, 11])
+    with pytest.raises(RuntimeError, match="no forward-mode derivative"):
+        torch.func.jvp(lambda t: oeq.packed_attention(t, q, q, ptr), (q,), (q,))
+    with pytest.raises(RuntimeError, match="no forward-mode derivative"):
+        torch.func.jvp(lambda t: oeq.qk_norm_rotary(t, q, torch.arange(11, device="cuda"), oeq.rotary_table(11, 8, device="cuda")),
+                       (q,), (q,))
