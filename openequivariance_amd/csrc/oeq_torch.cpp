@@ -101,11 +101,11 @@ int64_t without_terms(int64_t kid) {
     return g_py->without_terms(kid).cast<int64_t>();
 }
 
-void check_weights(const Entry& e, const Tensor& w, int64_t rows, const char* name) {
+void check_weights(const Entry& e, const Tensor& w, int64_t rows, const char* name, const Tensor& beside) {
     if (e.shared)
-        check_tensor(w, {e.WN}, e.dtype, name);
+        check_tensor(w, {e.WN}, e.dtype, name, beside);
     else
-        check_tensor(w, {rows, e.WN}, e.dtype, name);
+        check_tensor(w, {rows, e.WN}, e.dtype, name, beside);
 }
 
 int64_t rows_of(const Tensor& t) { return t.dim() > 0 ? t.size(0) : -1; }
@@ -126,9 +126,9 @@ Tensor tp_forward_gpu(const Tensor& L1_in, const Tensor& L2_in, const Tensor& W,
     const EntryRef ref = entry_of(kid, spec);
     const Entry& e = *ref;
     const int64_t n = rows_of(L1_in);
-    check_tensor(L1_in, {n, e.L1}, e.dtype, "L1_in");
-    check_tensor(L2_in, {n, e.L2}, e.dtype, "L2_in");
-    check_weights(e, W, n, "W");
+    check_tensor(L1_in, {n, e.L1}, e.dtype, "L1_in", L1_in);
+    check_tensor(L2_in, {n, e.L2}, e.dtype, "L2_in", L1_in);
+    check_weights(e, W, n, "W", L1_in);
     const Tensor x = operand(e, L1_in), y = operand(e, L2_in), w = operand(e, W);
     OnDevice dev(x);
     Tensor out = at::empty({n, e.L3}, x.options());
@@ -141,10 +141,10 @@ Tensor3 tp_backward_gpu(const Tensor& L1_in, const Tensor& L2_in, const Tensor& 
     const EntryRef ref = entry_of(kid, spec);
     const Entry& e = *ref;
     const int64_t n = rows_of(L1_in);
-    check_tensor(L1_in, {n, e.L1}, e.dtype, "L1_in");
-    check_tensor(L2_in, {n, e.L2}, e.dtype, "L2_in");
-    check_weights(e, W, n, "W");
-    check_tensor(L3_grad, {n, e.L3}, e.dtype, "L3_grad");
+    check_tensor(L1_in, {n, e.L1}, e.dtype, "L1_in", L1_in);
+    check_tensor(L2_in, {n, e.L2}, e.dtype, "L2_in", L1_in);
+    check_weights(e, W, n, "W", L1_in);
+    check_tensor(L3_grad, {n, e.L3}, e.dtype, "L3_grad", L1_in);
     const Tensor x = operand(e, L1_in), y = operand(e, L2_in), w = operand(e, W), g = operand(e, L3_grad);
     OnDevice dev(x);
     Tensor dx = at::empty_like(x), dy = at::empty_like(y), dw = at::empty_like(w);
@@ -163,13 +163,13 @@ Tensor4 tp_double_backward_gpu(const Tensor& L1_in, const Tensor& L2_in, const T
     const EntryRef ref = entry_of(kid, spec);
     const Entry& e = *ref;
     const int64_t n = rows_of(L1_in);
-    check_tensor(L1_in, {n, e.L1}, e.dtype, "L1_in");
-    check_tensor(L1_dgrad, {n, e.L1}, e.dtype, "L1_dgrad");
-    check_tensor(L2_in, {n, e.L2}, e.dtype, "L2_in");
-    check_tensor(L2_dgrad, {n, e.L2}, e.dtype, "L2_dgrad");
-    check_weights(e, W, n, "W");
-    check_weights(e, W_dgrad, n, "W_dgrad");
-    check_tensor(L3_grad, {n, e.L3}, e.dtype, "L3_grad");
+    check_tensor(L1_in, {n, e.L1}, e.dtype, "L1_in", L1_in);
+    check_tensor(L1_dgrad, {n, e.L1}, e.dtype, "L1_dgrad", L1_in);
+    check_tensor(L2_in, {n, e.L2}, e.dtype, "L2_in", L1_in);
+    check_tensor(L2_dgrad, {n, e.L2}, e.dtype, "L2_dgrad", L1_in);
+    check_weights(e, W, n, "W", L1_in);
+    check_weights(e, W_dgrad, n, "W_dgrad", L1_in);
+    check_tensor(L3_grad, {n, e.L3}, e.dtype, "L3_grad", L1_in);
     const Tensor x = operand(e, L1_in), y = operand(e, L2_in), w = operand(e, W), g = operand(e, L3_grad);
     const Tensor a = operand(e, L1_dgrad), b = operand(e, L2_dgrad), c = operand(e, W_dgrad);
     OnDevice dev(x);
@@ -194,13 +194,13 @@ struct GraphSize {
 GraphSize conv_checks(const Entry& e, const Tensor& L1_in, const Tensor& L2_in, const Tensor& W, const Tensor& rows,
                       const Tensor& cols, const Tensor& perm, const Tensor* L3_grad) {
     const int64_t nodes = rows_of(L1_in), nnz = rows_of(rows);
-    check_tensor(L1_in, {nodes, e.L1}, e.dtype, "L1_in");
-    check_tensor(L2_in, {nnz, e.L2}, e.dtype, "L2_in");
-    check_weights(e, W, nnz, "W");
-    if (L3_grad) check_tensor(*L3_grad, {nodes, e.L3}, e.dtype, "L3_grad");
-    check_tensor(rows, {nnz}, at::kLong, "rows");
-    check_tensor(cols, {nnz}, at::kLong, "cols");
-    if (e.deterministic) check_tensor(perm, {nnz}, at::kLong, "transpose perm");
+    check_tensor(L1_in, {nodes, e.L1}, e.dtype, "L1_in", L1_in);
+    check_tensor(L2_in, {nnz, e.L2}, e.dtype, "L2_in", L1_in);
+    check_weights(e, W, nnz, "W", L1_in);
+    if (L3_grad) check_tensor(*L3_grad, {nodes, e.L3}, e.dtype, "L3_grad", L1_in);
+    check_tensor(rows, {nnz}, at::kLong, "rows", L1_in);
+    check_tensor(cols, {nnz}, at::kLong, "cols", L1_in);
+    if (e.deterministic) check_tensor(perm, {nnz}, at::kLong, "transpose perm", L1_in);
     // counterpart of at::globalContext().alertNotDeterministic (torch_core.hpp:448) for the calls that use float
     // atomics: the backward of deterministic=False (sender gradients), and both directions of the float-atomics
     // kernels. The grouped forward sums in a fixed order and needs no alert.
@@ -424,9 +424,9 @@ Tensor4 conv_double_backward_gpu(const Tensor& L1_in, const Tensor& L2_in, const
     }
     const Entry& e = *ref;
     const GraphSize n = conv_checks(e, L1_in, L2_in, W, rows, cols, transpose_perm, &L3_grad);
-    check_tensor(L1_dgrad, {n.nodes, e.L1}, e.dtype, "L1_in");
-    check_tensor(L2_dgrad, {n.edges, e.L2}, e.dtype, "L2_in");
-    check_weights(e, W_dgrad, n.edges, "W");
+    check_tensor(L1_dgrad, {n.nodes, e.L1}, e.dtype, "L1_in", L1_in);
+    check_tensor(L2_dgrad, {n.edges, e.L2}, e.dtype, "L2_in", L1_in);
+    check_weights(e, W_dgrad, n.edges, "W", L1_in);
     const Tensor x = operand(e, L1_in), y = operand(e, L2_in), w = operand(e, W), g = operand(e, L3_grad);
     const Tensor a = operand(e, L1_dgrad), b = operand(e, L2_dgrad), c = operand(e, W_dgrad);
     const Tensor r = rows.contiguous(), cc = cols.contiguous(), p = transpose_perm.contiguous();

@@ -42,9 +42,13 @@ inline std::string dtype_text(at::ScalarType t) {
     return code ? std::to_string(code) : std::string(at::toString(t));
 }
 
-inline void check_tensor(const Tensor& t, at::IntArrayRef shape, at::ScalarType dtype, const char* name) {
+// `beside`: another operand of the call, on whose device all of them have to be (a kernel would read another device's
+// memory through a pointer that need not mean anything on its own).
+inline void check_tensor(const Tensor& t, at::IntArrayRef shape, at::ScalarType dtype, const char* name, const Tensor& beside) {
     TORCH_CHECK(t.sizes() == shape, "Shape mismatch for tensor '", name, "'. Expected: ", shape, ". Got: ", t.sizes());
     TORCH_CHECK(t.is_cuda(), "Tensor '", name, "' is not on the GPU.");
+    TORCH_CHECK(t.device() == beside.device(), "Tensor '", name, "' is on ", t.device(), ", not on ", beside.device(),
+                " as the operands before it.");
     TORCH_CHECK(t.scalar_type() == dtype, "Dtype mismatch for tensor '", name, "'. Expected: ", dtype_text(dtype),
                 ". Got: ", dtype_text(t.scalar_type()));
 }

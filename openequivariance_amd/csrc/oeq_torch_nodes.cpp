@@ -80,17 +80,17 @@ struct Attention {
         TORCH_CHECK(d > 0 && d <= 128 && d % 8 == 0, "Shape mismatch for tensor 'q'. Expected: head_dim a multiple of 8 up to ",
                     "128. Got: ", q_.sizes());
         check_heads(k_, "k");
-        check_tensor(q_, q_.sizes(), q_.scalar_type(), "q");
-        check_tensor(k_, {k_.size(0), k_.size(1), d}, q_.scalar_type(), "k");
-        check_tensor(v_, k_.sizes(), q_.scalar_type(), "v");
+        check_tensor(q_, q_.sizes(), q_.scalar_type(), "q", q_);
+        check_tensor(k_, {k_.size(0), k_.size(1), d}, q_.scalar_type(), "k", q_);
+        check_tensor(v_, k_.sizes(), q_.scalar_type(), "v", q_);
         TORCH_CHECK(q_.size(1) > 0 && k_.size(1) > 0 && q_.size(1) % k_.size(1) == 0,
                     "Shape mismatch for tensor 'k'. Expected: a number of heads that divides the ", q_.size(1),
                     " heads of 'q'. Got: ", k_.sizes());
         TORCH_CHECK(q_ptr_.dim() == 1 && q_ptr_.size(0) > 0,
                     "Shape mismatch for tensor 'q_ptr'. Expected: [segments + 1]. Got: ", q_ptr_.sizes());
-        check_tensor(q_ptr_, q_ptr_.sizes(), at::kLong, "q_ptr");
-        check_tensor(k_ptr_, q_ptr_.sizes(), at::kLong, "k_ptr");
-        if (k_len_.has_value()) check_tensor(*k_len_, {q_ptr_.size(0) - 1}, at::kLong, "k_len");
+        check_tensor(q_ptr_, q_ptr_.sizes(), at::kLong, "q_ptr", q_);
+        check_tensor(k_ptr_, q_ptr_.sizes(), at::kLong, "k_ptr", q_);
+        if (k_len_.has_value()) check_tensor(*k_len_, {q_ptr_.size(0) - 1}, at::kLong, "k_len", q_);
         TORCH_CHECK(scale > 0 && std::isfinite(scale), "packed_attention: scale must be positive, got ", scale);
         q = Rows(q_), k = Rows(k_), v = Rows(v_);
         q_ptr = q_ptr_.contiguous(), k_ptr = k_ptr_.contiguous();
@@ -131,11 +131,12 @@ Tensor3 packed_attention_gpu(const Tensor& q, const Tensor& k, const Tensor& v, 
 Tensor3 packed_attention_backward_gpu(const Tensor& grad, const Tensor& q, const Tensor& k, const Tensor& v,
                                       const Tensor& out, const Tensor& log2_sum, const Tensor& rest, const Tensor& q_ptr,
                                       const Tensor& k_ptr, const OptTensor& k_len, bool causal, double scale) {
+    check_heads(q, "q");
+    check_tensor(grad, q.sizes(), q.scalar_type(), "grad", q);
+    check_tensor(out, q.sizes(), q.scalar_type(), "out", q);
+    check_tensor(log2_sum, {q.size(1), oeq_attention_stat_stride(q.size(0))}, at::kFloat, "log2_sum", q);
+    if (rest.numel()) check_tensor(rest, q.sizes(), q.scalar_type(), "rest", q);
     const Attention call(q, k, v, q_ptr, k_ptr, k_len, causal, scale);
-    check_tensor(grad, q.sizes(), q.scalar_type(), "grad");
-    check_tensor(out, q.sizes(), q.scalar_type(), "out");
-    check_tensor(log2_sum, {q.size(1), oeq_attention_stat_stride(q.size(0))}, at::kFloat, "log2_sum");
-    if (rest.numel()) check_tensor(rest, q.sizes(), q.scalar_type(), "rest");
     OnDevice dev(q);
     const Rows g(grad);
     const Tensor o = whole(out), sums = log2_sum.contiguous(), r = whole(rest);
@@ -166,15 +167,15 @@ struct Rotary {
         TORCH_CHECK(d > 0 && d <= 128 && d % 8 == 0, "Shape mismatch for tensor 'q'. Expected: head_dim a multiple of 8 up to ",
                     "128. Got: ", q_.sizes());
         check_heads(k_, "k");
-        check_tensor(q_, q_.sizes(), q_.scalar_type(), "q");
-        check_tensor(k_, {n, k_.size(1), d}, q_.scalar_type(), "k");
-        check_tensor(positions_, {n}, at::kLong, "positions");
+        check_tensor(q_, q_.sizes(), q_.scalar_type(), "q", q_);
+        check_tensor(k_, {n, k_.size(1), d}, q_.scalar_type(), "k", q_);
+        check_tensor(positions_, {n}, at::kLong, "positions", q_);
         TORCH_CHECK(table_.dim() == 3 && table_.size(1) == 2 && table_.size(2) % 4 == 0 && 2 * table_.size(2) <= d,
                     "Shape mismatch for tensor 'table'. Expected: [positions, 2, rotary_dim / 2] with rotary_dim a multiple ",
                     "of 8 up to ", d, ". Got: ", table_.sizes());
-        check_tensor(table_, table_.sizes(), at::kFloat, "table");
-        if (q_weight_.has_value()) check_tensor(*q_weight_, {d}, q_.scalar_type(), "q_weight");
-        if (k_weight_.has_value()) check_tensor(*k_weight_, {d}, q_.scalar_type(), "k_weight");
+        check_tensor(table_, table_.sizes(), at::kFloat, "table", q_);
+        if (q_weight_.has_value()) check_tensor(*q_weight_, {d}, q_.scalar_type(), "q_weight", q_);
+        if (k_weight_.has_value()) check_tensor(*k_weight_, {d}, q_.scalar_type(), "k_weight", q_);
         TORCH_CHECK(eps >= 0, "qk_norm_rotary: eps must not be negative, got ", eps);
         q = Rows(q_), k = Rows(k_);
         positions = positions_.contiguous(), table = whole(table_);
@@ -205,9 +206,9 @@ Tensor2 qk_norm_rotary_gpu(const Tensor& q, const Tensor& k, const Tensor& posit
 Tensor4 qk_norm_rotary_backward_gpu(const Tensor& q_grad, const Tensor& k_grad, const Tensor& q, const Tensor& k,
                                     const Tensor& positions, const Tensor& table, const OptTensor& q_weight,
                                     const OptTensor& k_weight, double eps, bool interleaved) {
+    check_tensor(q_grad, q.sizes(), q.scalar_type(), "q_grad", q);
+    check_tensor(k_grad, k.sizes(), q.scalar_type(), "k_grad", q);
     const Rotary call(q, k, positions, table, q_weight, k_weight, eps, interleaved);
-    check_tensor(q_grad, q.sizes(), q.scalar_type(), "q_grad");
-    check_tensor(k_grad, k.sizes(), q.scalar_type(), "k_grad");
     OnDevice dev(q);
     const Rows gq(q_grad), gk(k_grad);
     Tensor dq = at::empty(q.sizes(), q.options()), dk = at::empty(k.sizes(), k.options());
@@ -226,12 +227,14 @@ Tensor4 qk_norm_rotary_backward_gpu(const Tensor& q_grad, const Tensor& k_grad, 
 Tensor qk_norm_rotary_append_gpu(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& positions,
                                  const Tensor& table, const Tensor& k_cache, const Tensor& v_cache, const Tensor& slots,
                                  const OptTensor& q_weight, const OptTensor& k_weight, double eps, bool interleaved) {
-    const Rotary call(q, k, positions, table, q_weight, k_weight, eps, interleaved);
-    check_tensor(v, k.sizes(), q.scalar_type(), "v");
+    check_heads(q, "q");
+    check_heads(k, "k");
+    check_tensor(v, k.sizes(), q.scalar_type(), "v", q);
     check_heads(k_cache, "k_cache");
-    check_tensor(k_cache, {k_cache.size(0), k.size(1), k.size(2)}, q.scalar_type(), "k_cache");
-    check_tensor(v_cache, k_cache.sizes(), q.scalar_type(), "v_cache");
-    check_tensor(slots, {q.size(0)}, at::kLong, "slots");
+    check_tensor(k_cache, {k_cache.size(0), k.size(1), k.size(2)}, q.scalar_type(), "k_cache", q);
+    check_tensor(v_cache, k_cache.sizes(), q.scalar_type(), "v_cache", q);
+    check_tensor(slots, {q.size(0)}, at::kLong, "slots", q);
+    const Rotary call(q, k, positions, table, q_weight, k_weight, eps, interleaved);
     // the caches are written in place: a copy would not do
     TORCH_CHECK(Rows::fits(k_cache) && Rows::fits(v_cache), "qk_norm_rotary_append: the caches need heads whose elements are ",
                 "contiguous and rows and heads that begin at multiples of 16 bytes");
@@ -253,10 +256,10 @@ Tensor qk_norm_rotary_append_gpu(const Tensor& q, const Tensor& k, const Tensor&
 Tensor irrep_dropout_gpu(const Tensor& x, const OptTensor& residual, const Tensor& channels, const Tensor& seed, double p) {
     TORCH_CHECK(x.dim() == 2, "Shape mismatch for tensor 'x'. Expected: [rows, irreps.dim]. Got: ", x.sizes());
     const int type = element_of(x, "x", true);
-    check_tensor(x, {x.size(0), channels.dim() == 1 ? channels.size(0) : -1}, x.scalar_type(), "x");
-    check_tensor(channels, {x.size(1)}, at::kInt, "channels");
-    check_tensor(seed, {2}, at::kLong, "seed");
-    if (residual.has_value()) check_tensor(*residual, x.sizes(), x.scalar_type(), "residual");
+    check_tensor(x, {x.size(0), channels.dim() == 1 ? channels.size(0) : -1}, x.scalar_type(), "x", x);
+    check_tensor(channels, {x.size(1)}, at::kInt, "channels", x);
+    check_tensor(seed, {2}, at::kLong, "seed", x);
+    if (residual.has_value()) check_tensor(*residual, x.sizes(), x.scalar_type(), "residual", x);
     TORCH_CHECK(p >= 0 && p <= 1, "irrep_dropout: p must be between 0 and 1, got ", p);
     OnDevice dev(x);
     const Tensor in = whole(x), index = channels.contiguous(), key = seed.contiguous();

@@ -228,3 +228,60 @@ def test_forward_mode_derivatives_are_right_or_refused():
         assert forward_ad.unpack_dual(module(x, x, seed=seed)).tangent is None
     value, tangent = torch.func.jvp(lambda t: module(t, seed=seed), (x,), (x,))
     assert value.shape == tangent.shape == x.shape
+
+
+class _Elsewhere(torch.Tensor):
+    """A tensor that says which GPU it is on and has no memory."""
+
+    @staticmethod
+    def __new__(cls, *shape, device=0, dtype=torch.float32):
+        return torch.Tensor._make_wrapper_subclass(cls, shape, dtype=dtype, device=f"cuda:{device}")
+
+    @classmethod
+    def __torch_dispatch__(cls, func, types, args=(), kwargs=None):
+        raise NotImplementedError(func)
+
+
+def test_operands_on_another_gpu_are_refused():
+    """Every operand in turn, by the GPU's code of the op itself (which ends at its checks)."""
+    t, i64 = _Elsewhere, torch.int64
+
+    def make(shape, device):
+        dtype = shape[-1] if isinstance(shape[-1], torch.dtype) else torch.float32
+        return t(*[n for n in shape if not isinstance(n, torch.dtype)], device=device, dtype=dtype)
+
+    problem = oeq.TPProblem("4x0e", "1x0e", "4x0e", [(0, 0, 0, "uvu", True)], shared_weights=False, internal_weights=False)
+    product, conv = oeq.TensorProduct(problem), oeq.TensorProductConv(problem)
+    n, wn = 5, problem.weight_numel
+    attention = dict(q=(7, 4, 32), k=(9, 2, 32), v=(9, 2, 32), q_ptr=(3, i64), k_ptr=(3, i64), k_len=(2, i64))
+    rotary = dict(q=(7, 4, 32), k=(7, 2, 32), positions=(7, i64), table=(5, 2, 8), q_weight=(32,), k_weight=(32,))
+    ops = torch.ops.oeq_amd
+    calls = [
+        (attention, lambda a: ops.packed_attention.default.redispatch(_cuda(), *a.values(), False, 0.5)),
+        (dict(grad=(7, 4, 32), **{n: s for n, s in attention.items() if n in "qkv"}, out=(7, 4, 32), log2_sum=(4, 128),
+              rest=(0,), q_ptr=(3, i64), k_ptr=(3, i64)),
+         lambda a: ops.packed_attention_backward.default.redispatch(_cuda(), *a.values(), None, False, 0.5)),
+        (rotary, lambda a: ops.qk_norm_rotary.default.redispatch(_cuda(), *a.values(), 1e-6, False)),
+        (dict(q_grad=(7, 4, 32), k_grad=(7, 2, 32), **rotary),
+         lambda a: ops.qk_norm_rotary_backward.default.redispatch(_cuda(), *a.values(), 1e-6, False)),
+        (dict(q=(7, 4, 32), k=(7, 2, 32), v=(7, 2, 32), positions=(7, i64), table=(5, 2, 8), k_cache=(20, 2, 32),
+              v_cache=(20, 2, 32), slots=(7, i64)),
+         lambda a: ops.qk_norm_rotary_append.default.redispatch(_cuda(), *a.values(), None, None, 1e-6, False)),
+        (dict(x=(5, 4), residual=(5, 4), channels=(4, torch.int32), seed=(2, i64)),
+         lambda a: ops.irrep_dropout.default.redispatch(_cuda(), *a.values(), 0.5)),
+        (dict(x=(n, 4), y=(n, 1), w=(n, wn)),
+         lambda a: ops.tp_forward.default.redispatch(_cuda(), *a.values(), product.kid, None)),
+        (dict(x=(6, 4), y=(n, 1), w=(n, wn), rows=(n, i64), cols=(n, i64)),
+         lambda a: ops.conv_forward.default.redispatch(_cuda(), *a.values(), make((0, i64), 0), conv.kid, None)),
+    ]
+    for shapes, call in calls:
+        for name in shapes:
+            if name == "rest":  # (empty: not read)
+                continue
+            args = {m: make(s, int(m == name)) for m, s in shapes.items()}
+            with pytest.raises(RuntimeError, match="is on cuda:"):
+                call(args)
+
+
+def _cuda():
+    return torch._C.DispatchKeySet(torch._C.DispatchKey.CUDA)
