@@ -177,6 +177,9 @@ class IrrepDropout(torch.nn.Module):
     :param irreps: of the features' last dimension, e.g. ``"128x0e+128x1o"``.
     :param p: probability of a channel to be dropped, in steps of 2^-16.
     :param layout: ``"mul_ir"`` or ``"ir_mul"``, as in :class:`TPProblem`.
+
+    A module that was not moved to the GPU moves its table there with its first call, except while a graph is captured:
+    move the module before.
     """
 
     def __init__(self, irreps, p: float, layout: str = "mul_ir"):
@@ -197,6 +200,21 @@ class IrrepDropout(torch.nn.Module):
     def extra_repr(self) -> str:
         return f"{self.irreps}, p={self.p}, layout={self.layout!r}"
 
+    def _channels_on(self, x: torch.Tensor) -> torch.Tensor:
+        """The table of a module that was not moved to its input's device: it moves with the first call. Not while a graph
+        is captured (the copy from host memory would end the capture, and what it allocates belong to the graph), and
+        not as a tensor of inference mode, which later training steps could not save."""
+        if torch.compiler.is_compiling():
+            return self.channels.to(x.device)
+        if x.is_cuda and torch.cuda.is_current_stream_capturing():
+            raise RuntimeError(f"IrrepDropout is on {self.channels.device} and its input on {x.device}: move the module there "
+                               "before a graph is captured")
+        with torch.inference_mode(False):
+            channels = self.channels.to(x.device)
+        if type(channels) is torch.Tensor:  # (not a traced stand-in)
+            self.channels = channels
+        return channels
+
     def forward(self, x: torch.Tensor, residual: Optional[torch.Tensor] = None, *,
                 seed: Optional[torch.Tensor] = None) -> torch.Tensor:
         r"""
@@ -210,11 +228,7 @@ class IrrepDropout(torch.nn.Module):
             return x if residual is None else x + residual
         if seed is None:
             seed = torch.empty(2, dtype=torch.int64, device=x.device).random_()
-        channels = self.channels
-        if channels.device != x.device:  # (a module that was not moved: its table moves with the first call)
-            channels = channels.to(x.device)
-            if not torch.compiler.is_compiling():
-                self.channels = channels
+        channels = self.channels if self.channels.device == x.device else self._channels_on(x)
         if residual is not None and torch.is_autocast_enabled("cuda"):
             x = x.to(residual.dtype)  # (a projection in 16 bits on its way into a stream in 32)
         return _irrep_dropout(x, residual, channels, seed, self.p)

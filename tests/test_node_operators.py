@@ -285,3 +285,14 @@ def test_operands_on_another_gpu_are_refused():
 
 def _cuda():
     return torch._C.DispatchKeySet(torch._C.DispatchKey.CUDA)
+
+
+def test_dropout_of_a_module_first_called_in_inference_mode():
+    """Its table moves to the input's device with that call and stays good for training."""
+    x, seed = torch.empty(3, 4, device="meta"), torch.empty(2, dtype=torch.int64, device="meta")
+    for mode in (torch.inference_mode, torch.no_grad):
+        module = oeq.IrrepDropout("1x0e+1x1o", 0.1)
+        with mode():
+            module(x, seed=seed)
+        assert module.channels.device.type == "meta" and not module.channels.is_inference()
+        assert module(x.clone().requires_grad_(), seed=seed).requires_grad

@@ -663,3 +663,25 @@ def test_forward_mode_derivative_of_dropout():
     with pytest.raises(RuntimeError, match="no forward-mode derivative"):
         torch.func.jvp(lambda t: oeq.qk_norm_rotary(t, q, torch.arange(11, device="cuda"), oeq.rotary_table(11, 8, device="cuda")),
                        (q,), (q,))
+
+
+def test_dropout_of_a_module_that_was_not_moved():
+    x, seed = normal(20, 11), on_gpu([7, 8])
+    want = oeq.IrrepDropout("5x0e+2x1o", 0.4).cuda()(x, seed=seed)
+    module = oeq.IrrepDropout("5x0e+2x1o", 0.4)
+    graph = torch.cuda.CUDAGraph()
+    y = torch.zeros(4, device="cuda")
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        y.add_(1)
+        with pytest.raises(RuntimeError, match="before a graph is captured"):
+            module(x, seed=seed)
+    assert module.channels.device.type == "cpu"
+    graph.replay()
+    torch.cuda.synchronize()
+    assert (y == 1).all()  # the capture went on
+    with torch.inference_mode():
+        assert torch.equal(module(x, seed=seed), want)
+    leaf = x.clone().requires_grad_()
+    grad, = torch.autograd.grad(module(leaf, seed=seed).sum(), leaf)
+    assert torch.equal(grad != 0, want != 0)
