@@ -445,6 +445,15 @@ Tensor qk_norm_rotary_append_autograd(const Tensor& q, const Tensor& k, const Te
     TORCH_CHECK(!records(q, k, v, k_cache, v_cache, q_weight, k_weight),
                 "qk_norm_rotary_append writes into the caches and has no gradient: call it under torch.no_grad(), or ",
                 "qk_norm_rotary where gradients are needed");
+    at::AutoDispatchBelowAutograd below;
+    return OEQ_OP(qk_norm_rotary_append)
+        .call(q, k, v, positions, table, k_cache, v_cache, slots, q_weight, k_weight, eps, interleaved);
+}
+
+// Also in inference mode, which skips the function above: a cache that autograd has saved is known to have changed.
+Tensor qk_norm_rotary_append_in_place(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& positions,
+                                      const Tensor& table, const Tensor& k_cache, const Tensor& v_cache, const Tensor& slots,
+                                      const OptTensor& q_weight, const OptTensor& k_weight, double eps, bool interleaved) {
     at::AutoDispatchBelowADInplaceOrView below;
     Tensor out = OEQ_OP(qk_norm_rotary_append)
         .call(q, k, v, positions, table, k_cache, v_cache, slots, q_weight, k_weight, eps, interleaved);
@@ -484,3 +493,5 @@ TORCH_LIBRARY_IMPL(oeq_amd, Autograd, m) {
     m.impl("qk_norm_rotary_append", qk_norm_rotary_append_autograd);
     m.impl("irrep_dropout", irrep_dropout_autograd);
 }
+
+TORCH_LIBRARY_IMPL(oeq_amd, ADInplaceOrView, m) { m.impl("qk_norm_rotary_append", qk_norm_rotary_append_in_place); }

@@ -296,3 +296,20 @@ def test_dropout_of_a_module_first_called_in_inference_mode():
             module(x, seed=seed)
         assert module.channels.device.type == "meta" and not module.channels.is_inference()
         assert module(x.clone().requires_grad_(), seed=seed).requires_grad
+
+
+def test_caches_that_are_written_count_it():
+    """What autograd saved of a cache is known to have changed, whatever mode wrote to it."""
+    def operands():
+        q, k = torch.empty(7, 4, 32, device="meta"), torch.empty(7, 2, 32, device="meta")
+        at, table = torch.empty(7, device="meta", dtype=torch.int64), torch.empty(5, 2, 8, device="meta")
+        return q, k, k, at, table, torch.empty(20, 2, 32, device="meta"), torch.empty(20, 2, 32, device="meta"), at
+
+    args = operands()
+    written = args[5:7]
+    for n, mode in enumerate((torch.no_grad, torch.inference_mode, torch.enable_grad), 1):
+        with mode():
+            oeq.qk_norm_rotary_append(*args)
+        assert [c._version for c in written] == [n, n] and args[0]._version == 0
+    with torch.inference_mode():
+        assert oeq.qk_norm_rotary_append(*operands()).shape == (7, 4, 32)  # caches without a count
