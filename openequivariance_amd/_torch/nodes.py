@@ -146,7 +146,7 @@ def qk_norm_rotary(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, ta
         :func:`packed_attention`.
     :param positions: ``[rows]``, int64, each a row of ``table`` (another gives NaN).
     :param table: ``[positions, 2, rotary_dim / 2]`` cosines and sines (:func:`rotary_table`). The first ``rotary_dim``
-        elements of a head are turned, the rest only normed.
+        elements of a head are turned, the rest only normed. It has no gradient.
     :param q_weight, k_weight: ``[head_dim]``: ``x -> weight x / sqrt(mean(x^2) + eps)``; no norm where left out.
     :param interleaved: pairs are neighbours ``2 i, 2 i + 1`` instead of ``i, i + rotary_dim / 2``.
     """

@@ -398,9 +398,14 @@ Tensor3 packed_attention_backward_autograd(const Tensor& grad, const Tensor& q, 
     return OEQ_OP(packed_attention_backward).call(grad, q, k, v, out, log2_sum, rest, q_ptr, k_ptr, k_len, causal, scale);
 }
 
+void check_table(const Tensor& table) {
+    TORCH_CHECK(!records(table), "qk_norm_rotary: the table has no gradient (pass table.detach())");
+}
+
 Tensor2 qk_norm_rotary_autograd(const Tensor& q, const Tensor& k, const Tensor& positions, const Tensor& table,
                                 const OptTensor& q_weight, const OptTensor& k_weight, double eps, bool interleaved) {
     refuse_tangents("oeq_amd::qk_norm_rotary", q, k, table, q_weight, k_weight);
+    check_table(table);
     if (records(q, k, q_weight, k_weight)) {
         const auto out = QkNormRotary::apply(q, k, positions, table, q_weight, k_weight, eps, interleaved);
         return {out[0], out[1]};
@@ -428,6 +433,7 @@ Tensor4 qk_norm_rotary_backward_autograd(const Tensor& q_grad, const Tensor& k_g
                                          const Tensor& positions, const Tensor& table, const OptTensor& q_weight,
                                          const OptTensor& k_weight, double eps, bool interleaved) {
     refuse_tangents("oeq_amd::qk_norm_rotary_backward", q_grad, k_grad, q, k, table, q_weight, k_weight);
+    check_table(table);
     if (records(q_grad, k_grad, q, k, q_weight, k_weight)) {
         const auto g = QkNormRotaryGradient::apply(q_grad, k_grad, q, k, positions, table, q_weight, k_weight, eps, interleaved);
         return {g[0], g[1], g[2], g[3]};

@@ -313,3 +313,13 @@ def test_caches_that_are_written_count_it():
         assert [c._version for c in written] == [n, n] and args[0]._version == 0
     with torch.inference_mode():
         assert oeq.qk_norm_rotary_append(*operands()).shape == (7, 4, 32)  # caches without a count
+
+
+def test_a_table_that_wants_a_gradient_is_refused():
+    q, k = torch.empty(7, 4, 32, device="meta", requires_grad=True), torch.empty(7, 2, 32, device="meta")
+    at, table = torch.empty(7, device="meta", dtype=torch.int64), torch.empty(5, 2, 8, device="meta", requires_grad=True)
+    with pytest.raises(RuntimeError, match="table has no gradient"):
+        oeq.qk_norm_rotary(q, k, at, table)
+    assert oeq.qk_norm_rotary(q, k, at, table.detach())[0].requires_grad
+    with torch.no_grad():
+        oeq.qk_norm_rotary(q, k, at, table)
