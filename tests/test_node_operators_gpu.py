@@ -635,7 +635,7 @@ def test_autocast():
 def test_causal_ends_past_the_tensors_have_one_diagonal(dtype, end, rows, keys):
     """A segment that is said to go on behind the tensors is the one that is cut off there: its last row sees every key,
     in the output and in all gradients."""
-    end += rows
+    end += max(rows, keys)
     leaves = [normal(n, h, 32, dtype=dtype, seed=s).requires_grad_() for s, (n, h) in enumerate(((rows, 4), (keys, 2), (keys, 2)))]
     g = normal(rows, 4, 32, dtype=dtype, seed=5)
     results = []
