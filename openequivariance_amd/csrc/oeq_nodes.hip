@@ -263,7 +263,9 @@ int oeq_attention_forward(const oeq_attention* a, void* out, void* out_rest, flo
 size_t oeq_attention_backward_workspace_bytes(const oeq_attention* a) {
     if (!a || a->q_heads <= 0 || a->q_rows < 0 || a->k_rows < 0) return 0;
     const size_t delta = (size_t)a->q_heads * oeq_attention_stat_stride(a->q_rows) * sizeof(float);
-    return delta + (ordered(*a) ? 2 * (size_t)(query_tiles(*a) + key_tiles(*a)) * sizeof(int) : 0);
+    // (of float16 a number for each tile of each head, where a tile has 64 rows or more)
+    const size_t lifts = a->type == OEQ_FLOAT16 ? (size_t)a->q_heads * ((a->q_rows + 63) / 64) * sizeof(float) : 0;
+    return delta + lifts + (ordered(*a) ? 2 * (size_t)(query_tiles(*a) + key_tiles(*a)) * sizeof(int) : 0);
 }
 
 int oeq_attention_backward(const oeq_attention* a, const void* out, const void* out_rest, const float* log2_sum,
@@ -286,8 +288,10 @@ int oeq_attention_backward(const oeq_attention* a, const void* out, const void* 
     g.dq = q_grad, g.dk = k_grad, g.dv = v_grad, g.lse = (float*)log2_sum, g.delta = (float*)workspace;
     const auto s = (hipStream_t)stream;
     const int ktiles = (int)key_tiles(*a);
+    g.lifts = g.delta + a->q_heads * g.stat_stride;
+    g.q_tiles = g.tiles;
     if (ordered(*a)) {
-        int* q_order = (int*)(g.delta + a->q_heads * g.stat_stride);
+        int* q_order = (int*)(g.lifts + (a->type == OEQ_FLOAT16 ? (int64_t)a->q_heads * g.tiles : 0));
         int* k_order = q_order + 2 * (int64_t)g.tiles;
         g.q_order = q_order, g.k_order = k_order;
         packed_attention::order_tiles<<<2, 1024, 0, s>>>(g, q_order, g.tiles, k_order, ktiles);

@@ -51,6 +51,8 @@ struct Args {
     const int *q_order, *k_order;  // tiles by the length of their walks, or NULL
     int parts;  // the form for few queries: shares of a row's keys, and their results
     float* partial;
+    float* lifts;  // what the queries' gradient lifted ds by in each tile (see lifted_operands): [q_heads, q_tiles]
+    int q_tiles;
 };
 
 typedef float float4_t __attribute__((ext_vector_type(4)));
@@ -70,7 +72,8 @@ typedef __attribute__((address_space(3))) short4_t* ltr_t;
 // Powers of two that p and ds carry while they are operands, so that small ones keep their bits (v_exp_f32 knows no
 // numbers below 2^-126, and 16-bit floats of eleven bits end at 2^-24, a weight among 10^7 equal ones); they leave the
 // sums at the end. In the forward pass p reaches 2^8 before that (its maximum is an older one), in the gradients 1.
-// ds of eleven bits is left as it is: its size is that of the output's gradient, whose scale is the caller's choice.
+// ds of eleven bits has no fixed power of two: its size is that of the output's gradient, which may be anything that the
+// caller's scale of the loss makes of it (see lifted_operands).
 template <typename T>
 struct Types;
 template <>
@@ -83,7 +86,7 @@ template <>
 struct Types<_Float16> {
     typedef half8_t frag;
     typedef half4_t quad;
-    static constexpr int kForward = 7, kP = 12, kDs = 0;
+    static constexpr int kForward = 7, kP = 12, kDs = 60;  // (kDs: before any is seen)
 };
 template <>
 struct Types<__bf16> {
@@ -91,6 +94,8 @@ struct Types<__bf16> {
     typedef bf4_t quad;
     static constexpr int kForward = 0, kP = 40, kDs = 40;
 };
+template <typename T>
+constexpr bool kLifted = Types<T>::kForward > 0;  // elements of eleven bits
 template <int N>
 constexpr float power = N > 0 ? (float)(1ull << (N > 0 ? N : 0)) : 1.0f / (float)(1ull << (N < 0 ? -N : 0));
 
@@ -132,6 +137,11 @@ __device__ __forceinline__ float wave_sum(float x) {
 __device__ __forceinline__ int wave_min(int x) {
 #pragma unroll
     for (int m = 1; m < 64; m <<= 1) x = min(x, __shfl_xor(x, m));
+    return x;
+}
+__device__ __forceinline__ float wave_least(float x) {
+#pragma unroll
+    for (int m = 1; m < 64; m <<= 1) x = fminf(x, __shfl_xor(x, m));
     return x;
 }
 __device__ __forceinline__ int wave_max(int x) {
@@ -249,6 +259,32 @@ __device__ __forceinline__ typename Types<T>::frag operand(const float16_t& s, i
         for (int j = 0; j < 4; ++j) x[j] = s[4 * f + j];
     }
     return x;
+}
+
+// ds of eleven bits as operands. Every lane carries it at a power of two of its own: 2^kDs until it has seen one, less
+// where one would pass 2, so that the largest is about 2^-4. Terms then keep their bits, or are off by 2^-21 of the largest
+// seen, whatever the size of the output's gradient, and none overflows (gradients of size 1e-4 at 4 096 keys without that:
+// an error of 5 %, not 0.7). `lowered` is called with what changes that power of two. The operands' own bits tell: one of their
+// exponents has its highest bit set from 2 on. (Only in the queries' gradient, which 9 sequences, heads of 128, take 219
+// us for instead of 204. The keys' one, with one wave to a SIMD, took 450 instead of 390 that way; it goes by what the
+// queries' found, one power of two for a block, and takes no longer.)
+template <typename T, typename L>
+__device__ __forceinline__ void lifted_operands(float16_t& x, typename Types<T>::frag (&d)[2], L lowered) {
+#pragma unroll
+    for (int f = 0; f < 2; ++f) d[f] = operand<T>(x, f);
+    const uint4_t a = __builtin_bit_cast(uint4_t, d[0]), b = __builtin_bit_cast(uint4_t, d[1]);
+    const unsigned any = a[0] | a[1] | a[2] | a[3] | b[0] | b[1] | b[2] | b[3];
+    if (!__any(any & 0x40004000u)) return;
+    float top = 0;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) top = fmaxf(top, fabsf(x[r]));
+    top = max_halves(top);
+    const int n = top >= 2.0f && finite(top) ? __builtin_amdgcn_frexp_expf(top) + 3 : 0;  // (an infinity stays)
+    const float by = __builtin_amdgcn_ldexpf(1.0f, -n);
+    lowered(by);
+    x *= by;
+#pragma unroll
+    for (int f = 0; f < 2; ++f) d[f] = operand<T>(x, f);
 }
 
 // Fragments of a lane's row straight from memory; `chunks` of 16 bytes exist.
@@ -1061,10 +1097,12 @@ __global__ __launch_bounds__(256, (blocks_per_unit<T, DP>())) void query_gradien
     if (mine && half == 0) a.delta[h * a.stat_stride + i] = delta;
     const float lse = a.lse[h * a.stat_stride + i], c = a.scale_log2;
     settle();
+    float lift = power<Types<T>::kDs>, low = delta * (kLifted<T> ? lift : 1.0f);
     float16_t acc[DT];
 #pragma unroll
     for (int t = 0; t < DT; ++t) acc[t] = 0.0f;
 
+    constexpr bool kAnew = kLifted<T> && DP == 128 && SPLIT == 1;  // (no register is left for the places)
     auto products = [&](const char* kt, const char* vt, int first) {
 #pragma unroll
         for (int n = 0; n < SUB; ++n) {
@@ -1077,8 +1115,10 @@ __global__ __launch_bounds__(256, (blocks_per_unit<T, DP>())) void query_gradien
             for (int f = 0; f < L::kFrags; ++f) x = mma(L::row(vt, 32 * u + (lane & 31), f, half), g[f], x);
 #pragma unroll
             for (int r = 0; r < 16; ++r) {
-                const float p = raised<T, Types<T>::kDs>(fmaf(s[r], c, -lse));
-                x[r] = p * (x[r] - delta);
+                if constexpr (kLifted<T>)
+                    x[r] = __builtin_amdgcn_exp2f(fmaf(s[r], c, -lse)) * fmaf(x[r], lift, -low);
+                else
+                    x[r] = raised<T, Types<T>::kDs>(fmaf(s[r], c, -lse)) * (x[r] - low);
             }
             if (!(SPLIT == 2 || kSparse<T, DP> ? walk.whole(first + 32 * u, 32) : walk.whole(first, BK))) {
                 const int shift = first + 32 * u + 4 * half - b.lo;
@@ -1087,11 +1127,19 @@ __global__ __launch_bounds__(256, (blocks_per_unit<T, DP>())) void query_gradien
                 for (int r = 0; r < 16; ++r)
                     if ((unsigned)(shift + 8 * (r / 4) + r % 4) >= n) x[r] = 0.0f;
             }
+            const Lane anew = Lane::of<kAnew>(lane, half);
+            typename L::frag lifted[2];
+            if constexpr (kLifted<T>)
+                lifted_operands<T>(x, lifted, [&](float by) {
+                    lift *= by, low *= by;
+#pragma unroll
+                    for (int t = 0; t < DT; ++t) acc[t] *= by;
+                });
 #pragma unroll
             for (int f = 0; f < PF; ++f) {
-                const auto p = operand<T>(x, f);
+                const auto d = kLifted<T> ? lifted[f & 1] : operand<T>(x, f);
 #pragma unroll
-                for (int t = 0; t < DT; ++t) acc[t] = mma(column_of<T, DP, BK>(kt, 32 * u, f, t, lane), p, acc[t]);
+                for (int t = 0; t < DT; ++t) acc[t] = mma(column_of<T, DP, BK>(kt, 32 * u, f, t, kAnew ? anew.at : lane), d, acc[t]);
             }
             __builtin_amdgcn_sched_barrier(0);  // (reads of the next 32 keys this early would take registers that are not there)
         }
@@ -1108,10 +1156,19 @@ __global__ __launch_bounds__(256, (blocks_per_unit<T, DP>())) void query_gradien
         step(key0, val0, key1, val1, first);
         if (first + BK < all.hi) step(key1, val1, key0, val0, first + BK);
     }
+    const float scale = c * 0.6931471805599453f * (kLifted<T> ? 1.0f / lift : power<-Types<T>::kDs>);
+    if constexpr (kLifted<T>) {
+        __shared__ float least[4];
+        const float mine = wave_least(lift);
+        if (lane == 0) least[wave] = mine;
+        __syncthreads();
+        if (threadIdx.x == 0) a.lifts[(int64_t)h * a.q_tiles + tile] = fminf(fminf(least[0], least[1]), fminf(least[2], least[3]));
+    }
     if constexpr (SPLIT == 2) {
         // the wave with the second groups of keys hands its sums to the one with the first, 32 columns of the head at a time
 #pragma unroll
         for (int t = 0; t < DT; ++t) {
+            acc[t] *= scale;  // (the two may be lifted differently)
             __syncthreads();
             if (part)
 #pragma unroll
@@ -1127,7 +1184,7 @@ __global__ __launch_bounds__(256, (blocks_per_unit<T, DP>())) void query_gradien
         if (part) return;
     }
     if (mine)
-        store_row<T, DT>((T*)a.dq + ((int64_t)i * a.hq + h) * a.d, acc, c * (0.6931471805599453f * power<-Types<T>::kDs>), a.d, half);
+        store_row<T, DT>((T*)a.dq + ((int64_t)i * a.hq + h) * a.d, acc, SPLIT == 2 ? 1.0f : scale, a.d, half);
     uint64_t bad = __ballot(mine && !all_finite<DT>(acc));
     bad = (bad | bad >> 32) & 0xffffffffu;
     while (bad) {
@@ -1201,7 +1258,14 @@ __global__ __launch_bounds__(256, UNIT) void key_gradient(Args a) {
     for (int t = 0; t < DT; ++t) dk[t] = 0.0f, dv[t] = 0.0f;
     settle();
 
-    constexpr float kRatio = power<Types<T>::kDs - Types<T>::kP>;
+    // What ds carries over what p does; where it is lifted, as far as the queries' gradient has found that none passes 2^14.
+    float ratio = power<Types<T>::kDs - Types<T>::kP>;
+    if constexpr (kLifted<T>) {
+        float lift = power<Types<T>::kDs>;
+        const int each = 128 / a.split, tile0 = all.lo / each, tiles = all.lo < all.hi ? (all.hi - 1) / each - tile0 + 1 : 0;
+        for (int n = lane; n < tiles * group; n += 64) lift = fminf(lift, a.lifts[(int64_t)(kh * group + n / tiles) * a.q_tiles + tile0 + n % tiles]);
+        ratio = wave_least(lift) * power<13 - Types<T>::kP>;
+    }
     // p and ds from the scores and g.v
     auto weigh = [&](float16_t& s, float16_t& x, const float* st) {
 #pragma unroll
@@ -1212,7 +1276,7 @@ __global__ __launch_bounds__(256, UNIT) void key_gradient(Args a) {
             for (int e = 0; e < 4; ++e) {
                 const int r = 4 * g + e;
                 s[r] = raised<T, Types<T>::kP>(fmaf(s[r], c, -lse[e]));
-                if (DK) x[r] = s[r] * fmaf(x[r], kRatio, -delta[e] * kRatio);
+                if (DK) x[r] = s[r] * fmaf(x[r], ratio, -delta[e] * ratio);
             }
         }
     };
@@ -1325,7 +1389,7 @@ __global__ __launch_bounds__(256, UNIT) void key_gradient(Args a) {
     const bool mine = row < a.nk;
     if (mine) {
         const int64_t at = ((int64_t)j * a.hk + kh) * a.d;
-        if (DK) store_row<T, DT>((T*)a.dk + at, dk, c * (0.6931471805599453f * power<-Types<T>::kDs>), a.d, half);
+        if (DK) store_row<T, DT>((T*)a.dk + at, dk, c * (0.6931471805599453f * power<-Types<T>::kP> / ratio), a.d, half);
         if (DV) store_row<T, DT>((T*)a.dv + at, dv, power<-Types<T>::kP>, a.d, half);
     }
     uint64_t bad = __ballot(mine && !((!DK || all_finite<DT>(dk)) && (!DV || all_finite<DT>(dv))));

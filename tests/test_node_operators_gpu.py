@@ -685,3 +685,49 @@ def test_dropout_of_a_module_that_was_not_moved():
     leaf = x.clone().requires_grad_()
     grad, = torch.autograd.grad(module(leaf, seed=seed).sum(), leaf)
     assert torch.equal(grad != 0, want != 0)
+
+
+# ---------------------------------------------------------------------------
+# errors as a whole
+# ---------------------------------------------------------------------------
+
+
+def gradients_64(q, k, v, g, causal=False):
+    """(values, sums of the squared terms) of out, dq, dk and dv of one segment with a head of keys for each of queries,
+    in 64 bits: {name: (value, terms)}. The terms of a sum carry the roundings of its operands."""
+    q, k, v, g = (t.detach().double().transpose(0, 1).contiguous() for t in (q, k, v, g))
+    c = q.shape[2] ** -0.5
+    kt, vt = k.transpose(1, 2).contiguous(), v.transpose(1, 2).contiguous()
+    s = torch.bmm(q, kt) * c
+    if causal:
+        s += torch.full(s.shape[1:], -math.inf, dtype=s.dtype, device=s.device).triu(1 + s.shape[2] - s.shape[1])
+    p = torch.softmax(s, 2)
+    out = torch.bmm(p, v)
+    ds = p * (torch.bmm(g, vt) - (g * out).sum(2, keepdim=True))
+    pt, dst = p.transpose(1, 2).contiguous(), ds.transpose(1, 2).contiguous()
+    pairs = dict(out=(p, v, 1.0), dq=(ds, k, c), dk=(dst, q, c), dv=(pt, g, 1.0))
+    return {n: ((torch.bmm(a, b) * f).transpose(0, 1), (torch.bmm(a * a, b * b) * f * f).transpose(0, 1))
+            for n, (a, b, f) in pairs.items()}
+
+
+def check_norm(got, value, terms, dtype, what, more=0.0):
+    """The norm of the error, against that of independent roundings of one operand of each term (16-bit types) and of the
+    result, every one taken at its largest and the whole twice: `more` is what 32-bit sums may add of the value's norm."""
+    u, tiny = N.HALF_UNIT[dtype], N.TINY[dtype]
+    allowed = ((u * u * value * value + tiny * tiny).sum() + (u * u * terms.sum() if dtype != F32 else 0.0)).sqrt()
+    error = (got.double() - value).norm()
+    assert error <= 2 * allowed + more * value.norm(), f"{what}: {error / value.norm():.2e} of its norm, {allowed / value.norm():.2e}"
+
+
+@pytest.mark.parametrize("size", [1e-5, 1e-4, 1e-2, 1.0, 1e4])
+@pytest.mark.parametrize("d", [64, 96, 128])
+@pytest.mark.parametrize("rows,keys", [(256, 4096), (4096, 300), (4, 3)])
+def test_float16_gradients_of_any_size(rows, keys, d, size):
+    """The size of the output's gradient is the caller's choice (a loss that is scaled, or is not): it costs gradients no bits."""
+    q, k, v = (normal(n, 2, d, dtype=F16, seed=s).requires_grad_() for s, n in enumerate((rows, keys, keys)))
+    g = (size * normal(rows, 2, d, seed=5)).to(F16)
+    out = oeq.packed_attention(q, k, v, on_gpu([0, rows]), on_gpu([0, keys]))
+    want = gradients_64(q, k, v, g)
+    for name, x in zip(("dq", "dk", "dv"), torch.autograd.grad(out, (q, k, v), g)):
+        # (32-bit sums of a few thousand terms: some 2^-24 of them each)
+        check_norm(x, *want[name], F16, name, more=2.0 ** -18)
