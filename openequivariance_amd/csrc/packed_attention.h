@@ -8,7 +8,8 @@
 // dq_i = c sum_j ds_ij k_j,  dk_j = c sum_i ds_ij q_i, the last two sums over the query heads that share a key head too.
 // Scores, p, ds and all sums are held in 32 bits; where operands have 16, p and ds are rounded to their type as
 // operands of the second products (the products themselves are exact in 32 bits), which costs an error of the size of
-// the output's own rounding. delta would add a third such error where rows see few keys, were it taken from the rounded
+// the output's own rounding and halves the work of these products, which bound the tiles of rows (the form for few queries,
+// bound by memory, does without it). delta would add a third such error where rows see few keys, were it taken from the rounded
 // output: a pass that will be differentiated keeps what the rounding took off beside it (`rest`, 16 bits).
 //
 // Layout of the products. All of them run on the 32x32 matrix instructions with the *transposed* result in registers:
@@ -786,7 +787,9 @@ __global__ __launch_bounds__(256, (blocks_per_unit<T, DP>())) void forward(Args 
 // the query heads that share the key head (up to 32) are the columns of the products, so that keys and values are read
 // once for all of them. Each wave walks tiles of 32 keys of its own through LDS, the next one always on its way, and
 // meets the others only at the end. Rows past the share's end are cut off by the reads' bounds and arrive as zeros. Shares
-// of more than one block's row meet in `join`, in the order of the keys. Bound by memory: a token against 65 537 keys, 32 / 8
+// of more than one block's row meet in `join`, in the order of the keys. p of 16 bits goes in two parts, itself and what its
+// rounding took off, so that nothing but the output is rounded: the second products are done while memory is waited for.
+// Bound by memory: a token against 65 537 keys, 32 / 8
 // heads of 128, bf16, 59 us with the join (6), 4.5 TB/s of 268 MB where a copy reaches 4.7; 64 tokens against 1 to 4 096 keys
 // each, 16 / 4 heads, fp16, 70 us for the same bytes; 7 tokens against up to 60 keys 7 us, about a launch.
 
@@ -901,8 +904,19 @@ __global__ __launch_bounds__((64 * Few<T, DP>::kWaves), 1) void forward_few(Args
 #pragma unroll
         for (int f = 0; f < PF; ++f) {
             const auto p = operand<T>(s, f);
+            auto rest = p;
+            if constexpr (sizeof(T) == 2) {
+                float8_t w;
 #pragma unroll
-            for (int t = 0; t < DT; ++t) acc[t] = mma(column_of<T, DP, 32>(vt, 0, f, t, lane), p, acc[t]);
+                for (int j = 0; j < 8; ++j) w[j] = s[8 * f + j] - (float)p[j];
+                rest = __builtin_convertvector(w, typename L::frag);
+            }
+#pragma unroll
+            for (int t = 0; t < DT; ++t) {
+                const auto column = column_of<T, DP, 32>(vt, 0, f, t, lane);
+                acc[t] = mma(column, p, acc[t]);
+                if constexpr (sizeof(T) == 2) acc[t] = mma(column, rest, acc[t]);
+            }
         }
     };
     for (int first = start; first < mine.last; first += 2 * kStep) {

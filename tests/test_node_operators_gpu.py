@@ -731,3 +731,21 @@ def test_float16_gradients_of_any_size(rows, keys, d, size):
     for name, x in zip(("dq", "dk", "dv"), torch.autograd.grad(out, (q, k, v), g)):
         # (32-bit sums of a few thousand terms: some 2^-24 of them each)
         check_norm(x, *want[name], F16, name, more=2.0 ** -18)
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("segments,keys,hq,hk,d,few", [(1, 20011, 8, 2, 128, True), (1, 900, 4, 4, 64, True), (9, 700, 5, 1, 72, True),
+                                                       (64, 60, 8, 8, 32, True), (1, 300, 4, 4, 64, False)])
+def test_single_rows_lose_no_more_than_the_outputs_rounding(dtype, segments, keys, hq, hk, d, few):
+    """The error is what rounding the exact result once would leave, and twice what comes before that: weights of two
+    parts (the half unit squared; in one part the half unit where a call is so short that it takes the form for tiles) and
+    sums of 32 bits."""
+    q, k, v = (normal(segments * n, h, d, dtype=dtype, seed=s) for s, (n, h) in enumerate(((1, hq), (keys, hk), (keys, hk))))
+    ptr = torch.arange(segments + 1, device="cuda")
+    out = oeq.packed_attention(q, k, v, ptr, keys * ptr).double()
+    qq = q.double().view(segments, hk, hq // hk, d).reshape(-1, hq // hk, d)
+    kk, vv = (t.double().view(segments, keys, hk, d).transpose(1, 2).reshape(-1, keys, d) for t in (k, v))
+    p = torch.softmax(torch.bmm(qq, kk.transpose(1, 2).contiguous()) * d ** -0.5, 2)
+    want = torch.bmm(p, vv).view(segments, hq, d)
+    before = N.HALF_UNIT[dtype] ** (2 if few else 1) * torch.bmm(p * p, vv * vv).sum().sqrt() + 2.0 ** -17 * want.norm()
+    assert (out - want).norm() <= (want.to(dtype) - want).norm() + 2 * before
