@@ -27,8 +27,12 @@
 //
 // What a mask hides has no influence, whatever it holds: hidden scores are replaced before the maximum, hidden p and ds
 // are set to zero. A product still multiplies that zero with the hidden row, which is no zero if that row holds an
-// infinity or NaN; such a product leaves NaN in the sums. So a wave that finds its result not finite computes those rows
-// again one by one from the visible rows alone. Nothing is paid for that where results are finite.
+// infinity or NaN; such a product leaves NaN in the sums. So a block with a result that is not finite, for whatever reason,
+// walks its tiles a second time (Pass), with the infinities and NaN of the rows that its lanes share taken out of the products
+// and counted for each lane by products of their own. Results that were finite stay, and one that is finite now has the
+// bits that it has where hidden rows are finite. A causal sequence of 4 000 rows, 8 / 2 heads of 64, bf16: forward 43 us, with an
+// infinity among the values 152; gradients 187, with one in the output's gradient 1 050 (fp16 200 and 710). Where all is
+// finite it costs a barrier at the end: 512 molecules, float32, training step 132.6 and 134.2 us, large launches within 1 %.
 #ifndef OEQ_PACKED_ATTENTION_H
 #define OEQ_PACKED_ATTENTION_H
 
@@ -36,6 +40,7 @@
 
 #include <climits>
 #include <cstdint>
+#include <type_traits>
 
 namespace packed_attention {
 
@@ -100,13 +105,13 @@ constexpr bool kLifted = Types<T>::kForward > 0;  // elements of eleven bits
 template <int N>
 constexpr float power = N > 0 ? (float)(1ull << (N > 0 ? N : 0)) : 1.0f / (float)(1ull << (N < 0 ? -N : 0));
 
-// 2^(x + N). Where results keep 24 bits the sum would cost some of x's: x is raised only where it is large enough not to
-// lose any, else the result is.
-template <typename T, int N>
-__device__ __forceinline__ float raised(float x) {
-    if constexpr (sizeof(T) == 2 || N == 0) return __builtin_amdgcn_exp2f(x + N);
+// 2^(x + n), pn = 2^n. Where results keep 24 bits the sum would cost some of x's: x is raised only where it is large enough not
+// to lose any, else the result is.
+template <typename T>
+__device__ __forceinline__ float raised(float x, float n, float pn) {
+    if constexpr (sizeof(T) == 2) return __builtin_amdgcn_exp2f(x + n);
     const bool low = x < -100.0f;
-    return __builtin_amdgcn_exp2f(low ? x + N : x) * (low ? 1.0f : power<N>);
+    return __builtin_amdgcn_exp2f(low ? x + n : x) * (low ? 1.0f : pn);
 }
 
 __device__ __forceinline__ float16_t mma(float4_t a, float4_t b, float16_t c) {
@@ -151,6 +156,11 @@ __device__ __forceinline__ int wave_max(int x) {
     return x;
 }
 __device__ __forceinline__ bool finite(float x) { return fabsf(x) < INFINITY; }
+// Its bits without the sign: from 0x7f800000, an infinity, on it is not finite. (Compared as a number in the scalar unit's
+// registers where many of them are asked for at a time.)
+__device__ __forceinline__ unsigned magnitude(float x) { return __float_as_uint(x) & 0x7fffffffu; }
+// x times a factor that may have come out as zero: an infinity stays one.
+__device__ __forceinline__ float scaled(float x, float by) { return finite(x) ? x * by : x; }
 
 // ---------------------------------------------------------------------------
 // tiles in LDS
@@ -302,6 +312,7 @@ __device__ __forceinline__ void load_row(typename Types<T>::frag (&x)[FRAGS], co
 // `rest`, if there is one, what rounding takes off.
 template <typename T, int DT>
 __device__ __forceinline__ void store_row(T* row, const float16_t (&acc)[DT], float by, int d, int half, T* rest = nullptr) {
+#pragma clang fp contract(off)  // (a product is rounded to 32 bits first, here and in store_part)
 #pragma unroll
     for (int t = 0; t < DT; ++t)
 #pragma unroll
@@ -407,18 +418,23 @@ struct Walk {
     __device__ __forceinline__ bool whole(int first, int n) const { return first >= full_lo && first + n <= full_hi; }
 };
 
+struct Shared {
+    int range[8], bad[2];  // the waves' unions; whether a pass left results that are not finite (any_of_block)
+};
+
 // The union over the block's four waves.
-__device__ __forceinline__ Bounds block_range(const Walk& w, int (&shared)[8], int wave, int lane) {
+__device__ __forceinline__ Bounds block_range(const Walk& w, Shared& shared, int wave, int lane) {
     if (lane == 0) {
-        shared[2 * wave] = w.lo;
-        shared[2 * wave + 1] = w.hi;
+        shared.range[2 * wave] = w.lo;
+        shared.range[2 * wave + 1] = w.hi;
     }
+    if (threadIdx.x < 2) shared.bad[threadIdx.x] = 0;
     __syncthreads();
-    Bounds b = {shared[0], shared[1]};
+    Bounds b = {shared.range[0], shared.range[1]};
 #pragma unroll
     for (int i = 1; i < 4; ++i) {
-        b.lo = min(b.lo, shared[2 * i]);
-        b.hi = max(b.hi, shared[2 * i + 1]);
+        b.lo = min(b.lo, shared.range[2 * i]);
+        b.hi = max(b.hi, shared.range[2 * i + 1]);
     }
     b.lo = __builtin_amdgcn_readfirstlane(b.lo);
     b.hi = __builtin_amdgcn_readfirstlane(b.hi);
@@ -498,11 +514,16 @@ constexpr bool kSparse = sizeof(T) == 4 && DP == 32;
 // registers. In key_gradient: kSparse, 192 registers a lane or 138, a wave more to a SIMD: 512 molecules, float32, all
 // gradients 139 / 132 us, 2 048 460 / 424, but a segment of 3 000 rows 260 / 266. (bf16 heads of 32, whose products are 8 times as
 // fast: 2 048 molecules 185 / 177, a segment of 3 000 rows 64 / 73, so they keep them.)
+template <typename X>
+__device__ __forceinline__ X anew(X x) {
+    asm volatile("" : "+v"(x));
+    return x;
+}
 struct Lane {
     int at, half;
     template <bool ANEW>
     static __device__ __forceinline__ Lane of(int lane, int half) {
-        if constexpr (ANEW) asm volatile("" : "+v"(lane));
+        if constexpr (ANEW) lane = anew(lane);
         return {lane, ANEW ? lane >> 5 : half};
     }
 };
@@ -533,84 +554,8 @@ __device__ __forceinline__ void clear(char* lds) {
 }
 
 // ---------------------------------------------------------------------------
-// rows one by one (see the beginning: results that are not finite)
+// results that are not finite (see the beginning)
 // ---------------------------------------------------------------------------
-
-template <typename T>
-__device__ __forceinline__ float dot_row(const T* x, const T* y, int d, int lane) {
-    float s = 0;
-    for (int e = lane; e < d; e += 64) s += (float)x[e] * (float)y[e];
-    return wave_sum(s);
-}
-
-template <typename T>
-__device__ __forceinline__ void forward_row(const Args& a, int i, int h, int lo, int hi, int lane) {
-    const int kh = h / (a.hq / a.hk);
-    const T* q = (const T*)a.q + i * a.q_row + h * a.q_head;
-    const T *k = (const T*)a.k + kh * a.k_head, *v = (const T*)a.v + kh * a.v_head;
-    float m = -INFINITY, l = 0, o0 = 0, o1 = 0;
-    const int e0 = lane, e1 = lane + 64;
-    for (int j = lo; j < hi; ++j) {
-        const float s = dot_row(q, k + j * a.k_row, a.d, lane) * a.scale_log2;
-        const float top = fmaxf(m, s);
-        if (top == -INFINITY && !(s != s)) continue;  // exp(-inf) of nothing yet
-        const float keep = m == -INFINITY ? 0.0f : exp2f(m - top), p = exp2f(s - top);
-        m = top;
-        l = l * keep + p;
-        if (e0 < a.d) o0 = o0 * keep + p * (float)v[j * a.v_row + e0];
-        if (e1 < a.d) o1 = o1 * keep + p * (float)v[j * a.v_row + e1];
-    }
-    const int64_t at = ((int64_t)i * a.hq + h) * a.d;
-    const float by = hi > lo ? 1.0f / l : 0.0f;
-    const auto put = [&](int e, float x) {
-        const T y = (T)x;
-        ((T*)a.o)[at + e] = y;
-        if (a.rest) ((T*)a.rest)[at + e] = (T)(x - (float)y);
-    };
-    if (e0 < a.d) put(e0, hi > lo ? o0 * by : 0.0f);
-    if (e1 < a.d) put(e1, hi > lo ? o1 * by : 0.0f);
-    if (lane == 0) a.lse[h * a.stat_stride + i] = hi > lo ? m + log2f(l) : -INFINITY;
-}
-
-template <typename T>
-__device__ __forceinline__ void query_gradient_row(const Args& a, int i, int h, int lo, int hi, int lane) {
-    const int kh = h / (a.hq / a.hk);
-    const T *q = (const T*)a.q + i * a.q_row + h * a.q_head, *g = (const T*)a.grad + i * a.g_row + h * a.g_head;
-    const T *k = (const T*)a.k + kh * a.k_head, *v = (const T*)a.v + kh * a.v_head;
-    const float lse = a.lse[h * a.stat_stride + i], delta = a.delta[h * a.stat_stride + i];
-    float x0 = 0, x1 = 0;
-    const int e0 = lane, e1 = lane + 64;
-    for (int j = lo; j < hi; ++j) {
-        const float p = exp2f(dot_row(q, k + j * a.k_row, a.d, lane) * a.scale_log2 - lse);
-        const float ds = p * (dot_row(g, v + j * a.v_row, a.d, lane) - delta);
-        if (e0 < a.d) x0 += ds * (float)k[j * a.k_row + e0];
-        if (e1 < a.d) x1 += ds * (float)k[j * a.k_row + e1];
-    }
-    const float by = a.scale_log2 * 0.6931471805599453f;
-    T* dq = (T*)a.dq + ((int64_t)i * a.hq + h) * a.d;
-    if (e0 < a.d) dq[e0] = (T)(x0 * by);
-    if (e1 < a.d) dq[e1] = (T)(x1 * by);
-}
-
-template <typename T>
-__device__ __forceinline__ void key_gradient_row(const Args& a, int j, int kh, int lo, int hi, int lane) {
-    const int group = a.hq / a.hk;
-    const T *k = (const T*)a.k + j * a.k_row + kh * a.k_head, *v = (const T*)a.v + j * a.v_row + kh * a.v_head;
-    float k0 = 0, k1 = 0, v0 = 0, v1 = 0;
-    const int e0 = lane, e1 = lane + 64;
-    for (int h = kh * group; h < (kh + 1) * group; ++h)
-        for (int i = lo; i < hi; ++i) {
-            const T *q = (const T*)a.q + i * a.q_row + h * a.q_head, *g = (const T*)a.grad + i * a.g_row + h * a.g_head;
-            const float p = exp2f(dot_row(q, k, a.d, lane) * a.scale_log2 - a.lse[h * a.stat_stride + i]);
-            const float ds = p * (dot_row(g, v, a.d, lane) - a.delta[h * a.stat_stride + i]);
-            if (e0 < a.d) v0 += p * (float)g[e0], k0 += ds * (float)q[e0];
-            if (e1 < a.d) v1 += p * (float)g[e1], k1 += ds * (float)q[e1];
-        }
-    const float by = a.scale_log2 * 0.6931471805599453f;
-    const int64_t at = ((int64_t)j * a.hk + kh) * a.d;
-    if (e0 < a.d) ((T*)a.dk)[at + e0] = (T)(k0 * by), ((T*)a.dv)[at + e0] = (T)v0;
-    if (e1 < a.d) ((T*)a.dk)[at + e1] = (T)(k1 * by), ((T*)a.dv)[at + e1] = (T)v1;
-}
 
 template <int DT>
 __device__ __forceinline__ bool all_finite(const float16_t (&acc)[DT]) {
@@ -620,6 +565,138 @@ __device__ __forceinline__ bool all_finite(const float16_t (&acc)[DT]) {
 #pragma unroll
         for (int r = 0; r < 16; ++r) z = fmaf(acc[t][r], 0.0f, z);
     return z == 0.0f;
+}
+
+// Where a careful pass has an element that is not finite and does not know why: its sum may have been too large on the way.
+__device__ __forceinline__ bool all_known(const float16_t& acc, unsigned known) {
+    unsigned open = 0;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) open |= (~(magnitude(acc[r]) - 0x7f800000u) >> 31) << r;
+    return (open & ~known) == 0;
+}
+
+// store_row for 32 columns. `keep`: what is there already and finite stays.
+template <typename T>
+__device__ __forceinline__ void store_part(T* row, const float16_t& acc, float by, int d, int half, T* rest, bool keep) {
+#pragma clang fp contract(off)
+    typedef typename Types<T>::quad quad;
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+        const int at = 8 * g + 4 * half;
+        if (at >= d) break;
+        float4_t w;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) w[j] = acc[4 * g + j] * by;
+        quad x = __builtin_convertvector(w, quad), y = __builtin_convertvector(w - __builtin_convertvector(x, float4_t), quad);
+        if (keep) {
+            const quad was = *(const quad*)(row + at);
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                if (finite((float)was[j])) {
+                    x[j] = was[j];
+                    if (rest) y[j] = rest[at + j];
+                }
+        }
+        *(quad*)(row + at) = x;
+        if (rest) *(quad*)(rest + at) = y;
+        __builtin_amdgcn_sched_barrier(0);
+    }
+}
+
+// Passes of a block over its tiles: the first, a second one if results are not finite, and a third if some are not for a reason
+// that the second has not found in the operands: sums may have passed the largest number on the way (in 24 and 8 bits, whose
+// range is that of the sums). There p and ds carry no power of two and p never passes 1.
+enum Pass { kFirst, kCareful, kCarefulSmall };
+template <typename T>
+constexpr int kLastPass = kLifted<T> ? kCareful : kCarefulSmall;
+
+// Whether any thread of the block says so. A barrier; every pass has a place of its own.
+__device__ __forceinline__ bool any_of_block(bool bad, int& shared) {
+    if (__any(bad)) shared = 1;  // (the same from every lane)
+    __syncthreads();
+    return __builtin_amdgcn_readfirstlane(shared) != 0;
+}
+
+// The second and third pass of a block. They take 32 columns of the head at a time, with the scores computed anew for each, so
+// that they need hardly more registers than the first. `walk(t, raise, bad)` is a walk for columns 32 t ... that stores the
+// results where bad and says whether some of them are not finite for no known reason.
+template <typename T, int DT, typename F>
+__device__ __forceinline__ void careful_passes(int (&shared)[2], bool bad, F walk) {
+#pragma unroll 1
+    for (int n = kCareful; n <= kLastPass<T> && any_of_block(bad, shared[n - 1]); ++n) {
+        bool still = false;
+#pragma unroll 1
+        for (int t = 0; t < DT; ++t) {
+            if (t) __syncthreads();  // (all are done with the last walk's tiles)
+            int raise = n == kCareful;
+            asm volatile("" : "+s"(raise));  // (one walk for both passes)
+            if (walk(t, raise, bad)) still = true;
+        }
+        bad = still;
+    }
+}
+
+// acc += columns 32 t ... of the rows at `first`, transposed, times the weights of a result with these rows (and their `rest`),
+// by the rows' finite elements alone. Returns whether there were others. `known`: a bit for each register whose result is not
+// finite for what the operands hold, not for the size of its sum.
+template <typename T, int DP, int ROWS, bool REST = false>
+__device__ __forceinline__ bool finite_product_of(const char* lds, int first, int t, int lane, const float16_t& weights,
+                                                  const float16_t& rest, float16_t& acc, unsigned& known) {
+    unsigned left = 0;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) left = max(left, magnitude(weights[r]));
+    const float both = sum_halves(__uint_as_float(left));  // (a product sums over the weights of either half)
+    if (both != both) known = ~0u;
+    left = 0;
+#pragma unroll
+    for (int f = 0; f < (int)sizeof(T); ++f) {
+        auto x = column_of<T, DP, ROWS>(lds, first, f, t, lane);
+#pragma unroll
+        for (int j = 0; j < 16 / (int)sizeof(T); ++j) {
+            const unsigned size = magnitude((float)x[j]);
+            left = max(left, size);
+            x[j] = size < 0x7f800000u ? x[j] : (T)0.0f;
+        }
+        acc = mma(x, operand<T>(weights, f), acc);
+        if (REST) acc = mma(x, operand<T>(rest, f), acc);
+        __builtin_amdgcn_sched_barrier(0);
+    }
+    return kSparse<T, DP> || __any(left >= 0x7f800000u);  // (small heads: a branch around what follows would take registers)
+}
+
+// And what the rows' other elements come to in each result whose lane sees them (rows are numbered from `number` on):
+// infinities as they are, where weights are above zero (SIGNED), else NaN. A product of 1 where a lane sees a row with 1 for
+// each +inf, 2^7 for -inf and 2^14 for NaN counts up to 32 of each exactly.
+template <typename T, int DP, int ROWS, bool SIGNED, int BIT = 0>
+__device__ __forceinline__ void add_others(const char* lds, int first, int t, int lane, int number, Bounds b, float16_t& acc,
+                                           unsigned& known) {
+    constexpr int E = 16 / (int)sizeof(T);
+    float16_t count = 0.0f;
+#pragma unroll
+    for (int f = 0; f < 16 / E; ++f) {
+        auto x = column_of<T, DP, ROWS>(lds, first, f, t, lane), sees = x;
+#pragma unroll
+        for (int j = 0; j < E; ++j) {
+            const float y = (float)x[j];
+            const int r = E * f + j;
+            float code = y == INFINITY ? 1.0f : 0.0f;
+            code = y == -INFINITY ? 128.0f : code;
+            code = y != y ? 16384.0f : code;
+            x[j] = (T)code;
+            sees[j] = (unsigned)(number + 8 * (r / 4) + 4 * (lane >> 5) + r % 4 - b.lo) < (unsigned)(b.hi - b.lo) ? (T)1.0f : (T)0.0f;
+        }
+        count = mma(x, sees, count);
+        __builtin_amdgcn_sched_barrier(0);
+    }
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+        const int n = (int)count[r];
+        float other = n & 127 ? INFINITY : 0.0f;
+        if (n >> 7) other -= INFINITY;
+        if (n >> 14 || !SIGNED) other = NAN;
+        if (n) acc[r] += other, known |= 1u << (r + BIT);
+        __builtin_amdgcn_sched_barrier(0);
+    }
 }
 
 // ---------------------------------------------------------------------------
@@ -633,14 +710,15 @@ __device__ __forceinline__ bool all_finite(const float16_t (&acc)[DT]) {
 // Short ones by a block's chain of waits: 512 molecules, 8 heads of 32, float32, 35 us, of which the matrix units work 13;
 // 33 crystals, 6 / 2 heads of 72, fp16, 20 us.
 template <typename T, int DP, int SPLIT>
-__global__ __launch_bounds__(256, (blocks_per_unit<T, DP>())) void forward(Args a) {
+__global__ __launch_bounds__(256, (kSparse<T, DP> && SPLIT == 1 ? 4 : blocks_per_unit<T, DP>())) void forward(Args a) {
     constexpr int BK = SPLIT == 2 ? 64 : tile_rows<T, DP>(), SUB = SPLIT == 2 || kSparse<T, DP> ? 1 : BK / 32, DT = DP / 32;
     constexpr int PF = sizeof(T) == 2 ? 2 : 4;  // fragments of 32 keys
     typedef Tile<T, DP, BK> L;
     __shared__ __align__(1024) char key0[L::kBytes], key1[L::kBytes], val0[L::kBytes], val1[L::kBytes];
-    __shared__ int shared[8];
+    __shared__ Shared shared;
     __shared__ __align__(16) float4_t swap[SPLIT == 2 ? 512 : 1];
     __shared__ float swap_m[SPLIT == 2 ? 64 : 1], swap_l[SPLIT == 2 ? 64 : 1];
+    __shared__ unsigned swap_known[SPLIT == 2 ? 128 : 1];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5;
     int tile, h;
     place(a, a.hq, a.q_order, a.causal, tile, h);
@@ -659,123 +737,156 @@ __global__ __launch_bounds__(256, (blocks_per_unit<T, DP>())) void forward(Args 
     const char* vbase = (const char*)((const T*)a.v + kh * a.v_head);
     const int krow = (int)a.k_row * (int)sizeof(T), vrow = (int)a.v_row * (int)sizeof(T);
     const typename L::Places kplaces(krow, chunks, wave, lane), vplaces(vrow, chunks, wave, lane);
-    float16_t acc[DT];
-#pragma unroll
-    for (int t = 0; t < DT; ++t) acc[t] = 0.0f;
-    float m = -INFINITY, l = 0;
+    float m, l;
+    unsigned known;
     const float c = a.scale_log2;
     settle();
 
-    auto products = [&](const char* kt, const char* vt, int first, int r0) {
-        float16_t s[SUB];
+    // Sums are scaled to another maximum only where it grew by more than 2^grow: up to 2^8 p fits every type.
+    auto pass = [&](auto& acc, auto care, int t0, float grow) {
+        constexpr bool CARE = decltype(care)::value;
+        constexpr int NT = CARE ? 1 : DT;
 #pragma unroll
-        for (int u = 0; u < SUB; ++u) {
-            s[u] = 0.0f;
+        for (int t = 0; t < NT; ++t) acc[t] = 0.0f;
+        m = -INFINITY, l = 0, known = 0;
+        auto products = [&](const char* kt, const char* vt, int first, int r0) {
+            const Lane w = Lane::of<CARE>(lane, half);
+            float16_t s[SUB];
 #pragma unroll
-            for (int f = 0; f < L::kFrags; ++f) s[u] = mma(L::row(kt, r0 + 32 * u + (lane & 31), f, half), q[f], s[u]);
-        }
-        if (!walk.whole(first + r0, 32 * SUB)) {
-            const int shift = first + r0 + 4 * half - b.lo;
-            const unsigned n = b.hi - b.lo;
+            for (int u = 0; u < SUB; ++u) {
+                s[u] = 0.0f;
+#pragma unroll
+                for (int f = 0; f < L::kFrags; ++f) s[u] = mma(L::row(kt, r0 + 32 * u + (w.at & 31), f, w.half), q[f], s[u]);
+            }
+            if (!walk.whole(first + r0, 32 * SUB)) {
+                const int shift = first + r0 + 4 * half - b.lo;
+                const unsigned n = b.hi - b.lo;
+#pragma unroll
+                for (int u = 0; u < SUB; ++u)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r)
+                        if ((unsigned)(shift + 32 * u + 8 * (r / 4) + r % 4) >= n) s[u][r] = -INFINITY;
+            }
+            float top = s[0][0];
 #pragma unroll
             for (int u = 0; u < SUB; ++u)
 #pragma unroll
-                for (int r = 0; r < 16; ++r)
-                    if ((unsigned)(shift + 32 * u + 8 * (r / 4) + r % 4) >= n) s[u][r] = -INFINITY;
-        }
-        float top = s[0][0];
+                for (int r = 0; r < 16; ++r) top = fmaxf(top, s[u][r]);
+            top = max_halves(top);
+            if (__any((top - m) * c > grow)) {
+                const float now = fmaxf(m, top);
+                const float by = now == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f((m - now) * c);
+                m = now;
+                l *= by;
+                if constexpr (CARE) {
 #pragma unroll
-        for (int u = 0; u < SUB; ++u)
+                    for (int r = 0; r < 16; ++r) acc[0][r] = scaled(acc[0][r], by);
+                } else {
 #pragma unroll
-            for (int r = 0; r < 16; ++r) top = fmaxf(top, s[u][r]);
-        top = max_halves(top);
-        // sums are scaled to another maximum only where it grew by a factor of 2^8: up to there p fits every type
-        if (__any((top - m) * c > 8.0f)) {
-            const float now = fmaxf(m, top);
-            const float by = now == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f((m - now) * c);
-            m = now;
-            l *= by;
-#pragma unroll
-            for (int t = 0; t < DT; ++t) acc[t] *= by;
-        }
-        const float mc = m == -INFINITY ? 0.0f : m * c - Types<T>::kForward;
-#pragma unroll
-        for (int u = 0; u < SUB; ++u) {
-#pragma unroll
-            for (int r = 0; r < 16; ++r) {
-                s[u][r] = __builtin_amdgcn_exp2f(fmaf(s[u][r], c, -mc));
-                l += s[u][r];
+                    for (int t = 0; t < NT; ++t) acc[t] *= by;
+                }
             }
+            const float mc = m == -INFINITY ? 0.0f : m * c - Types<T>::kForward;
 #pragma unroll
-            for (int f = 0; f < PF; ++f) {
-                const auto p = operand<T>(s[u], f);
+            for (int u = 0; u < SUB; ++u) {
 #pragma unroll
-                for (int t = 0; t < DT; ++t) acc[t] = mma(column_of<T, DP, BK>(vt, r0 + 32 * u, f, t, lane), p, acc[t]);
+                for (int r = 0; r < 16; ++r) {
+                    s[u][r] = __builtin_amdgcn_exp2f(fmaf(s[u][r], c, -mc));
+                    l += s[u][r];
+                }
+                if constexpr (CARE) {
+                    if (finite_product_of<T, DP, BK>(vt, r0 + 32 * u, t0, w.at, s[u], s[u], acc[0], known))
+                        add_others<T, DP, BK, true>(vt, r0 + 32 * u, t0, w.at, first + r0 + 32 * u, b, acc[0], known);
+                } else {
+#pragma unroll
+                    for (int f = 0; f < PF; ++f) {
+                        const auto p = operand<T>(s[u], f);
+#pragma unroll
+                        for (int t = 0; t < DT; ++t) acc[t] = mma(column_of<T, DP, BK>(vt, r0 + 32 * u, f, t, lane), p, acc[t]);
+                    }
+                }
             }
+        };
+        auto step = [&](char* kt, char* vt, char* kn, char* vn, int first) {
+            arrived();
+            if (first + BK < all.hi) {
+                L::request(kn, kbase, krow, kplaces, first + BK, all.hi, chunks, wave);
+                L::request(vn, vbase, vrow, vplaces, first + BK, all.hi, chunks, wave);
+            }
+            if constexpr (SPLIT == 2) {
+                if (walk.needs(first + 32 * part, 32)) products(kt, vt, first, 32 * part);
+            } else {
+#pragma unroll
+                for (int r0 = 0; r0 < BK; r0 += 32 * SUB)
+                    if (walk.needs(first + r0, 32 * SUB)) products(kt, vt, first, r0);
+            }
+        };
+        if (all.lo < all.hi) {
+            L::request(key0, kbase, krow, kplaces, all.lo, all.hi, chunks, wave);
+            L::request(val0, vbase, vrow, vplaces, all.lo, all.hi, chunks, wave);
         }
-    };
-    auto step = [&](char* kt, char* vt, char* kn, char* vn, int first) {
-        arrived();
-        if (first + BK < all.hi) {
-            L::request(kn, kbase, krow, kplaces, first + BK, all.hi, chunks, wave);
-            L::request(vn, vbase, vrow, vplaces, first + BK, all.hi, chunks, wave);
+        for (int first = all.lo; first < all.hi; first += 2 * BK) {
+            step(key0, val0, key1, val1, first);
+            if (first + BK < all.hi) step(key1, val1, key0, val0, first + BK);
         }
+        l = sum_halves(l);
         if constexpr (SPLIT == 2) {
-            if (walk.needs(first + 32 * part, 32)) products(kt, vt, first, 32 * part);
-        } else {
+            // the wave with the second groups of keys hands its sums to the one with the first, 32 columns of the head at a time
+            if (part && half == 0) swap_m[32 * rows + lane] = m, swap_l[32 * rows + lane] = l;
+            if (CARE && part) swap_known[64 * rows + lane] = known;
+            __syncthreads();
+            if (CARE && !part) known |= swap_known[64 * rows + lane];
+            const float other = swap_m[32 * rows + (lane & 31)], top = fmaxf(m, other);
+            const float by = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((m - top) * c);
+            const float others = other == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((other - top) * c);
+            if (!part) l = l * by + swap_l[32 * rows + (lane & 31)] * others, m = top;
 #pragma unroll
-            for (int r0 = 0; r0 < BK; r0 += 32 * SUB)
-                if (walk.needs(first + r0, 32 * SUB)) products(kt, vt, first, r0);
+            for (int t = 0; t < NT; ++t) {
+                if (part)
+#pragma unroll
+                    for (int g = 0; g < 4; ++g)
+                        swap[(rows * 4 + g) * 64 + lane] = float4_t{acc[t][4 * g], acc[t][4 * g + 1], acc[t][4 * g + 2], acc[t][4 * g + 3]};
+                __syncthreads();
+                if (!part)
+#pragma unroll
+                    for (int g = 0; g < 4; ++g)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const float x = acc[t][4 * g + e], y = swap[(rows * 4 + g) * 64 + lane][e];
+                            acc[t][4 * g + e] = CARE && !(finite(x) && finite(y)) ? scaled(x, by) + scaled(y, others) : fmaf(x, by, y * others);
+                        }
+                __syncthreads();
+            }
         }
     };
-    if (all.lo < all.hi) {
-        L::request(key0, kbase, krow, kplaces, all.lo, all.hi, chunks, wave);
-        L::request(val0, vbase, vrow, vplaces, all.lo, all.hi, chunks, wave);
-    }
-    for (int first = all.lo; first < all.hi; first += 2 * BK) {
-        step(key0, val0, key1, val1, first);
-        if (first + BK < all.hi) step(key1, val1, key0, val0, first + BK);
-    }
-    l = sum_halves(l);
-    if constexpr (SPLIT == 2) {
-        // the wave with the second groups of keys hands its sums to the one with the first, 32 columns of the head at a time
-        if (part && half == 0) swap_m[32 * rows + lane] = m, swap_l[32 * rows + lane] = l;
-        __syncthreads();
-        const float other = swap_m[32 * rows + (lane & 31)], top = fmaxf(m, other);
-        const float by = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((m - top) * c);
-        const float others = other == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((other - top) * c);
-        if (!part) l = l * by + swap_l[32 * rows + (lane & 31)] * others, m = top;
-#pragma unroll
-        for (int t = 0; t < DT; ++t) {
-            if (part)
-#pragma unroll
-                for (int g = 0; g < 4; ++g)
-                    swap[(rows * 4 + g) * 64 + lane] = float4_t{acc[t][4 * g], acc[t][4 * g + 1], acc[t][4 * g + 2], acc[t][4 * g + 3]};
-            __syncthreads();
-            if (!part)
-#pragma unroll
-                for (int g = 0; g < 4; ++g)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e)
-                        acc[t][4 * g + e] = acc[t][4 * g + e] * by + swap[(rows * 4 + g) * 64 + lane][e] * others;
-            __syncthreads();
-        }
-        if (part) return;
-    }
-    const bool seen = b.lo < b.hi, mine = row < a.nq;
-    const float by = seen ? 1.0f / l : 0.0f;
-    if (mine) {
-        const int64_t at = ((int64_t)i * a.hq + h) * a.d;
-        store_row<T, DT>((T*)a.o + at, acc, by, a.d, half, a.rest ? (T*)a.rest + at : nullptr);
+    const bool seen = b.lo < b.hi;
+    auto put_sum = [&](int i) {
         if (half == 0) a.lse[h * a.stat_stride + i] = seen ? m * c + (__builtin_amdgcn_logf(l) - Types<T>::kForward) : -INFINITY;
+    };
+    bool bad = row < a.nq && !part;
+    {
+        float16_t acc[DT];
+        pass(acc, std::false_type(), 0, 8.0f);
+        const float by = seen ? 1.0f / l : 0.0f;
+        if (bad) {
+            const int64_t at = ((int64_t)i * a.hq + h) * a.d;
+            store_row<T, DT>((T*)a.o + at, acc, by, a.d, half, a.rest ? (T*)a.rest + at : nullptr);
+            put_sum(i);
+        }
+        bad = bad && !(all_finite<DT>(acc) && finite(by));
     }
-    uint64_t bad = __ballot(mine && !(all_finite<DT>(acc) && finite(by)));
-    bad = (bad | bad >> 32) & 0xffffffffu;
-    while (bad) {
-        const int at = __builtin_ctzll(bad);
-        bad &= bad - 1;
-        forward_row<T>(a, (tile * (4 / SPLIT) + rows) * 32 + at, h, __shfl(b.lo, at), __shfl(b.hi, at), lane);
-    }
+    careful_passes<T, DT>(shared.bad, bad, [&](int t, int raise, bool mine) {
+        float16_t acc[1];
+        pass(acc, std::true_type(), t, 8.0f * raise);
+        const float by = seen ? 1.0f / l : 0.0f;
+        if (mine) {
+            const int r = anew(i);
+            const int64_t at = ((int64_t)r * a.hq + h) * a.d + 32 * t;
+            store_part<T>((T*)a.o + at, acc[0], by, a.d - 32 * t, half, a.rest ? (T*)a.rest + at : nullptr, !raise);
+            if (raise) put_sum(r);
+        }
+        return mine && !all_known(acc[0], known);
+    });
 }
 
 // ---------------------------------------------------------------------------
@@ -825,7 +936,7 @@ __global__ __launch_bounds__((64 * Few<T, DP>::kWaves), 1) void forward_few(Args
     typedef typename Few<T, DP>::L L;
     __shared__ __align__(1024) char key0[W * L::kBytes], key1[W * L::kBytes], val0[W * L::kBytes], val1[W * L::kBytes];
     __shared__ float top_of[W][32], sum_of[W][32];
-    __shared__ int bad;
+    __shared__ int bad[2];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5;
     const int group = a.hq / a.hk, stacks = (group + 31) / 32;
     int id = blockIdx.x;
@@ -841,11 +952,13 @@ __global__ __launch_bounds__((64 * Few<T, DP>::kWaves), 1) void forward_few(Args
     if (part && mine.first >= mine.last) return;
     char *kt0 = key0 + wave * L::kBytes, *kt1 = key1 + wave * L::kBytes;
     char *vt0 = val0 + wave * L::kBytes, *vt1 = val1 + wave * L::kBytes;
-    if (chunks < L::kChunks) {  // (a wave's own part of the buffers: no barrier)
+    auto clear_own = [&] {  // (a wave's own part of the buffers: no barrier)
+        if (chunks >= L::kChunks) return;
         for (int n = lane * 16; n < L::kBytes; n += 1024)
             *(uint4_t*)(kt0 + n) = 0, *(uint4_t*)(kt1 + n) = 0, *(uint4_t*)(vt0 + n) = 0, *(uint4_t*)(vt1 + n) = 0;
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-    }
+    };
+    clear_own();
     const char* kbase = (const char*)((const T*)a.k + kh * a.k_head);
     const char* vbase = (const char*)((const T*)a.v + kh * a.v_head);
     const int krow = (int)a.k_row * (int)sizeof(T), vrow = (int)a.v_row * (int)sizeof(T);
@@ -861,128 +974,159 @@ __global__ __launch_bounds__((64 * Few<T, DP>::kWaves), 1) void forward_few(Args
     const bool live = column < heads;
     load_row<T, L::kFrags>(q, (const char*)((const T*)a.q + i * a.q_row + (h0 + (live ? column : 0)) * a.q_head),
                            live ? chunks : 0, half);
-    float16_t acc[DT];
-#pragma unroll
-    for (int t = 0; t < DT; ++t) acc[t] = 0.0f;
-    float m = -INFINITY, l = 0;
+    float m, l;
+    unsigned known;
     const float c = a.scale_log2;
 
-    auto step = [&](char* kt, char* vt, char* kn, char* vn, int first) {
-        if (first + kStep < mine.last) {
-            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // what was read from there has come
-            request(kn, vn, first + kStep);
-            asm volatile("s_waitcnt vmcnt(%0)" ::"n"(kAhead) : "memory");
-        } else {
-            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-        }
-        float16_t s = 0.0f;
+    auto pass = [&](auto& acc, auto care, int t0, float grow) {  // (see forward)
+        constexpr bool CARE = decltype(care)::value;
+        constexpr int NT = CARE ? 1 : DT;
 #pragma unroll
-        for (int f = 0; f < L::kFrags; ++f) s = mma(L::row(kt, lane & 31, f, half), q[f], s);
-        if (first + 32 > mine.last) {
-#pragma unroll
-            for (int r = 0; r < 16; ++r)
-                if (first + 4 * half + 8 * (r / 4) + r % 4 >= mine.last) s[r] = -INFINITY;
-        }
-        float top = s[0];
-#pragma unroll
-        for (int r = 1; r < 16; ++r) top = fmaxf(top, s[r]);
-        top = max_halves(top);
-        if (__any((top - m) * c > 8.0f)) {
-            const float now = fmaxf(m, top);
-            const float by = now == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f((m - now) * c);
-            m = now;
-            l *= by;
-#pragma unroll
-            for (int t = 0; t < DT; ++t) acc[t] *= by;
-        }
-        const float mc = m == -INFINITY ? 0.0f : m * c - Types<T>::kForward;
-#pragma unroll
-        for (int r = 0; r < 16; ++r) {
-            s[r] = __builtin_amdgcn_exp2f(fmaf(s[r], c, -mc));
-            l += s[r];
-        }
-#pragma unroll
-        for (int f = 0; f < PF; ++f) {
-            const auto p = operand<T>(s, f);
-            auto rest = p;
-            if constexpr (sizeof(T) == 2) {
-                float8_t w;
-#pragma unroll
-                for (int j = 0; j < 8; ++j) w[j] = s[8 * f + j] - (float)p[j];
-                rest = __builtin_convertvector(w, typename L::frag);
+        for (int t = 0; t < NT; ++t) acc[t] = 0.0f;
+        m = -INFINITY, l = 0, known = 0;
+        auto step = [&](char* kt, char* vt, char* kn, char* vn, int first) {
+            if (first + kStep < mine.last) {
+                asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // what was read from there has come
+                request(kn, vn, first + kStep);
+                asm volatile("s_waitcnt vmcnt(%0)" ::"n"(kAhead) : "memory");
+            } else {
+                asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
             }
+            const Lane w = Lane::of<CARE>(lane, half);
+            float16_t s = 0.0f;
 #pragma unroll
-            for (int t = 0; t < DT; ++t) {
-                const auto column = column_of<T, DP, 32>(vt, 0, f, t, lane);
-                acc[t] = mma(column, p, acc[t]);
-                if constexpr (sizeof(T) == 2) acc[t] = mma(column, rest, acc[t]);
+            for (int f = 0; f < L::kFrags; ++f) s = mma(L::row(kt, w.at & 31, f, w.half), q[f], s);
+            if (first + 32 > mine.last) {
+#pragma unroll
+                for (int r = 0; r < 16; ++r)
+                    if (first + 4 * half + 8 * (r / 4) + r % 4 >= mine.last) s[r] = -INFINITY;
             }
+            float top = s[0];
+#pragma unroll
+            for (int r = 1; r < 16; ++r) top = fmaxf(top, s[r]);
+            top = max_halves(top);
+            if (__any((top - m) * c > grow)) {
+                const float now = fmaxf(m, top);
+                const float by = now == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f((m - now) * c);
+                m = now;
+                l *= by;
+                if constexpr (CARE) {
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) acc[0][r] = scaled(acc[0][r], by);
+                } else {
+#pragma unroll
+                    for (int t = 0; t < NT; ++t) acc[t] *= by;
+                }
+            }
+            const float mc = m == -INFINITY ? 0.0f : m * c - Types<T>::kForward;
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                s[r] = __builtin_amdgcn_exp2f(fmaf(s[r], c, -mc));
+                l += s[r];
+            }
+            if constexpr (!CARE) {
+#pragma unroll
+                for (int f = 0; f < PF; ++f) {
+                    const auto p = operand<T>(s, f);
+                    auto rest = p;
+                    if constexpr (sizeof(T) == 2) {
+                        float8_t w;
+#pragma unroll
+                        for (int j = 0; j < 8; ++j) w[j] = s[8 * f + j] - (float)p[j];
+                        rest = __builtin_convertvector(w, typename L::frag);
+                    }
+#pragma unroll
+                    for (int t = 0; t < DT; ++t) {
+                        const auto column = column_of<T, DP, 32>(vt, 0, f, t, lane);
+                        acc[t] = mma(column, p, acc[t]);
+                        if constexpr (sizeof(T) == 2) acc[t] = mma(column, rest, acc[t]);
+                    }
+                }
+            } else {
+                float16_t rest = 0.0f;
+#pragma unroll
+                for (int r = 0; r < 16; ++r) rest[r] = s[r] - (float)(T)s[r];
+                if (finite_product_of<T, DP, 32, sizeof(T) == 2>(vt, 0, t0, w.at, s, rest, acc[0], known))
+                    add_others<T, DP, 32, true>(vt, 0, t0, w.at, first, Bounds{mine.first, mine.last}, acc[0], known);
+            }
+        };
+        for (int first = start; first < mine.last; first += 2 * kStep) {
+            step(kt0, vt0, kt1, vt1, first);
+            if (first + kStep < mine.last) step(kt1, vt1, kt0, vt0, first + kStep);
         }
     };
-    for (int first = start; first < mine.last; first += 2 * kStep) {
-        step(kt0, vt0, kt1, vt1, first);
-        if (first + kStep < mine.last) step(kt1, vt1, kt0, vt0, first + kStep);
-    }
-    // the waves' results: sums under the largest maximum, added in order
-    l = sum_halves(l);
-    if (half == 0) top_of[wave][column] = m, sum_of[wave][column] = l;
-    if (threadIdx.x == 0) bad = 0;
-    __syncthreads();
-    float top = top_of[0][column];
+    // The waves' results, columns 32 t0 ... of the head: sums under the largest maximum, added in order.
+    const bool seen = mine.count > 0;
+    auto finish = [&](auto& acc, auto care, int t0) {
+        constexpr bool CARE = decltype(care)::value;
+        constexpr int NT = CARE ? 1 : DT, QUADS = 8 * NT;
+        l = sum_halves(l);
+        if (half == 0) top_of[wave][column] = m, sum_of[wave][column] = l;
+        if (!CARE && threadIdx.x < 2) bad[threadIdx.x] = 0;
+        __syncthreads();
+        float top = top_of[0][column];
 #pragma unroll
-    for (int w = 1; w < W; ++w) top = fmaxf(top, top_of[w][column]);
-    {
+        for (int w = 1; w < W; ++w) top = fmaxf(top, top_of[w][column]);
         const float by = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((m - top) * c);
         if (live)
 #pragma unroll
-            for (int t = 0; t < DT; ++t)
+            for (int t = 0; t < NT; ++t)
 #pragma unroll
                 for (int g = 0; g < 4; ++g) {
                     float4_t x;
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) x[e] = acc[t][4 * g + e] * by;
-                    *Few<T, DP>::sums(key0, val0, wave, column, 32 * t + 8 * g + 4 * half) = x;
+                    for (int e = 0; e < 4; ++e) x[e] = CARE ? scaled(acc[t][4 * g + e], by) : acc[t][4 * g + e] * by;
+                    *Few<T, DP>::sums(key0, val0, wave, column, 32 * (t0 + t) + 8 * g + 4 * half) = x;
                 }
-    }
-    __syncthreads();
-    const bool seen = mine.count > 0;
-    bool finite_all = true;
-    for (int at = threadIdx.x; at < heads * (DP / 4); at += 64 * W) {
-        const int col = at / (DP / 4), e = at % (DP / 4) * 4, h = h0 + col;
-        if (e >= a.d) continue;
-        float high = top_of[0][col], total = 0;
-        float4_t x = 0.0f;
+        __syncthreads();
+        bool all = true;
+        for (int at = threadIdx.x; at < heads * QUADS; at += 64 * W) {
+            const int col = at / QUADS, e = 32 * t0 + at % QUADS * 4, h = h0 + col;
+            if (e >= a.d) continue;
+            float high = top_of[0][col], total = 0;
+            float4_t x = 0.0f;
 #pragma unroll
-        for (int w = 1; w < W; ++w) high = fmaxf(high, top_of[w][col]);
+            for (int w = 1; w < W; ++w) high = fmaxf(high, top_of[w][col]);
 #pragma unroll
-        for (int w = 0; w < W; ++w) {
-            const float one = top_of[w][col];
-            total += one == -INFINITY ? 0.0f * sum_of[w][col] : sum_of[w][col] * __builtin_amdgcn_exp2f((one - high) * c);
-            x += *Few<T, DP>::sums(key0, val0, w, col, e);
+            for (int w = 0; w < W; ++w) {
+                const float one = top_of[w][col];
+                total += one == -INFINITY ? 0.0f * sum_of[w][col] : sum_of[w][col] * __builtin_amdgcn_exp2f((one - high) * c);
+                x += *Few<T, DP>::sums(key0, val0, w, col, e);
+            }
+            all = all && finite(x[0]) && finite(x[1]) && finite(x[2]) && finite(x[3]);
+            const float log2_top = high == -INFINITY ? high : high * c - Types<T>::kForward;
+            if (mine.count > 1) {
+                float* to = a.partial + (((int64_t)i * a.hq + h) * a.parts + part) * ROW;
+                *(float4_t*)(to + e) = x;
+                if (e == 0) to[DP] = log2_top, to[DP + 1] = total;
+                continue;
+            }
+            const int64_t out = ((int64_t)i * a.hq + h) * a.d + e;
+            const float by = seen ? 1.0f / total : 0.0f;
+            x *= by;
+            const auto y = __builtin_convertvector(x, typename Types<T>::quad);
+            *(typename Types<T>::quad*)((T*)a.o + out) = y;
+            if (a.rest)
+                *(typename Types<T>::quad*)((T*)a.rest + out) =
+                    __builtin_convertvector(x - __builtin_convertvector(y, float4_t), typename Types<T>::quad);
+            if (e == 0) a.lse[h * a.stat_stride + i] = seen ? log2_top + __builtin_amdgcn_logf(total) : -INFINITY;
         }
-        const float log2_top = high == -INFINITY ? high : high * c - Types<T>::kForward;
-        if (mine.count > 1) {
-            float* to = a.partial + (((int64_t)i * a.hq + h) * a.parts + part) * ROW;
-            *(float4_t*)(to + e) = x;
-            if (e == 0) to[DP] = log2_top, to[DP + 1] = total;
-            continue;
-        }
-        const int64_t out = ((int64_t)i * a.hq + h) * a.d + e;
-        const float by = seen ? 1.0f / total : 0.0f;
-        x *= by;
-        const auto y = __builtin_convertvector(x, typename Types<T>::quad);
-        *(typename Types<T>::quad*)((T*)a.o + out) = y;
-        if (a.rest)
-            *(typename Types<T>::quad*)((T*)a.rest + out) =
-                __builtin_convertvector(x - __builtin_convertvector(y, float4_t), typename Types<T>::quad);
-        if (e == 0) a.lse[h * a.stat_stride + i] = seen ? log2_top + __builtin_amdgcn_logf(total) : -INFINITY;
-        finite_all = finite_all && finite(x[0] + x[1] + x[2] + x[3]) && finite(by);
+        return !all;
+    };
+    bool open;
+    {
+        float16_t acc[DT];
+        pass(acc, std::false_type(), 0, 8.0f);
+        open = finish(acc, std::false_type(), 0);
     }
-    if (mine.count > 1) return;
-    if (!finite_all) bad = 1;
-    __syncthreads();
-    if (!bad) return;
-    for (int n = wave; n < heads; n += W) forward_row<T>(a, i, h0 + n, b.lo, b.hi, lane);
+    careful_passes<T, DT>(bad, open, [&](int t, int raise, bool) {
+        float16_t acc[1];
+        clear_own();
+        if (start < mine.last) request(kt0, vt0, start);
+        pass(acc, std::true_type(), t, 8.0f * raise);
+        finish(acc, std::true_type(), t);
+        return live && !all_known(acc[0], known);
+    });
 }
 
 // Adds up the shares of one row's head: eight groups of 32 lanes take every eighth share, then in order. A chain of waits: what
@@ -993,7 +1137,6 @@ __global__ __launch_bounds__(256) void join(Args a) {
     constexpr int ROW = Few<T, DP>::kRow;
     __shared__ float weight[kMostParts], tops[4], totals[4];
     __shared__ __align__(16) float sums[8][DP];
-    __shared__ int bad;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int h = blockIdx.x % a.hq, i = blockIdx.x / a.hq;
     const float* from = a.partial + ((int64_t)i * a.hq + h) * a.parts * ROW;
@@ -1015,7 +1158,6 @@ __global__ __launch_bounds__(256) void join(Args a) {
 #pragma unroll
     for (int n = 1; n < 64; n <<= 1) top = fmaxf(top, __shfl_xor(top, n));
     if (lane == 0) tops[wave] = top;
-    if (threadIdx.x == 0) bad = 0;
     __syncthreads();
     top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
     const float by = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - top);
@@ -1025,12 +1167,25 @@ __global__ __launch_bounds__(256) void join(Args a) {
     __syncthreads();
     if (e < DP) {
         float4_t x = 0.0f;
+        auto add = [&](float4_t y, float by) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) x[j] = fmaf(by, y[j], x[j]);
+        };
         if (e < a.d) {
 #pragma unroll
             for (int n = 0; n < kAhead; ++n)
-                if (n0 + 8 * n < count) x += weight[n0 + 8 * n] * ahead[n];
+                if (n0 + 8 * n < count) add(ahead[n], weight[n0 + 8 * n]);
 #pragma unroll 8
-            for (int n = n0 + 8 * kAhead; n < count; n += 8) x += weight[n] * *(const float4_t*)(from + (int64_t)n * ROW + e);
+            for (int n = n0 + 8 * kAhead; n < count; n += 8) add(*(const float4_t*)(from + (int64_t)n * ROW + e), weight[n]);
+            if (!(finite(x[0]) && finite(x[1]) && finite(x[2]) && finite(x[3]))) {  // (an infinity under a weight of zero stays one)
+                x = 0.0f;
+                for (int n = n0; n < count; n += 8)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const float y = from[(int64_t)n * ROW + e + j];
+                        x[j] = finite(y) ? fmaf(weight[n], y, x[j]) : x[j] + y;
+                    }
+            }
         }
         *(float4_t*)&sums[n0][e] = x;
     }
@@ -1046,10 +1201,7 @@ __global__ __launch_bounds__(256) void join(Args a) {
         ((T*)a.o)[out] = y;
         if (a.rest) ((T*)a.rest)[out] = (T)(x - (float)y);
         if (threadIdx.x == 0) a.lse[h * a.stat_stride + i] = top + __builtin_amdgcn_logf(all);
-        if (!finite(x)) bad = 1;
     }
-    __syncthreads();
-    if (bad && wave == 0) forward_row<T>(a, i, h, b.lo, b.hi, lane);
 }
 
 // ---------------------------------------------------------------------------
@@ -1066,8 +1218,10 @@ __global__ __launch_bounds__(256, (blocks_per_unit<T, DP>())) void query_gradien
     constexpr int PF = sizeof(T) == 2 ? 2 : 4;
     typedef Tile<T, DP, BK> L;
     __shared__ __align__(1024) char key0[L::kBytes], key1[L::kBytes], val0[L::kBytes], val1[L::kBytes];
-    __shared__ int shared[8];
+    __shared__ Shared shared;
+    __shared__ float least[4];
     __shared__ __align__(16) float4_t swap[SPLIT == 2 ? 512 : 1];
+    __shared__ unsigned swap_known[SPLIT == 2 ? 128 : 1];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5;
     int tile, h;
     place(a, a.hq, a.q_order, a.causal, tile, h);
@@ -1084,10 +1238,12 @@ __global__ __launch_bounds__(256, (blocks_per_unit<T, DP>())) void query_gradien
     const char* vbase = (const char*)((const T*)a.v + kh * a.v_head);
     const int krow = (int)a.k_row * (int)sizeof(T), vrow = (int)a.v_row * (int)sizeof(T);
     const typename L::Places kplaces(krow, chunks, wave, lane), vplaces(vrow, chunks, wave, lane);
-    if (all.lo < all.hi) {
+    auto request_first = [&] {
+        if (all.lo >= all.hi) return;
         L::request(key0, kbase, krow, kplaces, all.lo, all.hi, chunks, wave);
         L::request(val0, vbase, vrow, vplaces, all.lo, all.hi, chunks, wave);
-    }
+    };
+    request_first();
     const bool mine = row < a.nq;
     typename L::frag q[L::kFrags], g[L::kFrags];
     load_row<T, L::kFrags>(q, (const char*)((const T*)a.q + i * a.q_row + h * a.q_head), chunks, half);
@@ -1111,101 +1267,120 @@ __global__ __launch_bounds__(256, (blocks_per_unit<T, DP>())) void query_gradien
     if (mine && half == 0) a.delta[h * a.stat_stride + i] = delta;
     const float lse = a.lse[h * a.stat_stride + i], c = a.scale_log2;
     settle();
-    float lift = power<Types<T>::kDs>, low = delta * (kLifted<T> ? lift : 1.0f);
-    float16_t acc[DT];
-#pragma unroll
-    for (int t = 0; t < DT; ++t) acc[t] = 0.0f;
 
-    constexpr bool kAnew = kLifted<T> && DP == 128 && SPLIT == 1;  // (no register is left for the places)
-    auto products = [&](const char* kt, const char* vt, int first) {
+    unsigned known;
+    // `times`, 2^up, is what ds is raised by (first). Returns what to multiply the sums by.
+    auto pass = [&](auto& acc, auto care, int t0, float up, float times) {
+        constexpr bool CARE = decltype(care)::value;
+        constexpr int NT = CARE ? 1 : DT;
+        float lift = times, low = delta * (kLifted<T> ? lift : 1.0f);
+        known = 0;
 #pragma unroll
-        for (int n = 0; n < SUB; ++n) {
-            const int u = SPLIT == 2 ? part : n;
-            if ((SPLIT == 2 || kSparse<T, DP>) && !walk.needs(first + 32 * u, 32)) continue;
-            float16_t s = 0.0f, x = 0.0f;
+        for (int t = 0; t < NT; ++t) acc[t] = 0.0f;
+        auto products = [&](const char* kt, const char* vt, int first) {
 #pragma unroll
-            for (int f = 0; f < L::kFrags; ++f) s = mma(L::row(kt, 32 * u + (lane & 31), f, half), q[f], s);
+            for (int n = 0; n < SUB; ++n) {
+                const int u = SPLIT == 2 ? part : n;
+                if ((SPLIT == 2 || kSparse<T, DP>) && !walk.needs(first + 32 * u, 32)) continue;
+                constexpr bool kAnew = CARE || (kLifted<T> && DP == 128 && SPLIT == 1);  // (no register is left for the places)
+                const Lane l = Lane::of<kAnew>(lane, half);
+                float16_t s = 0.0f, x = 0.0f;
 #pragma unroll
-            for (int f = 0; f < L::kFrags; ++f) x = mma(L::row(vt, 32 * u + (lane & 31), f, half), g[f], x);
+                for (int f = 0; f < L::kFrags; ++f) s = mma(L::row(kt, 32 * u + (CARE ? l.at & 31 : lane & 31), f, CARE ? l.half : half), q[f], s);
 #pragma unroll
-            for (int r = 0; r < 16; ++r) {
+                for (int f = 0; f < L::kFrags; ++f) x = mma(L::row(vt, 32 * u + (CARE ? l.at & 31 : lane & 31), f, CARE ? l.half : half), g[f], x);
+#pragma unroll
+                for (int r = 0; r < 16; ++r) {
+                    if constexpr (kLifted<T>)
+                        x[r] = __builtin_amdgcn_exp2f(fmaf(s[r], c, -lse)) * fmaf(x[r], lift, -low);
+                    else
+                        x[r] = raised<T>(fmaf(s[r], c, -lse), up, times) * (x[r] - low);
+                }
+                if (!(SPLIT == 2 || kSparse<T, DP> ? walk.whole(first + 32 * u, 32) : walk.whole(first, BK))) {
+                    const int shift = first + 32 * u + 4 * half - b.lo;
+                    const unsigned n = b.hi - b.lo;
+#pragma unroll
+                    for (int r = 0; r < 16; ++r)
+                        if ((unsigned)(shift + 8 * (r / 4) + r % 4) >= n) x[r] = 0.0f;
+                }
+                typename L::frag lifted[2];
                 if constexpr (kLifted<T>)
-                    x[r] = __builtin_amdgcn_exp2f(fmaf(s[r], c, -lse)) * fmaf(x[r], lift, -low);
-                else
-                    x[r] = raised<T, Types<T>::kDs>(fmaf(s[r], c, -lse)) * (x[r] - low);
+                    lifted_operands<T>(x, lifted, [&](float by) {
+                        lift *= by, low *= by;
+#pragma unroll
+                        for (int t = 0; t < NT; ++t) acc[t] *= by;
+                    });
+                if constexpr (CARE) {
+                    if (finite_product_of<T, DP, BK>(kt, 32 * u, t0, l.at, x, x, acc[0], known))
+                        add_others<T, DP, BK, false>(kt, 32 * u, t0, l.at, first + 32 * u, b, acc[0], known);
+                } else {
+#pragma unroll
+                    for (int f = 0; f < PF; ++f) {
+                        const auto d = kLifted<T> ? lifted[f & 1] : operand<T>(x, f);
+#pragma unroll
+                        for (int t = 0; t < DT; ++t) acc[t] = mma(column_of<T, DP, BK>(kt, 32 * u, f, t, kAnew ? l.at : lane), d, acc[t]);
+                    }
+                }
+                __builtin_amdgcn_sched_barrier(0);  // (reads of the next 32 keys this early would take registers that are not there)
             }
-            if (!(SPLIT == 2 || kSparse<T, DP> ? walk.whole(first + 32 * u, 32) : walk.whole(first, BK))) {
-                const int shift = first + 32 * u + 4 * half - b.lo;
-                const unsigned n = b.hi - b.lo;
-#pragma unroll
-                for (int r = 0; r < 16; ++r)
-                    if ((unsigned)(shift + 8 * (r / 4) + r % 4) >= n) x[r] = 0.0f;
+        };
+        auto step = [&](char* kt, char* vt, char* kn, char* vn, int first) {
+            arrived();
+            if (first + BK < all.hi) {
+                L::request(kn, kbase, krow, kplaces, first + BK, all.hi, chunks, wave);
+                L::request(vn, vbase, vrow, vplaces, first + BK, all.hi, chunks, wave);
             }
-            const Lane anew = Lane::of<kAnew>(lane, half);
-            typename L::frag lifted[2];
-            if constexpr (kLifted<T>)
-                lifted_operands<T>(x, lifted, [&](float by) {
-                    lift *= by, low *= by;
-#pragma unroll
-                    for (int t = 0; t < DT; ++t) acc[t] *= by;
-                });
-#pragma unroll
-            for (int f = 0; f < PF; ++f) {
-                const auto d = kLifted<T> ? lifted[f & 1] : operand<T>(x, f);
-#pragma unroll
-                for (int t = 0; t < DT; ++t) acc[t] = mma(column_of<T, DP, BK>(kt, 32 * u, f, t, kAnew ? anew.at : lane), d, acc[t]);
-            }
-            __builtin_amdgcn_sched_barrier(0);  // (reads of the next 32 keys this early would take registers that are not there)
+            if (walk.needs(first, BK)) products(kt, vt, first);
+        };
+        for (int first = all.lo; first < all.hi; first += 2 * BK) {
+            step(key0, val0, key1, val1, first);
+            if (first + BK < all.hi) step(key1, val1, key0, val0, first + BK);
         }
-    };
-    auto step = [&](char* kt, char* vt, char* kn, char* vn, int first) {
-        arrived();
-        if (first + BK < all.hi) {
-            L::request(kn, kbase, krow, kplaces, first + BK, all.hi, chunks, wave);
-            L::request(vn, vbase, vrow, vplaces, first + BK, all.hi, chunks, wave);
-        }
-        if (walk.needs(first, BK)) products(kt, vt, first);
-    };
-    for (int first = all.lo; first < all.hi; first += 2 * BK) {
-        step(key0, val0, key1, val1, first);
-        if (first + BK < all.hi) step(key1, val1, key0, val0, first + BK);
-    }
-    const float scale = c * 0.6931471805599453f * (kLifted<T> ? 1.0f / lift : power<-Types<T>::kDs>);
-    if constexpr (kLifted<T>) {
-        __shared__ float least[4];
-        const float mine = wave_least(lift);
-        if (lane == 0) least[wave] = mine;
-        __syncthreads();
-        if (threadIdx.x == 0) a.lifts[(int64_t)h * a.q_tiles + tile] = fminf(fminf(least[0], least[1]), fminf(least[2], least[3]));
-    }
-    if constexpr (SPLIT == 2) {
-        // the wave with the second groups of keys hands its sums to the one with the first, 32 columns of the head at a time
-#pragma unroll
-        for (int t = 0; t < DT; ++t) {
-            acc[t] *= scale;  // (the two may be lifted differently)
+        if constexpr (kLifted<T> && !CARE) {
+            const float mine = wave_least(lift);
+            if (lane == 0) least[wave] = mine;
             __syncthreads();
-            if (part)
-#pragma unroll
-                for (int g = 0; g < 4; ++g)
-                    swap[(rows * 4 + g) * 64 + lane] = float4_t{acc[t][4 * g], acc[t][4 * g + 1], acc[t][4 * g + 2], acc[t][4 * g + 3]};
-            __syncthreads();
-            if (!part)
-#pragma unroll
-                for (int g = 0; g < 4; ++g)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) acc[t][4 * g + e] += swap[(rows * 4 + g) * 64 + lane][e];
+            if (threadIdx.x == 0) a.lifts[(int64_t)h * a.q_tiles + tile] = fminf(fminf(least[0], least[1]), fminf(least[2], least[3]));
         }
-        if (part) return;
+        if constexpr (SPLIT == 2) {
+            // the wave with the second groups of keys hands its sums to the one with the first, 32 columns of the head at a time
+#pragma unroll
+            for (int t = 0; t < NT; ++t) {
+                acc[t] *= 1.0f / lift;  // (the two may be lifted differently)
+                if (CARE && part) swap_known[64 * rows + lane] = known;
+                __syncthreads();
+                if (part)
+#pragma unroll
+                    for (int g = 0; g < 4; ++g)
+                        swap[(rows * 4 + g) * 64 + lane] = float4_t{acc[t][4 * g], acc[t][4 * g + 1], acc[t][4 * g + 2], acc[t][4 * g + 3]};
+                __syncthreads();
+                if (CARE && !part) known |= swap_known[64 * rows + lane];
+                if (!part)
+#pragma unroll
+                    for (int g = 0; g < 4; ++g)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) acc[t][4 * g + e] += swap[(rows * 4 + g) * 64 + lane][e];
+            }
+        }
+        return SPLIT == 2 ? 1.0f : 1.0f / lift;
+    };
+    const float ln2 = 0.6931471805599453f;
+    bool bad = mine && !part;
+    {
+        float16_t acc[DT];
+        const float by = pass(acc, std::false_type(), 0, (float)Types<T>::kDs, power<Types<T>::kDs>);
+        if (bad) store_row<T, DT>((T*)a.dq + ((int64_t)i * a.hq + h) * a.d, acc, c * ln2 * by, a.d, half);
+        bad = bad && !all_finite<DT>(acc);
     }
-    if (mine)
-        store_row<T, DT>((T*)a.dq + ((int64_t)i * a.hq + h) * a.d, acc, SPLIT == 2 ? 1.0f : scale, a.d, half);
-    uint64_t bad = __ballot(mine && !all_finite<DT>(acc));
-    bad = (bad | bad >> 32) & 0xffffffffu;
-    while (bad) {
-        const int at = __builtin_ctzll(bad);
-        bad &= bad - 1;
-        query_gradient_row<T>(a, (tile * (4 / SPLIT) + rows) * 32 + at, h, __shfl(b.lo, at), __shfl(b.hi, at), lane);
-    }
+    careful_passes<T, DT>(shared.bad, bad, [&](int t, int raise, bool which) {
+        float16_t acc[1];
+        request_first();
+        const int up = Types<T>::kDs * raise;
+        const float by = pass(acc, std::true_type(), t, (float)up, __builtin_amdgcn_ldexpf(1.0f, up));
+        T* dq = (T*)a.dq + ((int64_t)i * a.hq + h) * a.d;
+        if (which) store_part<T>(dq + 32 * t, acc[0], c * ln2 * by, a.d - 32 * t, half, nullptr, !raise);
+        return which && !all_known(acc[0], known);
+    });
 }
 
 // ---------------------------------------------------------------------------
@@ -1230,7 +1405,8 @@ __global__ __launch_bounds__(256, UNIT) void key_gradient(Args a) {
     __shared__ __align__(1024) char gra0[L::kBytes], gra1[L::kBytes];
     __shared__ __align__(1024) float sta0[2 * BQ], sta1[2 * BQ];  // lse, then delta, of the tile's rows
     __shared__ __align__(16) float4_t swap[4 - KEYS][4][64];
-    __shared__ int shared[8];
+    __shared__ unsigned swap_known[4 - KEYS][64];
+    __shared__ Shared shared;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5;
     const int keys = wave % KEYS, r0 = 32 * (wave / KEYS);  // which 32 keys, and the wave's first row of a tile
     int tile, kh;
@@ -1252,7 +1428,7 @@ __global__ __launch_bounds__(256, UNIT) void key_gradient(Args a) {
     // Tiles of rows are walked from the last on. Causal: blocks of neighbouring keys, which run at the same time on an XCD,
     // see the same last rows and differ in their first, and this way they read the same tiles at the same time.
     const int top = all.lo < all.hi ? all.lo + (all.hi - all.lo - 1) / BQ * BQ : 0, last_head = (kh + 1) * group;
-    int next_h = all.lo < all.hi ? kh * group : last_head, next_first = top;  // the tile to be requested
+    int next_h = last_head, next_first = top;  // the tile to be requested
     auto request = [&](char* qt, char* gt, float* st) {
         if (next_h == last_head) return;
         L::request(qt, (const char*)((const T*)a.q + next_h * a.q_head), qrow, qplaces, next_first, all.hi, chunks, wave);
@@ -1265,13 +1441,12 @@ __global__ __launch_bounds__(256, UNIT) void key_gradient(Args a) {
         next_first -= BQ;
         if (next_first < all.lo) next_first = top, ++next_h;
     };
-    request(que0, gra0, sta0);
+    auto request_first = [&] {
+        if (all.lo < all.hi) next_h = kh * group;
+        request(que0, gra0, sta0);
+    };
+    request_first();
     const float c = a.scale_log2;
-    float16_t dk[DT], dv[DT];
-#pragma unroll
-    for (int t = 0; t < DT; ++t) dk[t] = 0.0f, dv[t] = 0.0f;
-    settle();
-
     // What ds carries over what p does; where it is lifted, as far as the queries' gradient has found that none passes 2^14.
     float ratio = power<Types<T>::kDs - Types<T>::kP>;
     if constexpr (kLifted<T>) {
@@ -1280,139 +1455,169 @@ __global__ __launch_bounds__(256, UNIT) void key_gradient(Args a) {
         for (int n = lane; n < tiles * group; n += 64) lift = fminf(lift, a.lifts[(int64_t)(kh * group + n / tiles) * a.q_tiles + tile0 + n % tiles]);
         ratio = wave_least(lift) * power<13 - Types<T>::kP>;
     }
-    // p and ds from the scores and g.v
-    auto weigh = [&](float16_t& s, float16_t& x, const float* st) {
+    settle();
+
+    unsigned known;
+    // `times`, 2^up, is what p is raised by. Leaves the sums in the first waves' registers.
+    auto pass = [&](auto& dk, auto& dv, auto care, int t0, float up, float times) {
+        constexpr bool CARE = decltype(care)::value;
+        constexpr int NT = CARE ? 1 : DT;
 #pragma unroll
-        for (int g = 0; g < 4; ++g) {
-            const float4_t lse = *(const float4_t*)(st + r0 + 8 * g + 4 * half);
-            const float4_t delta = *(const float4_t*)(st + BQ + r0 + 8 * g + 4 * half);
+        for (int t = 0; t < NT; ++t) dk[t] = 0.0f, dv[t] = 0.0f;
+        known = 0;
+        // p and ds from the scores and g.v
+        auto weigh = [&](float16_t& s, float16_t& x, const float* st) {
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const int r = 4 * g + e;
-                s[r] = raised<T, Types<T>::kP>(fmaf(s[r], c, -lse[e]));
-                if (DK) x[r] = s[r] * fmaf(x[r], ratio, -delta[e] * ratio);
+            for (int g = 0; g < 4; ++g) {
+                const float4_t lse = *(const float4_t*)(st + r0 + 8 * g + 4 * half);
+                const float4_t delta = *(const float4_t*)(st + BQ + r0 + 8 * g + 4 * half);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const int r = 4 * g + e;
+                    s[r] = raised<T>(fmaf(s[r], c, -lse[e]), up, times);
+                    if (DK) x[r] = s[r] * fmaf(x[r], ratio, -delta[e] * ratio);
+                }
             }
-        }
-    };
-    auto hide = [&](float16_t& s, float16_t& x, int first) {
-        if (walk.whole(first + r0, 32)) return;
-        const int shift = first + r0 + 4 * half - b.lo;
-        const unsigned n = b.hi - b.lo;
+        };
+        auto hide = [&](float16_t& s, float16_t& x, int first) {
+            if (walk.whole(first + r0, 32)) return;
+            const int shift = first + r0 + 4 * half - b.lo;
+            const unsigned n = b.hi - b.lo;
 #pragma unroll
-        for (int r = 0; r < 16; ++r)
-            if ((unsigned)(shift + 8 * (r / 4) + r % 4) >= n) s[r] = 0.0f, x[r] = 0.0f;
-    };
-    const int steps = all.lo < all.hi ? ((all.hi - all.lo - 1) / BQ + 1) * group : 0;
-    int first = top;
-    auto step = [&](char* qt, char* gt, float* st, char* qn, char* gn, float* sn) {
-        arrived();
-        request(qn, gn, sn);
-        const int now = first;
-        first -= BQ;
-        if (first < all.lo) first = top;
-        if (kSparse<T, DP> && !walk.needs(now + r0, 32)) return;
-        float16_t s = 0.0f, x = 0.0f;
-        if constexpr (kFenced<T, DP> && WHAT == 3) {
-            const Lane l = Lane::of<UNIT == 2>(lane, half);  // (kept, the places would take registers that are not there)
-            constexpr int kBatch = L::kFrags / 2;
-            typename L::frag rows[2][2 * kBatch], columns[2][2 * DT];
-            auto load_rows = [&](int n) {
+            for (int r = 0; r < 16; ++r)
+                if ((unsigned)(shift + 8 * (r / 4) + r % 4) >= n) s[r] = 0.0f, x[r] = 0.0f;
+        };
+        const int steps = all.lo < all.hi ? ((all.hi - all.lo - 1) / BQ + 1) * group : 0;
+        int first = top;
+        auto step = [&](char* qt, char* gt, float* st, char* qn, char* gn, float* sn) {
+            arrived();
+            request(qn, gn, sn);
+            const int now = first;
+            first -= BQ;
+            if (first < all.lo) first = top;
+            if (kSparse<T, DP> && !walk.needs(now + r0, 32)) return;
+            float16_t s = 0.0f, x = 0.0f;
+            if constexpr (kFenced<T, DP> && WHAT == 3 && !CARE) {
+                const Lane l = Lane::of<UNIT == 2>(lane, half);  // (kept, the places would take registers that are not there)
+                constexpr int kBatch = L::kFrags / 2;
+                typename L::frag rows[2][2 * kBatch], columns[2][2 * DT];
+                auto load_rows = [&](int n) {
 #pragma unroll
-                for (int f = 0; f < kBatch; ++f) {
-                    rows[n][2 * f] = L::row(qt, r0 + (l.at & 31), kBatch * n + f, l.half);
-                    rows[n][2 * f + 1] = L::row(gt, r0 + (l.at & 31), kBatch * n + f, l.half);
+                    for (int f = 0; f < kBatch; ++f) {
+                        rows[n][2 * f] = L::row(qt, r0 + (l.at & 31), kBatch * n + f, l.half);
+                        rows[n][2 * f + 1] = L::row(gt, r0 + (l.at & 31), kBatch * n + f, l.half);
+                    }
+                    __builtin_amdgcn_sched_barrier(0);
+                };
+                auto load_columns = [&](int f) {
+#pragma unroll
+                    for (int t = 0; t < DT; ++t) {
+                        columns[f][2 * t] = column_of<T, DP, BQ>(gt, r0, f, t, l.at);
+                        columns[f][2 * t + 1] = column_of<T, DP, BQ>(qt, r0, f, t, l.at);
+                    }
+                    __builtin_amdgcn_sched_barrier(0);
+                };
+                load_rows(0);
+                load_rows(1);
+#pragma unroll
+                for (int f = 0; f < L::kFrags; ++f) {
+                    s = mma(rows[f / kBatch][2 * (f % kBatch)], k[f], s);
+                    x = mma(rows[f / kBatch][2 * (f % kBatch) + 1], v[f], x);
                 }
                 __builtin_amdgcn_sched_barrier(0);
-            };
-            auto load_columns = [&](int f) {
+                load_columns(0);
+                weigh(s, x, st);
+                hide(s, x, now);
+                load_columns(1);
 #pragma unroll
-                for (int t = 0; t < DT; ++t) {
-                    columns[f][2 * t] = column_of<T, DP, BQ>(gt, r0, f, t, l.at);
-                    columns[f][2 * t + 1] = column_of<T, DP, BQ>(qt, r0, f, t, l.at);
+                for (int f = 0; f < 2; ++f) {
+                    const auto p = operand<T>(s, f), d = operand<T>(x, f);
+#pragma unroll
+                    for (int t = 0; t < DT; ++t) {
+                        dv[t] = mma(columns[f][2 * t], p, dv[t]);
+                        dk[t] = mma(columns[f][2 * t + 1], d, dk[t]);
+                    }
                 }
-                __builtin_amdgcn_sched_barrier(0);
-            };
-            load_rows(0);
-            load_rows(1);
+            } else {
+                const Lane l = Lane::of<CARE || kSparse<T, DP>>(lane, half);
 #pragma unroll
-            for (int f = 0; f < L::kFrags; ++f) {
-                s = mma(rows[f / kBatch][2 * (f % kBatch)], k[f], s);
-                x = mma(rows[f / kBatch][2 * (f % kBatch) + 1], v[f], x);
+                for (int f = 0; f < L::kFrags; ++f) s = mma(L::row(qt, r0 + (l.at & 31), f, l.half), k[f], s);
+#pragma unroll
+                for (int f = 0; f < L::kFrags; ++f)
+                    if (DK) x = mma(L::row(gt, r0 + (l.at & 31), f, l.half), v[f], x);
+                weigh(s, x, st);
+                hide(s, x, now);
+                if constexpr (CARE) {
+                    __builtin_amdgcn_sched_barrier(0);
+                    bool others = DV && finite_product_of<T, DP, BQ>(gt, r0, t0, l.at, s, s, dv[0], known);
+                    if (DK && finite_product_of<T, DP, BQ>(qt, r0, t0, l.at, x, x, dk[0], known)) others = true;
+                    if (DV && others) add_others<T, DP, BQ, true>(gt, r0, t0, l.at, now + r0, b, dv[0], known);
+                    if (DK && others) add_others<T, DP, BQ, false, 16>(qt, r0, t0, l.at, now + r0, b, dk[0], known);
+                } else {
+#pragma unroll
+                    for (int f = 0; f < PF; ++f) {
+                        if (DV) {
+                            const auto p = operand<T>(s, f);
+#pragma unroll
+                            for (int t = 0; t < DT; ++t) dv[t] = mma(column_of<T, DP, BQ>(gt, r0, f, t, l.at), p, dv[t]);
+                        }
+                        if (DK) {
+                            const auto d = operand<T>(x, f);
+#pragma unroll
+                            for (int t = 0; t < DT; ++t) dk[t] = mma(column_of<T, DP, BQ>(qt, r0, f, t, l.at), d, dk[t]);
+                        }
+                    }
+                }
             }
-            __builtin_amdgcn_sched_barrier(0);
-            load_columns(0);
-            weigh(s, x, st);
-            hide(s, x, now);
-            load_columns(1);
-#pragma unroll
-            for (int f = 0; f < 2; ++f) {
-                const auto p = operand<T>(s, f), d = operand<T>(x, f);
-#pragma unroll
-                for (int t = 0; t < DT; ++t) {
-                    dv[t] = mma(columns[f][2 * t], p, dv[t]);
-                    dk[t] = mma(columns[f][2 * t + 1], d, dk[t]);
-                }
-            }
-        } else {
-            const Lane l = Lane::of<kSparse<T, DP>>(lane, half);
-#pragma unroll
-            for (int f = 0; f < L::kFrags; ++f) s = mma(L::row(qt, r0 + (l.at & 31), f, l.half), k[f], s);
-#pragma unroll
-            for (int f = 0; f < L::kFrags; ++f)
-                if (DK) x = mma(L::row(gt, r0 + (l.at & 31), f, l.half), v[f], x);
-            weigh(s, x, st);
-            hide(s, x, now);
-#pragma unroll
-            for (int f = 0; f < PF; ++f) {
-                if (DV) {
-                    const auto p = operand<T>(s, f);
-#pragma unroll
-                    for (int t = 0; t < DT; ++t) dv[t] = mma(column_of<T, DP, BQ>(gt, r0, f, t, l.at), p, dv[t]);
-                }
-                if (DK) {
-                    const auto d = operand<T>(x, f);
-#pragma unroll
-                    for (int t = 0; t < DT; ++t) dk[t] = mma(column_of<T, DP, BQ>(qt, r0, f, t, l.at), d, dk[t]);
-                }
-                }
+        };
+        for (int n = 0; n < steps; n += 2) {
+            step(que0, gra0, sta0, que1, gra1, sta1);
+            if (n + 1 < steps) step(que1, gra1, sta1, que0, gra0, sta0);
         }
-    };
-    for (int n = 0; n < steps; n += 2) {
-        step(que0, gra0, sta0, que1, gra1, sta1);
-        if (n + 1 < steps) step(que1, gra1, sta1, que0, gra0, sta0);
-    }
-    // the waves with a tile's later rows hand their sums to those with the first ones, 32 columns of the head at a time
+        // the waves with a tile's later rows hand their sums to those with the first ones, 32 columns of the head at a time
 #pragma unroll
-    for (int t = DK ? 0 : DT; t < (DV ? 2 * DT : DT); ++t) {
-        float16_t& x = t < DT ? dk[t] : dv[t - DT];
-        __syncthreads();
-        if (r0)
-#pragma unroll
-            for (int g = 0; g < 4; ++g)
-                swap[wave - KEYS][g][lane] = float4_t{x[4 * g], x[4 * g + 1], x[4 * g + 2], x[4 * g + 3]};
-        __syncthreads();
-        if (!r0)
-#pragma unroll
-            for (int n = 0; n < GROUPS - 1; ++n)
+        for (int t = DK ? 0 : NT; t < (DV ? 2 * NT : NT); ++t) {
+            float16_t& x = t < NT ? dk[t] : dv[t - NT];
+            if (CARE && r0) swap_known[wave - KEYS][lane] = known;
+            __syncthreads();
+            if (r0)
 #pragma unroll
                 for (int g = 0; g < 4; ++g)
+                    swap[wave - KEYS][g][lane] = float4_t{x[4 * g], x[4 * g + 1], x[4 * g + 2], x[4 * g + 3]};
+            __syncthreads();
+            if (!r0)
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) x[4 * g + e] += swap[n * KEYS + keys][g][lane][e];
-    }
-    if (r0) return;
-    const bool mine = row < a.nk;
-    if (mine) {
+                for (int n = 0; n < GROUPS - 1; ++n) {
+                    if (CARE) known |= swap_known[n * KEYS + keys][lane];
+#pragma unroll
+                    for (int g = 0; g < 4; ++g)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) x[4 * g + e] += swap[n * KEYS + keys][g][lane][e];
+                }
+        }
+    };
+    const float ln2 = 0.6931471805599453f;
+    bool bad = row < a.nk && !r0;
+    {
+        constexpr float by = power<-Types<T>::kP>;
+        float16_t dk[DT], dv[DT];
+        pass(dk, dv, std::false_type(), 0, (float)Types<T>::kP, power<Types<T>::kP>);
         const int64_t at = ((int64_t)j * a.hk + kh) * a.d;
-        if (DK) store_row<T, DT>((T*)a.dk + at, dk, c * (0.6931471805599453f * power<-Types<T>::kP> / ratio), a.d, half);
-        if (DV) store_row<T, DT>((T*)a.dv + at, dv, power<-Types<T>::kP>, a.d, half);
+        if (DK && bad) store_row<T, DT>((T*)a.dk + at, dk, c * (ln2 * by / ratio), a.d, half);
+        if (DV && bad) store_row<T, DT>((T*)a.dv + at, dv, by, a.d, half);
+        bad = bad && !((!DK || all_finite<DT>(dk)) && (!DV || all_finite<DT>(dv)));
     }
-    uint64_t bad = __ballot(mine && !((!DK || all_finite<DT>(dk)) && (!DV || all_finite<DT>(dv))));
-    bad = (bad | bad >> 32) & 0xffffffffu;
-    while (bad) {
-        const int at = __builtin_ctzll(bad);
-        bad &= bad - 1;
-        key_gradient_row<T>(a, (tile * KEYS + keys) * 32 + at, kh, __shfl(b.lo, at), __shfl(b.hi, at), lane);
-    }
+    careful_passes<T, DT>(shared.bad, bad, [&](int t, int raise, bool mine) {
+        float16_t dk[1], dv[1];
+        request_first();
+        const int up = Types<T>::kP * raise;
+        pass(dk, dv, std::true_type(), t, (float)up, __builtin_amdgcn_ldexpf(1.0f, up));
+        const float by = __builtin_amdgcn_ldexpf(1.0f, -up);
+        const int64_t at = ((int64_t)anew(j) * a.hk + kh) * a.d;
+        if (DK && mine) store_part<T>((T*)a.dk + at + 32 * t, dk[0], c * (ln2 * by / ratio), a.d - 32 * t, half, nullptr, !raise);
+        if (DV && mine) store_part<T>((T*)a.dv + at + 32 * t, dv[0], by, a.d - 32 * t, half, nullptr, !raise);
+        return mine && !((!DK || all_known(dk[0], known >> 16)) && (!DV || all_known(dv[0], known)));
+    });
 }
 
 }  // namespace packed_attention

@@ -749,3 +749,174 @@ def test_single_rows_lose_no_more_than_the_outputs_rounding(dtype, segments, key
     want = torch.bmm(p, vv).view(segments, hq, d)
     before = N.HALF_UNIT[dtype] ** (2 if few else 1) * torch.bmm(p * p, vv * vv).sum().sqrt() + 2.0 ** -17 * want.norm()
     assert (out - want).norm() <= (want.to(dtype) - want).norm() + 2 * before
+
+
+# ---------------------------------------------------------------------------
+# results that are not finite
+# ---------------------------------------------------------------------------
+
+
+def all_of(leaves, q_ptr, k_ptr, k_len, causal, g):
+    out, lse = oeq.packed_attention(*leaves, q_ptr, k_ptr, k_len=k_len, causal=causal, return_lse=True)
+    return dict(zip(("out", "lse", "dq", "dk", "dv"), (out, lse) + torch.autograd.grad(out, leaves, g)))
+
+
+SPOILT = {
+    "small": ([20, 30, 1, 9] * 5, [25, 33, 40, 9] * 5, [20, 30, 7, 9] * 5, 4, 2),
+    "long": ([700, 61], [900, 200], [700, 90], 2, 1),
+    "many": ([50] * 90, [70] * 90, [50] * 90, 8, 8),
+    "single": ([1] * 9, [1500] * 9, [900, 3, 0, 1499, 600, 1, 256, 700, 64], 8, 2),
+}
+
+
+@pytest.mark.parametrize("d", [32, 72, 128])
+@pytest.mark.parametrize("case", SPOILT)
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+def test_hidden_rows_change_no_bit(dtype, case, d):
+    """Slots behind a cache's filled part and rows outside all segments: whatever they hold, every result is the same."""
+    q_lens, k_lens, k_len, hq, hk = SPOILT[case]
+    q_ptr, k_ptr = starts(q_lens, 2), starts(k_lens, 3)
+    nq, nk = q_ptr[-1] + 2, k_ptr[-1] + 4
+    seen_q = torch.zeros(nq, dtype=torch.bool, device="cuda")
+    seen_q[2:-2] = True
+    seen_k = torch.zeros(nk, dtype=torch.bool, device="cuda")
+    for first, n in zip(k_ptr, k_len):
+        seen_k[first:first + n] = True
+    base = [normal(n, h, d, dtype=dtype, seed=s) for s, (n, h) in enumerate(((nq, hq), (nk, hk), (nk, hk), (nq, hq)))]
+    want = None
+    for causal in (False, True):
+        for value in (0.0, math.nan, math.inf, -math.inf):
+            leaves = []
+            for n, t in enumerate(base):
+                t = t.clone()
+                t[~(seen_k if n in (1, 2) else seen_q)] = value
+                leaves.append(t)
+            got = all_of([t.requires_grad_() for t in leaves[:3]], on_gpu(q_ptr), on_gpu(k_ptr), on_gpu(k_len), causal, leaves[3])
+            if value == 0.0:
+                want = got
+            for name, x in got.items():
+                assert torch.equal(x, want[name]), (name, value, causal)
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("rows", [150, 700])
+def test_later_tokens_change_no_bit(dtype, rows):
+    """Causal: what comes after a row, in the same tile or a later one."""
+    bad = rows - 45
+    base = [normal(rows, h, 64, dtype=dtype, seed=s) for s, h in enumerate((4, 2, 2, 4))]
+    ptr, results = on_gpu([0, rows]), []
+    for value in (1.0, math.nan, math.inf, -math.inf):
+        leaves = [t.clone() for t in base]
+        leaves[1][bad], leaves[2][bad + 1, 1, 5], leaves[2][bad] = value, value, value
+        results.append(all_of([t.requires_grad_() for t in leaves[:3]], ptr, ptr, None, True, leaves[3]))
+        for name in ("out", "lse", "dq"):
+            assert torch.equal(results[-1][name][:bad], results[0][name][:bad]), (name, value)
+            if value != 1.0 and name != "lse":
+                assert not torch.isfinite(results[-1][name][bad:, 2:]).all()
+
+
+@pytest.mark.parametrize("form", ["tiles", "few", "shares"])
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+def test_visible_infinities_come_to_what_they_are(dtype, form):
+    """A weight is above zero: an infinity of either sign stays one, both together and a NaN are NaN, columns apart."""
+    segments, rows, keys = {"tiles": (3, 70, 90), "few": (40, 1, 200), "shares": (1, 1, 9000)}[form]
+    q, k, v = (normal(segments * n, h, 40, dtype=dtype, seed=s) for s, (n, h) in enumerate(((rows, 4), (keys, 2), (keys, 2))))
+    want = torch.zeros(segments, keys, 2, 40)
+    for value, keys_at, column in ((math.inf, [3], 0), (-math.inf, [0, 88], 7), (math.inf, [5], 11), (-math.inf, [70], 11),
+                                   (math.nan, [60], 39)):
+        for at in keys_at:
+            v.view(segments, keys, 2, 40)[-1, at, 1, column] = value
+            want[-1, at, 1, column] = value
+    q_ptr, k_ptr = (on_gpu([n * i for i in range(segments + 1)]) for n in (rows, keys))
+    clean = v.clone()
+    clean[~torch.isfinite(v)] = 0.5
+    out = oeq.packed_attention(q, k, v, q_ptr, k_ptr, causal=rows > 1).view(segments, rows, 4, 40)
+    other = oeq.packed_attention(q, k, clean, q_ptr, k_ptr, causal=rows > 1).view(segments, rows, 4, 40)
+    for i in range(rows):
+        seen = want[-1, :keys - rows + 1 + i, 1]
+        expect = seen.sum(0)  # (infinities and NaN add up as they should; elsewhere zero)
+        for h in (2, 3):
+            got = out[-1, i, h].float().cpu()
+            special = ~torch.isfinite(expect)
+            assert torch.equal(got[special].nan_to_num(nan=2.0), expect[special].nan_to_num(nan=2.0)), i
+            untouched = torch.isfinite(want[-1, :, 1]).all(0)
+            assert torch.equal(got[untouched], other[-1, i, h].float().cpu()[untouched])
+    assert torch.equal(out[..., :2, :], other[..., :2, :]) and torch.equal(out[:-1], other[:-1])
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+def test_gradients_that_are_not_finite_stay_with_what_sees_them(dtype):
+    n, ptr = 300, on_gpu([0, 130, 300])
+    leaves = [normal(n, h, 64, dtype=dtype, seed=s).requires_grad_() for s, h in enumerate((4, 2, 2))]
+    g = normal(n, 4, 64, dtype=dtype, seed=4)
+    clean = all_of(leaves, ptr, ptr, None, True, g)
+    g[200, 3, 9] = -math.inf
+    got = all_of(leaves, ptr, ptr, None, True, g)
+    seen = torch.arange(n, device="cuda")
+    seen = (seen >= 130) & (seen <= 200)
+    assert torch.equal(got["dv"][:, 0], clean["dv"][:, 0]) and torch.equal(got["dv"][~seen], clean["dv"][~seen])
+    assert (got["dv"][seen, 1, 9] == -math.inf).all()
+    others = torch.arange(64, device="cuda") != 9
+    assert torch.equal(got["dv"][..., others], clean["dv"][..., others])
+    assert torch.equal(got["dk"][~seen], clean["dk"][~seen]) and torch.equal(got["dk"][:, 0], clean["dk"][:, 0])
+    assert torch.isnan(got["dq"][200, 3]).all()
+    row = torch.arange(n, device="cuda") != 200
+    assert torch.equal(got["dq"][row], clean["dq"][row]) and torch.equal(got["dq"][200, :3], clean["dq"][200, :3])
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("rows,keys", [(90, 90), (1, 5000)])
+def test_numbers_near_the_largest(dtype, rows, keys):
+    """Values and output gradients whose sums stay in the type's range though raised weights times them do not."""
+    q, k, v = (normal(n, 2, 64, dtype=dtype, seed=s) for s, n in enumerate((rows, keys, keys)))
+    q_ptr, k_ptr = on_gpu([0, rows]), on_gpu([0, keys])
+    big = (v * 5e36).requires_grad_(False)
+    out = oeq.packed_attention(4 * q, k, big, q_ptr, k_ptr)
+    want = gradients_64(4 * q, k, big, torch.zeros_like(q))["out"]
+    assert torch.isfinite(out).all()
+    check_norm(out, *want, dtype, "out", more=2.0 ** -16)
+    leaves = [t.requires_grad_() for t in (q, k, v)]
+    g = 1e28 * normal(rows, 2, 64, dtype=dtype, seed=6)
+    want = gradients_64(q, k, v, g)
+    for name, x in zip(("dq", "dk", "dv"), torch.autograd.grad(oeq.packed_attention(q, k, v, q_ptr, k_ptr), leaves, g)):
+        check_norm(x, *want[name], dtype, name, more=2.0 ** -16)
+
+
+def test_results_that_are_not_finite_take_a_few_times_as_long():
+    """Uninitialised slots of a cache, and an overflow in the output's gradient, as loss scaling makes them."""
+    n, slots, ptr = 4000, 512, on_gpu([0, 4000])
+    leaves = [normal(n, h, 64, dtype=BF16, seed=s).requires_grad_() for s, h in enumerate((8, 2, 2))]
+    q_ptr, k_ptr, k_len = on_gpu(starts([64] * 16)), on_gpu(starts([slots] * 16)), on_gpu([300] * 16)
+    prompt = [normal(16 * m, h, 64, dtype=BF16, seed=s) for s, (m, h) in enumerate(((64, 8), (slots, 2), (slots, 2)))]
+    g = normal(n, 8, 64, dtype=BF16, seed=5)
+
+    def train():
+        torch.autograd.grad(oeq.packed_attention(*leaves, ptr, causal=True), leaves, g)
+
+    def read():
+        oeq.packed_attention(*prompt, q_ptr, k_ptr, k_len=k_len, causal=True)
+
+    def spoil_gradient():
+        g[3990, 3, 7] = math.inf
+
+    def spoil_slots():
+        for t in prompt[1:]:
+            t.view(16, slots, 2, 64)[:, 300:] = math.nan
+
+    for call, spoil in ((train, spoil_gradient), (read, spoil_slots)):
+        times = []
+        for change in (None, spoil):
+            if change:
+                change()
+            call()
+            best = math.inf
+            for _ in range(3):
+                a, b = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+                a.record()
+                call()
+                call()
+                b.record()
+                b.synchronize()
+                best = min(best, a.elapsed_time(b))
+            times.append(best)
+        assert times[1] <= 10 * times[0] + 0.1, times
