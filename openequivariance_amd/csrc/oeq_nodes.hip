@@ -54,6 +54,51 @@ int check_attention(const char* who, const oeq_attention* a) {
     return OEQ_OK;
 }
 
+// Tiles of rows by falling length of their walks: the longest first, so that a launch does not end with a few compute
+// units at work on them. Lengths are those between the first and the last row's bounds; tiles of about the same length come in
+// any order, on which no result depends. One block for query tiles, one for key tiles; order[tiles ..] is scratch.
+__global__ __launch_bounds__(1024) void order_tiles(packed_attention::Args a, int* q_order, int q_tiles, int* k_order, int k_tiles) {
+    __shared__ int count[256], longest;
+    const bool keys = blockIdx.x == 1;
+    int* order = keys ? k_order : q_order;
+    const int tiles = keys ? k_tiles : q_tiles, rows = keys ? a.nk : a.nq, each = keys ? packed_attention::kKeyTile : packed_attention::kQueryTile;
+    const int lane = threadIdx.x & 63;
+    if (threadIdx.x < 256) count[threadIdx.x] = 0;
+    if (threadIdx.x == 0) longest = 1;
+    __syncthreads();
+    for (int base = 0; base < tiles; base += 1024) {
+        const int t = base + threadIdx.x, first = min(t * each, rows - 1), last = min(first + each - 1, rows - 1);
+        const packed_attention::Bounds x = keys ? packed_attention::queries_of(a, first, lane) : packed_attention::keys_of(a, first, lane);
+        const packed_attention::Bounds y = keys ? packed_attention::queries_of(a, last, lane) : packed_attention::keys_of(a, last, lane);
+        const int n = x.lo < x.hi && y.lo < y.hi ? y.hi - x.lo : max(x.hi - x.lo, y.hi - y.lo);
+        if (t < tiles) {
+            order[tiles + t] = max(n, 0);
+            atomicMax(&longest, n);
+        }
+    }
+    __syncthreads();
+    const float by = 255.0f / longest;
+    for (int t = threadIdx.x; t < tiles; t += 1024) atomicAdd(&count[255 - min(255, (int)(order[tiles + t] * by))], 1);
+    __syncthreads();
+    if (threadIdx.x < 64) {  // where each class begins
+        int c[4], sum = 0;
+#pragma unroll
+        for (int n = 0; n < 4; ++n) c[n] = count[4 * lane + n], sum += c[n];
+        int before = sum;
+#pragma unroll
+        for (int n = 1; n < 64; n <<= 1) {
+            const int x = __shfl_up(before, n);
+            if (lane >= n) before += x;
+        }
+        before -= sum;
+#pragma unroll
+        for (int n = 0; n < 4; ++n) count[4 * lane + n] = before, before += c[n];
+    }
+    __syncthreads();
+    for (int t = threadIdx.x; t < tiles; t += 1024)
+        order[atomicAdd(&count[255 - min(255, (int)(order[tiles + t] * by))], 1)] = t;
+}
+
 int64_t query_tiles(const oeq_attention& a) { return (a.q_rows + packed_attention::kQueryTile - 1) / packed_attention::kQueryTile; }
 int64_t key_tiles(const oeq_attention& a) { return (a.k_rows + packed_attention::kKeyTile - 1) / packed_attention::kKeyTile; }
 
@@ -251,7 +296,7 @@ int oeq_attention_forward(const oeq_attention* a, void* out, void* out_rest, flo
     const auto s = (hipStream_t)stream;
     if (g.parts == 0 && ordered(*a)) {
         g.q_order = (int*)workspace;
-        packed_attention::order_tiles<<<1, 1024, 0, s>>>(g, (int*)workspace, g.tiles, nullptr, 0);
+        order_tiles<<<1, 1024, 0, s>>>(g, (int*)workspace, g.tiles, nullptr, 0);
         HIP_TRY(hipGetLastError());
     }
     HIP_TRY(a->type == OEQ_FLOAT32 ? packed_attention::Launch<float>::forward(g, s)
@@ -294,7 +339,7 @@ int oeq_attention_backward(const oeq_attention* a, const void* out, const void* 
         int* q_order = (int*)(g.lifts + (a->type == OEQ_FLOAT16 ? (int64_t)a->q_heads * g.tiles : 0));
         int* k_order = q_order + 2 * (int64_t)g.tiles;
         g.q_order = q_order, g.k_order = k_order;
-        packed_attention::order_tiles<<<2, 1024, 0, s>>>(g, q_order, g.tiles, k_order, ktiles);
+        order_tiles<<<2, 1024, 0, s>>>(g, q_order, g.tiles, k_order, ktiles);
         HIP_TRY(hipGetLastError());
     }
     HIP_TRY(a->type == OEQ_FLOAT32 ? packed_attention::Launch<float>::backward(g, ktiles, s)

@@ -454,52 +454,6 @@ __device__ __forceinline__ void place(const Args& a, int heads, const int* order
     head = heads % 8 == 0 ? (at % 8) * (heads / 8) + at / 8 : at;
 }
 
-// Tiles of rows by falling length of their walks: the longest first, so that a launch does not end with a few compute
-// units at work on them. Lengths are
-// those between the first and the last row's bounds; tiles of about the same length come in any order, on which no
-// result depends. One block for query tiles, one for key tiles; order[tiles ..] is scratch.
-[[maybe_unused]] static __global__ __launch_bounds__(1024) void order_tiles(Args a, int* q_order, int q_tiles, int* k_order, int k_tiles) {
-    __shared__ int count[256], longest;
-    const bool keys = blockIdx.x == 1;
-    int* order = keys ? k_order : q_order;
-    const int tiles = keys ? k_tiles : q_tiles, rows = keys ? a.nk : a.nq, each = keys ? 64 : 128;
-    const int lane = threadIdx.x & 63;
-    if (threadIdx.x < 256) count[threadIdx.x] = 0;
-    if (threadIdx.x == 0) longest = 1;
-    __syncthreads();
-    for (int base = 0; base < tiles; base += 1024) {
-        const int t = base + threadIdx.x, first = min(t * each, rows - 1), last = min(first + each - 1, rows - 1);
-        const Bounds x = keys ? queries_of(a, first, lane) : keys_of(a, first, lane);
-        const Bounds y = keys ? queries_of(a, last, lane) : keys_of(a, last, lane);
-        const int n = x.lo < x.hi && y.lo < y.hi ? y.hi - x.lo : max(x.hi - x.lo, y.hi - y.lo);
-        if (t < tiles) {
-            order[tiles + t] = max(n, 0);
-            atomicMax(&longest, n);
-        }
-    }
-    __syncthreads();
-    const float by = 255.0f / longest;
-    for (int t = threadIdx.x; t < tiles; t += 1024) atomicAdd(&count[255 - min(255, (int)(order[tiles + t] * by))], 1);
-    __syncthreads();
-    if (threadIdx.x < 64) {  // where each class begins
-        int c[4], sum = 0;
-#pragma unroll
-        for (int n = 0; n < 4; ++n) c[n] = count[4 * lane + n], sum += c[n];
-        int before = sum;
-#pragma unroll
-        for (int n = 1; n < 64; n <<= 1) {
-            const int x = __shfl_up(before, n);
-            if (lane >= n) before += x;
-        }
-        before -= sum;
-#pragma unroll
-        for (int n = 0; n < 4; ++n) count[4 * lane + n] = before, before += c[n];
-    }
-    __syncthreads();
-    for (int t = threadIdx.x; t < tiles; t += 1024)
-        order[atomicAdd(&count[255 - min(255, (int)(order[tiles + t] * by))], 1)] = t;
-}
-
 // Blocks of four waves on a compute unit: 256 registers a lane for two, 512 where a head of 128 four-byte elements needs
 // more for its row alone.
 template <typename T, int DP>

@@ -46,12 +46,15 @@ struct Kernels {
             // of 128 159 / 161; 504 217 / 278. All of them run at once, so they need no order (which is of tiles of 64 keys).
             b.tiles = (a.nk + 31) / 32, b.k_order = nullptr;
             key_gradient<T, DP, 3, 1, kAlone ? 1 : key_blocks_per_unit<T, DP, 3>()><<<(unsigned)(b.tiles * a.hk), 256, 0, stream>>>(b);
-        } else if (kAlone && a.causal && blocks <= 512) {
-            // Two blocks share a compute unit, or one has it alone and all registers, where the longest of few uneven walks
-            // decides. bf16, 16 heads of 96, gradients, shared / alone: causal, 284 blocks 485 / 431 us, 376 169 / 155, 500 556 / 492, 628
-            // 1 372 / 1 431, 2 000 170 / 215; not causal, 500 blocks 1 524 / 1 687.
-            key_gradient<T, DP, 3, 2, 1><<<blocks, 256, 0, stream>>>(b);
         } else {
+            if constexpr (kAlone)
+                if (a.causal && blocks <= 512) {
+                    // Two blocks share a compute unit, or one has it alone and all registers, where the longest of few
+                    // uneven walks decides. bf16, 16 heads of 96, gradients, shared / alone: causal, 284 blocks 485 / 431 us,
+                    // 376 169 / 155, 500 556 / 492, 628 1 372 / 1 431, 2 000 170 / 215; not causal, 500 blocks 1 524 / 1 687.
+                    key_gradient<T, DP, 3, 2, 1><<<blocks, 256, 0, stream>>>(b);
+                    return hipGetLastError();
+                }
             key_gradient<T, DP, 3, 2><<<blocks, 256, 0, stream>>>(b);
         }
         return hipGetLastError();
