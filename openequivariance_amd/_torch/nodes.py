@@ -98,8 +98,8 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_ptr: t
     :return: ``[rows, q_heads, head_dim]``. Rows that see no key are 0. What a row does not see has no influence on it
         and gets no gradient from it, infinities and NaN included. Runs and their gradients are reproducible bit by bit.
     """
-    if scale is None:
-        scale = q.shape[-1] ** -0.5
+    if scale is None:  # (heads without elements: the op says so)
+        scale = q.shape[-1] ** -0.5 if q.dim() and q.shape[-1] else 1.0
     out, log2_sum, _rest = _packed_attention(q, k, v, q_ptr, q_ptr if k_ptr is None else k_ptr, k_len, causal, scale)
     if return_lse:
         return out, (log2_sum[:, :q.shape[0]] * math.log(2.0)).t()

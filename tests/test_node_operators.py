@@ -323,3 +323,25 @@ def test_a_table_that_wants_a_gradient_is_refused():
     assert oeq.qk_norm_rotary(q, k, at, table.detach())[0].requires_grad
     with torch.no_grad():
         oeq.qk_norm_rotary(q, k, at, table)
+
+
+def test_attention_without_elements_is_the_ops_to_refuse():
+    ptr = _Elsewhere(2, dtype=torch.int64)
+    for shape in ((5, 2, 0), ()):
+        q = _Elsewhere(*shape)
+        calls = []
+
+        def op(*args):
+            calls.append(args)
+            return (None, None, None)
+
+        from openequivariance_amd._torch import nodes
+        real, nodes._packed_attention = nodes._packed_attention, op
+        try:
+            oeq.packed_attention(q, q, q, ptr)
+        finally:
+            nodes._packed_attention = real
+        assert calls[0][-1] == 1.0
+    with pytest.raises(RuntimeError, match="multiple of 8"):
+        q = _Elsewhere(5, 2, 0)
+        torch.ops.oeq_amd.packed_attention.default.redispatch(_cuda(), q, q, q, ptr, ptr, None, False, 1.0)
