@@ -920,3 +920,21 @@ def test_results_that_are_not_finite_take_a_few_times_as_long():
                 best = min(best, a.elapsed_time(b))
             times.append(best)
         assert times[1] <= 10 * times[0] + 0.1, times
+
+
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("lens,d", [([5, 1, 9, 31, 32, 33], 32), ([700, 61], 32), ([70, 1, 97], 128), ([1500], 96), ([300] * 12, 64)])
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+def test_errors_of_attention_as_a_whole(dtype, lens, d, causal):
+    """The bounds of single elements allow for the worst of every rounding; as a whole they are far apart. float32: a weight
+    is off by 2^-24 of what stands in the exponent (here up to some 8) and of the exponential itself, sums of up to
+    1 500 terms by less: 2^-19 of the norm. Operands of 11 or 8 bits would show at once (2^-12 and more)."""
+    ptr = starts(lens)
+    leaves = [normal(ptr[-1], 3, d, dtype=dtype, seed=s).requires_grad_() for s in range(3)]
+    g = normal(ptr[-1], 3, d, dtype=dtype, seed=3)
+    out = oeq.packed_attention(*leaves, on_gpu(ptr), causal=causal)
+    got = dict(zip(("out", "dq", "dk", "dv"), (out.detach(),) + torch.autograd.grad(out, leaves, g)))
+    parts = [gradients_64(*(t[a:b] for t in leaves), g[a:b], causal) for a, b in zip(ptr, ptr[1:])]
+    for name, x in got.items():
+        value, terms = (torch.cat([p[name][i] for p in parts]) for i in (0, 1))
+        check_norm(x, value, terms, dtype, name, more=2.0 ** -19)
