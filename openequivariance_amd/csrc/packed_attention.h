@@ -8,8 +8,8 @@
 // dq_i = c sum_j ds_ij k_j,  dk_j = c sum_i ds_ij q_i, the last two sums over the query heads that share a key head too.
 // Scores, p, ds and all sums are held in 32 bits; where operands have 16, p and ds are rounded to their type as
 // operands of the second products (the products themselves are exact in 32 bits), which costs an error of the size of
-// the output's own rounding and halves the work of these products, which bound the tiles of rows (the form for few queries,
-// bound by memory, does without it). delta would add a third such error where rows see few keys, were it taken from the rounded
+// the output's own rounding and halves the work of these products, which bound the tiles of rows (p in the form for few queries,
+// bound by memory, and in walks of few keys has two parts instead). delta would add a third such error where rows see few keys, were it taken from the rounded
 // output: a pass that will be differentiated keeps what the rounding took off beside it (`rest`, 16 bits).
 //
 // Layout of the products. All of them run on the 32x32 matrix instructions with the *transposed* result in registers:
@@ -270,6 +270,15 @@ __device__ __forceinline__ typename Types<T>::frag operand(const float16_t& s, i
         for (int j = 0; j < 4; ++j) x[j] = s[4 * f + j];
     }
     return x;
+}
+
+// What the rounding of an operand of 16 bits took off.
+template <typename T>
+__device__ __forceinline__ typename Types<T>::frag rest_of(const float16_t& s, typename Types<T>::frag x, int f) {
+    float8_t w;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) w[j] = s[8 * f + j] - (float)x[j];
+    return __builtin_convertvector(w, typename Types<T>::frag);
 }
 
 // ds of eleven bits as operands. Every lane carries it at a power of two of its own: 2^kDs until it has seen one, less
@@ -663,6 +672,15 @@ __device__ __forceinline__ void add_others(const char* lds, int first, int t, in
 // pairs (a large library product 1.16, both at some 2 GHz); 9 of 200 to 4 001 rows, 16 / 4 heads, 152 us, the longest walk.
 // Short ones by a block's chain of waits: 512 molecules, 8 heads of 32, float32, 35 us, of which the matrix units work 13;
 // 33 crystals, 6 / 2 heads of 72, fp16, 20 us.
+//
+// Where a row sees few keys, each weight is a large part of its sum, and so is what its rounding to 16 bits takes off; delta has
+// that error too and with it the gradients, whose errors it would raise from 1.41 times those of one rounding (ds has one, the
+// result another) to above 1.5. A block that walks no more than kFewKeys keys has p in two parts as the form for few queries has. Forward,
+// us, one part / two, bf16: 512 segments of 9 to 61 rows, heads of 32 16.6 / 18.2, 256 of 120, heads of 128 127 / 136, of 32 51 / 60; a
+// training step on the 33 crystals 78.0 / 78.3. For walks of up to 2 048 keys it would cost 9 sequences, heads of 128, 660 / 678,
+// and take the gradients' errors from 1.44 to 1.41.
+constexpr int kFewKeys = 256;
+
 template <typename T, int DP, int SPLIT>
 __global__ __launch_bounds__(256, (kSparse<T, DP> && SPLIT == 1 ? 4 : blocks_per_unit<T, DP>())) void forward(Args a) {
     constexpr int BK = SPLIT == 2 ? 64 : tile_rows<T, DP>(), SUB = SPLIT == 2 || kSparse<T, DP> ? 1 : BK / 32, DT = DP / 32;
@@ -694,11 +712,12 @@ __global__ __launch_bounds__(256, (kSparse<T, DP> && SPLIT == 1 ? 4 : blocks_per
     float m, l;
     unsigned known;
     const float c = a.scale_log2;
+    const bool in_parts = sizeof(T) == 2 && all.hi - all.lo <= kFewKeys;
     settle();
 
     // Sums are scaled to another maximum only where it grew by more than 2^grow: up to 2^8 p fits every type.
-    auto pass = [&](auto& acc, auto care, int t0, float grow) {
-        constexpr bool CARE = decltype(care)::value;
+    auto pass = [&](auto& acc, auto care, auto two, int t0, float grow) {
+        constexpr bool CARE = decltype(care)::value, TWO = decltype(two)::value;
         constexpr int NT = CARE ? 1 : DT;
 #pragma unroll
         for (int t = 0; t < NT; ++t) acc[t] = 0.0f;
@@ -749,14 +768,23 @@ __global__ __launch_bounds__(256, (kSparse<T, DP> && SPLIT == 1 ? 4 : blocks_per
                     l += s[u][r];
                 }
                 if constexpr (CARE) {
-                    if (finite_product_of<T, DP, BK>(vt, r0 + 32 * u, t0, w.at, s[u], s[u], acc[0], known))
+                    float16_t rest = 0.0f;
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) rest[r] = in_parts ? s[u][r] - (float)(T)s[u][r] : 0.0f;
+                    if (finite_product_of<T, DP, BK, sizeof(T) == 2>(vt, r0 + 32 * u, t0, w.at, s[u], rest, acc[0], known))
                         add_others<T, DP, BK, true>(vt, r0 + 32 * u, t0, w.at, first + r0 + 32 * u, b, acc[0], known);
                 } else {
 #pragma unroll
                     for (int f = 0; f < PF; ++f) {
                         const auto p = operand<T>(s[u], f);
+                        auto rest = p;
+                        if constexpr (TWO) rest = rest_of<T>(s[u], p, f);
 #pragma unroll
-                        for (int t = 0; t < DT; ++t) acc[t] = mma(column_of<T, DP, BK>(vt, r0 + 32 * u, f, t, lane), p, acc[t]);
+                        for (int t = 0; t < DT; ++t) {
+                            const auto column = column_of<T, DP, BK>(vt, r0 + 32 * u, f, t, lane);
+                            acc[t] = mma(column, p, acc[t]);
+                            if constexpr (TWO) acc[t] = mma(column, rest, acc[t]);
+                        }
                     }
                 }
             }
@@ -820,7 +848,10 @@ __global__ __launch_bounds__(256, (kSparse<T, DP> && SPLIT == 1 ? 4 : blocks_per
     bool bad = row < a.nq && !part;
     {
         float16_t acc[DT];
-        pass(acc, std::false_type(), 0, 8.0f);
+        if (in_parts)
+            pass(acc, std::false_type(), std::integral_constant<bool, sizeof(T) == 2>(), 0, 8.0f);
+        else
+            pass(acc, std::false_type(), std::false_type(), 0, 8.0f);
         const float by = seen ? 1.0f / l : 0.0f;
         if (bad) {
             const int64_t at = ((int64_t)i * a.hq + h) * a.d;
@@ -831,7 +862,7 @@ __global__ __launch_bounds__(256, (kSparse<T, DP> && SPLIT == 1 ? 4 : blocks_per
     }
     careful_passes<T, DT>(shared.bad, bad, [&](int t, int raise, bool mine) {
         float16_t acc[1];
-        pass(acc, std::true_type(), t, 8.0f * raise);
+        pass(acc, std::true_type(), std::false_type(), t, 8.0f * raise);
         const float by = seen ? 1.0f / l : 0.0f;
         if (mine) {
             const int r = anew(i);
@@ -983,12 +1014,7 @@ __global__ __launch_bounds__((64 * Few<T, DP>::kWaves), 1) void forward_few(Args
                 for (int f = 0; f < PF; ++f) {
                     const auto p = operand<T>(s, f);
                     auto rest = p;
-                    if constexpr (sizeof(T) == 2) {
-                        float8_t w;
-#pragma unroll
-                        for (int j = 0; j < 8; ++j) w[j] = s[8 * f + j] - (float)p[j];
-                        rest = __builtin_convertvector(w, typename L::frag);
-                    }
+                    if constexpr (sizeof(T) == 2) rest = rest_of<T>(s, p, f);
 #pragma unroll
                     for (int t = 0; t < DT; ++t) {
                         const auto column = column_of<T, DP, 32>(vt, 0, f, t, lane);
