@@ -585,6 +585,10 @@ __device__ __forceinline__ bool any_of_block(bool bad, int& shared) {
 // results where bad and says whether some of them are not finite for no known reason.
 template <typename T, int DT, typename F>
 __device__ __forceinline__ void careful_passes(int (&shared)[2], bool bad, F walk) {
+    if (__builtin_expect(!any_of_block(bad, shared[0]), 1)) {
+        asm volatile("s_endpgm");  // (the program's own end is a jump away, in instructions that would have to be fetched first:
+        return;                    // 6 single rows, 32 / 8 heads of 96, 13.6 us and not 12.9)
+    }
 #pragma unroll 1
     for (int n = kCareful; n <= kLastPass<T> && any_of_block(bad, shared[n - 1]); ++n) {
         bool still = false;
@@ -599,12 +603,12 @@ __device__ __forceinline__ void careful_passes(int (&shared)[2], bool bad, F wal
     }
 }
 
-// acc += columns 32 t ... of the rows at `first`, transposed, times the weights of a result with these rows (and their `rest`),
+// acc += columns 32 t ... of the rows at `first`, transposed, times the weights of a result with these rows (in `two` parts or one),
 // by the rows' finite elements alone. Returns whether there were others. `known`: a bit for each register whose result is not
 // finite for what the operands hold, not for the size of its sum.
-template <typename T, int DP, int ROWS, bool REST = false>
-__device__ __forceinline__ bool finite_product_of(const char* lds, int first, int t, int lane, const float16_t& weights,
-                                                  const float16_t& rest, float16_t& acc, unsigned& known) {
+template <typename T, int DP, int ROWS>
+__device__ __forceinline__ bool finite_product_of(const char* lds, int first, int t, int lane, const float16_t& weights, bool two,
+                                                  float16_t& acc, unsigned& known) {
     unsigned left = 0;
 #pragma unroll
     for (int r = 0; r < 16; ++r) left = max(left, magnitude(weights[r]));
@@ -620,8 +624,10 @@ __device__ __forceinline__ bool finite_product_of(const char* lds, int first, in
             left = max(left, size);
             x[j] = size < 0x7f800000u ? x[j] : (T)0.0f;
         }
-        acc = mma(x, operand<T>(weights, f), acc);
-        if (REST) acc = mma(x, operand<T>(rest, f), acc);
+        const auto w = operand<T>(weights, f);
+        acc = mma(x, w, acc);
+        if constexpr (sizeof(T) == 2)
+            if (two) acc = mma(x, rest_of<T>(weights, w, f), acc);
         __builtin_amdgcn_sched_barrier(0);
     }
     return kSparse<T, DP> || __any(left >= 0x7f800000u);  // (small heads: a branch around what follows would take registers)
@@ -676,13 +682,13 @@ __device__ __forceinline__ void add_others(const char* lds, int first, int t, in
 // Where a row sees few keys, each weight is a large part of its sum, and so is what its rounding to 16 bits takes off; delta has
 // that error too and with it the gradients, whose errors it would raise from 1.41 times those of one rounding (ds has one, the
 // result another) to above 1.5. A block that walks no more than kFewKeys keys has p in two parts as the form for few queries has. Forward,
-// us, one part / two, bf16: 512 segments of 9 to 61 rows, heads of 32 16.6 / 18.2, 256 of 120, heads of 128 127 / 136, of 32 51 / 60; a
-// training step on the 33 crystals 78.0 / 78.3. For walks of up to 2 048 keys it would cost 9 sequences, heads of 128, 660 / 678,
+// us, one part / two, bf16: 512 segments of 9 to 61 rows, heads of 32 14.8 / 16.7, 256 of 120, heads of 128 125 / 135, of 32 45 / 54; a
+// training step on the 33 crystals 79.3 either way. For walks of up to 2 048 keys it would cost 9 sequences, heads of 128, 649 / 665,
 // and take the gradients' errors from 1.44 to 1.41.
 constexpr int kFewKeys = 256;
 
-template <typename T, int DP, int SPLIT>
-__global__ __launch_bounds__(256, (kSparse<T, DP> && SPLIT == 1 ? 4 : blocks_per_unit<T, DP>())) void forward(Args a) {
+template <typename T, int DP, int SPLIT>  // (heads of 32: without the bound bf16 takes 139 registers, three waves to a SIMD)
+__global__ __launch_bounds__(256, (DP == 32 && SPLIT == 1 ? 4 : blocks_per_unit<T, DP>())) void forward(Args a) {
     constexpr int BK = SPLIT == 2 ? 64 : tile_rows<T, DP>(), SUB = SPLIT == 2 || kSparse<T, DP> ? 1 : BK / 32, DT = DP / 32;
     constexpr int PF = sizeof(T) == 2 ? 2 : 4;  // fragments of 32 keys
     typedef Tile<T, DP, BK> L;
@@ -768,22 +774,22 @@ __global__ __launch_bounds__(256, (kSparse<T, DP> && SPLIT == 1 ? 4 : blocks_per
                     l += s[u][r];
                 }
                 if constexpr (CARE) {
-                    float16_t rest = 0.0f;
-#pragma unroll
-                    for (int r = 0; r < 16; ++r) rest[r] = in_parts ? s[u][r] - (float)(T)s[u][r] : 0.0f;
-                    if (finite_product_of<T, DP, BK, sizeof(T) == 2>(vt, r0 + 32 * u, t0, w.at, s[u], rest, acc[0], known))
+                    if (finite_product_of<T, DP, BK>(vt, r0 + 32 * u, t0, w.at, s[u], in_parts, acc[0], known))
                         add_others<T, DP, BK, true>(vt, r0 + 32 * u, t0, w.at, first + r0 + 32 * u, b, acc[0], known);
                 } else {
 #pragma unroll
                     for (int f = 0; f < PF; ++f) {
                         const auto p = operand<T>(s[u], f);
-                        auto rest = p;
-                        if constexpr (TWO) rest = rest_of<T>(s[u], p, f);
+                        typename L::frag column[TWO ? DT : 1];
 #pragma unroll
                         for (int t = 0; t < DT; ++t) {
-                            const auto column = column_of<T, DP, BK>(vt, r0 + 32 * u, f, t, lane);
-                            acc[t] = mma(column, p, acc[t]);
-                            if constexpr (TWO) acc[t] = mma(column, rest, acc[t]);
+                            column[TWO ? t : 0] = column_of<T, DP, BK>(vt, r0 + 32 * u, f, t, lane);
+                            acc[t] = mma(column[TWO ? t : 0], p, acc[t]);
+                        }
+                        if constexpr (TWO) {
+                            const auto rest = rest_of<T>(s[u], p, f);
+#pragma unroll
+                            for (int t = 0; t < DT; ++t) acc[t] = mma(column[t], rest, acc[t]);
                         }
                     }
                 }
@@ -916,7 +922,7 @@ struct Share {
 };
 
 template <typename T, int DP>
-__global__ __launch_bounds__((64 * Few<T, DP>::kWaves), 1) void forward_few(Args a) {
+__global__ __launch_bounds__((64 * Few<T, DP>::kWaves), (sizeof(T) * DP == 64 ? 4 : 1)) void forward_few(Args a) {
     constexpr int W = Few<T, DP>::kWaves, DT = DP / 32, PF = sizeof(T) == 2 ? 2 : 4, ROW = Few<T, DP>::kRow;
     typedef typename Few<T, DP>::L L;
     __shared__ __align__(1024) char key0[W * L::kBytes], key1[W * L::kBytes], val0[W * L::kBytes], val1[W * L::kBytes];
@@ -1013,20 +1019,20 @@ __global__ __launch_bounds__((64 * Few<T, DP>::kWaves), 1) void forward_few(Args
 #pragma unroll
                 for (int f = 0; f < PF; ++f) {
                     const auto p = operand<T>(s, f);
-                    auto rest = p;
-                    if constexpr (sizeof(T) == 2) rest = rest_of<T>(s, p, f);
+                    typename L::frag column[DT];
 #pragma unroll
                     for (int t = 0; t < DT; ++t) {
-                        const auto column = column_of<T, DP, 32>(vt, 0, f, t, lane);
-                        acc[t] = mma(column, p, acc[t]);
-                        if constexpr (sizeof(T) == 2) acc[t] = mma(column, rest, acc[t]);
+                        column[t] = column_of<T, DP, 32>(vt, 0, f, t, lane);
+                        acc[t] = mma(column[t], p, acc[t]);
+                    }
+                    if constexpr (sizeof(T) == 2) {
+                        const auto rest = rest_of<T>(s, p, f);
+#pragma unroll
+                        for (int t = 0; t < DT; ++t) acc[t] = mma(column[t], rest, acc[t]);
                     }
                 }
             } else {
-                float16_t rest = 0.0f;
-#pragma unroll
-                for (int r = 0; r < 16; ++r) rest[r] = s[r] - (float)(T)s[r];
-                if (finite_product_of<T, DP, 32, sizeof(T) == 2>(vt, 0, t0, w.at, s, rest, acc[0], known))
+                if (finite_product_of<T, DP, 32>(vt, 0, t0, w.at, s, true, acc[0], known))
                     add_others<T, DP, 32, true>(vt, 0, t0, w.at, first, Bounds{mine.first, mine.last}, acc[0], known);
             }
         };
@@ -1291,7 +1297,7 @@ __global__ __launch_bounds__(256, (blocks_per_unit<T, DP>())) void query_gradien
                         for (int t = 0; t < NT; ++t) acc[t] *= by;
                     });
                 if constexpr (CARE) {
-                    if (finite_product_of<T, DP, BK>(kt, 32 * u, t0, l.at, x, x, acc[0], known))
+                    if (finite_product_of<T, DP, BK>(kt, 32 * u, t0, l.at, x, false, acc[0], known))
                         add_others<T, DP, BK, false>(kt, 32 * u, t0, l.at, first + 32 * u, b, acc[0], known);
                 } else {
 #pragma unroll
@@ -1529,8 +1535,8 @@ __global__ __launch_bounds__(256, UNIT) void key_gradient(Args a) {
                 hide(s, x, now);
                 if constexpr (CARE) {
                     __builtin_amdgcn_sched_barrier(0);
-                    bool others = DV && finite_product_of<T, DP, BQ>(gt, r0, t0, l.at, s, s, dv[0], known);
-                    if (DK && finite_product_of<T, DP, BQ>(qt, r0, t0, l.at, x, x, dk[0], known)) others = true;
+                    bool others = DV && finite_product_of<T, DP, BQ>(gt, r0, t0, l.at, s, false, dv[0], known);
+                    if (DK && finite_product_of<T, DP, BQ>(qt, r0, t0, l.at, x, false, dk[0], known)) others = true;
                     if (DV && others) add_others<T, DP, BQ, true>(gt, r0, t0, l.at, now + r0, b, dv[0], known);
                     if (DK && others) add_others<T, DP, BQ, false, 16>(qt, r0, t0, l.at, now + r0, b, dk[0], known);
                 } else {
