@@ -200,6 +200,17 @@ def test_no_kernel_of_the_library_has_scratch_memory():
     assert not {n: r for n, r in attention.items() if r[1] > 0}
 
 
+def test_norm_rotation_dropout_and_ordering_have_no_scratch_memory():
+    blob, at, names = rt.lib_path().read_bytes(), 0, {}
+    while (at := blob.find(b"\x7fELF", at + 1)) >= 0:
+        if int.from_bytes(blob[at + 18:at + 20], "little") == 224:  # EM_AMDGPU
+            names.update(rt.kernel_resources(blob[at:]))
+    for part, least in (("qk_rotary", 9), ("irrep_dropout", 4), ("order_tiles", 1)):
+        found = {n: r for n, r in names.items() if part in n}
+        assert len(found) >= least, (part, len(found))
+        assert not {n: r for n, r in found.items() if r[1] > 0}
+
+
 def test_forward_mode_derivatives_are_right_or_refused():
     """A dual tensor need not require a gradient; its tangent must not get lost on the way."""
     import torch.autograd.forward_ad as forward_ad
