@@ -128,10 +128,12 @@ packed_attention::Args attention_args(const oeq_attention& a) {
 // steps of about a microsecond. Tiles: blocks of 128 rows walk the keys of all segments that their rows belong to, 64 a
 // step. Few: blocks of a row and a key head walk that row's keys alone, 80 a step after some 5 steps of latency (a block's
 // bounds, first reads and end). Either way two blocks a compute unit run at a time. Measured with 8 heads of 64, bf16,
-// tiles / few in us: 128 segments of 1 row, 512 keys 1 023 / 26, of 2 rows, 16 keys 22 / 21, of 4 rows, 64 keys 39 / 39, of 8 rows,
-// 64 keys 22 / 74, 512 keys 132 / 122; 1 024 segments of 1 row, 32 keys 72 / 73; a segment of 16 rows, 4 096 keys 57 / 22.
+// tiles / few in us: 128 segments of 1 row, 512 keys 336 / 26, of 2 rows, 16 keys 11 / 20, of 4 rows, 64 keys 17 / 39, of 8 rows,
+// 64 keys 11 / 74, 512 keys 47 / 124; 1 024 segments of 1 row, 32 keys 29 / 74; a segment of 16 rows, 4 096 keys 39 / 23.
+// (Means tell nothing of a prompt beside single tokens, or of one long cache among short ones: results are right there, but
+// tiles then walk the single tokens' caches, and the long one has as few shares as the others.)
 int parts_of(const oeq_attention& a) {
-    constexpr int64_t kBlocks = 1024;   // (one token against 65 537 keys: 512 and 1 024 blocks 62 us, 2 048 blocks 73)
+    constexpr int64_t kBlocks = 1024;   // (one token against 65 537 keys, again and again: 512 blocks 52 us, 1 024 51, 2 048 57)
     constexpr int64_t kLeastKeys = 256;  // a share is worth its block and its row of the join
     const int64_t segments = std::max(a.segments, 1), group = a.q_heads / a.k_heads;
     const int64_t blocks = a.q_rows * a.k_heads * ((group + 31) / 32);

@@ -30,9 +30,9 @@
 // infinity or NaN; such a product leaves NaN in the sums. So a block with a result that is not finite, for whatever reason,
 // walks its tiles a second time (Pass), with the infinities and NaN of the rows that its lanes share taken out of the products
 // and counted for each lane by products of their own. Results that were finite stay, and one that is finite now has the
-// bits that it has where hidden rows are finite. A causal sequence of 4 000 rows, 8 / 2 heads of 64, bf16: forward 43 us, with an
-// infinity among the values 152; gradients 187, with one in the output's gradient 1 050 (fp16 200 and 710). Where all is
-// finite it costs a barrier at the end: 512 molecules, float32, training step 132.6 and 134.2 us, large launches within 1 %.
+// bits that it has where hidden rows are finite. A causal sequence of 4 000 rows, 8 / 2 heads of 64, bf16: forward 45 us, with an
+// infinity among the values 159; gradients 194, with one in the output's gradient 1 040 (fp16 194 and 710). Where all is
+// finite it costs a barrier at the end: 512 molecules, float32, training step 132.7 and 133.5 us, large launches within 1 %.
 #ifndef OEQ_PACKED_ATTENTION_H
 #define OEQ_PACKED_ATTENTION_H
 
@@ -474,7 +474,7 @@ template <typename T, int DP>
 constexpr bool kSparse = sizeof(T) == 4 && DP == 32;
 
 // A lane's number, or the same hidden from the compiler, which then computes places in LDS anew instead of keeping them in
-// registers. In key_gradient: kSparse, 192 registers a lane or 138, a wave more to a SIMD: 512 molecules, float32, all
+// registers. In key_gradient: kSparse, 192 registers a lane or 138 (168 with the passes after the first), a wave more to a SIMD: 512 molecules, float32, all
 // gradients 139 / 132 us, 2 048 460 / 424, but a segment of 3 000 rows 260 / 266. (bf16 heads of 32, whose products are 8 times as
 // fast: 2 048 molecules 185 / 177, a segment of 3 000 rows 64 / 73, so they keep them.)
 template <typename X>
@@ -677,8 +677,8 @@ __device__ __forceinline__ void add_others(const char* lds, int first, int t, in
 // A wave has 32 query rows in registers (128 a block, 64 with SPLIT) and walks keys and values through two LDS buffers, the
 // next tile always on its way, with running maximum and sum in the row's lane. Long walks are bound by the matrix units and
 // the power they may draw: 7 segments of 500 to 8 192 rows, 32 / 8 heads of 128, bf16, causal, 1.71 ms, 1.03 PFLOP/s of visible
-// pairs (a large library product 1.16, both at some 2 GHz); 9 of 200 to 4 001 rows, 16 / 4 heads, 152 us, the longest walk.
-// Short ones by a block's chain of waits: 512 molecules, 8 heads of 32, float32, 35 us, of which the matrix units work 13;
+// pairs (a large library product 1.16, both at some 2 GHz); 9 of 200 to 4 001 rows, 16 / 4 heads, 140 us, the longest walk.
+// Short ones by a block's chain of waits: 512 molecules, 8 heads of 32, float32, 33 us, of which the matrix units work 13;
 // 33 crystals, 6 / 2 heads of 72, fp16, 20 us.
 //
 // Where a row sees few keys, each weight is a large part of its sum, and so is what its rounding to 16 bits takes off; delta has
@@ -894,7 +894,7 @@ __global__ __launch_bounds__(256, (DP == 32 && SPLIT == 1 ? 4 : blocks_per_unit<
 // of more than one block's row meet in `join`, in the order of the keys. p of 16 bits goes in two parts, itself and what its
 // rounding took off, so that nothing but the output is rounded: the second products are done while memory is waited for.
 // Bound by memory: a token against 65 537 keys, 32 / 8
-// heads of 128, bf16, 59 us with the join (6), 4.5 TB/s of 268 MB where a copy reaches 4.7; 64 tokens against 1 to 4 096 keys
+// heads of 128, bf16, 60 us with the join (6), 4.5 TB/s of 268 MB where a copy reaches 4.7; 64 tokens against 1 to 4 096 keys
 // each, 16 / 4 heads, fp16, 70 us for the same bytes; 7 tokens against up to 60 keys 7 us, about a launch.
 
 template <typename T, int DP>
@@ -1197,7 +1197,7 @@ __global__ __launch_bounds__(256) void join(Args a) {
 // ---------------------------------------------------------------------------
 //
 // As the forward pass, with the output's gradient beside the query and three products for each pair, and bound by the same: in the
-// cases there 204 us (9 sequences, 0.8 PFLOP/s of visible pairs), 52 (molecules) and 24 (crystals). Scores are computed again here
+// cases there 187 us (9 sequences, 0.87 PFLOP/s of visible pairs), 50 (molecules) and 25 (crystals). Scores are computed again here
 // and for the keys' gradient, 14 units of products in all with the forward's 4, where one kernel for both would do 10 + 4 but
 // add to dq from many blocks: by atomics, in no fixed order, or through memory.
 template <typename T, int DP, int SPLIT>
@@ -1382,8 +1382,8 @@ __global__ __launch_bounds__(256, (blocks_per_unit<T, DP>())) void query_gradien
 // sums and 64 elements of its key and value, so there is one wave to a SIMD and nothing else runs while it waits: reads from
 // LDS go ahead of their products in batches, with a fence behind each. (Left to itself the compiler puts every read right
 // before its product, and the wave waited for 45 % of its clocks.) WHAT: 1 the keys' gradient, 2 the values', 3 both.
-// In the cases of the forward kernel 383 us (9 sequences, 0.57 PFLOP/s: the longest walk, matrix units at work for 45 % of the clocks of busy
-// compute units, which is what a large library product reaches), 54 (molecules), 37 (crystals).
+// In the cases of the forward kernel 334 us (9 sequences, 0.65 PFLOP/s: the longest walk, matrix units at work for 45 % of the clocks of busy
+// compute units, which is what a large library product reaches), 51 (molecules), 36 (crystals).
 template <typename T, int DP, int WHAT, int KEYS, int UNIT = key_blocks_per_unit<T, DP, WHAT>()>
 __global__ __launch_bounds__(256, UNIT) void key_gradient(Args a) {
     constexpr bool DK = WHAT & 1, DV = WHAT & 2;

@@ -9,9 +9,9 @@
 // the r turned elements. So the only thing that passes between lanes is the sum of squares. A block has one row or several
 // and its groups of lanes walk the row's heads, kHeads of them requested at a time, with the row's cosines and sines in
 // registers. The kernels are bound by memory: every head is read once and written once. 16 411 rows of 32 and 8 heads of 128,
-// bf16: forward 70 us, 3.9 TB/s, gradient 121 + 5 us, 3.4 TB/s (a copy 4.7): four waves a SIMD, all that their registers allow, do
-// not hide a row's chain of loads. (Both kinds' heads requested before either is computed: 78 and 155 us, for the registers;
-// one head at a time in the gradient 149; fewer registers by scratch memory 250 to 630.) A batch of 64 rows takes 5 us, about
+// bf16, 168 MB: forward 68 us for two times that, 4.9 TB/s, gradient 119 for three times, 4.2, and 5 for the weights' sums (a copy of
+// 4 GiB 4.7). (Both kinds' heads requested before either is computed: 78 and 155 us, for the registers; one head at a time in
+// the gradient 149; fewer registers by scratch memory 250 to 630.) A batch of 64 rows takes 5 us, about
 // a launch.
 #ifndef OEQ_QK_ROTARY_H
 #define OEQ_QK_ROTARY_H
