@@ -22,7 +22,7 @@
 #include <stdint.h>
 
 /* Changes with every change of a struct, an argument list or an enumerator below. */
-#define OEQ_ABI_VERSION 9
+#define OEQ_ABI_VERSION 10
 
 #ifdef __cplusplus
 extern "C" {
@@ -441,6 +441,65 @@ int oeq_qk_norm_rotary_backward(const oeq_qk_rotary* a, const void* q_grad, int6
  * seed[0], seed[1] (on the device), the row and the channel alone. */
 int oeq_irrep_dropout(int type, int64_t rows, int64_t dim, const void* x, const void* residual, void* out,
                       const int32_t* channels, const int64_t* seed, double p, void* stream);
+
+/* ---- operators whose parameters are chosen row by row --------------------- */
+/* A batch of rows (nodes, tokens), each of one of `types` types (species, experts, adapters): type_of_row [rows], on the
+ * device. Rows whose type is not one of 0 .. types - 1 have no parameters. Element types are those of oeq_element up to
+ * OEQ_BFLOAT16; strides are in elements. The reference has no counterpart of these.
+ *
+ * The index that most of them go by: `order` [rows], the row numbers by type, ascending within a type, rows without a type last;
+ * `ptr` [types + 1], where each type begins in it. It depends on the types alone. */
+size_t oeq_group_rows_workspace_bytes(int64_t rows, int64_t types);
+int oeq_group_rows(int64_t rows, int64_t types, const int64_t* type_of_row, int32_t* order, int32_t* ptr, void* workspace,
+                   size_t workspace_bytes, void* stream);
+
+/* out[i] = scale table[type_of_row[i]], 0 for rows without a type. table: [types, channels], rows strided; out: contiguous. */
+int oeq_type_lookup(int type, int64_t rows, int64_t types, int64_t channels, const int64_t* type_of_row, const void* table,
+                    int64_t table_row_stride, double scale, void* out, void* stream);
+
+/* out[t] = scale times the sum of x over the rows of type t and their parts, in the index's order; x: [rows, parts, channels],
+ * rows and parts strided; out: [types, channels], contiguous. */
+size_t oeq_type_sum_workspace_bytes(int64_t rows, int64_t types, int64_t channels);
+int oeq_type_sum(int type, int64_t rows, int64_t parts, int64_t types, int64_t channels, const int64_t* type_of_row,
+                 const int32_t* order, const int32_t* ptr, const void* x, int64_t row_stride, int64_t part_stride, double scale,
+                 void* out, void* workspace, size_t workspace_bytes, void* stream);
+
+/* Products of rows with the matrix of their type: out[i] = w_t x_i (+ bias_t), or w_t^T x_i (across). */
+typedef struct {
+    int32_t type;
+    int32_t across;          /* w is [types, inner, outer], else [types, outer, inner] */
+    int32_t shared;          /* one w for all rows, those without a type too; w_type_stride is not used */
+    int32_t rank;            /* of the thin product, 0: none */
+    int64_t rows, parts;     /* every row has that many parts, all of its type */
+    int64_t types, inner, outer;
+    int64_t x_row_stride, x_part_stride, w_type_stride, w_row_stride, up_type_stride, up_outer_stride, up_rank_stride;
+    const void *x, *w;       /* their last dimension is contiguous */
+    const void* bias;        /* [types, outer], contiguous, or NULL; not with shared */
+    const float* thin;       /* [rows, oeq_thin_stride(rank)], filled up with zeros: plus up_t thin_i for rows with a type, */
+    const void* up;          /* up: [types, outer, rank] of any strides. One part a row. */
+    const int32_t *order, *ptr;
+} oeq_typed_rows;
+
+/* out: [rows, parts, outer], contiguous. Rows without a type become 0 (shared: their product with w). */
+int oeq_typed_product(const oeq_typed_rows* a, void* out, void* stream);
+/* The same with results in float, scale[t] times (NULL: 1); `outer` is the rank, out: [rows, oeq_thin_stride(outer)], filled up
+ * with zeros. */
+int64_t oeq_thin_stride(int64_t rank);
+int oeq_typed_thin_product(const oeq_typed_rows* a, const float* scale, float* out, void* stream);
+
+/* out[t] = sum over the rows of type t (and their parts) of a_i^T b_i: [types, a_columns, b_columns], contiguous. */
+typedef struct {
+    int32_t type;            /* of a, b and out */
+    int32_t thin;            /* 1: a is float, 2: b is float, else 0 */
+    int64_t rows, parts;
+    int64_t types, a_columns, b_columns;
+    int64_t a_row_stride, a_part_stride, b_row_stride, b_part_stride;
+    const void *a, *b;       /* [rows, parts, columns], their last dimension is contiguous */
+    const int32_t *order, *ptr;
+} oeq_typed_sum;
+
+size_t oeq_typed_sum_workspace_bytes(const oeq_typed_sum* a);
+int oeq_typed_sum_products(const oeq_typed_sum* a, void* out, void* workspace, size_t workspace_bytes, void* stream);
 
 /* ---- per-kernel timing --------------------------------------------------- */
 /* Replaces GPUTimer (extension/backend/backend_hip.hpp:67-101). While enabled,

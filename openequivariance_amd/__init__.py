@@ -20,6 +20,7 @@ if os.environ.get("OEQ_NOTORCH") != "1":
     from ._torch.nodes import (IrrepDropout, packed_attention, qk_norm_rotary, qk_norm_rotary_append, rotary_table)
     from ._torch.tensor_product import TensorProduct
     from ._torch.tensor_product_conv import TensorProductConv
+    from ._torch.typed import RowGroups, adapter_linear, group_rows, type_embedding, typed_linear
     from ._torch.utils import torch_to_oeq_dtype, transpose_irreps
 
     from .core.problems import ChannelwiseTPP, FullyConnectedTPProblem, SingleInstruction
@@ -37,5 +38,6 @@ def torch_ext_so_path():
 
 
 __all__ = ["TPProblem", "Irrep", "Irreps", "Instruction", "TensorProduct", "TensorProductConv",
+           "RowGroups", "adapter_linear", "group_rows", "type_embedding", "typed_linear",
            "IrrepDropout", "packed_attention", "qk_norm_rotary", "qk_norm_rotary_append", "rotary_table",
            "torch_to_oeq_dtype", "transpose_irreps", "torch_ext_so_path"]

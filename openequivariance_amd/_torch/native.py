@@ -1,5 +1,6 @@
-"""Loads ``_oeq_torch-*.so``, the torch ops over the C ABI (``csrc/oeq_torch.cpp``, ``csrc/oeq_torch_nodes.cpp``), and builds it where no built file
-exists. There is no other implementation of the ops: without the library every call of one is an error."""
+"""Loads ``_oeq_torch-*.so``, the torch ops over the C ABI (``csrc/oeq_torch.cpp``, ``csrc/oeq_torch_nodes.cpp``,
+``csrc/oeq_torch_typed.cpp``), and builds it where no built file exists. There is no other implementation of the ops:
+without the library every call of one is an error."""
 
 from __future__ import annotations
 
@@ -19,7 +20,7 @@ from .. import runtime as rt
 # The file is bound to the torch it was compiled against (its C++ interface changes between releases), to this Python
 # and to the C ABI: what was built for others has another name and is not loaded.
 _SO_PATH = rt._PKG_DIR / f"_oeq_torch-{torch.__version__}-{sys.implementation.cache_tag}-abi{rt.ABI_VERSION}.so"
-_SRC_PATHS = [rt._CSRC_DIR / "oeq_torch.cpp", rt._CSRC_DIR / "oeq_torch_nodes.cpp"]
+_SRC_PATHS = [rt._CSRC_DIR / "oeq_torch.cpp", rt._CSRC_DIR / "oeq_torch_nodes.cpp", rt._CSRC_DIR / "oeq_torch_typed.cpp"]
 _lock = threading.Lock()
 _module = None
 

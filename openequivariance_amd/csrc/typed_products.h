@@ -1,0 +1,596 @@
+// Device code of matrix products whose weights are chosen row by row (typed_products.hip has the launches).
+//
+// Rows x_i of type t become y_i = x_i W_t^T (+ b_t), and for a gradient g of y
+//
+//   dx_i = g_i W_t,   dW_t = sum_{i of type t} g_i^T x_i,   db_t = sum g_i.
+//
+// Rows are taken by type through an index (row_groups.h), so that a tile of them has one matrix; nothing is gathered or
+// padded in memory. The number of rows of a type is known to the device alone: a launch has a slot for every BM rows
+// and one more for every type, type t owns the slots from floor(begin_t / BM) + t on, which are as many as it can need
+// (floor(b / m) - floor(a / m) + 1 is never less than ceil((b - a) / m)), and a block whose slot is past its type's rows ends.
+// A row can have several parts (the components of an irrep), which share its type: they count as rows here.
+//
+// Products run on the 32x32 matrix instructions, sums in 32 bits. Tiles of both operands go from memory to LDS 128 bytes of
+// the summation at a time, into one of two buffers while the products read the other.
+#ifndef OEQ_TYPED_PRODUCTS_H
+#define OEQ_TYPED_PRODUCTS_H
+
+#include <hip/hip_runtime.h>
+
+#include <cstdint>
+#include <type_traits>
+
+namespace typed_products {
+
+// Rows and parts of x and the rows of w are strided, their elements contiguous; strides in elements.
+struct Args {
+    const void *x, *w, *bias, *up;
+    const float *thin, *scale;  // thin: [rows, thin_row]; scale: of each type
+    void* out;                  // [rows, parts, out_row]
+    const int *order, *ptr;
+    int64_t x_row, x_part, w_type, w_row, bias_type, up_type, up_col, up_rank, out_row;
+    int rows, types, parts, inner, outer, rank, thin_row;
+    int slots, tiles;  // of rows, of columns
+    int shared;        // rows without a type have w too
+};
+
+// Sums of products over rows: out[t] = sum a_i^T b_i, [types, a columns, b columns].
+struct SumArgs {
+    const void *a, *b;
+    void* out;
+    float* partial;  // [slots, a columns, b columns]
+    const int *order, *ptr;
+    int64_t a_row, a_part, b_row, b_part;
+    int rows, types, parts, a_columns, b_columns;
+    int chunk;  // rows (with their parts) that a block sums up
+    int slots, a_tiles, b_tiles;
+};
+
+typedef float float4_t __attribute__((ext_vector_type(4)));
+typedef float float8_t __attribute__((ext_vector_type(8)));
+typedef float float16_t __attribute__((ext_vector_type(16)));
+typedef _Float16 half4_t __attribute__((ext_vector_type(4)));
+typedef _Float16 half8_t __attribute__((ext_vector_type(8)));
+typedef __bf16 bf4_t __attribute__((ext_vector_type(4)));
+typedef __bf16 bf8_t __attribute__((ext_vector_type(8)));
+typedef short short4_t __attribute__((ext_vector_type(4)));
+typedef unsigned uint4_t __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(1))) const void* gptr_t;
+typedef __attribute__((address_space(3))) void* lptr_t;
+typedef __attribute__((address_space(3))) short4_t* ltr_t;
+
+// A fragment: 16 bytes of a row, the operand of a product over twice as many elements (one half in either half of a wave).
+template <typename T>
+struct Types;
+template <>
+struct Types<float> {
+    typedef float4_t frag;
+    typedef float4_t quad;
+};
+template <>
+struct Types<_Float16> {
+    typedef half8_t frag;
+    typedef half4_t quad;
+};
+template <>
+struct Types<__bf16> {
+    typedef bf8_t frag;
+    typedef bf4_t quad;
+};
+
+__device__ __forceinline__ float16_t mma(float4_t a, float4_t b, float16_t c) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) c = __builtin_amdgcn_mfma_f32_32x32x2f32(a[j], b[j], c, 0, 0, 0);
+    return c;
+}
+__device__ __forceinline__ float16_t mma(float8_t a, float8_t b, float16_t c) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) c = __builtin_amdgcn_mfma_f32_32x32x2f32(a[j], b[j], c, 0, 0, 0);
+    return c;
+}
+__device__ __forceinline__ float16_t mma(half8_t a, half8_t b, float16_t c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
+}
+__device__ __forceinline__ float16_t mma(bf8_t a, bf8_t b, float16_t c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+}
+
+// ---------------------------------------------------------------------------
+// slots
+// ---------------------------------------------------------------------------
+
+// Blocks go to the eight XCDs in turn, each with a cache of its own: each takes a run of neighbouring tiles.
+__device__ __forceinline__ int tile_of_block(int block, int blocks) {
+    const int xcd = block & 7, each = blocks >> 3, rest = blocks & 7;
+    return xcd * each + min(xcd, rest) + (block >> 3);
+}
+
+struct Range {
+    int type, lo, hi;  // places of the index times parts
+};
+
+// Where type t's rows begin (t = types: the rows without one).
+__device__ __forceinline__ int begin_of(const int* ptr, int t, int rows, int parts) { return min(max(ptr[t], 0), rows) * parts; }
+
+// The type that owns a slot of `each` rows, among `types` (and the rows without a type, if `rest`), and the slot's rows.
+__device__ __forceinline__ Range rows_of_slot(const int* ptr, int slot, int each, int types, bool rest, int rows, int parts) {
+    const int lane = threadIdx.x & 63;
+    int t = 0, n = types + rest;
+    while (n > 1) {  // 64 candidates at a time; the first of them always begins early enough
+        const int step = (n + 63) >> 6;
+        const int at = lane * step;
+        const bool early = lane == 0 || (at < n && begin_of(ptr, t + at, rows, parts) / each + t + at <= slot);
+        const int last = 63 - __builtin_clzll(__ballot(early));
+        t += last * step;
+        n = min(step, n - last * step);
+    }
+    Range r;
+    r.type = __builtin_amdgcn_readfirstlane(t);
+    const int begin = begin_of(ptr, r.type, rows, parts);
+    const int64_t lo = begin + (int64_t)(slot - begin / each - r.type) * each;
+    r.hi = r.type < types ? begin_of(ptr, r.type + 1, rows, parts) : rows * parts;
+    r.lo = lo < r.hi ? (int)lo : r.hi;
+    return r;
+}
+
+// Place of the index -> row and part. (An index that was not made here is kept inside the rows.)
+struct Place {
+    int row, part;
+    __device__ __forceinline__ Place(const int* order, int at, int parts, int rows) {
+        const int i = parts == 1 ? at : at / parts;
+        part = at - i * parts;
+        row = order ? order[i] : i;
+        if ((unsigned)row >= (unsigned)rows) row = 0;
+    }
+};
+
+// ---------------------------------------------------------------------------
+// tiles in LDS
+// ---------------------------------------------------------------------------
+
+__device__ const uint4_t kZeros = {0, 0, 0, 0};
+
+// ROWS rows of CH chunks of 16 bytes; chunk c of row r lies at place c ^ swizzle(r) of the row. LDS has 64 banks, 256 bytes.
+// A 16-byte read meets them with one chunk of 16 consecutive rows, a transposing read with four neighbouring chunks of four
+// rows that begin at a multiple of four: either way the 16 have to lie in different places modulo 16. Four-byte
+// reads of float columns have 32 columns of two rows that lie four apart: the rows' places have to differ in the half.
+template <typename T, int CH, int ROWS, int WAVES>
+struct Tile {
+    static constexpr int kRowBytes = CH * 16, kBytes = ROWS * kRowBytes, kElements = 16 / (int)sizeof(T);
+    static constexpr int kRowsPer = 64 / CH, kEach = kBytes / 1024 / WAVES;
+    static_assert(CH >= 8 && CH <= 64 && kEach * 1024 * WAVES == kBytes, "the waves share a tile");
+
+    static __device__ __forceinline__ int swizzle(int r) {
+        if constexpr (CH == 8) return (r >> 1 & 1) << 2 | (r >> 2 & 3);
+        else if constexpr (sizeof(T) == 4) return (r >> 2 & 1) << 3;
+        else return (r & 3) << 2 | (r >> 2 & 3);
+    }
+    // What a lane of a wave brings with its i-th request: 1 KB for the wave.
+    static __device__ __forceinline__ int row(int i, int wave, int lane) { return (i * WAVES + wave) * kRowsPer + lane / CH; }
+    static __device__ __forceinline__ int chunk(int i, int wave, int lane) { return (lane % CH) ^ swizzle(row(i, wave, lane)); }
+    static __device__ __forceinline__ void request(char* lds, const char* from, int i, int wave) {
+        __builtin_amdgcn_global_load_lds((gptr_t)from, (lptr_t)(lds + (i * WAVES + wave) * 1024), 16, 0, 0);
+    }
+    static __device__ __forceinline__ void put(char* lds, uint4_t x, int i, int wave, int lane) {
+        *(uint4_t*)(lds + (i * WAVES + wave) * 1024 + lane * 16) = x;
+    }
+
+    // 16 bytes of row r: fragment f of it.
+    static __device__ __forceinline__ typename Types<T>::frag along(const char* lds, int r, int f, int half) {
+        return *(const typename Types<T>::frag*)(lds + r * kRowBytes + (((2 * f + half) ^ swizzle(r)) << 4));
+    }
+    // The rows 2 E f + E half .. + E of column `first` + lane % 32.
+    static __device__ __forceinline__ typename Types<T>::frag down(const char* lds, int f, int first, int lane) {
+        typename Types<T>::frag x;
+        if constexpr (sizeof(T) == 2) {
+            // a transposing read gives each of 16 lanes four rows of its column out of the 4 x 16 block whose rows the lanes
+            // address by quarters
+            const int l = lane & 15, c = (first >> 3) + 2 * ((lane >> 4) & 1) + ((l & 3) >> 1);
+            union {
+                short4_t q[2];
+                typename Types<T>::frag f;
+            } u;
+#pragma unroll
+            for (int g = 0; g < 2; ++g) {
+                const int r = 16 * f + 8 * (lane >> 5) + 4 * g + (l >> 2);
+                u.q[g] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((ltr_t)(lds + r * kRowBytes + ((c ^ swizzle(r)) << 4) + ((l & 1) << 3)));
+            }
+            x = u.f;
+        } else {
+            const int d = first + (lane & 31);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const int r = 8 * f + 4 * (lane >> 5) + j;
+                x[j] = *(const float*)(lds + r * kRowBytes + (((d >> 2) ^ swizzle(r)) << 4) + ((d & 3) << 2));
+            }
+        }
+        return x;
+    }
+};
+
+// 16 bytes from anywhere, of which `left` elements are there; zeros for the others.
+template <typename T>
+__device__ __forceinline__ uint4_t fetch(const char* from, int left) {
+    constexpr int E = 16 / (int)sizeof(T);
+    uint4_t x = {0, 0, 0, 0};
+    if (left >= E) {
+        __builtin_memcpy(&x, from, 16);
+    } else {
+        union {
+            uint4_t v;
+            T e[E];
+        } u;
+        u.v = x;
+#pragma unroll
+        for (int j = 0; j < E; ++j)
+            if (j < left) u.e[j] = ((const T*)from)[j];
+        x = u.v;
+    }
+    return x;
+}
+
+// What this wave requested is in LDS; then the same for the others, and all are done with the other buffer.
+__device__ __forceinline__ void arrived() {
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+}
+
+// ---------------------------------------------------------------------------
+// products of rows
+// ---------------------------------------------------------------------------
+
+// A tile of BM rows and BN columns. ACROSS: the weights' rows run along the columns (w[k, n]), else along the summation
+// (w[n, k]). DIRECT: everything is aligned to 16 bytes and goes straight to LDS; else through registers, by elements where a
+// row ends. The result is transposed in registers: lane l has row l % 32, register r column 8 (r / 4) + 4 (l / 32) + r % 4.
+template <typename T, typename O, bool ACROSS, bool DIRECT, int BM, int BN, int WM, int WN>
+__global__ __launch_bounds__(64 * WM * WN) void row_products(Args g) {
+    constexpr int WAVES = WM * WN, BK = 128 / (int)sizeof(T), E = 16 / (int)sizeof(T);
+    constexpr int TM = BM / WM / 32, TN = BN / WN / 32;
+    typedef Tile<T, 8, BM, WAVES> X;
+    typedef Tile<T, ACROSS ? BN * (int)sizeof(T) / 16 : 8, ACROSS ? BK : BN, WAVES> W;
+    __shared__ __align__(1024) char x0[X::kBytes], x1[X::kBytes], w0[W::kBytes], w1[W::kBytes];
+
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), half = lane >> 5;
+    // neighbours in a run: eight slots, column by column
+    const int id = tile_of_block(blockIdx.x, g.slots * g.tiles);
+    const int group = id / (8 * g.tiles), in_group = id - group * 8 * g.tiles, size = min(8, g.slots - group * 8);
+    const int slot = group * 8 + in_group % size, n0 = in_group / size * BN;
+    const Range rows = rows_of_slot(g.ptr, slot, BM, g.types, true, g.rows, g.parts);
+    if (rows.lo >= rows.hi) return;
+    const int m0 = rows.lo;
+    const bool typed = rows.type < g.types;
+    const int steps = typed || g.shared ? (g.inner + BK - 1) / BK : 0;
+
+    // where this lane's chunks of the tiles come from
+    const char* xs[X::kEach];
+    const char* ws[W::kEach];
+    int w_left[W::kEach];  // elements of w from there on to the end of its row (ACROSS)
+    if (steps) {
+        const T* w = (const T*)g.w + (typed ? rows.type : 0) * g.w_type;
+#pragma unroll
+        for (int i = 0; i < X::kEach; ++i) {
+            const int at = m0 + X::row(i, wave, lane);
+            const Place p(g.order, at < rows.hi ? at : m0, g.parts, g.rows);
+            xs[i] = (const char*)((const T*)g.x + p.row * g.x_row + p.part * g.x_part) + X::chunk(i, wave, lane) * 16;
+        }
+#pragma unroll
+        for (int i = 0; i < W::kEach; ++i) {
+            const int r = W::row(i, wave, lane), c = W::chunk(i, wave, lane) * E;
+            if constexpr (ACROSS) {
+                const bool in = n0 + c < g.outer;
+                w_left[i] = in ? g.outer - n0 - c : 0;
+                ws[i] = (const char*)(w + r * g.w_row + (in ? n0 + c : 0));
+            } else {
+                ws[i] = (const char*)(w + (int64_t)min(n0 + r, g.outer - 1) * g.w_row + c);
+            }
+        }
+    }
+    const int64_t w_step = ACROSS ? BK * g.w_row * (int64_t)sizeof(T) : 128;
+    uint4_t x_reg[DIRECT ? 1 : X::kEach], w_reg[DIRECT ? 1 : W::kEach];
+
+    // the tiles of step k
+    auto request = [&](char* xt, char* wt, int k) {
+        const bool last = (k + 1) * BK > g.inner;
+#pragma unroll
+        for (int i = 0; i < X::kEach; ++i) {
+            const int left = g.inner - k * BK - X::chunk(i, wave, lane) * E;
+            if constexpr (DIRECT)
+                X::request(xt, last && left <= 0 ? (const char*)&kZeros : xs[i], i, wave);
+            else
+                x_reg[i] = fetch<T>(xs[i], left);
+            xs[i] += 128;
+        }
+#pragma unroll
+        for (int i = 0; i < W::kEach; ++i) {
+            if constexpr (ACROSS) {
+                const bool in = k * BK + W::row(i, wave, lane) < g.inner;
+                if constexpr (DIRECT)
+                    W::request(wt, last && !in ? (const char*)&kZeros : ws[i], i, wave);
+                else
+                    w_reg[i] = fetch<T>(ws[i], in ? w_left[i] : 0);
+            } else {
+                const int left = g.inner - k * BK - W::chunk(i, wave, lane) * E;
+                if constexpr (DIRECT)
+                    W::request(wt, last && left <= 0 ? (const char*)&kZeros : ws[i], i, wave);
+                else
+                    w_reg[i] = fetch<T>(ws[i], left);
+            }
+            ws[i] += w_step;
+        }
+    };
+    auto put = [&](char* xt, char* wt) {
+        if constexpr (!DIRECT) {
+#pragma unroll
+            for (int i = 0; i < X::kEach; ++i) X::put(xt, x_reg[i], i, wave, lane);
+#pragma unroll
+            for (int i = 0; i < W::kEach; ++i) W::put(wt, w_reg[i], i, wave, lane);
+        }
+    };
+
+    const int wm = wave % WM * (BM / WM), wn = wave / WM * (BN / WN);
+    float16_t acc[TM][TN];
+#pragma unroll
+    for (int m = 0; m < TM; ++m)
+#pragma unroll
+        for (int n = 0; n < TN; ++n) acc[m][n] = 0.0f;
+
+    auto products = [&](const char* xt, const char* wt) {
+#pragma unroll
+        for (int f = 0; f < 4; ++f) {
+            typename Types<T>::frag a[TN], b[TM];
+#pragma unroll
+            for (int n = 0; n < TN; ++n)
+                a[n] = ACROSS ? W::down(wt, f, wn + 32 * n, lane) : W::along(wt, wn + 32 * n + (lane & 31), f, half);
+#pragma unroll
+            for (int m = 0; m < TM; ++m) b[m] = X::along(xt, wm + 32 * m + (lane & 31), f, half);
+#pragma unroll
+            for (int m = 0; m < TM; ++m)
+#pragma unroll
+                for (int n = 0; n < TN; ++n) acc[m][n] = mma(a[n], b[m], acc[m][n]);
+        }
+    };
+    auto step = [&](char* xt, char* wt, char* xn, char* wn_, int k) {
+        arrived();
+        if (k + 1 < steps) request(xn, wn_, k + 1);
+        products(xt, wt);
+        if (k + 1 < steps) put(xn, wn_);
+    };
+    if (steps) {
+        request(x0, w0, 0);
+        put(x0, w0);
+    }
+    for (int k = 0; k < steps; k += 2) {
+        step(x0, w0, x1, w1, k);
+        if (k + 1 < steps) step(x1, w1, x0, w0, k + 1);
+    }
+
+    int64_t to[TM];
+    bool mine[TM];
+    float by = 1.0f;
+    if (g.scale) by = typed ? g.scale[rows.type] : 0.0f;
+#pragma unroll
+    for (int m = 0; m < TM; ++m) {
+        const int at = m0 + wm + 32 * m + (lane & 31);
+        mine[m] = at < rows.hi;
+        const Place p(g.order, mine[m] ? at : m0, g.parts, g.rows);
+        to[m] = ((int64_t)p.row * g.parts + p.part) * g.out_row;
+        if (g.thin && typed) {
+            // the second, thin product: its rows are float, so it is one of floats
+            const float* u = g.thin + (int64_t)p.row * g.thin_row;
+            for (int k = 0; k < g.rank; k += 8) {
+                const float4_t b = *(const float4_t*)(u + k + 4 * half);
+#pragma unroll
+                for (int n = 0; n < TN; ++n) {
+                    const int col = n0 + wn + 32 * n + (lane & 31);
+                    const T* v = (const T*)g.up + rows.type * g.up_type;
+                    float4_t a = 0.0f;
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const int r = k + 4 * half + j;
+                        if (r < g.rank && col < g.outer) a[j] = (float)v[col * g.up_col + r * g.up_rank];
+                    }
+                    acc[m][n] = mma(a, b, acc[m][n]);
+                }
+            }
+        }
+    }
+    O* out = (O*)g.out;
+    const bool quads = g.out_row % 4 == 0;
+#pragma unroll
+    for (int m = 0; m < TM; ++m) {
+        if (!mine[m]) continue;
+#pragma unroll
+        for (int n = 0; n < TN; ++n)
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                const int col = n0 + wn + 32 * n + 8 * q + 4 * half;
+                if (col >= g.out_row) continue;
+                typename Types<O>::quad y;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    float s = acc[m][n][4 * q + j] * by;
+                    if (g.bias && typed && col + j < g.outer) s += (float)((const T*)g.bias)[rows.type * g.bias_type + col + j];
+                    y[j] = (O)(col + j < g.outer ? s : 0.0f);
+                }
+                if (quads) {
+                    *(typename Types<O>::quad*)(out + to[m] + col) = y;
+                } else {
+#pragma unroll
+                    for (int j = 0; j < 4; ++j)
+                        if (col + j < g.out_row) out[to[m] + col + j] = y[j];
+                }
+            }
+    }
+}
+
+// ---------------------------------------------------------------------------
+// sums of products over rows
+// ---------------------------------------------------------------------------
+
+// Operands of which one is float and the other is not are multiplied as floats.
+template <typename T, bool WIDE>
+__device__ __forceinline__ auto widened(typename Types<T>::frag x) {
+    if constexpr (sizeof(T) == 2 && WIDE)
+        return __builtin_convertvector(x, float8_t);
+    else
+        return x;
+}
+
+// A tile of BM columns of a and BN columns of b, summed over the rows of a slot. BK rows at a time; rows past the end are zeros.
+template <typename A, typename B, typename O, bool DIRECT, int BM, int BN, int WM, int WN>
+__global__ __launch_bounds__(64 * WM * WN) void sum_products(SumArgs g) {
+    constexpr int WAVES = WM * WN, BK = sizeof(A) + sizeof(B) == 4 ? 64 : 32;
+    constexpr bool MIXED = sizeof(A) != sizeof(B);
+    constexpr int EA = 16 / (int)sizeof(A), EB = 16 / (int)sizeof(B);
+    constexpr int TM = BM / WM / 32, TN = BN / WN / 32;
+    typedef Tile<A, BM * (int)sizeof(A) / 16, BK, WAVES> TA;
+    typedef Tile<B, BN * (int)sizeof(B) / 16, BK, WAVES> TB;
+    __shared__ __align__(1024) char a0[TA::kBytes], a1[TA::kBytes], b0[TB::kBytes], b1[TB::kBytes];
+
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int id = tile_of_block(blockIdx.x, g.slots * g.a_tiles * g.b_tiles);
+    const int slot = id / (g.a_tiles * g.b_tiles), tile = id - slot * g.a_tiles * g.b_tiles;
+    const int m0 = tile / g.b_tiles * BM, n0 = tile % g.b_tiles * BN;
+    const Range rows = rows_of_slot(g.ptr, slot, g.chunk, g.types, false, g.rows, g.parts);
+    const int begin = begin_of(g.ptr, rows.type, g.rows, g.parts);
+    const bool whole = rows.hi - begin <= g.chunk;  // the type has no other slot
+    if (rows.lo >= rows.hi && !(whole && rows.type + begin / g.chunk == slot)) return;
+    const int end = min(rows.hi, rows.hi - rows.lo > g.chunk ? rows.lo + g.chunk : rows.hi);
+    const int steps = (end - rows.lo + BK - 1) / BK;
+
+    uint4_t a_reg[DIRECT ? 1 : TA::kEach], b_reg[DIRECT ? 1 : TB::kEach];
+    auto request = [&](char* at, char* bt, int k) {
+#pragma unroll
+        for (int i = 0; i < TA::kEach; ++i) {
+            const int j = rows.lo + k * BK + TA::row(i, wave, lane), c = m0 + TA::chunk(i, wave, lane) * EA;
+            const Place p(g.order, min(j, end - 1), g.parts, g.rows);
+            const char* from = (const char*)((const A*)g.a + p.row * g.a_row + p.part * g.a_part + (c < g.a_columns ? c : 0));
+            if constexpr (DIRECT)
+                TA::request(at, j < end ? from : (const char*)&kZeros, i, wave);
+            else
+                a_reg[i] = fetch<A>(from, j < end && c < g.a_columns ? g.a_columns - c : 0);
+        }
+#pragma unroll
+        for (int i = 0; i < TB::kEach; ++i) {
+            const int j = rows.lo + k * BK + TB::row(i, wave, lane), c = n0 + TB::chunk(i, wave, lane) * EB;
+            const Place p(g.order, min(j, end - 1), g.parts, g.rows);
+            const char* from = (const char*)((const B*)g.b + p.row * g.b_row + p.part * g.b_part + (c < g.b_columns ? c : 0));
+            if constexpr (DIRECT)
+                TB::request(bt, j < end ? from : (const char*)&kZeros, i, wave);
+            else
+                b_reg[i] = fetch<B>(from, j < end && c < g.b_columns ? g.b_columns - c : 0);
+        }
+    };
+    auto put = [&](char* at, char* bt) {
+        if constexpr (!DIRECT) {
+#pragma unroll
+            for (int i = 0; i < TA::kEach; ++i) TA::put(at, a_reg[i], i, wave, lane);
+#pragma unroll
+            for (int i = 0; i < TB::kEach; ++i) TB::put(bt, b_reg[i], i, wave, lane);
+        }
+    };
+
+    const int wm = wave % WM * (BM / WM), wn = wave / WM * (BN / WN);
+    float16_t acc[TM][TN];
+#pragma unroll
+    for (int m = 0; m < TM; ++m)
+#pragma unroll
+        for (int n = 0; n < TN; ++n) acc[m][n] = 0.0f;
+
+    // A fragment of floats has 8 of the rows that one of 16 bits has: 8 f + 4 half .. + 4 (16 f + 8 half .. + 8); where
+    // both meet, two reads of four rows make the longer one.
+    auto a_frag = [&](const char* at, int f, int first) {
+        if constexpr (MIXED && sizeof(A) == 4) {
+            float8_t x;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const int r = 16 * f + 8 * (lane >> 5) + j, d = first + (lane & 31);
+                x[j] = *(const float*)(at + r * TA::kRowBytes + (((d >> 2) ^ TA::swizzle(r)) << 4) + ((d & 3) << 2));
+            }
+            return x;
+        } else {
+            return widened<A, MIXED>(TA::down(at, f, first, lane));
+        }
+    };
+    auto b_frag = [&](const char* bt, int f, int first) {
+        if constexpr (MIXED && sizeof(B) == 4) {
+            float8_t x;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const int r = 16 * f + 8 * (lane >> 5) + j, d = first + (lane & 31);
+                x[j] = *(const float*)(bt + r * TB::kRowBytes + (((d >> 2) ^ TB::swizzle(r)) << 4) + ((d & 3) << 2));
+            }
+            return x;
+        } else {
+            return widened<B, MIXED>(TB::down(bt, f, first, lane));
+        }
+    };
+    constexpr int FRAGS = sizeof(A) == 4 && sizeof(B) == 4 ? BK / 8 : BK / 16;
+    auto products = [&](const char* at, const char* bt) {
+#pragma unroll
+        for (int f = 0; f < FRAGS; ++f) {
+            decltype(a_frag(at, 0, 0)) a[TM];
+            decltype(b_frag(bt, 0, 0)) b[TN];
+#pragma unroll
+            for (int m = 0; m < TM; ++m) a[m] = a_frag(at, f, wm + 32 * m);
+#pragma unroll
+            for (int n = 0; n < TN; ++n) b[n] = b_frag(bt, f, wn + 32 * n);
+#pragma unroll
+            for (int m = 0; m < TM; ++m)
+#pragma unroll
+                for (int n = 0; n < TN; ++n) acc[m][n] = mma(a[m], b[n], acc[m][n]);
+        }
+    };
+    auto step = [&](char* at, char* bt, char* an, char* bn, int k) {
+        arrived();
+        if (k + 1 < steps) request(an, bn, k + 1);
+        products(at, bt);
+        if (k + 1 < steps) put(an, bn);
+    };
+    if (steps > 0) {
+        request(a0, b0, 0);
+        put(a0, b0);
+    }
+    for (int k = 0; k < steps; k += 2) {
+        step(a0, b0, a1, b1, k);
+        if (k + 1 < steps) step(a1, b1, a0, b0, k + 1);
+    }
+
+    // lane l has column l % 32 of b, register r row 8 (r / 4) + 4 (l / 32) + r % 4
+    const int64_t size = (int64_t)g.a_columns * g.b_columns;
+    O* out = (O*)g.out + rows.type * size;
+    float* partial = g.partial + slot * size;
+#pragma unroll
+    for (int m = 0; m < TM; ++m)
+#pragma unroll
+        for (int n = 0; n < TN; ++n)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                const int i = m0 + wm + 32 * m + 8 * (r / 4) + 4 * (lane >> 5) + r % 4, j = n0 + wn + 32 * n + (lane & 31);
+                if (i >= g.a_columns || j >= g.b_columns) continue;
+                const int64_t at = (int64_t)i * g.b_columns + j;
+                if (whole)
+                    out[at] = (O)acc[m][n][r];
+                else
+                    partial[at] = acc[m][n][r];
+            }
+}
+
+// The slots of a type in order, where it has more than one.
+template <typename O>
+__global__ __launch_bounds__(256) void join_slots(SumArgs g) {
+    const int t = blockIdx.y;
+    const int begin = begin_of(g.ptr, t, g.rows, g.parts), n = begin_of(g.ptr, t + 1, g.rows, g.parts) - begin;
+    if (n <= g.chunk) return;
+    const int64_t size = (int64_t)g.a_columns * g.b_columns;
+    const float* from = g.partial + ((int64_t)begin / g.chunk + t) * size;
+    const int slots = (n - 1) / g.chunk + 1;
+    for (int64_t i = blockIdx.x * 256ll + threadIdx.x; i < size; i += gridDim.x * 256ll) {
+        float sum = 0;
+        for (int s = 0; s < slots; ++s) sum += from[s * size + i];
+        ((O*)g.out)[t * size + i] = (O)sum;
+    }
+}
+
+}  // namespace typed_products
+#endif

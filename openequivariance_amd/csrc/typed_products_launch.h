@@ -1,0 +1,22 @@
+// The launches that typed_products.hip defines for each element type.
+#ifndef OEQ_TYPED_PRODUCTS_LAUNCH_H
+#define OEQ_TYPED_PRODUCTS_LAUNCH_H
+
+#include "typed_products.h"
+
+namespace typed_products {
+
+enum Thin { kNeither, kFirst, kSecond };  // which operand of a sum of products is float beside elements of 16 bits
+
+template <typename T>
+struct Launch {
+    // across: the weights' rows run along the columns. wide: the result is float. direct: see row_products.
+    static hipError_t rows(Args a, bool across, bool wide, bool direct, hipStream_t stream);
+    static hipError_t sums(SumArgs a, Thin thin, bool direct, hipStream_t stream);
+};
+
+// Columns of a tile of sum_products of which there are few (float operands of a thin product), else.
+constexpr int kThinTile = 32, kSumTile = 128;
+
+}  // namespace typed_products
+#endif

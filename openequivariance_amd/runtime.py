@@ -62,7 +62,7 @@ ROLE_SLICE_PLACE = 24
 
 CONV_ATOMIC, CONV_SORTED, CONV_GROUPED = 0, 1, 2
 DX_TERMS, DX_ATOMIC, DX_ARRIVAL, DX_SENDER_WALK = 0, 1, 2, 3
-ABI_VERSION = 9
+ABI_VERSION = 10
 
 
 class OeqError(RuntimeError):
@@ -130,10 +130,28 @@ class _QkRotary(ctypes.Structure):
                 + [(n, ctypes.c_void_p) for n in ("q", "k", "q_weight", "k_weight", "positions", "table")])
 
 
-# What liboeq_amd.so is compiled from, with the macros of each object: the runtime and the operators on nodes, whose
-# attention kernels make one object per element type (they take the longest: compiled side by side).
-_OBJECTS = [("oeq_amd.cpp", []), ("oeq_nodes.hip", [])] + [
-    ("packed_attention.hip", [f"-DOEQ_ATTENTION_TYPE={t}"]) for t in ("float", "_Float16", "__bf16")]
+class _TypedRows(ctypes.Structure):
+    _fields_ = ([(n, ctypes.c_int32) for n in ("type", "across", "shared", "rank")]
+                + [(n, ctypes.c_int64) for n in ("rows", "parts", "types", "inner", "outer", "x_row_stride", "x_part_stride",
+                                                 "w_type_stride", "w_row_stride", "up_type_stride", "up_outer_stride",
+                                                 "up_rank_stride")]
+                + [(n, ctypes.c_void_p) for n in ("x", "w", "bias", "thin", "up", "order", "ptr")])
+
+
+class _TypedSum(ctypes.Structure):
+    _fields_ = ([(n, ctypes.c_int32) for n in ("type", "thin")]
+                + [(n, ctypes.c_int64) for n in ("rows", "parts", "types", "a_columns", "b_columns", "a_row_stride",
+                                                 "a_part_stride", "b_row_stride", "b_part_stride")]
+                + [(n, ctypes.c_void_p) for n in ("a", "b", "order", "ptr")])
+
+
+# What liboeq_amd.so is compiled from, with the macros of each object: the runtime, the operators on nodes and those with
+# parameters by type, whose kernels of attention and of products make one object per element type (they take the longest:
+# compiled side by side).
+_OBJECTS = [("oeq_amd.cpp", []), ("oeq_nodes.hip", []), ("oeq_typed.hip", [])] + [
+    (f"{kernels}.hip", [f"-D{macro}={t}"]) for kernels, macro in (("packed_attention", "OEQ_ATTENTION_TYPE"),
+                                                                  ("typed_products", "OEQ_PRODUCT_TYPE"))
+    for t in ("float", "_Float16", "__bf16")]
 
 
 def _sources() -> List[Path]:
@@ -242,6 +260,17 @@ EXPORTS = {
     "oeq_qk_norm_rotary_backward": (ctypes.c_int, [ctypes.POINTER(_QkRotary), _P, _I64, _I64, _P, _I64, _I64, _P, _P, _P,
                                                    _P, _P, _SZ, _P]),
     "oeq_irrep_dropout": (ctypes.c_int, [ctypes.c_int, _I64, _I64, _P, _P, _P, _P, _P, ctypes.c_double, _P]),
+    "oeq_group_rows_workspace_bytes": (_SZ, [_I64, _I64]),
+    "oeq_group_rows": (ctypes.c_int, [_I64, _I64, _P, _P, _P, _P, _SZ, _P]),
+    "oeq_type_lookup": (ctypes.c_int, [ctypes.c_int, _I64, _I64, _I64, _P, _P, _I64, ctypes.c_double, _P, _P]),
+    "oeq_type_sum_workspace_bytes": (_SZ, [_I64, _I64, _I64]),
+    "oeq_type_sum": (ctypes.c_int, [ctypes.c_int, _I64, _I64, _I64, _I64, _P, _P, _P, _P, _I64, _I64, ctypes.c_double, _P, _P,
+                                    _SZ, _P]),
+    "oeq_typed_product": (ctypes.c_int, [ctypes.POINTER(_TypedRows), _P, _P]),
+    "oeq_thin_stride": (_I64, [_I64]),
+    "oeq_typed_thin_product": (ctypes.c_int, [ctypes.POINTER(_TypedRows), _P, _P, _P]),
+    "oeq_typed_sum_workspace_bytes": (_SZ, [ctypes.POINTER(_TypedSum)]),
+    "oeq_typed_sum_products": (ctypes.c_int, [ctypes.POINTER(_TypedSum), _P, _P, _SZ, _P]),
     "oeq_last_error": (ctypes.c_char_p, []),
     "oeq_abi_version": (ctypes.c_int, []),
 }
