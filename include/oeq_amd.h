@@ -477,9 +477,12 @@ typedef struct {
     const void* bias;        /* [types, outer], contiguous, or NULL; not with shared */
     const float* thin;       /* [rows, oeq_thin_stride(rank)], filled up with zeros: plus up_t thin_i for rows with a type, */
     const void* up;          /* up: [types, outer, rank] of any strides. One part a row. */
-    const int32_t *order, *ptr;
+    const int64_t* type_of_row;
+    const int32_t *order, *ptr;  /* may be NULL where oeq_typed_needs_index() is 0 */
 } oeq_typed_rows;
 
+/* Whether a product goes by the index: those of few rows do without. */
+int oeq_typed_needs_index(const oeq_typed_rows* a);
 /* out: [rows, parts, outer], contiguous. Rows without a type become 0 (shared: their product with w). */
 int oeq_typed_product(const oeq_typed_rows* a, void* out, void* stream);
 /* The same with results in float, scale[t] times (NULL: 1); `outer` is the rank, out: [rows, oeq_thin_stride(outer)], filled up

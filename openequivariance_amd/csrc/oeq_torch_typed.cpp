@@ -36,9 +36,17 @@ void check_types(const Tensor& types, const Tensor& beside) {
     check_tensor(types, types.sizes(), at::kLong, "types", beside);
 }
 
-// The index of a batch's types: the caller's, or one made for this call.
+// The index of a batch's types: the caller's, or one made when a call needs it.
 struct Groups {
-    Tensor order, ptr;
+    Tensor types, order, ptr;
+    int64_t count;
+    Groups(const Tensor& types_, int64_t count_, const OptTensor& order_, const OptTensor& ptr_);
+    void make();
+    void set(oeq_typed_rows& a) {
+        if (!oeq_typed_needs_index(&a)) return;
+        make();
+        a.order = order.data_ptr<int32_t>(), a.ptr = ptr.data_ptr<int32_t>();
+    }
 };
 
 Tensor2 group_rows_gpu(const Tensor& types, int64_t count) {
@@ -57,15 +65,17 @@ Tensor2 group_rows_gpu(const Tensor& types, int64_t count) {
     return {order, ptr};
 }
 
-Groups groups_of(const Tensor& types, int64_t count, const OptTensor& order, const OptTensor& ptr) {
-    TORCH_CHECK(order.has_value() == ptr.has_value(), "an index has both 'order' and 'ptr'");
-    if (!order.has_value()) {
-        auto [o, p] = group_rows_gpu(types, count);
-        return {o, p};
-    }
-    check_tensor(*order, {types.size(0)}, at::kInt, "order", types);
-    check_tensor(*ptr, {count + 1}, at::kInt, "ptr", types);
-    return {order->contiguous(), ptr->contiguous()};
+Groups::Groups(const Tensor& types_, int64_t count_, const OptTensor& order_, const OptTensor& ptr_)
+    : types(types_.contiguous()), count(count_) {
+    TORCH_CHECK(order_.has_value() == ptr_.has_value(), "an index has both 'order' and 'ptr'");
+    if (!order_.has_value()) return;
+    check_tensor(*order_, {types.size(0)}, at::kInt, "order", types);
+    check_tensor(*ptr_, {count + 1}, at::kInt, "ptr", types);
+    order = order_->contiguous(), ptr = ptr_->contiguous();
+}
+
+void Groups::make() {
+    if (!order.defined()) std::tie(order, ptr) = group_rows_gpu(types, count);
 }
 
 // Rows as the kernels take them: elements one after the other, everything else strided. (Where strides or the first
@@ -123,16 +133,16 @@ Tensor type_embedding_gpu(const Tensor& types, const Tensor& weight, double scal
 }
 
 // Sums of rows [rows, channels] or [rows, parts, channels] by type.
-Tensor type_sum(const Tensor& x, const Tensor& types, const Groups& index, int64_t count, double scale, void* stream) {
+Tensor type_sum(const Tensor& x, Groups& index, double scale, void* stream) {
     const Strided rows(x);
-    const Tensor at = types.contiguous();
-    const int64_t channels = x.size(-1);
+    const int64_t channels = x.size(-1), count = index.count;
+    index.make();
     Tensor out = at::empty({count, channels}, x.options());
     if (rows.parts == 0) return out.zero_();
     const size_t nb = oeq_type_sum_workspace_bytes(x.size(0), count, channels);
     Tensor ws;
     if (nb) ws = scratch(x, nb);
-    check(oeq_type_sum(element_of(x, "grad"), x.size(0), rows.parts, count, channels, at.data_ptr<int64_t>(),
+    check(oeq_type_sum(element_of(x, "grad"), x.size(0), rows.parts, count, channels, index.types.data_ptr<int64_t>(),
                        index.order.data_ptr<int32_t>(), index.ptr.data_ptr<int32_t>(), rows.t.data_ptr(), rows.row, rows.part,
                        scale, out.data_ptr(), nb ? ws.data_ptr() : nullptr, nb, stream),
           "oeq_type_sum");
@@ -146,7 +156,8 @@ Tensor type_embedding_backward_gpu(const Tensor& grad, const Tensor& types, int6
     check_types(types, grad);
     check_tensor(grad, {types.size(0), grad.size(1)}, grad.scalar_type(), "grad", grad);
     OnDevice dev(grad);
-    return type_sum(grad, types, groups_of(types, count, order, ptr), count, scale, dev.stream);
+    Groups index(types, count, order, ptr);
+    return type_sum(grad, index, scale, dev.stream);
 }
 
 // ---------------------------------------------------------------------------
@@ -165,12 +176,13 @@ void check_linear(const Tensor& x, const Tensor& weight, const Tensor& types) {
     check_tensor(types, {x.size(0)}, at::kLong, "types", x);
 }
 
-oeq_typed_rows rows_of(const Tensor& like, const Strided& x, const Groups& index, int64_t types, int64_t inner, int64_t outer) {
+// (the index is set where a product needs one)
+oeq_typed_rows rows_of(const Tensor& like, const Strided& x, const Tensor& type_of_row, int64_t types, int64_t inner, int64_t outer) {
     oeq_typed_rows a{};
     a.type = element_of(like, "x");
     a.rows = like.size(0), a.parts = x.parts, a.types = types, a.inner = inner, a.outer = outer;
     a.x_row_stride = x.row, a.x_part_stride = x.part, a.x = x.t.data_ptr();
-    a.order = index.order.data_ptr<int32_t>(), a.ptr = index.ptr.data_ptr<int32_t>();
+    a.type_of_row = type_of_row.data_ptr<int64_t>();
     return a;
 }
 
@@ -180,8 +192,10 @@ void set_matrices(oeq_typed_rows& a, const Matrices& w, bool across) {
 
 // sum over rows of a^T b by type, of elements like `like`.
 Tensor typed_sum(const Tensor& a_, const Tensor& b_, int thin, int64_t a_columns, int64_t b_columns, const Tensor& like,
-                 const Groups& index, int64_t types, void* stream) {
+                 Groups& index, void* stream) {
     const Strided a(a_), b(b_);
+    const int64_t types = index.count;
+    index.make();
     Tensor out = at::empty({types, a_columns, b_columns}, like.options());
     if (a.parts == 0) return out.zero_();
     oeq_typed_sum d{};
@@ -210,13 +224,14 @@ Tensor typed_linear_gpu(const Tensor& x, const Tensor& weight, const Tensor& typ
     OnDevice dev(x);
     Tensor out = at::empty(with_last(x, weight.size(1)), x.options());
     if (out.numel() == 0) return out;
-    const Groups index = groups_of(types, weight.size(0), order, ptr);
+    Groups index(types, weight.size(0), order, ptr);
     const Strided in(x);
     const Matrices w(weight);
     Tensor b;
     if (bias.has_value()) b = bias->contiguous();
-    oeq_typed_rows a = rows_of(x, in, index, weight.size(0), weight.size(2), weight.size(1));
+    oeq_typed_rows a = rows_of(x, in, index.types, weight.size(0), weight.size(2), weight.size(1));
     set_matrices(a, w, !w.inner_first);
+    index.set(a);
     a.bias = b.defined() ? b.data_ptr() : nullptr;
     check(oeq_typed_product(&a, out.data_ptr(), dev.stream), "oeq_typed_product");
     return out;
@@ -229,7 +244,7 @@ Tensor3 typed_linear_backward_gpu(const Tensor& grad, const Tensor& x, const Ten
     check_tensor(grad, with_last(x, weight.size(1)), x.scalar_type(), "grad", x);
     OnDevice dev(x);
     const int64_t count = weight.size(0), outer = weight.size(1), inner = weight.size(2);
-    const Groups index = groups_of(types, count, order, ptr);
+    Groups index(types, count, order, ptr);
     const auto none = [&] { return at::empty({0}, x.options()); };
     Tensor dx = none(), dw = none(), db = none();
     if (want_x) {
@@ -237,13 +252,14 @@ Tensor3 typed_linear_backward_gpu(const Tensor& grad, const Tensor& x, const Ten
         if (dx.numel()) {
             const Strided g(grad);
             const Matrices w(weight);
-            oeq_typed_rows a = rows_of(x, g, index, count, outer, inner);
+            oeq_typed_rows a = rows_of(x, g, index.types, count, outer, inner);
             set_matrices(a, w, w.inner_first);
+            index.set(a);
             check(oeq_typed_product(&a, dx.data_ptr(), dev.stream), "oeq_typed_product");
         }
     }
-    if (want_weight) dw = typed_sum(grad, x, 0, outer, inner, x, index, count, dev.stream);
-    if (want_bias) db = type_sum(grad, types, index, count, 1.0, dev.stream);
+    if (want_weight) dw = typed_sum(grad, x, 0, outer, inner, x, index, dev.stream);
+    if (want_bias) db = type_sum(grad, index, 1.0, dev.stream);
     return {dx, dw, db};
 }
 
@@ -274,15 +290,16 @@ void set_thin(oeq_typed_rows& a, const Tensor& thin, const Tensor& matrices, int
 }
 
 // thin = scale_t m_t x, [rows, stride] in float.
-Tensor thin_product(const Tensor& x, const Tensor& matrices, bool transposed, const OptTensor& scale, const Groups& index,
+Tensor thin_product(const Tensor& x, const Tensor& matrices, bool transposed, const OptTensor& scale, Groups& index,
                     void* stream) {
     const Matrices w(matrices);
     const Strided in(x);
     const int64_t rank = matrices.size(transposed ? 2 : 1), inner = matrices.size(transposed ? 1 : 2);
     Tensor out = at::empty({x.size(0), oeq_thin_stride(rank)}, x.options().dtype(at::kFloat));
     if (out.numel() == 0) return out;
-    oeq_typed_rows a = rows_of(x, in, index, matrices.size(0), inner, rank);
+    oeq_typed_rows a = rows_of(x, in, index.types, matrices.size(0), inner, rank);
     set_matrices(a, w, w.inner_first == transposed);
+    index.set(a);
     const Tensor by = scale.has_value() ? scale->contiguous() : Tensor();
     check(oeq_typed_thin_product(&a, by.defined() ? by.data_ptr<float>() : nullptr, out.data_ptr<float>(), stream), "oeq_typed_thin_product");
     return out;
@@ -294,15 +311,16 @@ Tensor2 adapter_linear_gpu(const Tensor& x, const Tensor& weight, const Tensor& 
     check_adapters(x, weight, down, up, types, scale);
     OnDevice dev(x);
     const int64_t count = down.size(0), rank = down.size(1);
-    const Groups index = groups_of(types, count, order, ptr);
+    Groups index(types, count, order, ptr);
     Tensor thin = thin_product(x, down, false, scale, index, dev.stream);
     Tensor out = at::empty({x.size(0), weight.size(0)}, x.options());
     if (out.numel() == 0) return {out, thin};
     const Strided in(x);
     const Matrices w(weight);
-    oeq_typed_rows a = rows_of(x, in, index, count, weight.size(1), weight.size(0));
+    oeq_typed_rows a = rows_of(x, in, index.types, count, weight.size(1), weight.size(0));
     set_matrices(a, w, !w.inner_first);
     set_thin(a, thin, up, 1, 2);
+    index.set(a);
     check(oeq_typed_product(&a, out.data_ptr(), dev.stream), "oeq_typed_product");
     return {out, thin};
 }
@@ -315,7 +333,7 @@ Tensor4 adapter_linear_backward_gpu(const Tensor& grad, const Tensor& x, const T
     check_tensor(grad, {x.size(0), outer}, x.scalar_type(), "grad", x);
     check_tensor(thin, {x.size(0), oeq_thin_stride(rank)}, at::kFloat, "thin", x);
     OnDevice dev(x);
-    const Groups index = groups_of(types, count, order, ptr);
+    Groups index(types, count, order, ptr);
     const Tensor u = thin.contiguous();
     const auto none = [&] { return at::empty({0}, x.options()); };
     Tensor dx = none(), dw = none(), ddown = none(), dup = none(), v;
@@ -325,17 +343,19 @@ Tensor4 adapter_linear_backward_gpu(const Tensor& grad, const Tensor& x, const T
         if (dx.numel()) {
             const Strided g(grad);
             const Matrices w(weight);
-            oeq_typed_rows a = rows_of(x, g, index, count, outer, inner);
+            oeq_typed_rows a = rows_of(x, g, index.types, count, outer, inner);
             set_matrices(a, w, w.inner_first);
             set_thin(a, v, down, 2, 1);
+            index.set(a);
             check(oeq_typed_product(&a, dx.data_ptr(), dev.stream), "oeq_typed_product");
         }
     }
-    if (want_down) ddown = typed_sum(v, x, 1, rank, inner, x, index, count, dev.stream);
-    if (want_up) dup = typed_sum(grad, u, 2, outer, rank, x, index, count, dev.stream);
+    if (want_down) ddown = typed_sum(v, x, 1, rank, inner, x, index, dev.stream);
+    if (want_up) dup = typed_sum(grad, u, 2, outer, rank, x, index, dev.stream);
     if (want_weight) {
         const Tensor one = at::zeros({x.size(0)}, types.options());  // (all rows are of one type)
-        dw = typed_sum(grad, x, 0, outer, inner, x, groups_of(one, 1, {}, {}), 1, dev.stream).squeeze(0);
+        Groups all(one, 1, {}, {});
+        dw = typed_sum(grad, x, 0, outer, inner, x, all, dev.stream).squeeze(0);
     }
     return {dx, dw, ddown, dup};
 }

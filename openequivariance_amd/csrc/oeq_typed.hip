@@ -101,8 +101,9 @@ int check_rows(const char* who, const oeq_typed_rows* a, bool thin_result) {
         if (s < 0) return fail(OEQ_ERR_INVALID, "%s: a stride of %lld elements", who, (long long)s);
     if (a->bias && a->shared) return fail(OEQ_ERR_INVALID, "%s: a bias beside shared weights", who);
     if (a->rows == 0 || a->outer == 0) return OEQ_OK;
-    if ((a->inner && (!a->x || ((a->types || a->shared) && !a->w))) || !a->order || !a->ptr)
+    if ((a->inner && (!a->x || ((a->types || a->shared) && !a->w))) || !a->type_of_row)
         return fail(OEQ_ERR_INVALID, "%s: NULL buffer", who);
+    if (oeq_typed_needs_index(a) && (!a->order || !a->ptr)) return fail(OEQ_ERR_INVALID, "%s: NULL buffer", who);
     if (a->rank && a->types && (!a->thin || !a->up)) return fail(OEQ_ERR_INVALID, "%s: NULL buffer", who);
     const int bytes = element_bytes(a->type);
     if (!aligned(a->x, bytes) || !aligned(a->w, bytes) || !aligned(a->bias, bytes) || !aligned(a->up, bytes) || !aligned(a->thin))
@@ -113,7 +114,7 @@ int check_rows(const char* who, const oeq_typed_rows* a, bool thin_result) {
 typed_products::Args rows_args(const oeq_typed_rows& a) {
     typed_products::Args g = {};
     g.x = a.x, g.w = a.w, g.bias = a.bias, g.up = a.up, g.thin = a.rank ? a.thin : nullptr;
-    g.order = a.order, g.ptr = a.ptr;
+    g.order = a.order, g.ptr = a.ptr, g.type_of_row = a.type_of_row;
     g.x_row = a.x_row_stride, g.x_part = a.x_part_stride, g.w_type = a.shared ? 0 : a.w_type_stride, g.w_row = a.w_row_stride;
     g.bias_type = a.outer, g.out_row = a.outer;
     g.up_type = a.up_type_stride, g.up_col = a.up_outer_stride, g.up_rank = a.up_rank_stride;
@@ -256,6 +257,13 @@ int oeq_type_sum(int type, int64_t rows, int64_t parts, int64_t types, int64_t c
         case OEQ_FLOAT16: return vec ? launch_sum<_Float16, 8>(g, s) : launch_sum<_Float16, 1>(g, s);
         default: return vec ? launch_sum<__bf16, 8>(g, s) : launch_sum<__bf16, 1>(g, s);
     }
+}
+
+int oeq_typed_needs_index(const oeq_typed_rows* a) {
+    if (!a || a->rows <= 0 || a->parts < 1 || a->rows > kMostRows / a->parts) return 1;
+    typed_products::Args g = {};
+    g.rows = (int)a->rows, g.parts = (int)a->parts, g.shared = a->shared;
+    return !typed_products::few(g, a->across != 0);
 }
 
 int oeq_typed_product(const oeq_typed_rows* a, void* out, void* stream) {

@@ -28,6 +28,7 @@ struct Args {
     const float *thin, *scale;  // thin: [rows, thin_row]; scale: of each type
     void* out;                  // [rows, parts, out_row]
     const int *order, *ptr;
+    const int64_t* type_of_row;
     int64_t x_row, x_part, w_type, w_row, bias_type, up_type, up_col, up_rank, out_row;
     int rows, types, parts, inner, outer, rank, thin_row;
     int slots, tiles;  // of rows, of columns
@@ -424,6 +425,147 @@ __global__ __launch_bounds__(64 * WM * WN) void row_products(Args g) {
 }
 
 // ---------------------------------------------------------------------------
+// products of few rows
+// ---------------------------------------------------------------------------
+
+// Up to 64 rows, as in serving, where each matrix that has a row is read once and nothing else takes time: bound by memory.
+// A block has 16 columns and the rows of one type (of all types, where w is shared); its waves share the summation in turns of
+// 128 bytes of a row, straight from memory to registers, and are added up through LDS. No index: a wave holds the types of 64
+// rows in its lanes, and the block of the first row of a type takes all of them.
+template <typename T>
+struct Few;  // products on the 16x16 matrix instructions: lane l has row l % 16, register r column 4 (l / 16) + r
+template <>
+struct Few<float> {
+    static __device__ __forceinline__ float4_t mma(float4_t a, float4_t b, float4_t c) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a[j], b[j], c, 0, 0, 0);
+        return c;
+    }
+};
+template <>
+struct Few<_Float16> {
+    static __device__ __forceinline__ float4_t mma(half8_t a, half8_t b, float4_t c) {
+        return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
+    }
+};
+template <>
+struct Few<__bf16> {
+    static __device__ __forceinline__ float4_t mma(bf8_t a, bf8_t b, float4_t c) {
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+    }
+};
+
+constexpr int kFewRows = 64, kFewWaves = 8;
+
+// MT: tiles of 16 rows. blockIdx.x: columns; blockIdx.y: rows, of which the first of a type stands for all; with shared
+// weights: every 16 MT rows.
+template <typename T, typename O, bool DIRECT, int MT>
+__global__ __launch_bounds__(64 * kFewWaves) void few_products(Args g) {
+    constexpr int E = 16 / (int)sizeof(T), BK = 128 / (int)sizeof(T), AHEAD = MT <= 2 ? 4 : 2;
+    typedef typename Types<T>::frag frag;
+    __shared__ int members[kFewRows];
+    __shared__ float sums[kFewWaves][16 * MT][17];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int n0 = blockIdx.x * 16, total = g.rows * g.parts;
+    int type = g.types, count;
+    if (g.shared) {
+        const int first = blockIdx.y * 16 * MT;
+        count = min(16 * MT, total - first);
+        if (tid < count) members[tid] = first + tid;
+    } else {
+        const auto type_of = [&](int at) {
+            const int64_t t = g.type_of_row[g.parts == 1 ? at : at / g.parts];
+            return t >= 0 && t < g.types ? (int)t : g.types;
+        };
+        const int mine = lane < total ? type_of(lane) : -1;
+        type = __builtin_amdgcn_readlane(mine, blockIdx.y);
+        const uint64_t same = __ballot(mine == type);
+        if (__builtin_ctzll(same) != (int)blockIdx.y) return;
+        count = __popcll(same);
+        if (wave == 0 && mine == type) members[__popcll(same & ((1ull << lane) - 1))] = lane;
+    }
+    __syncthreads();
+    const bool typed = type < g.types;
+    const int tiles = (count + 15) / 16;
+
+    const T* w = (const T*)g.w + (typed ? type : 0) * g.w_type + min(n0 + (lane & 15), g.outer - 1) * g.w_row + 2 * E * (lane >> 4);
+    const T* x[MT];
+#pragma unroll
+    for (int m = 0; m < MT; ++m) {
+        const int at = members[min(16 * m + (lane & 15), count - 1)];
+        const int row = g.parts == 1 ? at : at / g.parts;
+        x[m] = (const T*)g.x + row * g.x_row + (at - row * g.parts) * g.x_part + 2 * E * (lane >> 4);
+    }
+    // 16 bytes from element k of a row on
+    const auto load = [&](const T* row, int k) -> frag {
+        if constexpr (DIRECT) {
+            return *(const frag*)(k + 2 * E * (lane >> 4) < g.inner ? row + k : (const T*)&kZeros);
+        } else {
+            union {
+                uint4_t v;
+                frag f;
+            } u;
+            u.v = fetch<T>((const char*)(row + k), g.inner - k - 2 * E * (lane >> 4));
+            return u.f;
+        }
+    };
+    float4_t acc[MT];
+#pragma unroll
+    for (int m = 0; m < MT; ++m) acc[m] = 0.0f;
+    const int steps = typed || g.shared ? (g.inner + BK - 1) / BK : 0;
+    for (int s0 = wave; s0 < steps; s0 += AHEAD * kFewWaves) {
+        frag a[AHEAD][2], b[AHEAD][MT][2];
+#pragma unroll
+        for (int u = 0; u < AHEAD; ++u) {
+            const int k = (s0 + u * kFewWaves) * BK;
+            if (s0 + u * kFewWaves < steps) {
+#pragma unroll
+                for (int h = 0; h < 2; ++h) a[u][h] = load(w, k + h * E);
+#pragma unroll
+                for (int m = 0; m < MT; ++m)
+                    if (m < tiles)
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) b[u][m][h] = load(x[m], k + h * E);
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < AHEAD; ++u)
+            if (s0 + u * kFewWaves < steps)
+#pragma unroll
+                for (int m = 0; m < MT; ++m)
+                    if (m < tiles)
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) acc[m] = Few<T>::mma(a[u][h], b[u][m][h], acc[m]);
+    }
+#pragma unroll
+    for (int m = 0; m < MT; ++m)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) sums[wave][16 * m + (lane & 15)][4 * (lane >> 4) + r] = acc[m][r];
+    __syncthreads();
+    const float by = g.scale ? (typed ? g.scale[type] : 0.0f) : 1.0f;
+    for (int i = tid; i < 16 * count; i += 64 * kFewWaves) {
+        const int r = i / 16, col = n0 + i % 16;
+        if (col >= g.out_row) continue;
+        float sum = 0;
+#pragma unroll
+        for (int v = 0; v < kFewWaves; ++v) sum += sums[v][r][i % 16];
+        sum *= by;
+        const int at = members[r];
+        if (col >= g.outer) sum = 0;
+        else if (g.bias && typed) sum += (float)((const T*)g.bias)[type * g.bias_type + col];
+        else if (g.thin) {
+            const int64_t t = g.type_of_row[at];
+            if (t >= 0 && t < g.types) {
+                const float* u = g.thin + (int64_t)at * g.thin_row;
+                const T* v = (const T*)g.up + t * g.up_type + col * g.up_col;
+                for (int k = 0; k < g.rank; ++k) sum += u[k] * (float)v[k * g.up_rank];
+            }
+        }
+        ((O*)g.out)[(int64_t)at * g.out_row + col] = (O)sum;
+    }
+}
+
+// ---------------------------------------------------------------------------
 // sums of products over rows
 // ---------------------------------------------------------------------------
 
@@ -457,14 +599,26 @@ __global__ __launch_bounds__(64 * WM * WN) void sum_products(SumArgs g) {
     if (rows.lo >= rows.hi && !(whole && rows.type + begin / g.chunk == slot)) return;
     const int end = min(rows.hi, rows.hi - rows.lo > g.chunk ? rows.lo + g.chunk : rows.hi);
     const int steps = (end - rows.lo + BK - 1) / BK;
+    const auto row_at = [&](int at) { return g.order[g.parts == 1 ? at : at / g.parts]; };
+    const auto inside = [&](int row) { return (unsigned)row < (unsigned)g.rows ? row : 0; };  // (an index not made here)
+    const auto part_of = [&](int at) { return g.parts == 1 ? 0 : min(at, end - 1) % g.parts; };
 
     uint4_t a_reg[DIRECT ? 1 : TA::kEach], b_reg[DIRECT ? 1 : TB::kEach];
+    // The rows of a step are looked up one step ahead: their numbers have come when the step before has its operands.
+    constexpr bool SAME = TA::kRowsPer == TB::kRowsPer && TA::kEach == TB::kEach;
+    int a_row[TA::kEach], b_row[SAME ? 1 : TB::kEach];
+    auto look_up = [&](int k) {
+#pragma unroll
+        for (int i = 0; i < TA::kEach; ++i) a_row[i] = row_at(min(rows.lo + k * BK + TA::row(i, wave, lane), end - 1));
+        if constexpr (!SAME)
+#pragma unroll
+            for (int i = 0; i < TB::kEach; ++i) b_row[i] = row_at(min(rows.lo + k * BK + TB::row(i, wave, lane), end - 1));
+    };
     auto request = [&](char* at, char* bt, int k) {
 #pragma unroll
         for (int i = 0; i < TA::kEach; ++i) {
             const int j = rows.lo + k * BK + TA::row(i, wave, lane), c = m0 + TA::chunk(i, wave, lane) * EA;
-            const Place p(g.order, min(j, end - 1), g.parts, g.rows);
-            const char* from = (const char*)((const A*)g.a + p.row * g.a_row + p.part * g.a_part + (c < g.a_columns ? c : 0));
+            const char* from = (const char*)((const A*)g.a + inside(a_row[i]) * g.a_row + part_of(j) * g.a_part + (c < g.a_columns ? c : 0));
             if constexpr (DIRECT)
                 TA::request(at, j < end ? from : (const char*)&kZeros, i, wave);
             else
@@ -473,8 +627,8 @@ __global__ __launch_bounds__(64 * WM * WN) void sum_products(SumArgs g) {
 #pragma unroll
         for (int i = 0; i < TB::kEach; ++i) {
             const int j = rows.lo + k * BK + TB::row(i, wave, lane), c = n0 + TB::chunk(i, wave, lane) * EB;
-            const Place p(g.order, min(j, end - 1), g.parts, g.rows);
-            const char* from = (const char*)((const B*)g.b + p.row * g.b_row + p.part * g.b_part + (c < g.b_columns ? c : 0));
+            const int row = inside(SAME ? a_row[i] : b_row[i]);
+            const char* from = (const char*)((const B*)g.b + row * g.b_row + part_of(j) * g.b_part + (c < g.b_columns ? c : 0));
             if constexpr (DIRECT)
                 TB::request(bt, j < end ? from : (const char*)&kZeros, i, wave);
             else
@@ -544,11 +698,14 @@ __global__ __launch_bounds__(64 * WM * WN) void sum_products(SumArgs g) {
     auto step = [&](char* at, char* bt, char* an, char* bn, int k) {
         arrived();
         if (k + 1 < steps) request(an, bn, k + 1);
+        if (k + 2 < steps) look_up(k + 2);
         products(at, bt);
         if (k + 1 < steps) put(an, bn);
     };
     if (steps > 0) {
+        look_up(0);
         request(a0, b0, 0);
+        if (steps > 1) look_up(1);
         put(a0, b0);
     }
     for (int k = 0; k < steps; k += 2) {

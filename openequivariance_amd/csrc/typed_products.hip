@@ -22,8 +22,20 @@ hipError_t rows_by(Args a, hipStream_t stream) {
     return hipGetLastError();
 }
 
+template <typename O, bool DIRECT, int MT>
+hipError_t few_by(const Args& a, hipStream_t stream) {
+    const int64_t rows = (int64_t)a.rows * a.parts;
+    few_products<T, O, DIRECT, MT><<<dim3((unsigned)divide_up(a.out_row, 16), (unsigned)(a.shared ? divide_up(rows, 16 * MT) : rows)),
+                                     64 * kFewWaves, 0, stream>>>(a);
+    return hipGetLastError();
+}
+
 template <typename O, bool ACROSS, bool DIRECT>
 hipError_t rows_of_size(const Args& a, hipStream_t stream) {
+    if constexpr (!ACROSS) {
+        const int64_t rows = (int64_t)a.rows * a.parts;
+        if (few(a, false)) return rows <= 16 ? few_by<O, DIRECT, 1>(a, stream) : rows <= 32 ? few_by<O, DIRECT, 2>(a, stream) : few_by<O, DIRECT, 4>(a, stream);
+    }
     if (a.out_row <= 64) return rows_by<O, ACROSS, DIRECT, 64, 64, 2, 2>(a, stream);
     return rows_by<O, ACROSS, DIRECT, 128, 128, 2, 2>(a, stream);
 }

@@ -6,6 +6,9 @@
 
 namespace typed_products {
 
+// Whether the form for few rows, which needs no index, takes a product.
+inline bool few(const Args& a, bool across) { return !across && (int64_t)a.rows * a.parts <= (a.shared ? 4 * kFewRows : kFewRows); }
+
 enum Thin { kNeither, kFirst, kSecond };  // which operand of a sum of products is float beside elements of 16 bits
 
 template <typename T>

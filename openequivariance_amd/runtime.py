@@ -135,7 +135,7 @@ class _TypedRows(ctypes.Structure):
                 + [(n, ctypes.c_int64) for n in ("rows", "parts", "types", "inner", "outer", "x_row_stride", "x_part_stride",
                                                  "w_type_stride", "w_row_stride", "up_type_stride", "up_outer_stride",
                                                  "up_rank_stride")]
-                + [(n, ctypes.c_void_p) for n in ("x", "w", "bias", "thin", "up", "order", "ptr")])
+                + [(n, ctypes.c_void_p) for n in ("x", "w", "bias", "thin", "up", "type_of_row", "order", "ptr")])
 
 
 class _TypedSum(ctypes.Structure):
@@ -266,6 +266,7 @@ EXPORTS = {
     "oeq_type_sum_workspace_bytes": (_SZ, [_I64, _I64, _I64]),
     "oeq_type_sum": (ctypes.c_int, [ctypes.c_int, _I64, _I64, _I64, _I64, _P, _P, _P, _P, _I64, _I64, ctypes.c_double, _P, _P,
                                     _SZ, _P]),
+    "oeq_typed_needs_index": (ctypes.c_int, [ctypes.POINTER(_TypedRows)]),
     "oeq_typed_product": (ctypes.c_int, [ctypes.POINTER(_TypedRows), _P, _P]),
     "oeq_thin_stride": (_I64, [_I64]),
     "oeq_typed_thin_product": (ctypes.c_int, [ctypes.POINTER(_TypedRows), _P, _P, _P]),

@@ -103,8 +103,8 @@ def test_c_abi_refuses_products():
     lib = rt.load_library()
 
     def rows(**changes):
-        fields = dict(type=2, across=0, shared=0, rank=0, rows=10, parts=1, types=3, inner=32, outer=16, x_row_stride=32, w_type_stride=512,
-                      w_row_stride=32, x=16, w=16, order=16, ptr=16)
+        fields = dict(type=2, across=0, shared=0, rank=0, rows=1000, parts=1, types=3, inner=32, outer=16, x_row_stride=32, w_type_stride=512,
+                      w_row_stride=32, x=16, w=16, type_of_row=16, order=16, ptr=16)
         fields.update(changes)
         return ctypes.byref(rt._TypedRows(**fields))
 
@@ -113,7 +113,7 @@ def test_c_abi_refuses_products():
     for changes, text in ((dict(type=3), "element type"), (dict(rows=-1), "rows"), (dict(rows=1 << 28, parts=4), "rows"), (dict(parts=0), "parts"),
                           (dict(types=-1), "types"), (dict(inner=-1), "inner"), (dict(outer=1 << 31), "outer"), (dict(rank=-1), "rank"),
                           (dict(rank=4, parts=2), "rank"), (dict(rank=4), "NULL"), (dict(x_row_stride=-1), "stride of -1"), (dict(x=0), "NULL"),
-                          (dict(w=0), "NULL"), (dict(order=0), "NULL"), (dict(ptr=0), "NULL"), (dict(shared=1, bias=16), "bias"),
+                          (dict(w=0), "NULL"), (dict(type_of_row=0), "NULL"), (dict(rows=9, type_of_row=0), "NULL"), (dict(order=0), "NULL"), (dict(ptr=0), "NULL"), (dict(shared=1, bias=16), "bias"),
                           (dict(x=17), "unaligned"), (dict(rows=1 << 28, outer=1 << 20), "too many")):
         refused(lib.oeq_typed_product(rows(**changes), 16, None), text)
     refused(lib.oeq_typed_product(rows(), None, None), "NULL")
@@ -121,6 +121,8 @@ def test_c_abi_refuses_products():
     for changes, text in ((dict(parts=2), "parts"), (dict(shared=1), "shared"), (dict(bias=16), "bias"), (dict(rank=3, thin=16, up=16), "rank")):
         refused(lib.oeq_typed_thin_product(rows(**changes), 16, 16, None), text)
     refused(lib.oeq_typed_thin_product(rows(), 16, None, None), "NULL")
+    assert lib.oeq_typed_needs_index(rows()) and not lib.oeq_typed_needs_index(rows(rows=9))
+    assert lib.oeq_typed_needs_index(rows(rows=9, across=1))
     assert [lib.oeq_thin_stride(r) for r in (0, 1, 8, 9)] == [0, 8, 8, 16]
 
 
