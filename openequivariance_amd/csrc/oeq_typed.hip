@@ -49,7 +49,7 @@ int passes_of(int64_t types) {
 
 // Rows of a block in a pass.
 int span_of(int64_t rows) {
-    const int64_t least = 2 * row_groups::kThreads, even = divide_up(rows, row_groups::kMostBlocks);
+    const int64_t least = row_groups::kThreads, even = divide_up(rows, row_groups::kMostBlocks);
     return (int)std::max(least, divide_up(even, row_groups::kThreads) * row_groups::kThreads);
 }
 
@@ -77,12 +77,15 @@ int launch_lookup(int64_t rows, int64_t types, int64_t channels, const int64_t* 
 
 template <typename T, int V>
 int launch_sum(const row_groups::Sums& g, hipStream_t s) {
-    const int across = lanes_across(g.channels / V);
-    const unsigned chunks = (unsigned)divide_up(g.n, row_groups::kChunk), wide = (unsigned)divide_up(g.channels / V, across);
-    row_groups::sum_types<T, V><<<dim3(g.count + chunks, wide), 256, 0, s>>>(g, across);
+    const int64_t vectors = g.channels / V;
+    const int across = lanes_across(vectors);
+    const unsigned chunks = g.n > row_groups::kChunk ? (unsigned)divide_up(g.n, row_groups::kChunk) : 0;
+    const unsigned blocks = (unsigned)divide_up(g.count, 256 / across * row_groups::kTypes);
+    row_groups::sum_types<T, V><<<dim3(blocks + chunks, (unsigned)divide_up(vectors, across)), 256, 0, s>>>(g, across, (int)blocks);
     HIP_TRY(hipGetLastError());
-    if (g.n > row_groups::kChunk) {
-        row_groups::join_chunks<T, V><<<dim3(chunks, wide), 256, 0, s>>>(g, across);
+    if (chunks) {
+        const int few = std::min(across, 16);
+        row_groups::join_chunks<T, V><<<dim3(chunks, (unsigned)divide_up(vectors, few)), 256, 0, s>>>(g, few);
         HIP_TRY(hipGetLastError());
     }
     return OEQ_OK;
@@ -140,16 +143,30 @@ int launch_rows(const char* who, const oeq_typed_rows& a, const typed_products::
     return OEQ_OK;
 }
 
-// Rows that a block sums up: all of a type's where the types' tiles fill the card, else shares whose partial sums pass
-// through memory.
-int64_t chunk_of(const oeq_typed_sum& a) {
-    using namespace typed_products;
-    constexpr int64_t kBlocks = 1024, kLeast = 256;
-    const int64_t tiles = divide_up(a.a_columns, a.thin == 1 ? kThinTile : kSumTile) *
-                          divide_up(a.b_columns, a.thin == 2 ? kThinTile : kSumTile);
-    const int64_t rows = a.rows * a.parts;
-    if (a.types * tiles >= kBlocks) return std::max<int64_t>(rows, 1);
-    return std::max(kLeast, divide_up(rows * tiles, kBlocks * 64) * 64);
+// How a sum over rows is cut: columns of a tile, and the rows that a block sums up, which are all of a type's where the tiles
+// of all types fill the card, else shares whose partial sums pass through memory.
+struct Cut {
+    int tile;
+    int64_t chunk;
+    Cut(const oeq_typed_sum& a, bool direct) {
+        using namespace typed_products;
+        constexpr int64_t kBlocks = 1024, kLeast = 256;
+        const auto tiles = [&](int to) {
+            return divide_up(a.a_columns, a.thin == 1 ? kThinTile : to) * divide_up(a.b_columns, a.thin == 2 ? kThinTile : to);
+        };
+        const int64_t rows = a.rows * a.parts;
+        // (through registers small tiles only, whose loads on their way fit beside the sums)
+        tile = a.thin || (direct && (a.types * tiles(kSumTile) >= kBlocks || rows / kLeast * tiles(kSumTile) >= kBlocks)) ? kSumTile
+                                                                                                                     : kSmallSumTile;
+        chunk = a.types * tiles(tile) >= kBlocks ? std::max<int64_t>(rows, 1)
+                                                 : std::max(kLeast, divide_up(rows * tiles(tile), kBlocks * 64) * 64);
+    }
+};
+
+bool direct_sum(const oeq_typed_sum& a) {
+    const int a_bytes = a.thin == 1 ? 4 : element_bytes(a.type), b_bytes = a.thin == 2 ? 4 : element_bytes(a.type);
+    return aligned(a.a, a_bytes, {a.a_row_stride, a.a_part_stride, a.a_columns}) &&
+           aligned(a.b, b_bytes, {a.b_row_stride, a.b_part_stride, a.b_columns});
 }
 
 }  // namespace
@@ -238,7 +255,7 @@ int oeq_type_sum(int type, int64_t rows, int64_t parts, int64_t types, int64_t c
     if (int rc = check_index(who, rows, parts, types)) return rc;
     if (types + divide_up(rows, row_groups::kChunk) > kMostBlocks)
         return fail(OEQ_ERR_INVALID, "%s: %lld rows of %lld types are too many for a launch", who, (long long)rows, (long long)types);
-    if (channels < 0 || channels > (1 << 23) || row_stride < 0 || part_stride < 0)
+    if (channels < 0 || channels > (1 << 19) || row_stride < 0 || part_stride < 0)
         return fail(OEQ_ERR_INVALID, "%s: %lld channels, strides of %lld and %lld elements", who, (long long)channels,
                     (long long)row_stride, (long long)part_stride);
     if (types == 0 || channels == 0) return OEQ_OK;
@@ -292,8 +309,8 @@ int oeq_typed_thin_product(const oeq_typed_rows* a, const float* scale, float* o
 }
 
 size_t oeq_typed_sum_workspace_bytes(const oeq_typed_sum* a) {
-    if (!a || a->rows <= 0 || a->parts < 1 || a->types <= 0 || a->a_columns <= 0 || a->b_columns <= 0) return 0;
-    const int64_t chunk = chunk_of(*a), rows = a->rows * a->parts;
+    if (!a || !element_bytes(a->type) || a->rows <= 0 || a->parts < 1 || a->types <= 0 || a->a_columns <= 0 || a->b_columns <= 0) return 0;
+    const int64_t chunk = Cut(*a, direct_sum(*a)).chunk, rows = a->rows * a->parts;
     return chunk >= rows ? 0 : (size_t)(rows / chunk + a->types) * a->a_columns * a->b_columns * sizeof(float);
 }
 
@@ -321,10 +338,10 @@ int oeq_typed_sum_products(const oeq_typed_sum* a, void* out, void* workspace, s
     g.rows = (int)a->rows, g.types = (int)a->types, g.parts = (int)a->parts;
     g.a_columns = (int)a->a_columns, g.b_columns = (int)a->b_columns;
     const int64_t rows = a->rows * a->parts;
-    g.chunk = (int)chunk_of(*a);
+    const bool direct = direct_sum(*a);
+    const Cut cut(*a, direct);
+    g.tile = cut.tile, g.chunk = (int)cut.chunk;
     g.slots = (int)(rows / g.chunk + a->types);
-    const bool direct = aligned(a->a, a_bytes, {a->a_row_stride, a->a_part_stride, a->a_columns}) &&
-                        aligned(a->b, b_bytes, {a->b_row_stride, a->b_part_stride, a->b_columns});
     const auto thin = (typed_products::Thin)a->thin;
     const auto s = (hipStream_t)stream;
     const hipError_t status = a->type == OEQ_FLOAT32 ? typed_products::Launch<float>::sums(g, thin, direct, s)

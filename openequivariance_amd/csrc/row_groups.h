@@ -324,6 +324,14 @@ __device__ __forceinline__ Row<T, V> sum_places(const Sums& s, int lo, int hi, i
     return sum;
 }
 
+template <typename T, int V>
+__device__ __forceinline__ void store_sum(const Sums& s, const Row<T, V>& sum, int t, int c) {
+    typename Row<T, V>::vec y;
+#pragma unroll
+    for (int e = 0; e < V; ++e) y[e] = (T)(sum.x[e] * s.scale);
+    *(typename Row<T, V>::vec*)((T*)s.out + (int64_t)t * s.channels + c) = y;
+}
+
 // Threads of a block: `across` lanes next to each other for the channels (V each), 256 / across groups.
 template <typename T, int V>
 __device__ __forceinline__ void join_groups(Row<T, V>& sum, float* lds, int across, int lane, int group, int groups) {
@@ -339,29 +347,32 @@ __device__ __forceinline__ void join_groups(Row<T, V>& sum, float* lds, int acro
     }
 }
 
-// Blocks 0 .. count - 1: types, the rest: chunks; blockIdx.y: channels.
+// The first blocks have a type for each of their groups of lanes, kTypes of them one after the other; the rest a chunk each.
+// blockIdx.y: channels.
+constexpr int kTypes = 4;
+
 template <typename T, int V>
-__global__ __launch_bounds__(256) void sum_types(Sums s, int across) {
+__global__ __launch_bounds__(256) void sum_types(Sums s, int across, int type_blocks) {
     __shared__ float lds[128 * V];
     const int lane = threadIdx.x % across, group = threadIdx.x / across, groups = 256 / across;
     const int c = (blockIdx.y * across + lane) * V;
     const bool valid = c < s.channels;
-    if ((int)blockIdx.x < s.count) {
-        const int t = blockIdx.x, lo = max(s.ptr[t], 0), hi = min(s.ptr[t + 1], s.n);
-        if (hi - lo > kChunk) return;
-        Row<T, V> sum;
-        sum.clear();
-        if (valid) sum = sum_places<T, V>(s, lo, hi, c, group, groups);
-        if (hi - lo > 1) join_groups(sum, lds, across, lane, group, groups);
-        if (valid && group == 0) {
-            typename Row<T, V>::vec y;
+    if ((int)blockIdx.x < type_blocks) {
+        if (!valid) return;
+        const int t0 = (blockIdx.x * groups + group) * kTypes;
+        int begin[kTypes + 1];
 #pragma unroll
-            for (int e = 0; e < V; ++e) y[e] = (T)(sum.x[e] * s.scale);
-            *(typename Row<T, V>::vec*)((T*)s.out + (int64_t)t * s.channels + c) = y;
+        for (int i = 0; i <= kTypes; ++i) begin[i] = t0 < s.count ? s.ptr[min(t0 + i, s.count)] : 0;
+#pragma unroll
+        for (int i = 0; i < kTypes; ++i) {
+            const int lo = max(begin[i], 0), hi = min(begin[i + 1], s.n);
+            if (t0 + i >= s.count || hi - lo > kChunk) continue;
+            const Row<T, V> sum = sum_places<T, V>(s, lo, hi, c, 0, 1);
+            store_sum(s, sum, t0 + i, c);
         }
         return;
     }
-    const int chunk = blockIdx.x - s.count, first = chunk * kChunk, last = min(s.n, s.ptr[s.count]);
+    const int chunk = blockIdx.x - type_blocks, first = chunk * kChunk, last = min(s.n, s.ptr[s.count]);
     if (first >= last) return;
     const int end = min(first + kChunk, last);
     const int ta = key_of(s.types[row_at(s.order, first, s.n)], s.count), tb = key_of(s.types[row_at(s.order, end - 1, s.n)], s.count);
@@ -380,7 +391,8 @@ __global__ __launch_bounds__(256) void sum_types(Sums s, int across) {
     }
 }
 
-// A block for each chunk: the longer types that begin in it.
+// A block for each chunk: the longer types that begin in it. Few channels a block and many groups, each with a few of the
+// chunks: what a long type waits for is one read after the other.
 template <typename T, int V>
 __global__ __launch_bounds__(256) void join_chunks(Sums s, int across) {
     __shared__ float lds[128 * V];
@@ -401,18 +413,14 @@ __global__ __launch_bounds__(256) void join_chunks(Sums s, int across) {
         sum.clear();
         // the first chunk's part is its end's, unless the type begins with the chunk; all others begin with the type
         if (valid)
+#pragma unroll 4
             for (int k = group; k < chunks; k += groups) {
                 const float* from = s.partial + ((int64_t)(chunk + k) * 2 + (k == 0 ? side : 0)) * s.channels + c;
 #pragma unroll
                 for (int e = 0; e < V; ++e) sum.x[e] += from[e];
             }
         join_groups(sum, lds, across, lane, group, groups);
-        if (valid && group == 0) {
-            typename Row<T, V>::vec y;
-#pragma unroll
-            for (int e = 0; e < V; ++e) y[e] = (T)(sum.x[e] * s.scale);
-            *(typename Row<T, V>::vec*)((T*)s.out + (int64_t)t * s.channels + c) = y;
-        }
+        if (valid && group == 0) store_sum(s, sum, t, c);
     }
 }
 

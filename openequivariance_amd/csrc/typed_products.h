@@ -44,6 +44,7 @@ struct SumArgs {
     int64_t a_row, a_part, b_row, b_part;
     int rows, types, parts, a_columns, b_columns;
     int chunk;  // rows (with their parts) that a block sums up
+    int tile;   // columns of a block
     int slots, a_tiles, b_tiles;
 };
 
@@ -243,7 +244,7 @@ __device__ __forceinline__ void arrived() {
 // A tile of BM rows and BN columns. ACROSS: the weights' rows run along the columns (w[k, n]), else along the summation
 // (w[n, k]). DIRECT: everything is aligned to 16 bytes and goes straight to LDS; else through registers, by elements where a
 // row ends. The result is transposed in registers: lane l has row l % 32, register r column 8 (r / 4) + 4 (l / 32) + r % 4.
-template <typename T, typename O, bool ACROSS, bool DIRECT, int BM, int BN, int WM, int WN>
+template <typename T, typename O, bool ACROSS, bool DIRECT, bool THIN, int BM, int BN, int WM, int WN>
 __global__ __launch_bounds__(64 * WM * WN) void row_products(Args g) {
     constexpr int WAVES = WM * WN, BK = 128 / (int)sizeof(T), E = 16 / (int)sizeof(T);
     constexpr int TM = BM / WM / 32, TN = BN / WN / 32;
@@ -356,10 +357,103 @@ __global__ __launch_bounds__(64 * WM * WN) void row_products(Args g) {
         products(xt, wt);
         if (k + 1 < steps) put(xn, wn_);
     };
-    if (steps) {
-        request(x0, w0, 0);
-        put(x0, w0);
+    if (steps) request(x0, w0, 0);
+    if constexpr (THIN) {
+        // The thin product first, from the other buffer. Its rows are float; as operands beside 16 bits they have two parts, u =
+        // hi + lo, next to each other along the summation: 16 bits of u or more, when what it adds to is rounded to 8 or 11.
+        if (typed && g.rank) {
+            constexpr int PARTS = sizeof(T) == 2 ? 2 : 1;
+            const int width = g.thin_row;
+            float* lift = (float*)w1;  // (done with before w1 is filled)
+            float down[TM];
+            float up_by[X::kEach];
+            if constexpr (std::is_same<T, _Float16>::value) {
+                // A power of two for each row: parts of 11 bits each, whatever the size of u.
+                for (int r = tid; r < BM; r += 64 * WAVES) {
+                    const int at = min(m0 + r, rows.hi - 1);
+                    const float* u = g.thin + (int64_t)Place(g.order, at, 1, g.rows).row * width;
+                    float most = 0;
+                    for (int k = 0; k < width; k += 4) {
+                        const float4_t v = *(const float4_t*)(u + k);
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) most = fmaxf(most, fabsf(v[j]));
+                    }
+                    // most 2^-e is between 1 / 2 and 1; infinities and NaN stay as they are
+                    const int e = most > 0 && most < INFINITY ? __builtin_amdgcn_frexp_expf(most) : 0;
+                    lift[r] = __builtin_amdgcn_ldexpf(1.0f, max(-e, -126) < 127 ? max(-e, -126) : 126);
+                }
+                __syncthreads();
+#pragma unroll
+                for (int m = 0; m < TM; ++m) down[m] = 1.0f / lift[wm + 32 * m + (lane & 31)];
+#pragma unroll
+                for (int i = 0; i < X::kEach; ++i) up_by[i] = lift[X::row(i, wave, lane)];
+                __syncthreads();
+            }
+            const T* up = (const T*)g.up + rows.type * g.up_type;
+            for (int k0 = 0; k0 < PARTS * width; k0 += BK) {
+#pragma unroll
+                for (int i = 0; i < X::kEach; ++i) {
+                    const int at = min(m0 + X::row(i, wave, lane), rows.hi - 1), kk = k0 + X::chunk(i, wave, lane) * E;
+                    const bool low = kk >= width;
+                    union {
+                        uint4_t v;
+                        T e[E];
+                    } y;
+                    y.v = uint4_t{0, 0, 0, 0};
+                    if (kk < PARTS * width) {
+                        const float* u = g.thin + (int64_t)Place(g.order, at, 1, g.rows).row * width + (low ? kk - width : kk);
+#pragma unroll
+                        for (int j = 0; j < E; ++j) {
+                            const float v = std::is_same<T, _Float16>::value ? u[j] * up_by[i] : u[j];
+                            const float hi = (float)(T)v;
+                            y.e[j] = PARTS == 2 && low ? (T)(fabsf(hi) < INFINITY ? v - hi : 0.0f) : (T)v;
+                        }
+                    }
+                    X::put(x1, y.v, i, wave, lane);
+                }
+#pragma unroll
+                for (int i = 0; i < W::kEach; ++i) {
+                    const int r = W::row(i, wave, lane), c = W::chunk(i, wave, lane) * E;
+                    union {
+                        uint4_t v;
+                        T e[E];
+                    } y;
+                    y.v = uint4_t{0, 0, 0, 0};
+                    if constexpr (ACROSS) {
+                        const int k = k0 + r >= width ? k0 + r - width : k0 + r;
+                        const int left = k0 + r < PARTS * width && k < g.rank ? g.outer - n0 - c : 0;
+                        const T* from = up + k * g.up_rank + (n0 + c) * g.up_col;
+                        if (g.up_col == 1)
+                            y.v = fetch<T>((const char*)from, left);
+                        else
+#pragma unroll
+                            for (int j = 0; j < E; ++j)
+                                if (j < left) y.e[j] = from[j * g.up_col];
+                    } else {
+                        const int kk = k0 + c, k = kk >= width ? kk - width : kk;
+                        const int left = kk < PARTS * width ? g.rank - k : 0;
+                        const T* from = up + min(n0 + r, g.outer - 1) * g.up_col + k * g.up_rank;
+                        if (g.up_rank == 1)
+                            y.v = fetch<T>((const char*)from, left);
+                        else
+#pragma unroll
+                            for (int j = 0; j < E; ++j)
+                                if (j < left) y.e[j] = from[j * g.up_rank];
+                    }
+                    W::put(w1, y.v, i, wave, lane);
+                }
+                __syncthreads();
+                products(x1, w1);
+                __syncthreads();
+            }
+            if constexpr (std::is_same<T, _Float16>::value)
+#pragma unroll
+                for (int m = 0; m < TM; ++m)
+#pragma unroll
+                    for (int n = 0; n < TN; ++n) acc[m][n] *= down[m];
+        }
     }
+    if (steps) put(x0, w0);
     for (int k = 0; k < steps; k += 2) {
         step(x0, w0, x1, w1, k);
         if (k + 1 < steps) step(x1, w1, x0, w0, k + 1);
@@ -375,25 +469,6 @@ __global__ __launch_bounds__(64 * WM * WN) void row_products(Args g) {
         mine[m] = at < rows.hi;
         const Place p(g.order, mine[m] ? at : m0, g.parts, g.rows);
         to[m] = ((int64_t)p.row * g.parts + p.part) * g.out_row;
-        if (g.thin && typed) {
-            // the second, thin product: its rows are float, so it is one of floats
-            const float* u = g.thin + (int64_t)p.row * g.thin_row;
-            for (int k = 0; k < g.rank; k += 8) {
-                const float4_t b = *(const float4_t*)(u + k + 4 * half);
-#pragma unroll
-                for (int n = 0; n < TN; ++n) {
-                    const int col = n0 + wn + 32 * n + (lane & 31);
-                    const T* v = (const T*)g.up + rows.type * g.up_type;
-                    float4_t a = 0.0f;
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        const int r = k + 4 * half + j;
-                        if (r < g.rank && col < g.outer) a[j] = (float)v[col * g.up_col + r * g.up_rank];
-                    }
-                    acc[m][n] = mma(a, b, acc[m][n]);
-                }
-            }
-        }
     }
     O* out = (O*)g.out;
     const bool quads = g.out_row % 4 == 0;
@@ -566,6 +641,94 @@ __global__ __launch_bounds__(64 * kFewWaves) void few_products(Args g) {
 }
 
 // ---------------------------------------------------------------------------
+// thin products
+// ---------------------------------------------------------------------------
+
+// Many rows, few columns, a long summation: bound by reading the rows. A block has 32 rows of a type and 16 NT columns; its
+// waves share the summation as those of few_products do, so that nothing passes through LDS but their sums.
+constexpr int kThinRows = 32;
+
+template <typename T, bool DIRECT, int NT>
+__global__ __launch_bounds__(64 * kFewWaves) void thin_products(Args g) {
+    constexpr int E = 16 / (int)sizeof(T), BK = 128 / (int)sizeof(T), MT = kThinRows / 16, AHEAD = 2;
+    typedef typename Types<T>::frag frag;
+    __shared__ float sums[kFewWaves][kThinRows][16 * NT + 1];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const Range rows = rows_of_slot(g.ptr, blockIdx.x, kThinRows, g.types, true, g.rows, 1);
+    if (rows.lo >= rows.hi) return;
+    const int n0 = blockIdx.y * 16 * NT, count = min(kThinRows, rows.hi - rows.lo);
+    const bool typed = rows.type < g.types;
+    const int begin = 2 * E * (lane >> 4);
+    const T *x[MT], *w[NT];
+#pragma unroll
+    for (int m = 0; m < MT; ++m)
+        x[m] = (const T*)g.x + Place(g.order, rows.lo + min(16 * m + (lane & 15), count - 1), 1, g.rows).row * g.x_row + begin;
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+        w[n] = (const T*)g.w + (typed ? rows.type : 0) * g.w_type + min(n0 + 16 * n + (lane & 15), g.outer - 1) * g.w_row + begin;
+    const auto load = [&](const T* row, int k) -> frag {
+        if constexpr (DIRECT) {
+            return *(const frag*)(k + begin < g.inner ? row + k : (const T*)&kZeros);
+        } else {
+            union {
+                uint4_t v;
+                frag f;
+            } u;
+            u.v = fetch<T>((const char*)(row + k), g.inner - k - begin);
+            return u.f;
+        }
+    };
+    float4_t acc[MT][NT];
+#pragma unroll
+    for (int m = 0; m < MT; ++m)
+#pragma unroll
+        for (int n = 0; n < NT; ++n) acc[m][n] = 0.0f;
+    const int steps = typed ? (g.inner + BK - 1) / BK : 0;
+    for (int s0 = wave; s0 < steps; s0 += AHEAD * kFewWaves) {
+        frag a[AHEAD][NT][2], b[AHEAD][MT][2];
+#pragma unroll
+        for (int u = 0; u < AHEAD; ++u)
+            if (s0 + u * kFewWaves < steps) {
+                const int k = (s0 + u * kFewWaves) * BK;
+#pragma unroll
+                for (int m = 0; m < MT; ++m)
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) b[u][m][h] = load(x[m], k + h * E);
+#pragma unroll
+                for (int n = 0; n < NT; ++n)
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) a[u][n][h] = load(w[n], k + h * E);
+            }
+#pragma unroll
+        for (int u = 0; u < AHEAD; ++u)
+            if (s0 + u * kFewWaves < steps)
+#pragma unroll
+                for (int m = 0; m < MT; ++m)
+#pragma unroll
+                    for (int n = 0; n < NT; ++n)
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) acc[m][n] = Few<T>::mma(a[u][n][h], b[u][m][h], acc[m][n]);
+    }
+#pragma unroll
+    for (int m = 0; m < MT; ++m)
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) sums[wave][16 * m + (lane & 15)][16 * n + 4 * (lane >> 4) + r] = acc[m][n][r];
+    __syncthreads();
+    const float by = typed ? (g.scale ? g.scale[rows.type] : 1.0f) : 0.0f;
+    for (int i = tid; i < 16 * NT * count; i += 64 * kFewWaves) {
+        const int r = i / (16 * NT), c = i % (16 * NT);
+        if (n0 + c >= g.out_row) continue;
+        float sum = 0;
+#pragma unroll
+        for (int v = 0; v < kFewWaves; ++v) sum += sums[v][r][c];
+        const int row = Place(g.order, rows.lo + r, 1, g.rows).row;
+        ((float*)g.out)[(int64_t)row * g.out_row + n0 + c] = n0 + c < g.outer ? sum * by : 0.0f;
+    }
+}
+
+// ---------------------------------------------------------------------------
 // sums of products over rows
 // ---------------------------------------------------------------------------
 
@@ -733,19 +896,32 @@ __global__ __launch_bounds__(64 * WM * WN) void sum_products(SumArgs g) {
             }
 }
 
-// The slots of a type in order, where it has more than one.
-template <typename O>
+// The slots of a type, where it has more than one: 16 lanes with V columns each, and 16 groups with every sixteenth slot.
+template <typename O, int V>
 __global__ __launch_bounds__(256) void join_slots(SumArgs g) {
-    const int t = blockIdx.y;
+    typedef float vec __attribute__((ext_vector_type(V)));
+    typedef O result __attribute__((ext_vector_type(V)));
+    __shared__ vec lds[16][16];
+    const int t = blockIdx.y, lane = threadIdx.x & 15, group = threadIdx.x >> 4;
     const int begin = begin_of(g.ptr, t, g.rows, g.parts), n = begin_of(g.ptr, t + 1, g.rows, g.parts) - begin;
     if (n <= g.chunk) return;
     const int64_t size = (int64_t)g.a_columns * g.b_columns;
     const float* from = g.partial + ((int64_t)begin / g.chunk + t) * size;
     const int slots = (n - 1) / g.chunk + 1;
-    for (int64_t i = blockIdx.x * 256ll + threadIdx.x; i < size; i += gridDim.x * 256ll) {
-        float sum = 0;
-        for (int s = 0; s < slots; ++s) sum += from[s * size + i];
-        ((O*)g.out)[t * size + i] = (O)sum;
+    for (int64_t block = blockIdx.x; block * 16 * V < size; block += gridDim.x) {
+        const int64_t i = (block * 16 + lane) * V;
+        vec sum = 0.0f;
+        if (i < size)
+#pragma unroll 4
+            for (int s = group; s < slots; s += 16) sum += *(const vec*)(from + s * size + i);
+        lds[group][lane] = sum;
+        __syncthreads();
+        if (group == 0 && i < size) {
+            sum = lds[0][lane];
+            for (int k = 1; k < min(slots, 16); ++k) sum += lds[k][lane];
+            *(result*)((O*)g.out + t * size + i) = __builtin_convertvector(sum, result);
+        }
+        __syncthreads();
     }
 }
 

@@ -12,13 +12,13 @@ typedef OEQ_PRODUCT_TYPE T;
 
 int64_t divide_up(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
-template <typename O, bool ACROSS, bool DIRECT, int BM, int BN, int WM, int WN>
+template <typename O, bool ACROSS, bool DIRECT, bool THIN, int BM, int BN, int WM, int WN>
 hipError_t rows_by(Args a, hipStream_t stream) {
     a.slots = (int)((int64_t)a.rows * a.parts / BM + a.types + 1);
     a.tiles = (int)divide_up(a.out_row, BN);
     const int64_t blocks = (int64_t)a.slots * a.tiles;
     if (blocks > (1 << 24) - 1) return hipErrorInvalidConfiguration;
-    row_products<T, O, ACROSS, DIRECT, BM, BN, WM, WN><<<(unsigned)blocks, 64 * WM * WN, 0, stream>>>(a);
+    row_products<T, O, ACROSS, DIRECT, THIN, BM, BN, WM, WN><<<(unsigned)blocks, 64 * WM * WN, 0, stream>>>(a);
     return hipGetLastError();
 }
 
@@ -30,14 +30,42 @@ hipError_t few_by(const Args& a, hipStream_t stream) {
     return hipGetLastError();
 }
 
+template <bool DIRECT, int NT>
+hipError_t thin_by(const Args& a, hipStream_t stream) {
+    const int64_t slots = a.rows / kThinRows + a.types + 1, tiles = divide_up(a.out_row, 16 * NT);
+    if (slots > (1 << 23) - 1 || tiles > 65535) return hipErrorInvalidConfiguration;
+    thin_products<T, DIRECT, NT><<<dim3((unsigned)slots, (unsigned)tiles), 64 * kFewWaves, 0, stream>>>(a);
+    return hipGetLastError();
+}
+
 template <typename O, bool ACROSS, bool DIRECT>
-hipError_t rows_of_size(const Args& a, hipStream_t stream) {
+hipError_t rows_of_size(const Args& a, bool thin_result, hipStream_t stream) {
     if constexpr (!ACROSS) {
         const int64_t rows = (int64_t)a.rows * a.parts;
         if (few(a, false)) return rows <= 16 ? few_by<O, DIRECT, 1>(a, stream) : rows <= 32 ? few_by<O, DIRECT, 2>(a, stream) : few_by<O, DIRECT, 4>(a, stream);
     }
-    if (a.out_row <= 64) return rows_by<O, ACROSS, DIRECT, 64, 64, 2, 2>(a, stream);
-    return rows_by<O, ACROSS, DIRECT, 128, 128, 2, 2>(a, stream);
+    if constexpr (std::is_same<O, float>::value && !ACROSS)
+        if (thin_result) return a.outer <= 16 ? thin_by<DIRECT, 1>(a, stream) : a.outer <= 32 ? thin_by<DIRECT, 2>(a, stream) : thin_by<DIRECT, 4>(a, stream);
+    // Tiles by how many blocks there are, with half a tile of each type's rows left over.
+    const auto blocks = [&](int64_t bm, int64_t bn) {
+        const int64_t rows = (int64_t)a.rows * a.parts;
+        return (rows / bm + std::min<int64_t>(a.types, rows) / 2 + 1) * divide_up(a.out_row, bn);
+    };
+    constexpr bool MAY_BE_THIN = std::is_same<O, T>::value;
+    if (a.out_row <= 64 || blocks(128, 128) < 256) {
+        if constexpr (MAY_BE_THIN)
+            if (a.rank) return rows_by<O, ACROSS, DIRECT, true, 64, 64, 2, 2>(a, stream);
+        return rows_by<O, ACROSS, DIRECT, false, 64, 64, 2, 2>(a, stream);
+    }
+    if constexpr (DIRECT && sizeof(T) == 2)
+        if (blocks(256, 256) >= 256) {
+            if constexpr (MAY_BE_THIN)
+                if (a.rank) return rows_by<O, ACROSS, DIRECT, true, 256, 256, 2, 4>(a, stream);
+            return rows_by<O, ACROSS, DIRECT, false, 256, 256, 2, 4>(a, stream);
+        }
+    if constexpr (MAY_BE_THIN)
+        if (a.rank) return rows_by<O, ACROSS, DIRECT, true, 128, 128, 2, 2>(a, stream);
+    return rows_by<O, ACROSS, DIRECT, false, 128, 128, 2, 2>(a, stream);
 }
 
 template <typename A, typename B, typename O, bool DIRECT, int BM, int BN, int WM, int WN>
@@ -48,8 +76,11 @@ hipError_t sums_by(SumArgs g, hipStream_t stream) {
     sum_products<A, B, O, DIRECT, BM, BN, WM, WN><<<(unsigned)blocks, 64 * WM * WN, 0, stream>>>(g);
     if (g.partial) {
         const int64_t size = (int64_t)g.a_columns * g.b_columns;
-        const dim3 grid((unsigned)std::min<int64_t>(divide_up(size, 256), 4096), (unsigned)g.types);
-        join_slots<O><<<grid, 256, 0, stream>>>(g);
+        const auto grid = [&](int each) { return dim3((unsigned)std::min<int64_t>(divide_up(size, 16 * each), 1 << 16), (unsigned)g.types); };
+        if (size % 4 == 0 && ((uintptr_t)g.out & 15) == 0)
+            join_slots<O, 4><<<grid(4), 256, 0, stream>>>(g);
+        else
+            join_slots<O, 1><<<grid(1), 256, 0, stream>>>(g);
     }
     return hipGetLastError();
 }
@@ -58,8 +89,9 @@ template <bool DIRECT>
 hipError_t sums_of(const SumArgs& g, Thin thin, hipStream_t stream) {
     if (thin == kFirst) return sums_by<float, T, T, DIRECT, kThinTile, kSumTile, 1, 4>(g, stream);
     if (thin == kSecond) return sums_by<T, float, T, DIRECT, kSumTile, kThinTile, 4, 1>(g, stream);
-    // (through registers: smaller tiles, whose loads on their way fit beside the sums)
-    return sums_by<T, T, T, DIRECT, DIRECT ? kSumTile : 64, DIRECT ? kSumTile : 64, 2, 2>(g, stream);
+    if constexpr (DIRECT)
+        if (g.tile == kSumTile) return sums_by<T, T, T, true, kSumTile, kSumTile, 2, 2>(g, stream);
+    return sums_by<T, T, T, DIRECT, kSmallSumTile, kSmallSumTile, 2, 2>(g, stream);
 }
 
 }  // namespace
@@ -67,10 +99,10 @@ hipError_t sums_of(const SumArgs& g, Thin thin, hipStream_t stream) {
 template <>
 hipError_t Launch<T>::rows(Args a, bool across, bool wide, bool direct, hipStream_t stream) {
     if (wide)
-        return across ? (direct ? rows_of_size<float, true, true>(a, stream) : rows_of_size<float, true, false>(a, stream))
-                      : (direct ? rows_of_size<float, false, true>(a, stream) : rows_of_size<float, false, false>(a, stream));
-    return across ? (direct ? rows_of_size<T, true, true>(a, stream) : rows_of_size<T, true, false>(a, stream))
-                  : (direct ? rows_of_size<T, false, true>(a, stream) : rows_of_size<T, false, false>(a, stream));
+        return across ? (direct ? rows_of_size<float, true, true>(a, true, stream) : rows_of_size<float, true, false>(a, true, stream))
+                      : (direct ? rows_of_size<float, false, true>(a, true, stream) : rows_of_size<float, false, false>(a, true, stream));
+    return across ? (direct ? rows_of_size<T, true, true>(a, false, stream) : rows_of_size<T, true, false>(a, false, stream))
+                  : (direct ? rows_of_size<T, false, true>(a, false, stream) : rows_of_size<T, false, false>(a, false, stream));
 }
 
 template <>
