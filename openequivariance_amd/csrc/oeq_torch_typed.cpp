@@ -85,7 +85,8 @@ struct Strided {
     int64_t row = 0, part = 0, parts = 1;
     explicit Strided(const Tensor& x) : t(x) {
         const int64_t last = x.dim() - 1;
-        if (x.size(last) > 1 && x.stride(last) != 1) t = x.contiguous();
+        const auto far = [&](int64_t dim) { return x.size(dim) > 1 && x.stride(dim) > INT32_MAX / 4; };  // (the C library refuses it)
+        if ((x.size(last) > 1 && x.stride(last) != 1) || far(0) || far(last - 1)) t = x.contiguous();
         row = t.size(0) > 1 ? t.stride(0) : 0;
         if (last == 2) {
             parts = t.size(1);

@@ -33,6 +33,9 @@ constexpr int64_t kMostBlocks = (1 << 24) - 1;
 // Rows (times parts) and types: slots and places are counted in 32 bits.
 constexpr int64_t kMostRows = 1 << 29, kMostTypes = 1 << 23;
 
+// Elements between rows of sums' operands: their bytes are counted in 32 bits.
+constexpr int64_t kMostStride = INT_MAX / 4;
+
 int check_index(const char* who, int64_t rows, int64_t parts, int64_t types) {
     if (rows < 0 || parts < 1 || types < 0 || types > kMostTypes || rows > kMostRows / parts)
         return fail(OEQ_ERR_INVALID, "%s: %lld rows of %lld parts, %lld types", who, (long long)rows, (long long)parts,
@@ -158,7 +161,8 @@ struct Cut {
         // (through registers small tiles only, whose loads on their way fit beside the sums)
         tile = a.thin || (direct && (a.types * tiles(kSumTile) >= kBlocks || rows / kLeast * tiles(kSumTile) >= kBlocks)) ? kSumTile
                                                                                                                      : kSmallSumTile;
-        chunk = a.types * tiles(tile) >= kBlocks ? std::max<int64_t>(rows, 1)
+        if (!a.thin && direct && a.parts == 1 && a.type != OEQ_FLOAT32 && a.types * tiles(kLargeSumTile) >= 256) tile = kLargeSumTile;
+        chunk = tile == kLargeSumTile || a.types * tiles(tile) >= kBlocks ? std::max<int64_t>(rows, 1)
                                                  : std::max(kLeast, divide_up(rows * tiles(tile), kBlocks * 64) * 64);
     }
 };
@@ -323,7 +327,7 @@ int oeq_typed_sum_products(const oeq_typed_sum* a, void* out, void* workspace, s
         return fail(OEQ_ERR_INVALID, "%s: %lld and %lld columns", who, (long long)a->a_columns, (long long)a->b_columns);
     if (a->thin < 0 || a->thin > 2) return fail(OEQ_ERR_INVALID, "%s: thin operand %d", who, a->thin);
     for (int64_t s : {a->a_row_stride, a->a_part_stride, a->b_row_stride, a->b_part_stride})
-        if (s < 0) return fail(OEQ_ERR_INVALID, "%s: a stride of %lld elements", who, (long long)s);
+        if (s < 0 || s > kMostStride) return fail(OEQ_ERR_INVALID, "%s: a stride of %lld elements", who, (long long)s);
     if (a->types == 0 || a->a_columns == 0 || a->b_columns == 0) return OEQ_OK;
     if (!out || !a->ptr || (a->rows && (!a->a || !a->b || !a->order))) return fail(OEQ_ERR_INVALID, "%s: NULL buffer", who);
     const int a_bytes = a->thin == 1 ? 4 : element_bytes(a->type), b_bytes = a->thin == 2 ? 4 : element_bytes(a->type);

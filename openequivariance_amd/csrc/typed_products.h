@@ -162,6 +162,7 @@ struct Tile {
     static constexpr int kRowsPer = 64 / CH, kEach = kBytes / 1024 / WAVES;
     static_assert(CH >= 8 && CH <= 64 && kEach * 1024 * WAVES == kBytes, "the waves share a tile");
 
+    static constexpr int kPeriod = CH > 8 && sizeof(T) == 4 ? 8 : 16;  // rows after which swizzles come again
     static __device__ __forceinline__ int swizzle(int r) {
         if constexpr (CH == 8) return (r >> 1 & 1) << 2 | (r >> 2 & 3);
         else if constexpr (sizeof(T) == 4) return (r >> 2 & 1) << 3;
@@ -290,37 +291,44 @@ __global__ __launch_bounds__(64 * WM * WN) void row_products(Args g) {
     const int64_t w_step = ACROSS ? BK * g.w_row * (int64_t)sizeof(T) : 128;
     uint4_t x_reg[DIRECT ? 1 : X::kEach], w_reg[DIRECT ? 1 : W::kEach];
 
-    // the tiles of step k
-    auto request = [&](char* xt, char* wt, int k) {
-        const bool last = (k + 1) * BK > g.inner;
-#pragma unroll
-        for (int i = 0; i < X::kEach; ++i) {
-            const int left = g.inner - k * BK - X::chunk(i, wave, lane) * E;
-            if constexpr (DIRECT)
-                X::request(xt, last && left <= 0 ? (const char*)&kZeros : xs[i], i, wave);
-            else
-                x_reg[i] = fetch<T>(xs[i], left);
-            xs[i] += 128;
-        }
-#pragma unroll
-        for (int i = 0; i < W::kEach; ++i) {
-            if constexpr (ACROSS) {
-                const bool in = k * BK + W::row(i, wave, lane) < g.inner;
-                if constexpr (DIRECT)
-                    W::request(wt, last && !in ? (const char*)&kZeros : ws[i], i, wave);
-                else
-                    w_reg[i] = fetch<T>(ws[i], in ? w_left[i] : 0);
-            } else {
-                const int left = g.inner - k * BK - W::chunk(i, wave, lane) * E;
-                if constexpr (DIRECT)
-                    W::request(wt, last && left <= 0 ? (const char*)&kZeros : ws[i], i, wave);
-                else
-                    w_reg[i] = fetch<T>(ws[i], left);
-            }
-            ws[i] += w_step;
-        }
+    // Requests the tiles of step k, a quarter at a time between the products. (Past the last step zeros come, which nobody reads.)
+    auto request_x = [&](char* xt, int k, int i) __attribute__((always_inline)) {
+        const int left = g.inner - k * BK - X::chunk(i, wave, lane) * E;
+        if constexpr (DIRECT)
+            X::request(xt, left <= 0 ? (const char*)&kZeros : xs[i], i, wave);
+        else
+            x_reg[i] = fetch<T>(xs[i], left);
+        xs[i] += 128;
     };
-    auto put = [&](char* xt, char* wt) {
+    auto request_w = [&](char* wt, int k, int i) __attribute__((always_inline)) {
+        if constexpr (ACROSS) {
+            const bool in = k * BK + W::row(i, wave, lane) < g.inner;
+            if constexpr (DIRECT)
+                W::request(wt, !in ? (const char*)&kZeros : ws[i], i, wave);
+            else
+                w_reg[i] = fetch<T>(ws[i], in ? w_left[i] : 0);
+        } else {
+            const int left = g.inner - k * BK - W::chunk(i, wave, lane) * E;
+            if constexpr (DIRECT)
+                W::request(wt, left <= 0 ? (const char*)&kZeros : ws[i], i, wave);
+            else
+                w_reg[i] = fetch<T>(ws[i], left);
+        }
+        ws[i] += w_step;
+    };
+    auto request = [&](char* xt, char* wt, int k, int quarter) __attribute__((always_inline)) {
+#pragma unroll
+        for (int i = 0; i < X::kEach; ++i)
+            if (i % 4 == quarter) request_x(xt, k, i);
+#pragma unroll
+        for (int i = 0; i < W::kEach; ++i)
+            if (i % 4 == quarter) request_w(wt, k, i);
+    };
+    auto request_all = [&](char* xt, char* wt, int k) __attribute__((always_inline)) {
+#pragma unroll
+        for (int quarter = 0; quarter < 4; ++quarter) request(xt, wt, k, quarter);
+    };
+    auto put = [&](char* xt, char* wt) __attribute__((always_inline)) {
         if constexpr (!DIRECT) {
 #pragma unroll
             for (int i = 0; i < X::kEach; ++i) X::put(xt, x_reg[i], i, wave, lane);
@@ -336,28 +344,40 @@ __global__ __launch_bounds__(64 * WM * WN) void row_products(Args g) {
 #pragma unroll
         for (int n = 0; n < TN; ++n) acc[m][n] = 0.0f;
 
-    auto products = [&](const char* xt, const char* wt) {
-#pragma unroll
-        for (int f = 0; f < 4; ++f) {
-            typename Types<T>::frag a[TN], b[TM];
+    // The fragments of a quarter are read while the products of the quarter before are computed: those of w into other registers,
+    // those of x each when the last product with it has been issued. (The barriers keep the compiler from moving reads down to
+    // where they are waited for.)
+    auto products = [&](const char* xt, const char* wt, auto between) __attribute__((always_inline)) {
+        typename Types<T>::frag a[2][TN], b[TM];
+        auto read_w = [&](int f) __attribute__((always_inline)) {
 #pragma unroll
             for (int n = 0; n < TN; ++n)
-                a[n] = ACROSS ? W::down(wt, f, wn + 32 * n, lane) : W::along(wt, wn + 32 * n + (lane & 31), f, half);
+                a[f & 1][n] = ACROSS ? W::down(wt, f, wn + 32 * n, lane) : W::along(wt, wn + 32 * n + (lane & 31), f, half);
+        };
+        auto read_x = [&](int f, int m) __attribute__((always_inline)) { b[m] = X::along(xt, wm + 32 * m + (lane & 31), f, half); };
+        read_w(0);
 #pragma unroll
-            for (int m = 0; m < TM; ++m) b[m] = X::along(xt, wm + 32 * m + (lane & 31), f, half);
+        for (int m = 0; m < TM; ++m) read_x(0, m);
 #pragma unroll
-            for (int m = 0; m < TM; ++m)
+        for (int f = 0; f < 4; ++f) {
+            if (f < 3) read_w(f + 1);
+            between(f);
+            __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-                for (int n = 0; n < TN; ++n) acc[m][n] = mma(a[n], b[m], acc[m][n]);
+            for (int m = 0; m < TM; ++m) {
+#pragma unroll
+                for (int n = 0; n < TN; ++n) acc[m][n] = mma(a[f & 1][n], b[m], acc[m][n]);
+                if (f < 3) read_x(f + 1, m);
+                __builtin_amdgcn_sched_barrier(0);
+            }
         }
     };
-    auto step = [&](char* xt, char* wt, char* xn, char* wn_, int k) {
+    auto step = [&](char* xt, char* wt, char* xn, char* wn_, int k) __attribute__((always_inline)) {
         arrived();
-        if (k + 1 < steps) request(xn, wn_, k + 1);
-        products(xt, wt);
-        if (k + 1 < steps) put(xn, wn_);
+        products(xt, wt, [&](int f) { request(xn, wn_, k + 1, f); });
+        put(xn, wn_);
     };
-    if (steps) request(x0, w0, 0);
+    if (steps) request_all(x0, w0, 0);
     if constexpr (THIN) {
         // The thin product first, from the other buffer. Its rows are float; as operands beside 16 bits they have two parts, u =
         // hi + lo, next to each other along the summation: 16 bits of u or more, when what it adds to is rounded to 8 or 11.
@@ -443,7 +463,7 @@ __global__ __launch_bounds__(64 * WM * WN) void row_products(Args g) {
                     W::put(w1, y.v, i, wave, lane);
                 }
                 __syncthreads();
-                products(x1, w1);
+                products(x1, w1, [](int) {});
                 __syncthreads();
             }
             if constexpr (std::is_same<T, _Float16>::value)
@@ -458,44 +478,68 @@ __global__ __launch_bounds__(64 * WM * WN) void row_products(Args g) {
         step(x0, w0, x1, w1, k);
         if (k + 1 < steps) step(x1, w1, x0, w0, k + 1);
     }
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // (the zeros)
 
-    int64_t to[TM];
-    bool mine[TM];
+    // Results pass through LDS, a wave's 32 rows at a time, so that rows are written in pieces of up to 128 bytes. (From the
+    // registers, four columns of 32 rows at a time, a tile of 256 x 256 took 4 us to write.)
+    constexpr int SLAB = 128 / (int)sizeof(O) < 32 * TN ? 128 / (int)sizeof(O) : 32 * TN, CHUNKS = SLAB * (int)sizeof(O) / 16;
+    constexpr int EO = 16 / (int)sizeof(O), ROWS = 64 / CHUNKS;
+    constexpr bool FITS = WAVES * 32 * SLAB * (int)sizeof(O) <= X::kBytes;
+    __shared__ __align__(16) char results[FITS ? 16 : WAVES * 32 * SLAB * (int)sizeof(O)];
+    char* slab = (FITS ? x0 : results) + wave * 32 * SLAB * (int)sizeof(O);
+    const auto place = [&](int r, int c) { return slab + r * SLAB * (int)sizeof(O) + ((c ^ (r & (CHUNKS - 1))) << 4); };
     float by = 1.0f;
     if (g.scale) by = typed ? g.scale[rows.type] : 0.0f;
-#pragma unroll
-    for (int m = 0; m < TM; ++m) {
-        const int at = m0 + wm + 32 * m + (lane & 31);
-        mine[m] = at < rows.hi;
-        const Place p(g.order, mine[m] ? at : m0, g.parts, g.rows);
-        to[m] = ((int64_t)p.row * g.parts + p.part) * g.out_row;
-    }
     O* out = (O*)g.out;
-    const bool quads = g.out_row % 4 == 0;
+    const bool whole = g.out_row % EO == 0 && ((uintptr_t)out & 15) == 0;
+    const T* bias = g.bias && typed ? (const T*)g.bias + rows.type * g.bias_type : nullptr;
+    __syncthreads();  // (all are done with x0)
 #pragma unroll
     for (int m = 0; m < TM; ++m) {
-        if (!mine[m]) continue;
+        const int first = m0 + wm + 32 * m;
+        int64_t to = 0;
+        if (first < rows.hi) {
+            const Place p(g.order, min(first + (lane & 31), rows.hi - 1), g.parts, g.rows);
+            to = ((int64_t)p.row * g.parts + p.part) * g.out_row;
+        }
 #pragma unroll
-        for (int n = 0; n < TN; ++n)
+        for (int s = 0; s < 32 * TN / SLAB; ++s) {
+            const int col0 = n0 + wn + s * SLAB;
 #pragma unroll
-            for (int q = 0; q < 4; ++q) {
-                const int col = n0 + wn + 32 * n + 8 * q + 4 * half;
-                if (col >= g.out_row) continue;
-                typename Types<O>::quad y;
+            for (int n = 0; n < SLAB / 32; ++n)
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    float s = acc[m][n][4 * q + j] * by;
-                    if (g.bias && typed && col + j < g.outer) s += (float)((const T*)g.bias)[rows.type * g.bias_type + col + j];
-                    y[j] = (O)(col + j < g.outer ? s : 0.0f);
+                for (int q = 0; q < 4; ++q) {
+                    const int c = 32 * n + 8 * q + 4 * half;  // of the slab
+                    typename Types<O>::quad y;
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        float v = acc[m][s * (SLAB / 32) + n][4 * q + j] * by;
+                        const bool in = col0 + c + j < g.outer;
+                        if (bias && in) v += (float)bias[col0 + c + j];
+                        y[j] = (O)(in ? v : 0.0f);
+                    }
+                    *(typename Types<O>::quad*)(place(lane & 31, c / EO) + c % EO * (int)sizeof(O)) = y;
                 }
-                if (quads) {
-                    *(typename Types<O>::quad*)(out + to[m] + col) = y;
-                } else {
 #pragma unroll
-                    for (int j = 0; j < 4; ++j)
-                        if (col + j < g.out_row) out[to[m] + col + j] = y[j];
+            for (int i = 0; i < 32 / ROWS; ++i) {
+                const int r = i * ROWS + lane / CHUNKS, c = lane % CHUNKS, col = col0 + c * EO;
+                const int64_t at = __shfl(to, r) + col;
+                const uint4_t y = *(const uint4_t*)place(r, c);
+                if (first + r >= rows.hi || col >= g.out_row) continue;
+                if (whole) {
+                    *(uint4_t*)(out + at) = y;
+                } else {
+                    union {
+                        uint4_t v;
+                        O e[EO];
+                    } u;
+                    u.v = y;
+#pragma unroll
+                    for (int j = 0; j < EO; ++j)
+                        if (col + j < g.out_row) out[at + j] = u.e[j];
                 }
             }
+        }
     }
 }
 
@@ -742,7 +786,8 @@ __device__ __forceinline__ auto widened(typename Types<T>::frag x) {
 }
 
 // A tile of BM columns of a and BN columns of b, summed over the rows of a slot. BK rows at a time; rows past the end are zeros.
-template <typename A, typename B, typename O, bool DIRECT, int BM, int BN, int WM, int WN>
+// PARTS: rows have more than one. (A kernel of its own: branches inside the loop send the sums through other registers and back.)
+template <typename A, typename B, typename O, bool DIRECT, bool PARTS, int BM, int BN, int WM, int WN>
 __global__ __launch_bounds__(64 * WM * WN) void sum_products(SumArgs g) {
     constexpr int WAVES = WM * WN, BK = sizeof(A) + sizeof(B) == 4 ? 64 : 32;
     constexpr bool MIXED = sizeof(A) != sizeof(B);
@@ -753,52 +798,66 @@ __global__ __launch_bounds__(64 * WM * WN) void sum_products(SumArgs g) {
     __shared__ __align__(1024) char a0[TA::kBytes], a1[TA::kBytes], b0[TB::kBytes], b1[TB::kBytes];
 
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    // slot by slot; in a slot neighbours are eight tiles of a, column by column of b
     const int id = tile_of_block(blockIdx.x, g.slots * g.a_tiles * g.b_tiles);
     const int slot = id / (g.a_tiles * g.b_tiles), tile = id - slot * g.a_tiles * g.b_tiles;
-    const int m0 = tile / g.b_tiles * BM, n0 = tile % g.b_tiles * BN;
+    const int group = tile / (8 * g.b_tiles), in_group = tile - group * 8 * g.b_tiles, high = min(8, g.a_tiles - group * 8);
+    const int m0 = (group * 8 + in_group % high) * BM, n0 = in_group / high * BN;
     const Range rows = rows_of_slot(g.ptr, slot, g.chunk, g.types, false, g.rows, g.parts);
     const int begin = begin_of(g.ptr, rows.type, g.rows, g.parts);
     const bool whole = rows.hi - begin <= g.chunk;  // the type has no other slot
     if (rows.lo >= rows.hi && !(whole && rows.type + begin / g.chunk == slot)) return;
     const int end = min(rows.hi, rows.hi - rows.lo > g.chunk ? rows.lo + g.chunk : rows.hi);
     const int steps = (end - rows.lo + BK - 1) / BK;
-    const auto row_at = [&](int at) { return g.order[g.parts == 1 ? at : at / g.parts]; };
-    const auto inside = [&](int row) { return (unsigned)row < (unsigned)g.rows ? row : 0; };  // (an index not made here)
-    const auto part_of = [&](int at) { return g.parts == 1 ? 0 : min(at, end - 1) % g.parts; };
 
+    // Requests of an operand: the rows of a step are looked up one step ahead, their numbers have come when the step before
+    // has its operands. Lanes keep their columns.
     uint4_t a_reg[DIRECT ? 1 : TA::kEach], b_reg[DIRECT ? 1 : TB::kEach];
-    // The rows of a step are looked up one step ahead: their numbers have come when the step before has its operands.
     constexpr bool SAME = TA::kRowsPer == TB::kRowsPer && TA::kEach == TB::kEach;
     int a_row[TA::kEach], b_row[SAME ? 1 : TB::kEach];
-    auto look_up = [&](int k) {
+    const int a_column = m0 + TA::chunk(0, wave, lane) * EA, b_column = n0 + TB::chunk(0, wave, lane) * EB;
+    const int a_left = max(g.a_columns - a_column, 0), b_left = max(g.b_columns - b_column, 0);
+    const char* a_from = (const char*)((const A*)g.a + (a_left ? a_column : 0));
+    const char* b_from = (const char*)((const B*)g.b + (b_left ? b_column : 0));
+    const unsigned a_stride = (unsigned)g.a_row * (unsigned)sizeof(A), b_stride = (unsigned)g.b_row * (unsigned)sizeof(B);
+    const auto look_up = [&](int k) __attribute__((always_inline)) {
+        const auto row_at = [&](int at) { return g.order[PARTS ? min(at, end - 1) / g.parts : min(at, end - 1)]; };
 #pragma unroll
-        for (int i = 0; i < TA::kEach; ++i) a_row[i] = row_at(min(rows.lo + k * BK + TA::row(i, wave, lane), end - 1));
+        for (int i = 0; i < TA::kEach; ++i) a_row[i] = row_at(rows.lo + k * BK + TA::row(i, wave, lane));
         if constexpr (!SAME)
 #pragma unroll
-            for (int i = 0; i < TB::kEach; ++i) b_row[i] = row_at(min(rows.lo + k * BK + TB::row(i, wave, lane), end - 1));
+            for (int i = 0; i < TB::kEach; ++i) b_row[i] = row_at(rows.lo + k * BK + TB::row(i, wave, lane));
     };
-    auto request = [&](char* at, char* bt, int k) {
+    const auto place = [&](const char* from, int row, unsigned stride, int j, int64_t part) __attribute__((always_inline)) {
+        row = (unsigned)row < (unsigned)g.rows ? row : 0;  // (an index that was not made here)
+        const char* p = from + (uint64_t)(unsigned)row * stride;
+        return PARTS ? p + min(j, end - 1) % g.parts * part : p;
+    };
+    auto request = [&](char* at, char* bt, int k, int quarter) __attribute__((always_inline)) {
 #pragma unroll
         for (int i = 0; i < TA::kEach; ++i) {
-            const int j = rows.lo + k * BK + TA::row(i, wave, lane), c = m0 + TA::chunk(i, wave, lane) * EA;
-            const char* from = (const char*)((const A*)g.a + inside(a_row[i]) * g.a_row + part_of(j) * g.a_part + (c < g.a_columns ? c : 0));
+            if (i % 4 != quarter) continue;
+            static_assert(TA::kEach == 1 || WAVES * TA::kRowsPer % TA::kPeriod == 0, "a lane's chunks are of one column");
+            const int j = rows.lo + k * BK + TA::row(i, wave, lane);
+            const char* from = place(a_from, a_row[i], a_stride, j, g.a_part * (int64_t)sizeof(A));
             if constexpr (DIRECT)
                 TA::request(at, j < end ? from : (const char*)&kZeros, i, wave);
             else
-                a_reg[i] = fetch<A>(from, j < end && c < g.a_columns ? g.a_columns - c : 0);
+                a_reg[i] = fetch<A>(from, j < end ? a_left : 0);
         }
 #pragma unroll
         for (int i = 0; i < TB::kEach; ++i) {
-            const int j = rows.lo + k * BK + TB::row(i, wave, lane), c = n0 + TB::chunk(i, wave, lane) * EB;
-            const int row = inside(SAME ? a_row[i] : b_row[i]);
-            const char* from = (const char*)((const B*)g.b + row * g.b_row + part_of(j) * g.b_part + (c < g.b_columns ? c : 0));
+            if (i % 4 != quarter) continue;
+            static_assert(TB::kEach == 1 || WAVES * TB::kRowsPer % TB::kPeriod == 0, "a lane's chunks are of one column");
+            const int j = rows.lo + k * BK + TB::row(i, wave, lane);
+            const char* from = place(b_from, SAME ? a_row[i] : b_row[i], b_stride, j, g.b_part * (int64_t)sizeof(B));
             if constexpr (DIRECT)
                 TB::request(bt, j < end ? from : (const char*)&kZeros, i, wave);
             else
-                b_reg[i] = fetch<B>(from, j < end && c < g.b_columns ? g.b_columns - c : 0);
+                b_reg[i] = fetch<B>(from, j < end ? b_left : 0);
         }
     };
-    auto put = [&](char* at, char* bt) {
+    auto put = [&](char* at, char* bt) __attribute__((always_inline)) {
         if constexpr (!DIRECT) {
 #pragma unroll
             for (int i = 0; i < TA::kEach; ++i) TA::put(at, a_reg[i], i, wave, lane);
@@ -816,7 +875,7 @@ __global__ __launch_bounds__(64 * WM * WN) void sum_products(SumArgs g) {
 
     // A fragment of floats has 8 of the rows that one of 16 bits has: 8 f + 4 half .. + 4 (16 f + 8 half .. + 8); where
     // both meet, two reads of four rows make the longer one.
-    auto a_frag = [&](const char* at, int f, int first) {
+    auto a_frag = [&](const char* at, int f, int first) __attribute__((always_inline)) {
         if constexpr (MIXED && sizeof(A) == 4) {
             float8_t x;
 #pragma unroll
@@ -829,7 +888,7 @@ __global__ __launch_bounds__(64 * WM * WN) void sum_products(SumArgs g) {
             return widened<A, MIXED>(TA::down(at, f, first, lane));
         }
     };
-    auto b_frag = [&](const char* bt, int f, int first) {
+    auto b_frag = [&](const char* bt, int f, int first) __attribute__((always_inline)) {
         if constexpr (MIXED && sizeof(B) == 4) {
             float8_t x;
 #pragma unroll
@@ -843,38 +902,53 @@ __global__ __launch_bounds__(64 * WM * WN) void sum_products(SumArgs g) {
         }
     };
     constexpr int FRAGS = sizeof(A) == 4 && sizeof(B) == 4 ? BK / 8 : BK / 16;
-    auto products = [&](const char* at, const char* bt) {
+    // As in row_products: fragments one ahead, requests between.
+    auto products = [&](const char* at, const char* bt, auto between) __attribute__((always_inline)) {
+        decltype(a_frag(at, 0, 0)) a[TM];
+        decltype(b_frag(bt, 0, 0)) b[2][TN];
+        auto read_b = [&](int f) __attribute__((always_inline)) {
+#pragma unroll
+            for (int n = 0; n < TN; ++n) b[f & 1][n] = b_frag(bt, f, wn + 32 * n);
+        };
+        read_b(0);
+#pragma unroll
+        for (int m = 0; m < TM; ++m) a[m] = a_frag(at, 0, wm + 32 * m);
 #pragma unroll
         for (int f = 0; f < FRAGS; ++f) {
-            decltype(a_frag(at, 0, 0)) a[TM];
-            decltype(b_frag(bt, 0, 0)) b[TN];
+            if (f + 1 < FRAGS) read_b(f + 1);
 #pragma unroll
-            for (int m = 0; m < TM; ++m) a[m] = a_frag(at, f, wm + 32 * m);
+            for (int quarter = f * 4 / FRAGS; quarter < (f + 1) * 4 / FRAGS; ++quarter) between(quarter);
+            __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-            for (int n = 0; n < TN; ++n) b[n] = b_frag(bt, f, wn + 32 * n);
+            for (int m = 0; m < TM; ++m) {
 #pragma unroll
-            for (int m = 0; m < TM; ++m)
-#pragma unroll
-                for (int n = 0; n < TN; ++n) acc[m][n] = mma(a[m], b[n], acc[m][n]);
+                for (int n = 0; n < TN; ++n) acc[m][n] = mma(a[m], b[f & 1][n], acc[m][n]);
+                if (f + 1 < FRAGS) a[m] = a_frag(at, f + 1, wm + 32 * m);
+                __builtin_amdgcn_sched_barrier(0);
+            }
         }
     };
-    auto step = [&](char* at, char* bt, char* an, char* bn, int k) {
+    // (Past the last step zeros are requested, and the last row is looked up again.)
+    auto step = [&](char* at, char* bt, char* an, char* bn, int k) __attribute__((always_inline)) {
         arrived();
-        if (k + 1 < steps) request(an, bn, k + 1);
-        if (k + 2 < steps) look_up(k + 2);
-        products(at, bt);
-        if (k + 1 < steps) put(an, bn);
+        products(at, bt, [&](int quarter) {
+            request(an, bn, k + 1, quarter);
+            if (quarter == 3) look_up(k + 2);
+        });
+        put(an, bn);
     };
     if (steps > 0) {
         look_up(0);
-        request(a0, b0, 0);
-        if (steps > 1) look_up(1);
+#pragma unroll
+        for (int quarter = 0; quarter < 4; ++quarter) request(a0, b0, 0, quarter);
+        look_up(1);
         put(a0, b0);
     }
     for (int k = 0; k < steps; k += 2) {
         step(a0, b0, a1, b1, k);
         if (k + 1 < steps) step(a1, b1, a0, b0, k + 1);
     }
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
 
     // lane l has column l % 32 of b, register r row 8 (r / 4) + 4 (l / 32) + r % 4
     const int64_t size = (int64_t)g.a_columns * g.b_columns;

@@ -73,7 +73,14 @@ hipError_t sums_by(SumArgs g, hipStream_t stream) {
     g.a_tiles = (int)divide_up(g.a_columns, BM), g.b_tiles = (int)divide_up(g.b_columns, BN);
     const int64_t blocks = (int64_t)g.slots * g.a_tiles * g.b_tiles;
     if (blocks > (1 << 24) - 1) return hipErrorInvalidConfiguration;
-    sum_products<A, B, O, DIRECT, BM, BN, WM, WN><<<(unsigned)blocks, 64 * WM * WN, 0, stream>>>(g);
+    if constexpr (sizeof(A) == sizeof(B) && BM < kLargeSumTile) {
+        if (g.parts > 1)
+            sum_products<A, B, O, DIRECT, true, BM, BN, WM, WN><<<(unsigned)blocks, 64 * WM * WN, 0, stream>>>(g);
+        else
+            sum_products<A, B, O, DIRECT, false, BM, BN, WM, WN><<<(unsigned)blocks, 64 * WM * WN, 0, stream>>>(g);
+    } else {
+        sum_products<A, B, O, DIRECT, false, BM, BN, WM, WN><<<(unsigned)blocks, 64 * WM * WN, 0, stream>>>(g);
+    }
     if (g.partial) {
         const int64_t size = (int64_t)g.a_columns * g.b_columns;
         const auto grid = [&](int each) { return dim3((unsigned)std::min<int64_t>(divide_up(size, 16 * each), 1 << 16), (unsigned)g.types); };
@@ -89,6 +96,8 @@ template <bool DIRECT>
 hipError_t sums_of(const SumArgs& g, Thin thin, hipStream_t stream) {
     if (thin == kFirst) return sums_by<float, T, T, DIRECT, kThinTile, kSumTile, 1, 4>(g, stream);
     if (thin == kSecond) return sums_by<T, float, T, DIRECT, kSumTile, kThinTile, 4, 1>(g, stream);
+    if constexpr (DIRECT && sizeof(T) == 2)
+        if (g.tile == kLargeSumTile) return sums_by<T, T, T, true, kLargeSumTile, kLargeSumTile, 2, 4>(g, stream);
     if constexpr (DIRECT)
         if (g.tile == kSumTile) return sums_by<T, T, T, true, kSumTile, kSumTile, 2, 2>(g, stream);
     return sums_by<T, T, T, DIRECT, kSmallSumTile, kSmallSumTile, 2, 2>(g, stream);

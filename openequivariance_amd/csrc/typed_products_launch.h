@@ -19,7 +19,7 @@ struct Launch {
 };
 
 // Columns of a tile of sum_products of which there are few (float operands of a thin product), else.
-constexpr int kThinTile = 32, kSumTile = 128, kSmallSumTile = 64;
+constexpr int kThinTile = 32, kSumTile = 128, kSmallSumTile = 64, kLargeSumTile = 256;
 
 }  // namespace typed_products
 #endif
