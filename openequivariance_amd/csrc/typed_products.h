@@ -101,10 +101,14 @@ __device__ __forceinline__ float16_t mma(bf8_t a, bf8_t b, float16_t c) {
 // slots
 // ---------------------------------------------------------------------------
 
-// Blocks go to the eight XCDs in turn, each with a cache of its own: each takes a run of neighbouring tiles.
+// Blocks go to the eight XCDs in turn, each with a cache of its own: an XCD takes 32 neighbouring tiles, one for each of its
+// compute units, then the 32 that follow those of the other seven. (Longer runs leave some XCDs with the slots that have no rows: 8 192
+// rows, 8192 x 8192, bf16: 1 028 us with an eighth of all tiles to each XCD, 953 so.)
 __device__ __forceinline__ int tile_of_block(int block, int blocks) {
-    const int xcd = block & 7, each = blocks >> 3, rest = blocks & 7;
-    return xcd * each + min(xcd, rest) + (block >> 3);
+    constexpr int kRun = 32;
+    if (block >= blocks / (8 * kRun) * (8 * kRun)) return block;
+    const int xcd = block & 7, turn = block >> 3;
+    return (turn / kRun * 8 + xcd) * kRun + turn % kRun;
 }
 
 struct Range {
@@ -162,7 +166,9 @@ struct Tile {
     static constexpr int kRowsPer = 64 / CH, kEach = kBytes / 1024 / WAVES;
     static_assert(CH >= 8 && CH <= 64 && kEach * 1024 * WAVES == kBytes, "the waves share a tile");
 
-    static constexpr int kPeriod = CH > 8 && sizeof(T) == 4 ? 8 : 16;  // rows after which swizzles come again
+    // After this many of a lane's requests the same chunk comes again.
+    static constexpr int kPeriod = CH > 8 && sizeof(T) == 4 ? 8 : 16, kApart = WAVES * kRowsPer;
+    static constexpr int kColumns = kApart >= kPeriod ? 1 : kEach < kPeriod / kApart ? kEach : kPeriod / kApart;
     static __device__ __forceinline__ int swizzle(int r) {
         if constexpr (CH == 8) return (r >> 1 & 1) << 2 | (r >> 2 & 3);
         else if constexpr (sizeof(T) == 4) return (r >> 2 & 1) << 3;
@@ -231,6 +237,10 @@ __device__ __forceinline__ uint4_t fetch(const char* from, int left) {
     }
     return x;
 }
+
+// Quarters of a step's products, between which the next step's operands are requested: early enough to be there in time.
+// 8 192 rows, 8192 x 8192, bf16, us: 1 1 064, 2 1 028, 4 1 135.
+constexpr int kEarly = 2;
 
 // What this wave requested is in LDS; then the same for the others, and all are done with the other buffer.
 __device__ __forceinline__ void arrived() {
@@ -374,7 +384,11 @@ __global__ __launch_bounds__(64 * WM * WN) void row_products(Args g) {
     };
     auto step = [&](char* xt, char* wt, char* xn, char* wn_, int k) __attribute__((always_inline)) {
         arrived();
-        products(xt, wt, [&](int f) { request(xn, wn_, k + 1, f); });
+        products(xt, wt, [&](int f) __attribute__((always_inline)) {
+            if (f < kEarly)
+#pragma unroll
+                for (int quarter = f * 4 / kEarly; quarter < (f + 1) * 4 / kEarly; ++quarter) request(xn, wn_, k + 1, quarter);
+        });
         put(xn, wn_);
     };
     if (steps) request_all(x0, w0, 0);
@@ -788,7 +802,7 @@ __device__ __forceinline__ auto widened(typename Types<T>::frag x) {
 // A tile of BM columns of a and BN columns of b, summed over the rows of a slot. BK rows at a time; rows past the end are zeros.
 // PARTS: rows have more than one. (A kernel of its own: branches inside the loop send the sums through other registers and back.)
 template <typename A, typename B, typename O, bool DIRECT, bool PARTS, int BM, int BN, int WM, int WN>
-__global__ __launch_bounds__(64 * WM * WN) void sum_products(SumArgs g) {
+__global__ __launch_bounds__(64 * WM * WN, BM * BN == WM * WN * 128 * 128 ? 1 : 2) void sum_products(SumArgs g) {
     constexpr int WAVES = WM * WN, BK = sizeof(A) + sizeof(B) == 4 ? 64 : 32;
     constexpr bool MIXED = sizeof(A) != sizeof(B);
     constexpr int EA = 16 / (int)sizeof(A), EB = 16 / (int)sizeof(B);
@@ -815,10 +829,21 @@ __global__ __launch_bounds__(64 * WM * WN) void sum_products(SumArgs g) {
     uint4_t a_reg[DIRECT ? 1 : TA::kEach], b_reg[DIRECT ? 1 : TB::kEach];
     constexpr bool SAME = TA::kRowsPer == TB::kRowsPer && TA::kEach == TB::kEach;
     int a_row[TA::kEach], b_row[SAME ? 1 : TB::kEach];
-    const int a_column = m0 + TA::chunk(0, wave, lane) * EA, b_column = n0 + TB::chunk(0, wave, lane) * EB;
-    const int a_left = max(g.a_columns - a_column, 0), b_left = max(g.b_columns - b_column, 0);
-    const char* a_from = (const char*)((const A*)g.a + (a_left ? a_column : 0));
-    const char* b_from = (const char*)((const B*)g.b + (b_left ? b_column : 0));
+    constexpr int CA = TA::kColumns, CB = TB::kColumns;
+    int a_left[CA], b_left[CB];  // elements from a lane's columns on
+    const char *a_from[CA], *b_from[CB];
+#pragma unroll
+    for (int i = 0; i < CA; ++i) {
+        const int column = m0 + TA::chunk(i, wave, lane) * EA;
+        a_left[i] = max(g.a_columns - column, 0);
+        a_from[i] = (const char*)((const A*)g.a + (a_left[i] ? column : 0));
+    }
+#pragma unroll
+    for (int i = 0; i < CB; ++i) {
+        const int column = n0 + TB::chunk(i, wave, lane) * EB;
+        b_left[i] = max(g.b_columns - column, 0);
+        b_from[i] = (const char*)((const B*)g.b + (b_left[i] ? column : 0));
+    }
     const unsigned a_stride = (unsigned)g.a_row * (unsigned)sizeof(A), b_stride = (unsigned)g.b_row * (unsigned)sizeof(B);
     const auto look_up = [&](int k) __attribute__((always_inline)) {
         const auto row_at = [&](int at) { return g.order[PARTS ? min(at, end - 1) / g.parts : min(at, end - 1)]; };
@@ -837,24 +862,22 @@ __global__ __launch_bounds__(64 * WM * WN) void sum_products(SumArgs g) {
 #pragma unroll
         for (int i = 0; i < TA::kEach; ++i) {
             if (i % 4 != quarter) continue;
-            static_assert(TA::kEach == 1 || WAVES * TA::kRowsPer % TA::kPeriod == 0, "a lane's chunks are of one column");
             const int j = rows.lo + k * BK + TA::row(i, wave, lane);
-            const char* from = place(a_from, a_row[i], a_stride, j, g.a_part * (int64_t)sizeof(A));
+            const char* from = place(a_from[i % CA], a_row[i], a_stride, j, g.a_part * (int64_t)sizeof(A));
             if constexpr (DIRECT)
                 TA::request(at, j < end ? from : (const char*)&kZeros, i, wave);
             else
-                a_reg[i] = fetch<A>(from, j < end ? a_left : 0);
+                a_reg[i] = fetch<A>(from, j < end ? a_left[i % CA] : 0);
         }
 #pragma unroll
         for (int i = 0; i < TB::kEach; ++i) {
             if (i % 4 != quarter) continue;
-            static_assert(TB::kEach == 1 || WAVES * TB::kRowsPer % TB::kPeriod == 0, "a lane's chunks are of one column");
             const int j = rows.lo + k * BK + TB::row(i, wave, lane);
-            const char* from = place(b_from, SAME ? a_row[i] : b_row[i], b_stride, j, g.b_part * (int64_t)sizeof(B));
+            const char* from = place(b_from[i % CB], SAME ? a_row[i] : b_row[i], b_stride, j, g.b_part * (int64_t)sizeof(B));
             if constexpr (DIRECT)
                 TB::request(bt, j < end ? from : (const char*)&kZeros, i, wave);
             else
-                b_reg[i] = fetch<B>(from, j < end ? b_left : 0);
+                b_reg[i] = fetch<B>(from, j < end ? b_left[i % CB] : 0);
         }
     };
     auto put = [&](char* at, char* bt) __attribute__((always_inline)) {
@@ -916,8 +939,7 @@ __global__ __launch_bounds__(64 * WM * WN) void sum_products(SumArgs g) {
 #pragma unroll
         for (int f = 0; f < FRAGS; ++f) {
             if (f + 1 < FRAGS) read_b(f + 1);
-#pragma unroll
-            for (int quarter = f * 4 / FRAGS; quarter < (f + 1) * 4 / FRAGS; ++quarter) between(quarter);
+            between(f);
             __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
             for (int m = 0; m < TM; ++m) {
@@ -931,9 +953,11 @@ __global__ __launch_bounds__(64 * WM * WN) void sum_products(SumArgs g) {
     // (Past the last step zeros are requested, and the last row is looked up again.)
     auto step = [&](char* at, char* bt, char* an, char* bn, int k) __attribute__((always_inline)) {
         arrived();
-        products(at, bt, [&](int quarter) {
-            request(an, bn, k + 1, quarter);
-            if (quarter == 3) look_up(k + 2);
+        products(at, bt, [&](int f) __attribute__((always_inline)) {
+            if (f < kEarly)
+#pragma unroll
+                for (int quarter = f * 4 / kEarly; quarter < (f + 1) * 4 / kEarly; ++quarter) request(an, bn, k + 1, quarter);
+            if (f == kEarly - 1) look_up(k + 2);
         });
         put(an, bn);
     };
@@ -950,7 +974,9 @@ __global__ __launch_bounds__(64 * WM * WN) void sum_products(SumArgs g) {
     }
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
 
-    // lane l has column l % 32 of b, register r row 8 (r / 4) + 4 (l / 32) + r % 4
+    // lane l has column l % 32 of b, register r row 8 (r / 4) + 4 (l / 32) + r % 4 (the lane counted again: kept over the loop it
+    // would leave no registers for the sums)
+    const int l = __builtin_amdgcn_mbcnt_hi(~0u, __builtin_amdgcn_mbcnt_lo(~0u, 0));
     const int64_t size = (int64_t)g.a_columns * g.b_columns;
     O* out = (O*)g.out + rows.type * size;
     float* partial = g.partial + slot * size;
@@ -960,7 +986,7 @@ __global__ __launch_bounds__(64 * WM * WN) void sum_products(SumArgs g) {
         for (int n = 0; n < TN; ++n)
 #pragma unroll
             for (int r = 0; r < 16; ++r) {
-                const int i = m0 + wm + 32 * m + 8 * (r / 4) + 4 * (lane >> 5) + r % 4, j = n0 + wn + 32 * n + (lane & 31);
+                const int i = m0 + wm + 32 * m + 8 * (r / 4) + 4 * (l >> 5) + r % 4, j = n0 + wn + 32 * n + (l & 31);
                 if (i >= g.a_columns || j >= g.b_columns) continue;
                 const int64_t at = (int64_t)i * g.b_columns + j;
                 if (whole)
