@@ -162,8 +162,10 @@ struct Cut {
         tile = a.thin || (direct && (a.types * tiles(kSumTile) >= kBlocks || rows / kLeast * tiles(kSumTile) >= kBlocks)) ? kSumTile
                                                                                                                      : kSmallSumTile;
         if (!a.thin && direct && a.parts == 1 && a.type != OEQ_FLOAT32 && a.types * tiles(kLargeSumTile) >= 256) tile = kLargeSumTile;
-        chunk = tile == kLargeSumTile || a.types * tiles(tile) >= kBlocks ? rows + 1  // (no type has a second slot)
-                                                 : std::max(kLeast, divide_up(rows * tiles(tile), kBlocks * 64) * 64);
+        // (short sums are done before a second launch has begun)
+        chunk = tile == kLargeSumTile || a.types * tiles(tile) >= kBlocks || rows / a.types <= 2 * kLeast
+                    ? rows + 1  // (no type has a second slot)
+                    : std::max(kLeast, divide_up(rows * tiles(tile), kBlocks * 64) * 64);
     }
 };
 

@@ -86,6 +86,8 @@ __global__ __launch_bounds__(kThreads) void sort_in_block(const int64_t* types, 
         if (tid < kDigits)
             for (int w = 0; w < kWaves; ++w) total += counts[w][tid];
         int before = before_digit(total, wave_sums);
+        const bool last = pass + 1 == passes;
+        if (passes == 1 && tid <= count) ptr[tid] = before;  // (the digit is the type)
         if (tid < kDigits)
             for (int w = 0; w < kWaves; ++w) {
                 const int c = counts[w][tid];
@@ -101,12 +103,13 @@ __global__ __launch_bounds__(kThreads) void sort_in_block(const int64_t* types, 
             const uint64_t same = same_digit(digit, at < rows);
             if (at < rows) {
                 const int to = counts[wave][digit] + lanes_before(same);
-                keys[to] = key[i], numbers[to] = number[i];
+                if (last) order[to] = number[i];
+                if (passes > 1) keys[to] = key[i], numbers[to] = number[i];
                 if (lanes_before(same) == __popcll(same) - 1) counts[wave][digit] = to + 1;
             }
         }
         __syncthreads();
-        if (pass + 1 < passes) {
+        if (!last) {
 #pragma unroll
             for (int i = 0; i < kEach; ++i) {
                 const int at = wave * span + i * 64 + lane;
@@ -114,7 +117,7 @@ __global__ __launch_bounds__(kThreads) void sort_in_block(const int64_t* types, 
             }
         }
     }
-    for (int at = tid; at < rows; at += kThreads) order[at] = numbers[at];
+    if (passes == 1) return;
     for (int t = tid; t <= count; t += kThreads) {  // the first place whose key is t or more
         int lo = 0, hi = rows;
         while (lo < hi) {
@@ -264,7 +267,7 @@ __global__ __launch_bounds__(256) void lookup(const T* table, int64_t table_row,
 // the blocks of the type, longer ones in two steps: chunks of kChunk places of the index sum what they hold of a longer
 // type (a chunk holds parts of two at most: the one that it begins in and the one that it ends in), and the chunk in which a
 // longer type begins adds up the chunks' sums in order.
-constexpr int kChunk = 64;
+constexpr int kChunk = 32;
 
 struct Sums {
     const void* rows;

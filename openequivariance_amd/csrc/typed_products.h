@@ -121,20 +121,29 @@ __device__ __forceinline__ int begin_of(const int* ptr, int t, int rows, int par
 // The type that owns a slot of `each` rows, among `types` (and the rows without a type, if `rest`), and the slot's rows.
 __device__ __forceinline__ Range rows_of_slot(const int* ptr, int slot, int each, int types, bool rest, int rows, int parts) {
     const int lane = threadIdx.x & 63;
-    int t = 0, n = types + rest;
-    while (n > 1) {  // 64 candidates at a time; the first of them always begins early enough
-        const int step = (n + 63) >> 6;
-        const int at = lane * step;
-        const bool early = lane == 0 || (at < n && begin_of(ptr, t + at, rows, parts) / each + t + at <= slot);
-        const int last = 63 - __builtin_clzll(__ballot(early));
-        t += last * step;
-        n = min(step, n - last * step);
-    }
     Range r;
-    r.type = __builtin_amdgcn_readfirstlane(t);
-    const int begin = begin_of(ptr, r.type, rows, parts);
+    int begin;
+    if (types < 64) {  // every type's beginning in a lane
+        const int mine = begin_of(ptr, min(lane, types), rows, parts);
+        const bool early = lane == 0 || (lane < types + rest && mine / each + lane <= slot);
+        r.type = __builtin_amdgcn_readfirstlane(63 - __builtin_clzll(__ballot(early)));
+        begin = __builtin_amdgcn_readlane(mine, r.type);
+        r.hi = r.type < types ? __builtin_amdgcn_readlane(mine, r.type + 1) : rows * parts;
+    } else {
+        int t = 0, n = types + rest;
+        while (n > 1) {  // 64 candidates at a time; the first of them always begins early enough
+            const int step = (n + 63) >> 6;
+            const int at = lane * step;
+            const bool early = lane == 0 || (at < n && begin_of(ptr, t + at, rows, parts) / each + t + at <= slot);
+            const int last = 63 - __builtin_clzll(__ballot(early));
+            t += last * step;
+            n = min(step, n - last * step);
+        }
+        r.type = __builtin_amdgcn_readfirstlane(t);
+        begin = begin_of(ptr, r.type, rows, parts);
+        r.hi = r.type < types ? begin_of(ptr, r.type + 1, rows, parts) : rows * parts;
+    }
     const int64_t lo = begin + (int64_t)(slot - begin / each - r.type) * each;
-    r.hi = r.type < types ? begin_of(ptr, r.type + 1, rows, parts) : rows * parts;
     r.lo = lo < r.hi ? (int)lo : r.hi;
     return r;
 }
@@ -217,25 +226,25 @@ struct Tile {
     }
 };
 
-// 16 bytes from anywhere, of which `left` elements are there; zeros for the others.
+typedef uint4_t anywhere2_t __attribute__((aligned(2)));
+typedef uint4_t anywhere4_t __attribute__((aligned(4)));
+
+// 16 bytes from anywhere in memory, of which `left` elements are there; zeros for the others. (Pointers are told to be global
+// ones: next to kZeros the compiler takes them for any, and such loads are waited for all at once.)
 template <typename T>
 __device__ __forceinline__ uint4_t fetch(const char* from, int left) {
     constexpr int E = 16 / (int)sizeof(T);
-    uint4_t x = {0, 0, 0, 0};
-    if (left >= E) {
-        __builtin_memcpy(&x, from, 16);
-    } else {
-        union {
-            uint4_t v;
-            T e[E];
-        } u;
-        u.v = x;
+    typedef typename std::conditional<sizeof(T) == 2, anywhere2_t, anywhere4_t>::type anywhere_t;
+    if (left >= E) return *(__attribute__((address_space(1))) const anywhere_t*)from;
+    union {
+        uint4_t v;
+        T e[E];
+    } u;
+    u.v = uint4_t{0, 0, 0, 0};
 #pragma unroll
-        for (int j = 0; j < E; ++j)
-            if (j < left) u.e[j] = ((const T*)from)[j];
-        x = u.v;
-    }
-    return x;
+    for (int j = 0; j < E; ++j)
+        if (j < left) u.e[j] = ((__attribute__((address_space(1))) const T*)from)[j];
+    return u.v;
 }
 
 // Quarters of a step's products, between which the next step's operands are requested: early enough to be there in time.
@@ -588,16 +597,82 @@ struct Few<__bf16> {
     }
 };
 
-constexpr int kFewRows = 64, kFewWaves = 8;
+constexpr int kFewRows = 64, kFewWaves = 4;
+
+// acc[m][n] += products of 16 x rows and 16 w rows for this wave's turns of the summation: 128 bytes of each row, from memory to a
+// part of LDS that is the wave's own (no barrier), two turns ahead of the products. rows(r) is where row r begins: first the x rows,
+// 16 X of them, then those of w. (Straight to registers a request has 16 bytes of 16 rows, lanes next to each other in different rows:
+// 27 accesses to the cache where 8 rows of 128 bytes take 8; 48 requests beside 4096 x 4096, bf16: 21 us, so 14.)
+template <typename T, bool DIRECT, int X, int W, typename Rows>
+__device__ __forceinline__ void sum_turns(float4_t (&acc)[X][W], char* stage0, char* stage1, char* stage2, const Rows& rows, int inner,
+                                          int wave, int lane) {
+    constexpr int E = 16 / (int)sizeof(T), BK = 128 / (int)sizeof(T), REQUESTS = 2 * (X + W);
+    typedef Tile<T, 8, 16 * (X + W), 1> L;
+    static_assert(L::kEach == REQUESTS, "1 KB a request");
+    const int steps = (inner + BK - 1) / BK;
+    if (wave >= steps) return;
+    const char* from[REQUESTS];
+#pragma unroll
+    for (int i = 0; i < REQUESTS; ++i) from[i] = (const char*)rows(L::row(i, 0, lane)) + L::chunk(i, 0, lane) * 16;
+    const auto request = [&](char* to, int step) __attribute__((always_inline)) {
+#pragma unroll
+        for (int i = 0; i < REQUESTS; ++i) {
+            const int left = inner - step * BK - L::chunk(i, 0, lane) * E;
+            const char* at = from[i] + (int64_t)step * 128;
+            if constexpr (DIRECT)
+                L::request(to, left <= 0 ? (const char*)&kZeros : at, i, 0);
+            else
+                L::put(to, fetch<T>(at, left), i, 0, lane);
+        }
+    };
+    const auto products = [&](const char* from_) __attribute__((always_inline)) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            typename Types<T>::frag a[W], b[X];
+            const auto read = [&](int r) __attribute__((always_inline)) {
+                return *(const typename Types<T>::frag*)(from_ + r * 128 + (((4 * h + (lane >> 4)) ^ L::swizzle(r)) << 4));
+            };
+#pragma unroll
+            for (int m = 0; m < X; ++m) b[m] = read(16 * m + (lane & 15));
+#pragma unroll
+            for (int n = 0; n < W; ++n) a[n] = read(16 * (X + n) + (lane & 15));
+#pragma unroll
+            for (int m = 0; m < X; ++m)
+#pragma unroll
+                for (int n = 0; n < W; ++n) acc[m][n] = Few<T>::mma(a[n], b[m], acc[m][n]);
+        }
+    };
+    const auto step = [&](const char* now, char* next, int k) __attribute__((always_inline)) {
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // what was read from `next` has come
+        request(next, k + 2 * kFewWaves);
+        if constexpr (DIRECT) {  // vmcnt(2 REQUESTS), as a builtin that the compiler counts with
+            __builtin_amdgcn_s_waitcnt((2 * REQUESTS & 15) | 0xf70 | (2 * REQUESTS >> 4) << 14);
+            asm volatile("" ::: "memory");
+        }
+        products(now);
+    };
+    // (No branch around a request: the compiler would not know how many are on their way, and wait for all. Past the last step
+    // zeros come, which nobody needs.)
+    request(stage0, wave);
+    request(stage1, wave + kFewWaves);
+    for (int k = wave; k < steps; k += 3 * kFewWaves) {
+        step(stage0, stage2, k);
+        step(stage1, stage0, k + kFewWaves);
+        step(stage2, stage1, k + 2 * kFewWaves);
+    }
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+}
 
 // MT: tiles of 16 rows. blockIdx.x: columns; blockIdx.y: rows, of which the first of a type stands for all; with shared
 // weights: every 16 MT rows.
 template <typename T, typename O, bool DIRECT, int MT>
 __global__ __launch_bounds__(64 * kFewWaves) void few_products(Args g) {
-    constexpr int E = 16 / (int)sizeof(T), BK = 128 / (int)sizeof(T), AHEAD = MT <= 2 ? 4 : 2;
-    typedef typename Types<T>::frag frag;
+    constexpr int E = 16 / (int)sizeof(T), STAGE = 16 * (MT + 1) * 128;
     __shared__ int members[kFewRows];
-    __shared__ float sums[kFewWaves][16 * MT][17];
+    __shared__ __align__(1024) char stage0[kFewWaves * STAGE], stage1[kFewWaves * STAGE], stage2[kFewWaves * STAGE];
+    typedef float Sums[kFewWaves][16 * MT][17];
+    static_assert(sizeof(Sums) <= sizeof(stage0), "the sums lie where the operands did");
+    Sums& sums = *(Sums*)stage0;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int n0 = blockIdx.x * 16, total = g.rows * g.parts;
     int type = g.types, count;
@@ -619,57 +694,35 @@ __global__ __launch_bounds__(64 * kFewWaves) void few_products(Args g) {
     }
     __syncthreads();
     const bool typed = type < g.types;
-    const int tiles = (count + 15) / 16;
-
-    const T* w = (const T*)g.w + (typed ? type : 0) * g.w_type + min(n0 + (lane & 15), g.outer - 1) * g.w_row + 2 * E * (lane >> 4);
-    const T* x[MT];
-#pragma unroll
-    for (int m = 0; m < MT; ++m) {
-        const int at = members[min(16 * m + (lane & 15), count - 1)];
-        const int row = g.parts == 1 ? at : at / g.parts;
-        x[m] = (const T*)g.x + row * g.x_row + (at - row * g.parts) * g.x_part + 2 * E * (lane >> 4);
-    }
-    // 16 bytes from element k of a row on
-    const auto load = [&](const T* row, int k) -> frag {
-        if constexpr (DIRECT) {
-            return *(const frag*)(k + 2 * E * (lane >> 4) < g.inner ? row + k : (const T*)&kZeros);
-        } else {
-            union {
-                uint4_t v;
-                frag f;
-            } u;
-            u.v = fetch<T>((const char*)(row + k), g.inner - k - 2 * E * (lane >> 4));
-            return u.f;
-        }
-    };
+    const T* w = (const T*)g.w + (typed ? type : 0) * g.w_type;
     float4_t acc[MT];
 #pragma unroll
     for (int m = 0; m < MT; ++m) acc[m] = 0.0f;
-    const int steps = typed || g.shared ? (g.inner + BK - 1) / BK : 0;
-    for (int s0 = wave; s0 < steps; s0 += AHEAD * kFewWaves) {
-        frag a[AHEAD][2], b[AHEAD][MT][2];
+    const auto sum_up = [&](auto tiles) __attribute__((always_inline)) {
+        constexpr int TILES = decltype(tiles)::value;
+        const auto rows = [&](int r) {
+            if (r >= 16 * TILES) return w + min(n0 + r - 16 * TILES, g.outer - 1) * g.w_row;
+            const int at = members[min(r, count - 1)], row = g.parts == 1 ? at : at / g.parts;
+            return (const T*)g.x + row * g.x_row + (at - row * g.parts) * g.x_part;
+        };
+        float4_t part[TILES][1];
 #pragma unroll
-        for (int u = 0; u < AHEAD; ++u) {
-            const int k = (s0 + u * kFewWaves) * BK;
-            if (s0 + u * kFewWaves < steps) {
+        for (int m = 0; m < TILES; ++m) part[m][0] = 0.0f;
+        sum_turns<T, DIRECT, TILES, 1>(part, stage0 + wave * STAGE, stage1 + wave * STAGE, stage2 + wave * STAGE, rows, g.inner, wave, lane);
 #pragma unroll
-                for (int h = 0; h < 2; ++h) a[u][h] = load(w, k + h * E);
-#pragma unroll
-                for (int m = 0; m < MT; ++m)
-                    if (m < tiles)
-#pragma unroll
-                        for (int h = 0; h < 2; ++h) b[u][m][h] = load(x[m], k + h * E);
-            }
-        }
-#pragma unroll
-        for (int u = 0; u < AHEAD; ++u)
-            if (s0 + u * kFewWaves < steps)
-#pragma unroll
-                for (int m = 0; m < MT; ++m)
-                    if (m < tiles)
-#pragma unroll
-                        for (int h = 0; h < 2; ++h) acc[m] = Few<T>::mma(a[u][h], b[u][m][h], acc[m]);
+        for (int m = 0; m < TILES; ++m) acc[m] = part[m][0];
+    };
+    if (typed || g.shared) {
+        const int tiles = (count + 15) / 16;
+        if (tiles == 1) sum_up(std::integral_constant<int, 1>());
+        if constexpr (MT >= 2)
+            if (tiles == 2) sum_up(std::integral_constant<int, 2>());
+        if constexpr (MT >= 3)
+            if (tiles == 3) sum_up(std::integral_constant<int, 3>());
+        if constexpr (MT >= 4)
+            if (tiles == 4) sum_up(std::integral_constant<int, 4>());
     }
+    __syncthreads();
 #pragma unroll
     for (int m = 0; m < MT; ++m)
 #pragma unroll
@@ -691,7 +744,24 @@ __global__ __launch_bounds__(64 * kFewWaves) void few_products(Args g) {
             if (t >= 0 && t < g.types) {
                 const float* u = g.thin + (int64_t)at * g.thin_row;
                 const T* v = (const T*)g.up + t * g.up_type + col * g.up_col;
-                for (int k = 0; k < g.rank; ++k) sum += u[k] * (float)v[k * g.up_rank];
+                if (g.up_rank == 1) {
+#pragma unroll 2
+                    for (int k = 0; k < g.rank; k += E) {
+                        union {
+                            uint4_t v;
+                            T e[E];
+                        } y;
+                        y.v = fetch<T>((const char*)(v + k), g.rank - k);
+#pragma unroll
+                        for (int j = 0; j < E; j += 4) {  // (thin rows are filled up with zeros)
+                            const float4_t z = *(const float4_t*)(u + k + j);
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) sum += z[i] * (float)y.e[j + i];
+                        }
+                    }
+                } else {
+                    for (int k = 0; k < g.rank; ++k) sum += u[k] * (float)v[k * g.up_rank];
+                }
             }
         }
         ((O*)g.out)[(int64_t)at * g.out_row + col] = (O)sum;
@@ -703,70 +773,35 @@ __global__ __launch_bounds__(64 * kFewWaves) void few_products(Args g) {
 // ---------------------------------------------------------------------------
 
 // Many rows, few columns, a long summation: bound by reading the rows. A block has 32 rows of a type and 16 NT columns; its
-// waves share the summation as those of few_products do, so that nothing passes through LDS but their sums.
+// waves share the summation as those of few_products do.
 constexpr int kThinRows = 32;
 
 template <typename T, bool DIRECT, int NT>
 __global__ __launch_bounds__(64 * kFewWaves) void thin_products(Args g) {
-    constexpr int E = 16 / (int)sizeof(T), BK = 128 / (int)sizeof(T), MT = kThinRows / 16, AHEAD = 2;
-    typedef typename Types<T>::frag frag;
-    __shared__ float sums[kFewWaves][kThinRows][16 * NT + 1];
+    constexpr int MT = kThinRows / 16, STAGE = 16 * (MT + NT) * 128;
+    __shared__ __align__(1024) char stage0[kFewWaves * STAGE], stage1[kFewWaves * STAGE], stage2[kFewWaves * STAGE];
+    typedef float Sums[kFewWaves][kThinRows][16 * NT + 1];
+    static_assert(sizeof(Sums) <= sizeof(stage0), "the sums lie where the operands did");
+    Sums& sums = *(Sums*)stage0;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const Range rows = rows_of_slot(g.ptr, blockIdx.x, kThinRows, g.types, true, g.rows, 1);
-    if (rows.lo >= rows.hi) return;
-    const int n0 = blockIdx.y * 16 * NT, count = min(kThinRows, rows.hi - rows.lo);
-    const bool typed = rows.type < g.types;
-    const int begin = 2 * E * (lane >> 4);
-    const T *x[MT], *w[NT];
-#pragma unroll
-    for (int m = 0; m < MT; ++m)
-        x[m] = (const T*)g.x + Place(g.order, rows.lo + min(16 * m + (lane & 15), count - 1), 1, g.rows).row * g.x_row + begin;
-#pragma unroll
-    for (int n = 0; n < NT; ++n)
-        w[n] = (const T*)g.w + (typed ? rows.type : 0) * g.w_type + min(n0 + 16 * n + (lane & 15), g.outer - 1) * g.w_row + begin;
-    const auto load = [&](const T* row, int k) -> frag {
-        if constexpr (DIRECT) {
-            return *(const frag*)(k + begin < g.inner ? row + k : (const T*)&kZeros);
-        } else {
-            union {
-                uint4_t v;
-                frag f;
-            } u;
-            u.v = fetch<T>((const char*)(row + k), g.inner - k - begin);
-            return u.f;
-        }
-    };
+    const Range range = rows_of_slot(g.ptr, blockIdx.x, kThinRows, g.types, true, g.rows, 1);
+    if (range.lo >= range.hi) return;
+    const int n0 = blockIdx.y * 16 * NT, count = min(kThinRows, range.hi - range.lo);
+    const bool typed = range.type < g.types;
     float4_t acc[MT][NT];
 #pragma unroll
     for (int m = 0; m < MT; ++m)
 #pragma unroll
         for (int n = 0; n < NT; ++n) acc[m][n] = 0.0f;
-    const int steps = typed ? (g.inner + BK - 1) / BK : 0;
-    for (int s0 = wave; s0 < steps; s0 += AHEAD * kFewWaves) {
-        frag a[AHEAD][NT][2], b[AHEAD][MT][2];
-#pragma unroll
-        for (int u = 0; u < AHEAD; ++u)
-            if (s0 + u * kFewWaves < steps) {
-                const int k = (s0 + u * kFewWaves) * BK;
-#pragma unroll
-                for (int m = 0; m < MT; ++m)
-#pragma unroll
-                    for (int h = 0; h < 2; ++h) b[u][m][h] = load(x[m], k + h * E);
-#pragma unroll
-                for (int n = 0; n < NT; ++n)
-#pragma unroll
-                    for (int h = 0; h < 2; ++h) a[u][n][h] = load(w[n], k + h * E);
-            }
-#pragma unroll
-        for (int u = 0; u < AHEAD; ++u)
-            if (s0 + u * kFewWaves < steps)
-#pragma unroll
-                for (int m = 0; m < MT; ++m)
-#pragma unroll
-                    for (int n = 0; n < NT; ++n)
-#pragma unroll
-                        for (int h = 0; h < 2; ++h) acc[m][n] = Few<T>::mma(a[u][n][h], b[u][m][h], acc[m][n]);
+    if (typed) {
+        const T* w = (const T*)g.w + range.type * g.w_type;
+        const auto rows = [&](int r) {
+            if (r >= kThinRows) return w + min(n0 + r - kThinRows, g.outer - 1) * g.w_row;
+            return (const T*)g.x + Place(g.order, range.lo + min(r, count - 1), 1, g.rows).row * g.x_row;
+        };
+        sum_turns<T, DIRECT, MT, NT>(acc, stage0 + wave * STAGE, stage1 + wave * STAGE, stage2 + wave * STAGE, rows, g.inner, wave, lane);
     }
+    __syncthreads();
 #pragma unroll
     for (int m = 0; m < MT; ++m)
 #pragma unroll
@@ -774,14 +809,14 @@ __global__ __launch_bounds__(64 * kFewWaves) void thin_products(Args g) {
 #pragma unroll
             for (int r = 0; r < 4; ++r) sums[wave][16 * m + (lane & 15)][16 * n + 4 * (lane >> 4) + r] = acc[m][n][r];
     __syncthreads();
-    const float by = typed ? (g.scale ? g.scale[rows.type] : 1.0f) : 0.0f;
+    const float by = typed ? (g.scale ? g.scale[range.type] : 1.0f) : 0.0f;
     for (int i = tid; i < 16 * NT * count; i += 64 * kFewWaves) {
         const int r = i / (16 * NT), c = i % (16 * NT);
         if (n0 + c >= g.out_row) continue;
         float sum = 0;
 #pragma unroll
         for (int v = 0; v < kFewWaves; ++v) sum += sums[v][r][c];
-        const int row = Place(g.order, rows.lo + r, 1, g.rows).row;
+        const int row = Place(g.order, range.lo + r, 1, g.rows).row;
         ((float*)g.out)[(int64_t)row * g.out_row + n0 + c] = n0 + c < g.outer ? sum * by : 0.0f;
     }
 }

@@ -42,7 +42,7 @@ template <typename O, bool ACROSS, bool DIRECT>
 hipError_t rows_of_size(const Args& a, bool thin_result, hipStream_t stream) {
     if constexpr (!ACROSS) {
         const int64_t rows = (int64_t)a.rows * a.parts;
-        if (few(a, false)) return rows <= 16 ? few_by<O, DIRECT, 1>(a, stream) : rows <= 32 ? few_by<O, DIRECT, 2>(a, stream) : few_by<O, DIRECT, 4>(a, stream);
+        if (few(a, false)) return rows <= 16 ? few_by<O, DIRECT, 1>(a, stream) : rows <= 32 ? few_by<O, DIRECT, 2>(a, stream) : rows <= 48 ? few_by<O, DIRECT, 3>(a, stream) : few_by<O, DIRECT, 4>(a, stream);
     }
     if constexpr (std::is_same<O, float>::value && !ACROSS)
         if (thin_result) return a.outer <= 16 ? thin_by<DIRECT, 1>(a, stream) : a.outer <= 32 ? thin_by<DIRECT, 2>(a, stream) : thin_by<DIRECT, 4>(a, stream);
