@@ -66,10 +66,10 @@ int lanes_across(int64_t vectors) {
 template <typename T, int V>
 int launch_lookup(int64_t rows, int64_t types, int64_t channels, const int64_t* type_of_row, const void* table,
                   int64_t table_row, float scale, void* out, hipStream_t s) {
-    const int across = lanes_across(channels / V);
-    const int64_t blocks = divide_up(rows, 256 / across);
+    const int across = lanes_across(channels / V), each = 256 / across * row_groups::kLookups;
+    const int64_t blocks = divide_up(rows, each);
     for (int64_t first = 0; first < blocks; first += kMostBlocks) {
-        const int64_t row = first * (256 / across);
+        const int64_t row = first * each;
         row_groups::lookup<T, V><<<(unsigned)std::min(kMostBlocks, blocks - first), 256, 0, s>>>(
             (const T*)table, table_row, type_of_row + row, rows - row, (int)types, (int)channels, across, scale,
             (T*)out + row * channels);

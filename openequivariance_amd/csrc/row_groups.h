@@ -235,27 +235,42 @@ __global__ __launch_bounds__(256) void find_types(const int* keys, int rows, int
 // ---------------------------------------------------------------------------
 
 // out[i] = scale table[types[i]], 0 where there is no type. V elements (16 bytes where everything is aligned, else one) at a
-// time; `across` lanes, a power of two, share a row. Bound by memory, or a launch.
+// time; `across` lanes, a power of two, share a row and have kLookups rows each, requested together. Bound by memory, or a launch.
+constexpr int kLookups = 4;
+
 template <typename T, int V>
 __global__ __launch_bounds__(256) void lookup(const T* table, int64_t table_row, const int64_t* types, int64_t rows, int count,
                                               int channels, int across, float scale, T* out) {
     typedef T vec __attribute__((ext_vector_type(V)));
-    const int lane = threadIdx.x & (across - 1);
-    const int64_t row = (int64_t)blockIdx.x * (256 / across) + threadIdx.x / across;
-    if (row >= rows) return;
-    const int64_t type = types[row];
-    const bool known = type >= 0 && type < count;
-    const T* from = table + (known ? type : 0) * table_row;
-    T* to = out + row * channels;
-#pragma unroll 4
-    for (int c = lane * V; c < channels; c += across * V) {
-        vec x = (T)0;
-        if (known) {
-            x = *(const vec*)(from + c);
+    const int lane = threadIdx.x & (across - 1), groups = 256 / across;
+    const int64_t row0 = (int64_t)blockIdx.x * groups * kLookups + threadIdx.x / across;
+    const T* from[kLookups];
+    bool known[kLookups];
 #pragma unroll
-            for (int e = 0; e < V; ++e) x[e] = (T)((float)x[e] * scale);
+    for (int i = 0; i < kLookups; ++i) {
+        const int64_t row = row0 + i * groups, type = row < rows ? types[row] : -1;
+        known[i] = type >= 0 && type < count;
+        from[i] = table + (known[i] ? type : 0) * table_row;
+    }
+    for (int c = lane * V; c < channels; c += across * V) {
+        vec x[kLookups];
+#pragma unroll
+        for (int i = 0; i < kLookups; ++i) {
+            x[i] = (T)0;
+            if (known[i]) x[i] = *(const vec*)(from[i] + c);
         }
-        *(vec*)(to + c) = x;
+#pragma unroll
+        for (int i = 0; i < kLookups; ++i) {
+            const int64_t row = row0 + i * groups;
+            if (row >= rows) break;
+#pragma unroll
+            for (int e = 0; e < V; ++e) {
+                float y = known[i] ? (float)x[i][e] * scale : 0.0f;
+                asm("" : "+v"(y));  // (a product of 32 bits, as elsewhere, not one that is rounded to 16 at once)
+                x[i][e] = (T)y;
+            }
+            *(vec*)(out + row * channels + c) = x[i];
+        }
     }
 }
 

@@ -4,6 +4,7 @@
 #include "typed_products_launch.h"
 
 #include <algorithm>
+#include <cmath>
 
 namespace typed_products {
 namespace {
@@ -46,23 +47,33 @@ hipError_t rows_of_size(const Args& a, bool thin_result, hipStream_t stream) {
     }
     if constexpr (std::is_same<O, float>::value && !ACROSS)
         if (thin_result) return a.outer <= 16 ? thin_by<DIRECT, 1>(a, stream) : a.outer <= 32 ? thin_by<DIRECT, 2>(a, stream) : thin_by<DIRECT, 4>(a, stream);
-    // Tiles by how many blocks there are, with half a tile of each type's rows left over.
-    const auto blocks = [&](int64_t bm, int64_t bn) {
-        const int64_t rows = (int64_t)a.rows * a.parts;
-        return (rows / bm + std::min<int64_t>(a.types, rows) / 2 + 1) * divide_up(a.out_row, bn);
+    // Tiles by an estimate, in us, of what measured tiles take: a block's beginning and end, and steps that last as long as one
+    // alone or as all blocks of a compute unit together. (Half a tile of each type's rows is left over; compute units hold four
+    // tiles of 64, two of 128, one of 256.) bf16, us with tiles of 64 / 128 / 256: 1 000 rows, 4 matrices of 1024 x 1024 10 / 16 / 31,
+    // 8 000 34 / 39 / 36, 16 000 63 / 48 / 68; 4 001 rows, 16 of 2048 x 2048 70 / 68 / 60, one of 4096 x 4096 207 / 148 / 125;
+    // float32: 5 000 rows, 5 of 512 x 512 36 / 43, 20 000 rows, 10 of 128 x 128 14 / 18.
+    constexpr bool SHORT = sizeof(T) == 2;
+    constexpr int64_t BK = 128 / (int)sizeof(T);
+    const int64_t rows = (int64_t)a.rows * a.parts;
+    const double steps = (double)(divide_up(a.inner, BK) + divide_up((SHORT ? 2 : 1) * (int64_t)(a.rank ? a.thin_row : 0), BK));
+    const auto takes = [&](int64_t tile, int at_once, double ends, double alone, double together) {
+        const int64_t blocks = (rows / tile + std::min<int64_t>(a.types, rows) / 2 + 1) * divide_up(a.out_row, tile);
+        const double mean = blocks / 256.0, each = mean < 1 ? mean : (mean + std::ceil(mean)) / 2;  // (of a compute unit)
+        return ends * std::max(1.0, each / at_once) + steps * std::max(alone, each * together);
     };
+    const double small = takes(64, 4, 6, SHORT ? 0.5 : 0.7, SHORT ? 0.22 : 0.5), middle = takes(128, 2, 6, SHORT ? 0.7 : 2, SHORT ? 0.62 : 1.95);
     constexpr bool MAY_BE_THIN = std::is_same<O, T>::value;
-    if (a.out_row <= 64 || blocks(128, 128) < 256) {
-        if constexpr (MAY_BE_THIN)
-            if (a.rank) return rows_by<O, ACROSS, DIRECT, true, 64, 64, 2, 2>(a, stream);
-        return rows_by<O, ACROSS, DIRECT, false, 64, 64, 2, 2>(a, stream);
-    }
-    if constexpr (DIRECT && sizeof(T) == 2)
-        if (blocks(256, 256) >= 256) {
+    if constexpr (DIRECT && SHORT)
+        if (takes(256, 1, 12, 1.37, 1.95) < std::min(small, middle)) {
             if constexpr (MAY_BE_THIN)
                 if (a.rank) return rows_by<O, ACROSS, DIRECT, true, 256, 256, 2, 4>(a, stream);
             return rows_by<O, ACROSS, DIRECT, false, 256, 256, 2, 4>(a, stream);
         }
+    if (small < middle) {
+        if constexpr (MAY_BE_THIN)
+            if (a.rank) return rows_by<O, ACROSS, DIRECT, true, 64, 64, 2, 2>(a, stream);
+        return rows_by<O, ACROSS, DIRECT, false, 64, 64, 2, 2>(a, stream);
+    }
     if constexpr (MAY_BE_THIN)
         if (a.rank) return rows_by<O, ACROSS, DIRECT, true, 128, 128, 2, 2>(a, stream);
     return rows_by<O, ACROSS, DIRECT, false, 128, 128, 2, 2>(a, stream);
