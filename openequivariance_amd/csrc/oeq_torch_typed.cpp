@@ -247,9 +247,8 @@ Tensor3 typed_linear_backward_gpu(const Tensor& grad, const Tensor& x, const Ten
     const int64_t count = weight.size(0), outer = weight.size(1), inner = weight.size(2);
     Groups index(types, count, order, ptr);
     const auto none = [&] { return at::empty({0}, x.options()); };
-    Tensor dx = none(), dw = none(), db = none();
+    Tensor dx = want_x ? at::empty(x.sizes(), x.options()) : none(), dw, db;
     if (want_x) {
-        dx = at::empty(x.sizes(), x.options());
         if (dx.numel()) {
             const Strided g(grad);
             const Matrices w(weight);
@@ -259,8 +258,8 @@ Tensor3 typed_linear_backward_gpu(const Tensor& grad, const Tensor& x, const Ten
             check(oeq_typed_product(&a, dx.data_ptr(), dev.stream), "oeq_typed_product");
         }
     }
-    if (want_weight) dw = typed_sum(grad, x, 0, outer, inner, x, index, dev.stream);
-    if (want_bias) db = type_sum(grad, index, 1.0, dev.stream);
+    dw = want_weight ? typed_sum(grad, x, 0, outer, inner, x, index, dev.stream) : none();
+    db = want_bias ? type_sum(grad, index, 1.0, dev.stream) : none();
     return {dx, dw, db};
 }
 
@@ -337,10 +336,9 @@ Tensor4 adapter_linear_backward_gpu(const Tensor& grad, const Tensor& x, const T
     Groups index(types, count, order, ptr);
     const Tensor u = thin.contiguous();
     const auto none = [&] { return at::empty({0}, x.options()); };
-    Tensor dx = none(), dw = none(), ddown = none(), dup = none(), v;
+    Tensor dx = want_x ? at::empty(x.sizes(), x.options()) : none(), dw, ddown, dup, v;
     if (want_x || want_down) v = thin_product(grad, up, true, scale, index, dev.stream);
     if (want_x) {
-        dx = at::empty(x.sizes(), x.options());
         if (dx.numel()) {
             const Strided g(grad);
             const Matrices w(weight);
@@ -351,12 +349,14 @@ Tensor4 adapter_linear_backward_gpu(const Tensor& grad, const Tensor& x, const T
             check(oeq_typed_product(&a, dx.data_ptr(), dev.stream), "oeq_typed_product");
         }
     }
-    if (want_down) ddown = typed_sum(v, x, 1, rank, inner, x, index, dev.stream);
-    if (want_up) dup = typed_sum(grad, u, 2, outer, rank, x, index, dev.stream);
+    ddown = want_down ? typed_sum(v, x, 1, rank, inner, x, index, dev.stream) : none();
+    dup = want_up ? typed_sum(grad, u, 2, outer, rank, x, index, dev.stream) : none();
     if (want_weight) {
         const Tensor one = at::zeros({x.size(0)}, types.options());  // (all rows are of one type)
         Groups all(one, 1, {}, {});
         dw = typed_sum(grad, x, 0, outer, inner, x, all, dev.stream).squeeze(0);
+    } else {
+        dw = none();
     }
     return {dx, dw, ddown, dup};
 }

@@ -20,7 +20,6 @@ constexpr int kBits = 8, kDigits = 1 << kBits;
 constexpr int kWaves = 16, kThreads = 64 * kWaves;
 constexpr int kOneBlock = 8 * kThreads;  // rows that one block sorts in LDS
 constexpr int kMostBlocks = 256;         // of a pass: every block adds up what all of them counted
-constexpr int kRound = kThreads;         // rows that a block places at a time
 
 __device__ __forceinline__ int key_of(int64_t type, int types) { return type >= 0 && type < types ? (int)type : types; }
 
@@ -184,7 +183,7 @@ __global__ __launch_bounds__(kThreads) void place_rows(Source from, int rows, in
         if (ptr && blockIdx.x == 0 && tid <= count) ptr[tid] = before;
     }
     const int first = blockIdx.x * span, end = first + min(rows - first, span);
-    for (int base = first; base < end; base += kRound) {
+    for (int base = first; base < end; base += kThreads) {
         __syncthreads();
         for (int i = tid; i < kWaves * kDigits; i += kThreads) ((int*)round)[i] = 0;
         __syncthreads();

@@ -837,7 +837,7 @@ __device__ __forceinline__ auto widened(typename Types<T>::frag x) {
 // A tile of BM columns of a and BN columns of b, summed over the rows of a slot. BK rows at a time; rows past the end are zeros.
 // PARTS: rows have more than one. (A kernel of its own: branches inside the loop send the sums through other registers and back.)
 template <typename A, typename B, typename O, bool DIRECT, bool PARTS, int BM, int BN, int WM, int WN>
-__global__ __launch_bounds__(64 * WM * WN, BM * BN == WM * WN * 128 * 128 ? 1 : 2) void sum_products(SumArgs g) {
+__global__ __launch_bounds__(64 * WM * WN) void sum_products(SumArgs g) {
     constexpr int WAVES = WM * WN, BK = sizeof(A) + sizeof(B) == 4 ? 64 : 32;
     constexpr bool MIXED = sizeof(A) != sizeof(B);
     constexpr int EA = 16 / (int)sizeof(A), EB = 16 / (int)sizeof(B);

@@ -33,7 +33,7 @@ def draw_types(gen, rows, count, outside=0.1):
 # ---------------------------------------------------------------------------------------------------------------------
 
 
-@pytest.mark.parametrize("rows", [0, 1, 63, 65, 1023, 8191, 8192, 8193, 20000, 300001])
+@pytest.mark.parametrize("rows", [0, 1, 63, 65, 1023, 8191, 8192, 8193, 20000, 32769, 300001])
 @pytest.mark.parametrize("count", [0, 1, 3, 255, 256, 65535, 65536, 70001])
 def test_group_rows(rows, count):
     gen = torch.Generator().manual_seed(rows + count)
@@ -190,6 +190,15 @@ def test_linear_of_nothing(rows, components, count, inner, outer):
         assert (dw[0] == n).all() and not dw[1:].any() and (db[0] == n).all() and not db[1:].any()
 
 
+def test_linear_of_no_components():
+    x, weight = torch.ones(5, 0, 8, device="cuda", requires_grad=True), torch.ones(2, 3, 8, device="cuda", requires_grad=True)
+    bias, types = torch.ones(2, 3, device="cuda", requires_grad=True), torch.zeros(5, dtype=torch.int64, device="cuda")
+    out = oeq.typed_linear(x, weight, types, bias)
+    assert out.shape == (5, 0, 3)
+    dx, dw, db = torch.autograd.grad(out, (x, weight, bias), torch.ones_like(out))
+    assert dx.shape == x.shape and not dw.any() and not db.any()
+
+
 def test_rows_without_a_type_have_no_influence():
     """Whatever such rows and the matrices of types without rows hold; nor do rows of one type reach another's results."""
     for dtype in DTYPES:
@@ -215,6 +224,26 @@ def test_linear_with_a_type_of_many_rows():
     for dtype in DTYPES:
         x, weight, types, bias, grad = linear_case(30001, 0, 2, 40, 24, True, dtype, outside=0.01)
         compare_linear(x, weight, types, bias, grad)
+
+
+def test_far_offsets():
+    """Rows, and matrices, that begin past 2^31 elements of their tensor."""
+    table = torch.zeros(9, 1 << 28, device="cuda", dtype=torch.float16)
+    table[8, :64] = torch.arange(64)
+    types = torch.tensor([8, 0, 8], device="cuda")
+    part = table[:, :64]
+    assert torch.equal(oeq.type_embedding(types, part)[0], part[8])
+    weight = table.view(9, 1 << 14, 1 << 14)[:, :8, :64]  # [types, 8, 64], 2^28 elements apart
+    for rows in (3, 200):
+        x = torch.ones(rows, 64, device="cuda", dtype=torch.float16)
+        out = oeq.typed_linear(x, weight, torch.full((rows,), 8, device="cuda"))
+        assert (out[:, 0] == 2016).all() and not out[:, 1:].any()
+    out = oeq.typed_linear(table[:, :64], torch.ones(1, 8, 64, device="cuda", dtype=torch.float16), torch.zeros(9, dtype=torch.int64, device="cuda"))
+    assert (out[8] == 2016).all() and not out[:8].any()
+    w = torch.ones(1, 8, 64, device="cuda", dtype=torch.float16, requires_grad=True)
+    grad = torch.ones(9, 8, device="cuda", dtype=torch.float16)
+    got, = torch.autograd.grad(oeq.typed_linear(table[:, :64], w, torch.zeros(9, dtype=torch.int64, device="cuda")), w, grad)
+    assert torch.equal(got[0, 0], table[8, :64])
 
 
 def test_linear_second_derivatives():
