@@ -7,6 +7,8 @@
 // equal, so the last leaves rows of a type ascending and every sum over a type's rows has one order. A pass has two launches:
 // blocks count the digits of their span of rows; then each block adds up the counts before its own (all digits below, and
 // the same digit in the blocks before) and places its rows. Up to kOneBlock rows one block does all passes in LDS in one launch.
+// Launches and chains of waits are all that it takes: 333 rows 3.7 us, 4 001 9, 20 000 3.5 and 6; of 32 003 types two passes and the
+// search for their beginnings 24. (Every block counting all rows instead of the first launch: 18 us, not 9.)
 #ifndef OEQ_ROW_GROUPS_H
 #define OEQ_ROW_GROUPS_H
 
@@ -277,10 +279,13 @@ __global__ __launch_bounds__(256) void lookup(const T* table, int64_t table_row,
 // sums of rows by type
 // ---------------------------------------------------------------------------
 
-// out[t] = scale sum_{i of type t} rows[i], in 32 bits and in the index's order. A type of up to kChunk rows is summed by
-// the blocks of the type, longer ones in two steps: chunks of kChunk places of the index sum what they hold of a longer
-// type (a chunk holds parts of two at most: the one that it begins in and the one that it ends in), and the chunk in which a
-// longer type begins adds up the chunks' sums in order.
+// out[t] = scale sum_{i of type t} rows[i], in 32 bits and in an order that the index alone decides. A type of up to kChunk rows is
+// summed by a group of lanes of its own, longer ones in two steps: chunks of kChunk places of the index sum what they hold of
+// a longer type (a chunk holds parts of two at most: the one that it begins in and the one that it ends in), and the chunk in
+// which a longer type begins adds up the chunks' sums.
+// Bound by memory and a chain of waits (place, type, bounds, row): 20 000 rows of 512 floats, 89 types of which one has 12 400,
+// 14 us and 9 for the long ones' join; 16 411 rows of 1 024, 32 003 types, bf16, 20 (98 MB, 4.8 TB/s) and 8. (Chunks of 64 rows:
+// 16 and 7, 20 and 5. The join with a few groups of lanes, each with many chunks: 28.)
 constexpr int kChunk = 32;
 
 struct Sums {

@@ -11,7 +11,15 @@
 // A row can have several parts (the components of an irrep), which share its type: they count as rows here.
 //
 // Products run on the 32x32 matrix instructions, sums in 32 bits. Tiles of both operands go from memory to LDS 128 bytes of
-// the summation at a time, into one of two buffers while the products read the other.
+// the summation at a time, into one of two buffers while the products read the other; there is one barrier a step. Nothing is
+// rounded to fewer bits but the results, and what lies between two thin products, which keeps 16 bits or more (row_products).
+//
+// What bounds them and what they reach, bf16 if nothing else is said: large products the matrix units and the card's power, 8 192 rows
+// of one 8192 x 8192 matrix 953 us, 1.15 PFLOP/s (1.13 to 1.26 for the library's product there, which has neither types nor
+// rows in another order; gradient of x 912, of the weights 983), float32 4096 x 4096 2.06 ms, 134 TFLOP/s of 154. Of shorter sums the beginning and end of a tile
+// take a share, some 12 us of a tile of 256 x 256 where all compute units write at a time: 32 768 rows, 16 matrices of
+// 2048 x 5632 800 us, 0.95 PFLOP/s. (Blocks that stay for several tiles took 820.) Few rows: memory, 64 rows of 64 types,
+// 2048 x 2048, 69 us, 4.9 TB/s of the matrices that are read.
 #ifndef OEQ_TYPED_PRODUCTS_H
 #define OEQ_TYPED_PRODUCTS_H
 
@@ -663,7 +671,7 @@ __device__ __forceinline__ void sum_turns(float4_t (&acc)[X][W], char* stage0, c
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
 }
 
-// MT: tiles of 16 rows. blockIdx.x: columns; blockIdx.y: rows, of which the first of a type stands for all; with shared
+// MT: tiles of 16 rows at a time. blockIdx.x: columns; blockIdx.y: rows, of which the first of a type stands for all; with shared
 // weights: every 16 MT rows.
 template <typename T, typename O, bool DIRECT, int MT>
 __global__ __launch_bounds__(64 * kFewWaves) void few_products(Args g) {
@@ -695,76 +703,80 @@ __global__ __launch_bounds__(64 * kFewWaves) void few_products(Args g) {
     __syncthreads();
     const bool typed = type < g.types;
     const T* w = (const T*)g.w + (typed ? type : 0) * g.w_type;
-    float4_t acc[MT];
-#pragma unroll
-    for (int m = 0; m < MT; ++m) acc[m] = 0.0f;
-    const auto sum_up = [&](auto tiles) __attribute__((always_inline)) {
-        constexpr int TILES = decltype(tiles)::value;
-        const auto rows = [&](int r) {
-            if (r >= 16 * TILES) return w + min(n0 + r - 16 * TILES, g.outer - 1) * g.w_row;
-            const int at = members[min(r, count - 1)], row = g.parts == 1 ? at : at / g.parts;
-            return (const T*)g.x + row * g.x_row + (at - row * g.parts) * g.x_part;
-        };
-        float4_t part[TILES][1];
-#pragma unroll
-        for (int m = 0; m < TILES; ++m) part[m][0] = 0.0f;
-        sum_turns<T, DIRECT, TILES, 1>(part, stage0 + wave * STAGE, stage1 + wave * STAGE, stage2 + wave * STAGE, rows, g.inner, wave, lane);
-#pragma unroll
-        for (int m = 0; m < TILES; ++m) acc[m] = part[m][0];
-    };
-    if (typed || g.shared) {
-        const int tiles = (count + 15) / 16;
-        if (tiles == 1) sum_up(std::integral_constant<int, 1>());
-        if constexpr (MT >= 2)
-            if (tiles == 2) sum_up(std::integral_constant<int, 2>());
-        if constexpr (MT >= 3)
-            if (tiles == 3) sum_up(std::integral_constant<int, 3>());
-        if constexpr (MT >= 4)
-            if (tiles == 4) sum_up(std::integral_constant<int, 4>());
-    }
-    __syncthreads();
-#pragma unroll
-    for (int m = 0; m < MT; ++m)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) sums[wave][16 * m + (lane & 15)][4 * (lane >> 4) + r] = acc[m][r];
-    __syncthreads();
     const float by = g.scale ? (typed ? g.scale[type] : 0.0f) : 1.0f;
-    for (int i = tid; i < 16 * count; i += 64 * kFewWaves) {
-        const int r = i / 16, col = n0 + i % 16;
-        if (col >= g.out_row) continue;
-        float sum = 0;
+    for (int first = 0; first < count; first += 16 * MT) {
+        const int here = min(16 * MT, count - first);
+        float4_t acc[MT];
 #pragma unroll
-        for (int v = 0; v < kFewWaves; ++v) sum += sums[v][r][i % 16];
-        sum *= by;
-        const int at = members[r];
-        if (col >= g.outer) sum = 0;
-        else if (g.bias && typed) sum += (float)((const T*)g.bias)[type * g.bias_type + col];
-        else if (g.thin) {
-            const int64_t t = g.type_of_row[at];
-            if (t >= 0 && t < g.types) {
-                const float* u = g.thin + (int64_t)at * g.thin_row;
-                const T* v = (const T*)g.up + t * g.up_type + col * g.up_col;
-                if (g.up_rank == 1) {
+        for (int m = 0; m < MT; ++m) acc[m] = 0.0f;
+        const auto sum_up = [&](auto tiles) __attribute__((always_inline)) {
+            constexpr int TILES = decltype(tiles)::value;
+            const auto rows = [&](int r) {
+                if (r >= 16 * TILES) return w + min(n0 + r - 16 * TILES, g.outer - 1) * g.w_row;
+                const int at = members[first + min(r, here - 1)], row = g.parts == 1 ? at : at / g.parts;
+                return (const T*)g.x + row * g.x_row + (at - row * g.parts) * g.x_part;
+            };
+            float4_t part[TILES][1];
+#pragma unroll
+            for (int m = 0; m < TILES; ++m) part[m][0] = 0.0f;
+            sum_turns<T, DIRECT, TILES, 1>(part, stage0 + wave * STAGE, stage1 + wave * STAGE, stage2 + wave * STAGE, rows, g.inner, wave, lane);
+#pragma unroll
+            for (int m = 0; m < TILES; ++m) acc[m] = part[m][0];
+        };
+        if (typed || g.shared) {
+            const int tiles = (here + 15) / 16;
+            if (tiles == 1) sum_up(std::integral_constant<int, 1>());
+            if constexpr (MT >= 2)
+                if (tiles == 2) sum_up(std::integral_constant<int, 2>());
+            if constexpr (MT >= 3)
+                if (tiles == 3) sum_up(std::integral_constant<int, 3>());
+            if constexpr (MT >= 4)
+                if (tiles == 4) sum_up(std::integral_constant<int, 4>());
+        }
+        __syncthreads();
+#pragma unroll
+        for (int m = 0; m < MT; ++m)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) sums[wave][16 * m + (lane & 15)][4 * (lane >> 4) + r] = acc[m][r];
+        __syncthreads();
+        for (int i = tid; i < 16 * here; i += 64 * kFewWaves) {
+            const int r = i / 16, col = n0 + i % 16;
+            if (col >= g.out_row) continue;
+            float sum = 0;
+#pragma unroll
+            for (int v = 0; v < kFewWaves; ++v) sum += sums[v][r][i % 16];
+            sum *= by;
+            const int at = members[first + r];
+            if (col >= g.outer) sum = 0;
+            else if (g.bias && typed) sum += (float)((const T*)g.bias)[type * g.bias_type + col];
+            else if (g.thin) {
+                const int64_t t = g.type_of_row[at];
+                if (t >= 0 && t < g.types) {
+                    const float* u = g.thin + (int64_t)at * g.thin_row;
+                    const T* v = (const T*)g.up + t * g.up_type + col * g.up_col;
+                    if (g.up_rank == 1) {
 #pragma unroll 2
-                    for (int k = 0; k < g.rank; k += E) {
-                        union {
-                            uint4_t v;
-                            T e[E];
-                        } y;
-                        y.v = fetch<T>((const char*)(v + k), g.rank - k);
+                        for (int k = 0; k < g.rank; k += E) {
+                            union {
+                                uint4_t v;
+                                T e[E];
+                            } y;
+                            y.v = fetch<T>((const char*)(v + k), g.rank - k);
 #pragma unroll
-                        for (int j = 0; j < E; j += 4) {  // (thin rows are filled up with zeros)
-                            const float4_t z = *(const float4_t*)(u + k + j);
+                            for (int j = 0; j < E; j += 4) {  // (thin rows are filled up with zeros)
+                                const float4_t z = *(const float4_t*)(u + k + j);
 #pragma unroll
-                            for (int i = 0; i < 4; ++i) sum += z[i] * (float)y.e[j + i];
+                                for (int i = 0; i < 4; ++i) sum += z[i] * (float)y.e[j + i];
+                            }
                         }
+                    } else {
+                        for (int k = 0; k < g.rank; ++k) sum += u[k] * (float)v[k * g.up_rank];
                     }
-                } else {
-                    for (int k = 0; k < g.rank; ++k) sum += u[k] * (float)v[k * g.up_rank];
                 }
             }
+            ((O*)g.out)[(int64_t)at * g.out_row + col] = (O)sum;
         }
-        ((O*)g.out)[(int64_t)at * g.out_row + col] = (O)sum;
+        __syncthreads();  // (the sums lie where the next rows' operands go)
     }
 }
 

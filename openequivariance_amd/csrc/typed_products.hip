@@ -42,8 +42,13 @@ hipError_t thin_by(const Args& a, hipStream_t stream) {
 template <typename O, bool ACROSS, bool DIRECT>
 hipError_t rows_of_size(const Args& a, bool thin_result, hipStream_t stream) {
     if constexpr (!ACROSS) {
-        const int64_t rows = (int64_t)a.rows * a.parts;
-        if (few(a, false)) return rows <= 16 ? few_by<O, DIRECT, 1>(a, stream) : rows <= 32 ? few_by<O, DIRECT, 2>(a, stream) : rows <= 48 ? few_by<O, DIRECT, 3>(a, stream) : few_by<O, DIRECT, 4>(a, stream);
+        if (few(a, false)) {
+            // As many rows at a time as a type has about twice: with more, fewer blocks fit a compute unit, with fewer a type's
+            // matrix is read again. 64 rows of 64 types, 2048 x 2048, bf16: 103 us for 64 rows at a time, 69 for 16.
+            const int64_t all = (int64_t)a.rows * a.parts, at_a_time = a.shared ? all : 2 * divide_up(all, std::max(1, std::min(a.types, a.rows)));
+            return at_a_time <= 16 ? few_by<O, DIRECT, 1>(a, stream) : at_a_time <= 32 ? few_by<O, DIRECT, 2>(a, stream)
+                   : at_a_time <= 48 ? few_by<O, DIRECT, 3>(a, stream) : few_by<O, DIRECT, 4>(a, stream);
+        }
     }
     if constexpr (std::is_same<O, float>::value && !ACROSS)
         if (thin_result) return a.outer <= 16 ? thin_by<DIRECT, 1>(a, stream) : a.outer <= 32 ? thin_by<DIRECT, 2>(a, stream) : thin_by<DIRECT, 4>(a, stream);
