@@ -72,7 +72,7 @@ class StructureTransformer(torch.nn.Module):
 
     def gather(self, species, xyz, rows, cols):
         """Scalar features of the atoms from the edges (receiver, sender) to atoms placed before them."""
-        own = self.embed(species)
+        own = oeq.type_embedding(species, self.embed.weight)
         vector = xyz[rows] - xyz[cols]
         length = vector.norm(dim=1, keepdim=True).clamp(min=1e-3)
         harmonics = torch.cat([torch.ones_like(length), math.sqrt(3.0) * vector / length], dim=1)
