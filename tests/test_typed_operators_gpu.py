@@ -113,7 +113,8 @@ SHAPES = [  # rows, components, types, in, out, bias
     (1, 0, 1, 1, 1, True), (1, 0, 5, 64, 64, False), (17, 0, 3, 8, 8, True), (63, 0, 64, 256, 96, False), (65, 0, 2, 72, 40, True),
     (129, 0, 1, 128, 128, False), (300, 3, 4, 64, 128, False), (200, 5, 10, 131, 93, True), (777, 0, 7, 131, 93, True),
     (1000, 0, 3, 512, 264, True), (257, 1, 2, 20, 300, False), (40, 7, 3, 136, 24, False), (2500, 0, 1, 64, 32, True),
-    (1500, 2, 2, 32, 64, False), (600, 0, 40, 200, 520, True), (30, 0, 3, 4, 2, False), (2100, 0, 2, 640, 768, False)]
+    (1500, 2, 2, 32, 64, False), (600, 0, 40, 200, 520, True), (30, 0, 3, 4, 2, False), (2100, 0, 2, 640, 768, False),
+    (300, 0, 63, 72, 40, False), (300, 0, 65, 72, 40, True), (900, 2, 300, 40, 24, False)]
 
 
 def linear_case(rows, components, count, inner, outer, bias, dtype, seed=0, outside=0.1):
@@ -316,7 +317,8 @@ def compare_adapters(x, weight, down, up, types, scale, grad, index=None):
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("rows,count,inner,outer,rank", [
     (1, 1, 8, 8, 1), (5, 3, 64, 128, 8), (48, 32, 256, 192, 16), (64, 2, 100, 36, 6), (65, 4, 128, 128, 4), (333, 5, 131, 67, 6),
-    (500, 3, 512, 264, 64), (150, 1, 64, 520, 128), (20, 2, 1024, 48, 130), (700, 40, 72, 80, 20), (33, 4, 40, 40, 0)])
+    (500, 3, 512, 264, 64), (150, 1, 64, 520, 128), (20, 2, 1024, 48, 130), (700, 40, 72, 80, 20), (33, 4, 40, 40, 0), (20, 0, 64, 72, 8),
+    (300, 0, 64, 72, 8), (400, 63, 64, 72, 8), (400, 70, 64, 72, 8), (100, 2, 64, 72, 8), (129, 2, 64, 72, 8)])
 def test_adapters(rows, count, inner, outer, rank, dtype):
     case = adapter_case(rows, count, inner, outer, rank, dtype)
     first = compare_adapters(*case)
