@@ -47,7 +47,7 @@ struct Args {
 struct SumArgs {
     const void *a, *b;
     void* out;
-    float* partial;  // [slots, a columns, b columns]
+    float* partial;  // [shares, a columns, b columns]
     const int *order, *ptr;
     int64_t a_row, a_part, b_row, b_part;
     int rows, types, parts, a_columns, b_columns;
@@ -846,6 +846,10 @@ __device__ __forceinline__ auto widened(typename Types<T>::frag x) {
         return x;
 }
 
+// Where the share of a slot lies, of a type that has more than one: such a type has more than `chunk` rows, so of the shares that begin in
+// a stretch of that many rows one at most is its type's first, and one at most is not.
+__device__ __forceinline__ int64_t share_of(int lo, int chunk, bool first) { return 2 * (int64_t)(lo / chunk) + first; }
+
 // A tile of BM columns of a and BN columns of b, summed over the rows of a slot. BK rows at a time; rows past the end are zeros.
 // PARTS: rows have more than one. (A kernel of its own: branches inside the loop send the sums through other registers and back.)
 template <typename A, typename B, typename O, bool DIRECT, bool PARTS, int BM, int BN, int WM, int WN>
@@ -1026,7 +1030,7 @@ __global__ __launch_bounds__(64 * WM * WN) void sum_products(SumArgs g) {
     const int l = __builtin_amdgcn_mbcnt_hi(~0u, __builtin_amdgcn_mbcnt_lo(~0u, 0));
     const int64_t size = (int64_t)g.a_columns * g.b_columns;
     O* out = (O*)g.out + rows.type * size;
-    float* partial = g.partial + slot * size;
+    float* partial = g.partial + share_of(rows.lo, g.chunk, rows.lo == begin) * size;
 #pragma unroll
     for (int m = 0; m < TM; ++m)
 #pragma unroll
@@ -1053,14 +1057,14 @@ __global__ __launch_bounds__(256) void join_slots(SumArgs g) {
     const int begin = begin_of(g.ptr, t, g.rows, g.parts), n = begin_of(g.ptr, t + 1, g.rows, g.parts) - begin;
     if (n <= g.chunk) return;
     const int64_t size = (int64_t)g.a_columns * g.b_columns;
-    const float* from = g.partial + ((int64_t)begin / g.chunk + t) * size;
+    const float* from = g.partial;
     const int slots = (n - 1) / g.chunk + 1;
     for (int64_t block = blockIdx.x; block * 16 * V < size; block += gridDim.x) {
         const int64_t i = (block * 16 + lane) * V;
         vec sum = 0.0f;
         if (i < size)
 #pragma unroll 4
-            for (int s = group; s < slots; s += 16) sum += *(const vec*)(from + s * size + i);
+            for (int s = group; s < slots; s += 16) sum += *(const vec*)(from + share_of(begin + s * g.chunk, g.chunk, s == 0) * size + i);
         lds[group][lane] = sum;
         __syncthreads();
         if (group == 0 && i < size) {

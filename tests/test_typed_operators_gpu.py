@@ -225,6 +225,17 @@ def test_linear_with_a_type_of_many_rows():
     for dtype in DTYPES:
         x, weight, types, bias, grad = linear_case(30001, 0, 2, 40, 24, True, dtype, outside=0.01)
         compare_linear(x, weight, types, bias, grad)
+        x, weight, types, bias, grad = linear_case(3000, 3, 5, 72, 40, False, dtype)
+        compare_linear(x, weight, types, bias, grad)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_linear_with_one_frequent_type_of_many(dtype):
+    """Types whose tiles fill the card together, of which two have most of the rows, next to each other in the index."""
+    x, weight, types, _, grad = linear_case(13001, 0, 80, 392, 392, False, dtype)
+    types[:] = torch.where(torch.arange(13001, device="cuda") % 4 == 0, types, 40 + torch.arange(13001, device="cuda") % 3 % 2)
+    compare_linear(x, weight, types, None, grad)
+    compare_linear(x[:, :131], weight[:, :65, :131], types, None, grad[:, :65])
 
 
 def test_far_offsets():
