@@ -165,9 +165,10 @@ struct Cut {
                                                                                                                      : kSmallSumTile;
         if (!a.thin && direct && a.parts == 1 && a.type != OEQ_FLOAT32 && a.types * tiles(kLargeSumTile) >= 256) tile = kLargeSumTile;
         chunk = rows + 1;
-        // Every type's tiles fill the card, or sums are so short that they end before a second launch has begun (whose grid has
-        // room for so many types).
-        if (tiles(tile) >= 256 || rows <= kShort || a.types > 65535) return;
+        // Every type's tiles fill the card, or large ones of all types together several times over (the second launch, which comes whether
+        // there is anything to join or not, cost 16 411 rows, 32 matrices of 1024 x 2048, a training step of 390 us, 10 % of it), or sums are
+        // so short that they end before that launch has begun (whose grid has room for so many types).
+        if (tiles(tile) >= 256 || (tile == kLargeSumTile && a.types * tiles(tile) >= kBlocks) || rows <= kShort || a.types > 65535) return;
         if (tile == kLargeSumTile || a.types * tiles(tile) >= kBlocks) {
             // All types' tiles together fill it: cut only what would go on when the others have ended. 20 000 rows, 89 types
             // of which one has 12 400, 512 x 512, float32: 208 us, 851 without.

@@ -100,7 +100,7 @@ hipError_t sums_by(SumArgs g, hipStream_t stream) {
     if (g.partial) {
         const int64_t size = (int64_t)g.a_columns * g.b_columns;
         // (most blocks are of types with nothing to join)
-        const int64_t most = std::max(32, (1 << 12) / g.types);
+        const int64_t most = std::max(32, (1 << 14) / g.types);
         const auto grid = [&](int each) { return dim3((unsigned)std::min(divide_up(size, 16 * each), most), (unsigned)g.types); };
         if (size % 4 == 0 && ((uintptr_t)g.out & 15) == 0)
             join_slots<O, 4><<<grid(4), 256, 0, stream>>>(g);
