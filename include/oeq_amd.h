@@ -493,7 +493,7 @@ int oeq_typed_thin_product(const oeq_typed_rows* a, const float* scale, float* o
 /* out[t] = sum over the rows of type t (and their parts) of a_i^T b_i: [types, a_columns, b_columns], contiguous. */
 typedef struct {
     int32_t type;            /* of a, b and out */
-    int32_t thin;            /* 1: a is float, 2: b is float, else 0 */
+    int32_t thin;            /* 1: a is float, 2: b is float (one part a row), else 0 */
     int64_t rows, parts;
     int64_t types, a_columns, b_columns;
     int64_t a_row_stride, a_part_stride, b_row_stride, b_part_stride;

@@ -340,6 +340,8 @@ int oeq_typed_sum_products(const oeq_typed_sum* a, void* out, void* workspace, s
     if (a->a_columns < 0 || a->b_columns < 0 || a->a_columns > INT_MAX - 256 || a->b_columns > INT_MAX - 256)
         return fail(OEQ_ERR_INVALID, "%s: %lld and %lld columns", who, (long long)a->a_columns, (long long)a->b_columns);
     if (a->thin < 0 || a->thin > 2) return fail(OEQ_ERR_INVALID, "%s: thin operand %d", who, a->thin);
+    // (the kernel of mixed operands is built for rows of one part: it would look places times parts up in the index)
+    if (a->thin && a->parts != 1) return fail(OEQ_ERR_INVALID, "%s: a thin operand of %lld parts", who, (long long)a->parts);
     for (int64_t s : {a->a_row_stride, a->a_part_stride, a->b_row_stride, a->b_part_stride})
         if (s < 0 || s > kMostStride) return fail(OEQ_ERR_INVALID, "%s: a stride of %lld elements", who, (long long)s);
     if (a->types == 0 || a->a_columns == 0 || a->b_columns == 0) return OEQ_OK;

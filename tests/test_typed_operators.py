@@ -150,6 +150,15 @@ def test_c_abi_refuses_sums_of_products():
     refused(call(many, 16, 16, need - 1, None), "workspace")
 
 
+@pytest.mark.parametrize("type_", [0, 1, 2])
+@pytest.mark.parametrize("thin", [1, 2])
+def test_c_abi_refuses_a_thin_operand_of_several_parts(type_, thin):
+    """A float operand beside others has one part a row: the kernel of mixed operands counts rows of the index."""
+    fields = dict(type=type_, thin=thin, rows=10, parts=2, types=3, a_columns=32, b_columns=16, a_row_stride=64, a_part_stride=32,
+                  b_row_stride=32, b_part_stride=16, a=16, b=16, order=16, ptr=16)
+    refused(rt.load_library().oeq_typed_sum_products(ctypes.byref(rt._TypedSum(**fields)), 16, None, 0, None), "parts")
+
+
 def test_no_kernel_has_scratch_memory():
     blob = rt.lib_path().read_bytes()
     names, at = {}, 0
