@@ -13,21 +13,25 @@ typedef OEQ_PRODUCT_TYPE T;
 
 int64_t divide_up(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
+// Threads along the first dimension of a launch are counted in 32 bits.
+bool too_many(int64_t blocks, int threads) { return blocks * threads > UINT32_MAX; }
+
 template <typename O, bool ACROSS, bool DIRECT, bool THIN, int BM, int BN, int WM, int WN>
 hipError_t rows_by(Args a, hipStream_t stream) {
     a.slots = (int)((int64_t)a.rows * a.parts / BM + a.types + 1);
     a.tiles = (int)divide_up(a.out_row, BN);
     const int64_t blocks = (int64_t)a.slots * a.tiles;
-    if (blocks > (1 << 24) - 1) return hipErrorInvalidConfiguration;
+    if (too_many(blocks, 64 * WM * WN)) return hipErrorInvalidConfiguration;
     row_products<T, O, ACROSS, DIRECT, THIN, BM, BN, WM, WN><<<(unsigned)blocks, 64 * WM * WN, 0, stream>>>(a);
     return hipGetLastError();
 }
 
 template <typename O, bool DIRECT, int MT>
 hipError_t few_by(const Args& a, hipStream_t stream) {
-    const int64_t rows = (int64_t)a.rows * a.parts;
-    few_products<T, O, DIRECT, MT><<<dim3((unsigned)divide_up(a.out_row, 16), (unsigned)(a.shared ? divide_up(rows, 16 * MT) : rows)),
-                                     64 * kFewWaves, 0, stream>>>(a);
+    const int64_t rows = (int64_t)a.rows * a.parts, columns = divide_up(a.out_row, 16);
+    if (too_many(columns, 64 * kFewWaves)) return hipErrorInvalidConfiguration;
+    few_products<T, O, DIRECT, MT><<<dim3((unsigned)columns, (unsigned)(a.shared ? divide_up(rows, 16 * MT) : rows)), 64 * kFewWaves, 0,
+                                     stream>>>(a);
     return hipGetLastError();
 }
 
@@ -88,7 +92,7 @@ template <typename A, typename B, typename O, bool DIRECT, int BM, int BN, int W
 hipError_t sums_by(SumArgs g, hipStream_t stream) {
     g.a_tiles = (int)divide_up(g.a_columns, BM), g.b_tiles = (int)divide_up(g.b_columns, BN);
     const int64_t blocks = (int64_t)g.slots * g.a_tiles * g.b_tiles;
-    if (blocks > (1 << 24) - 1) return hipErrorInvalidConfiguration;
+    if (too_many(blocks, 64 * WM * WN)) return hipErrorInvalidConfiguration;
     if constexpr (sizeof(A) == sizeof(B) && BM < kLargeSumTile) {
         if (g.parts > 1)
             sum_products<A, B, O, DIRECT, true, BM, BN, WM, WN><<<(unsigned)blocks, 64 * WM * WN, 0, stream>>>(g);

@@ -159,6 +159,18 @@ def test_c_abi_refuses_a_thin_operand_of_several_parts(type_, thin):
     refused(rt.load_library().oeq_typed_sum_products(ctypes.byref(rt._TypedSum(**fields)), 16, None, 0, None), "parts")
 
 
+def test_c_abi_refuses_more_threads_than_a_launch_counts():
+    """Threads of a launch are counted in 32 bits: blocks of 512 have half the room of blocks of 256."""
+    lib = rt.load_library()
+    d = rt._TypedSum(type=2, rows=10, parts=1, types=1 << 23, a_columns=16, b_columns=16, a_row_stride=16, b_row_stride=16, a=16, b=16,
+                     order=16, ptr=16)
+    refused(lib.oeq_typed_sum_products(ctypes.byref(d), 16, None, 0, None), "too many")
+    for rows, outer in ((9, 1 << 28), (64, (1 << 31) - 512)):  # the form for few rows: 16 columns to a block of 256
+        a = rt._TypedRows(type=2, rows=rows, parts=1, types=3, inner=8, outer=outer, x_row_stride=8, w_type_stride=8, w_row_stride=8,
+                          x=16, w=16, type_of_row=16)
+        refused(lib.oeq_typed_product(ctypes.byref(a), 16, None), "too many")
+
+
 def test_no_kernel_has_scratch_memory():
     blob = rt.lib_path().read_bytes()
     names, at = {}, 0
