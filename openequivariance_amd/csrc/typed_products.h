@@ -749,7 +749,7 @@ __global__ __launch_bounds__(64 * kFewWaves) void few_products(Args g) {
             const int at = members[first + r];
             if (col >= g.outer) sum = 0;
             else if (g.bias && typed) sum += (float)((const T*)g.bias)[type * g.bias_type + col];
-            else if (g.thin) {
+            if (col < g.outer && g.thin) {
                 const int64_t t = g.type_of_row[at];
                 if (t >= 0 && t < g.types) {
                     const float* u = g.thin + (int64_t)at * g.thin_row;
