@@ -269,6 +269,32 @@ __device__ __forceinline__ void arrived() {
 // products of rows
 // ---------------------------------------------------------------------------
 
+// A float u beside operands of 16 bits is hi + lo. Its products with weights that are not finite are those of hi alone (the weights of lo
+// are 0 there: lo inf would be NaN, or an infinity of the other sign), so hi is not 0 where u is not: then the smallest there is.
+template <typename T>
+__device__ __forceinline__ T upper_part(float u) {
+    union {
+        T t;
+        unsigned short bits;
+    } hi;
+    hi.t = (T)u;
+    if (!(hi.bits & 0x7fff) && u != 0.0f) hi.bits |= 1;
+    return hi.t;
+}
+template <typename T>
+__device__ __forceinline__ uint4_t finite_or_zero(uint4_t x) {
+    constexpr unsigned short kExponent = std::is_same<T, _Float16>::value ? 0x7c00 : 0x7f80;
+    union {
+        uint4_t v;
+        unsigned short e[8];
+    } y;
+    y.v = x;
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+        if ((y.e[j] & kExponent) == kExponent) y.e[j] = 0;
+    return y.v;
+}
+
 // A tile of BM rows and BN columns. ACROSS: the weights' rows run along the columns (w[k, n]), else along the summation
 // (w[n, k]). DIRECT: everything is aligned to 16 bytes and goes straight to LDS; else through registers, by elements where a
 // row ends. The result is transposed in registers: lane l has row l % 32, register r column 8 (r / 4) + 4 (l / 32) + r % 4.
@@ -456,8 +482,12 @@ __global__ __launch_bounds__(64 * WM * WN) void row_products(Args g) {
 #pragma unroll
                         for (int j = 0; j < E; ++j) {
                             const float v = std::is_same<T, _Float16>::value ? u[j] * up_by[i] : u[j];
-                            const float hi = (float)(T)v;
-                            y.e[j] = PARTS == 2 && low ? (T)(fabsf(hi) < INFINITY ? v - hi : 0.0f) : (T)v;
+                            if constexpr (PARTS == 2) {
+                                const T hi = upper_part<T>(v);
+                                y.e[j] = !low ? hi : (T)(fabsf((float)hi) < INFINITY ? v - (float)hi : 0.0f);
+                            } else {
+                                y.e[j] = v;
+                            }
                         }
                     }
                     X::put(x1, y.v, i, wave, lane);
@@ -480,6 +510,7 @@ __global__ __launch_bounds__(64 * WM * WN) void row_products(Args g) {
 #pragma unroll
                             for (int j = 0; j < E; ++j)
                                 if (j < left) y.e[j] = from[j * g.up_col];
+                        if (PARTS == 2 && k0 + r >= width) y.v = finite_or_zero<T>(y.v);
                     } else {
                         const int kk = k0 + c, k = kk >= width ? kk - width : kk;
                         const int left = kk < PARTS * width ? g.rank - k : 0;
@@ -490,6 +521,7 @@ __global__ __launch_bounds__(64 * WM * WN) void row_products(Args g) {
 #pragma unroll
                             for (int j = 0; j < E; ++j)
                                 if (j < left) y.e[j] = from[j * g.up_rank];
+                        if (PARTS == 2 && kk >= width) y.v = finite_or_zero<T>(y.v);
                     }
                     W::put(w1, y.v, i, wave, lane);
                 }

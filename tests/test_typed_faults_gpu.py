@@ -9,7 +9,7 @@ import torch
 import openequivariance_amd as oeq
 from openequivariance_amd import runtime as rt
 from tests import typed_oracle as O
-from tests.test_typed_operators_gpu import DTYPES, normal
+from tests.test_typed_operators_gpu import DTYPES, adapter_case, normal
 
 pytestmark = pytest.mark.gpu
 
@@ -44,3 +44,46 @@ def test_a_bias_and_a_thin_product_of_one_call_are_both_added(rows, dtype):
                     + bias[t].cpu().double().abs())
         err[at] = keep * (u.abs() @ b.abs().t())
     O.check(out, val, O.dot_error(inner + rank + 1, size) + 2 * err + O.rounded(val, dtype), "out")
+
+
+def plain_adapters(x, weight, down, up, types, scale):
+    """The definition in 64 bits, infinities and NaN included: products one by one, so that nothing is multiplied that a row has not."""
+    x, weight, down, up, scale = (t.detach().cpu().double() for t in (x, weight, down, up, scale))
+    out = x @ weight.t()
+    for t, at in O.rows_of(types.cpu(), down.shape[0]):
+        u = scale[t] * (x[at, None, :] * down[t]).sum(-1)
+        out[at] += (u[:, None, :] * up[t]).sum(-1)
+    return out
+
+
+def same_kind(got, want, dtype):
+    """Infinities, their signs and NaN as in the definition (which is rounded to the type first)."""
+    got, want = got.detach().cpu().double(), want.to(dtype).double()
+    assert torch.equal(got.isnan(), want.isnan())
+    assert torch.equal(got.isinf(), want.isinf()) and torch.equal(got[got.isinf()], want[want.isinf()])
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows", [40, 300])
+def test_adapters_with_infinities(rows, dtype):
+    """An infinite weight of an adapter: an infinity of the product's sign, whatever is left of the operand beside it in its lower part."""
+    x, weight, down, up, types, scale, grad = adapter_case(rows, 3, 64, 72, 8, dtype)
+    scale = torch.tensor([1.5, -1.0, 2.0], device="cuda")
+    down, up = down.clone(), up.clone()
+    up[0, 5, 2], up[1, 40, 0], up[2, 71, 7], up[2, 70, 7] = float("inf"), float("-inf"), float("inf"), float("nan")
+    # rows between whose products the upper part is all there is (0.5 s), or too small for float16 beside the row's largest (2^-28 s)
+    x[:9], down[:, 2], types[:9] = 0, 0, torch.arange(9, device="cuda") % 3
+    x[:9, 0], x[:9, 1], down[:, :, 0], down[:, 2, 1] = 0.5, 2.0 ** -14, 0.0, 2.0 ** -14
+    down[:, 0, 0] = down[:, 7, 0] = 1.0
+    out = oeq.adapter_linear(x, weight, down, up, types, scale=scale)
+    want = plain_adapters(x, weight, down, up, types, scale)
+    assert want.isinf().sum() > 20 and want[:, 70].isnan().any()
+    same_kind(out, want, dtype)
+    # dx: the same with the matrices of the other direction
+    up = adapter_case(rows, 3, 64, 72, 8, dtype)[3]
+    down[0, 3, 60], down[1, 0, 0], down[2, 1, 33] = float("-inf"), float("inf"), float("inf")
+    leaf = x.clone().requires_grad_()
+    dx, = torch.autograd.grad(oeq.adapter_linear(leaf, weight, down, up, types, scale=scale), leaf, grad)
+    want = plain_adapters(grad, weight.t(), up.transpose(1, 2), down.transpose(1, 2), types, scale)
+    assert want.isinf().sum() > 20
+    same_kind(dx, want, dtype)
