@@ -453,10 +453,10 @@ __global__ __launch_bounds__(64 * WM * WN) void row_products(Args g) {
                     for (int k = 0; k < width; k += 4) {
                         const float4_t v = *(const float4_t*)(u + k);
 #pragma unroll
-                        for (int j = 0; j < 4; ++j) most = fmaxf(most, fabsf(v[j]));
+                        for (int j = 0; j < 4; ++j) most = fmaxf(most, fabsf(v[j]) < INFINITY ? fabsf(v[j]) : 0.0f);
                     }
-                    // most 2^-e is between 1 / 2 and 1; infinities and NaN stay as they are
-                    const int e = most > 0 && most < INFINITY ? __builtin_amdgcn_frexp_expf(most) : 0;
+                    // the largest that is finite, most, times 2^-e is between 1 / 2 and 1; infinities and NaN stay what they are
+                    const int e = most > 0 ? __builtin_amdgcn_frexp_expf(most) : 0;
                     lift[r] = __builtin_amdgcn_ldexpf(1.0f, max(-e, -126) < 127 ? max(-e, -126) : 126);
                 }
                 __syncthreads();

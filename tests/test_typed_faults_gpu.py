@@ -87,3 +87,17 @@ def test_adapters_with_infinities(rows, dtype):
     want = plain_adapters(grad, weight.t(), up.transpose(1, 2), down.transpose(1, 2), types, scale)
     assert want.isinf().sum() > 20
     same_kind(dx, want, dtype)
+
+
+@pytest.mark.parametrize("rows", [40, 300])
+def test_adapters_between_whose_products_are_infinities(rows):
+    """One infinite element between the thin products leaves the others as they are, past float16's range too."""
+    dtype = torch.float16
+    x, weight = torch.zeros(rows, 64, device="cuda", dtype=dtype), torch.zeros(72, 64, device="cuda", dtype=dtype)
+    down, up = torch.zeros(1, 8, 64, device="cuda", dtype=dtype), torch.zeros(1, 72, 8, device="cuda", dtype=dtype)
+    x[:] = 1000.0
+    down[0, 0, 0], down[0, 1, 1:9] = float("inf"), 1000.0  # u = (inf, 8e6, 0, ..)
+    up[0, :, 0], up[0, :, 1] = 1.0, -1.0
+    types, scale = torch.zeros(rows, dtype=torch.int64, device="cuda"), torch.ones(1, device="cuda")
+    out = oeq.adapter_linear(x, weight, down, up, types, scale=scale)
+    same_kind(out, plain_adapters(x, weight, down, up, types, scale), dtype)
