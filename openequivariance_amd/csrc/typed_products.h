@@ -279,6 +279,8 @@ __device__ __forceinline__ T upper_part(float u) {
     } hi;
     hi.t = (T)u;
     if (!(hi.bits & 0x7fff) && u != 0.0f) hi.bits |= 1;
+    if constexpr (!std::is_same<T, _Float16>::value)  // (where u is past what 8 bits hold: the largest there is)
+        if ((hi.bits & 0x7fff) == 0x7f80 && fabsf(u) < INFINITY) --hi.bits;
     return hi.t;
 }
 template <typename T>

@@ -101,3 +101,20 @@ def test_adapters_between_whose_products_are_infinities(rows):
     types, scale = torch.zeros(rows, dtype=torch.int64, device="cuda"), torch.ones(1, device="cuda")
     out = oeq.adapter_linear(x, weight, down, up, types, scale=scale)
     same_kind(out, plain_adapters(x, weight, down, up, types, scale), dtype)
+
+
+@pytest.mark.parametrize("rows", [40, 300])
+def test_adapters_near_the_end_of_the_range(rows):
+    """A sum between the thin products that is finite, but past what bfloat16 holds: 2^128 (1 - 2^-9 - 2^-10) becomes infinite when it is
+    rounded to 8 bits."""
+    dtype = torch.bfloat16
+    x, weight = torch.zeros(rows, 64, device="cuda", dtype=dtype), torch.zeros(72, 64, device="cuda", dtype=dtype)
+    down, up = torch.zeros(1, 8, 64, device="cuda", dtype=dtype), torch.zeros(1, 72, 8, device="cuda", dtype=dtype)
+    x[:, 0], x[:, 1] = 2.0 ** 126, 2.0 ** 118
+    down[0, 0, 0], down[0, 0, 1] = 3.984375, 1.25  # 2^128 (1 - 2^-8) + 2^118 1.25
+    down[0, 0, 2], x[:, 2] = 1.0, 2.0 ** 118
+    up[0, :, 0] = 2.0 ** -10
+    types, scale = torch.zeros(rows, dtype=torch.int64, device="cuda"), torch.ones(1, device="cuda")
+    val, err = O.adapters(x, weight, down, up, types, scale)
+    assert val["out"].max() < 2.0 ** 118
+    O.check(oeq.adapter_linear(x, weight, down, up, types, scale=scale), val["out"], err["out"], "out")
