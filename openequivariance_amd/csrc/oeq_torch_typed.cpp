@@ -36,6 +36,17 @@ void check_types(const Tensor& types, const Tensor& beside) {
     check_tensor(types, types.sizes(), at::kLong, "types", beside);
 }
 
+void check_whole(const OptTensor& order, const OptTensor& ptr) {
+    TORCH_CHECK(order.has_value() == ptr.has_value(), "an index has both 'order' and 'ptr'");
+}
+
+void check_index(const Tensor& types, int64_t count, const OptTensor& order, const OptTensor& ptr) {
+    check_whole(order, ptr);
+    if (!order.has_value()) return;
+    check_tensor(*order, {types.size(0)}, at::kInt, "order", types);
+    check_tensor(*ptr, {count + 1}, at::kInt, "ptr", types);
+}
+
 // The index of a batch's types: the caller's, or one made when a call needs it.
 struct Groups {
     Tensor types, order, ptr;
@@ -67,11 +78,8 @@ Tensor2 group_rows_gpu(const Tensor& types, int64_t count) {
 
 Groups::Groups(const Tensor& types_, int64_t count_, const OptTensor& order_, const OptTensor& ptr_)
     : types(types_.contiguous()), count(count_) {
-    TORCH_CHECK(order_.has_value() == ptr_.has_value(), "an index has both 'order' and 'ptr'");
-    if (!order_.has_value()) return;
-    check_tensor(*order_, {types.size(0)}, at::kInt, "order", types);
-    check_tensor(*ptr_, {count + 1}, at::kInt, "ptr", types);
-    order = order_->contiguous(), ptr = ptr_->contiguous();
+    check_index(types, count, order_, ptr_);
+    if (order_.has_value()) order = order_->contiguous(), ptr = ptr_->contiguous();
 }
 
 void Groups::make() {
@@ -119,10 +127,12 @@ void check_table(const Tensor& weight) {
     check_tensor(weight, weight.sizes(), weight.scalar_type(), "weight", weight);
 }
 
-Tensor type_embedding_gpu(const Tensor& types, const Tensor& weight, double scale, const OptTensor&, const OptTensor&) {
+// (the lookup needs no index: one that is passed is checked all the same)
+Tensor type_embedding_gpu(const Tensor& types, const Tensor& weight, double scale, const OptTensor& order, const OptTensor& ptr) {
     check_table(weight);
     const int type = element_of(weight, "weight");
     check_types(types, weight);
+    check_index(types, weight.size(0), order, ptr);
     OnDevice dev(weight);
     const Tensor at = types.contiguous();
     const Strided table(weight);
@@ -377,7 +387,8 @@ OptTensor optional_of(const Tensor& t) { return t.defined() ? OptTensor(t) : Opt
 
 // The index of a call that will be differentiated: made now, so that the backward pass finds it.
 Tensor2 recorded_index(const Tensor& types, int64_t count, const OptTensor& order, const OptTensor& ptr) {
-    if (order.has_value() && ptr.has_value()) return {*order, *ptr};
+    check_whole(order, ptr);
+    if (order.has_value()) return {*order, *ptr};
     return OEQ_OP(group_rows).call(types, count);
 }
 

@@ -9,7 +9,7 @@ import torch
 import openequivariance_amd as oeq
 from openequivariance_amd import runtime as rt
 from tests import typed_oracle as O
-from tests.test_typed_operators_gpu import DTYPES, adapter_case, normal
+from tests.test_typed_operators_gpu import DTYPES, adapter_case, linear_case, normal
 
 pytestmark = pytest.mark.gpu
 
@@ -118,3 +118,13 @@ def test_adapters_near_the_end_of_the_range(rows):
     val, err = O.adapters(x, weight, down, up, types, scale)
     assert val["out"].max() < 2.0 ** 118
     O.check(oeq.adapter_linear(x, weight, down, up, types, scale=scale), val["out"], err["out"], "out")
+
+
+def test_an_index_is_checked_by_the_lookup_too():
+    x, weight, types, bias, grad = linear_case(10, 0, 3, 16, 24, True, torch.float32)
+    table, good = weight[:, 0], oeq.group_rows(types, 3)
+    for index, text in ((oeq.group_rows(types, 4), "Shape mismatch for tensor 'ptr'"), (good._replace(order=good.order[:5]), "Shape mismatch for tensor 'order'"),
+                        (good._replace(order=good.order.long()), "Dtype mismatch for tensor 'order'"), (good._replace(ptr=None), "both 'order' and 'ptr'")):
+        for leaf in (table, table.detach().requires_grad_()):
+            with pytest.raises(RuntimeError, match=text):
+                oeq.type_embedding(index, leaf)
