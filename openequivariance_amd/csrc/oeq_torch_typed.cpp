@@ -509,8 +509,13 @@ struct TypedLinearGradient : public torch::autograd::Function<TypedLinearGradien
             Tensor g;
             if (a.defined()) g = OEQ_OP(typed_linear).call(a, weight, types, {}, order, ptr);
             if (b.defined() || c.defined()) {
-                const Tensor w = b.defined() ? b : at::zeros_like(weight);
-                const Tensor more = OEQ_OP(typed_linear).call(x, w, types, optional_of(c), order, ptr);
+                Tensor more;
+                if (b.defined()) {
+                    more = OEQ_OP(typed_linear).call(x, b, types, optional_of(c), order, ptr);
+                } else {  // (no product with zeros: what a row holds has no part in c_t)
+                    more = OEQ_OP(type_embedding).call(types, c, 1.0, order, ptr);
+                    if (grad.dim() == 3) more = more.unsqueeze(1).expand_as(grad);
+                }
                 g = g.defined() ? g + more : more;
             }
             out[0] = g;

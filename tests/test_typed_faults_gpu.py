@@ -128,3 +128,17 @@ def test_an_index_is_checked_by_the_lookup_too():
         for leaf in (table, table.detach().requires_grad_()):
             with pytest.raises(RuntimeError, match=text):
                 oeq.type_embedding(index, leaf)
+
+
+@pytest.mark.parametrize("components", [0, 3])
+def test_a_bias_gradient_differentiated_alone_has_no_other_term(components):
+    """The sum of gradients by type is linear in them: its derivative is the lookup of its cotangent, whatever the rows hold."""
+    x, weight, types, bias, grad = linear_case(90, components, 4, 24, 40, True, torch.float32)
+    x[types == 1] = float("inf")
+    leaves = [bias.detach().requires_grad_(), grad.requires_grad_()]
+    db, = torch.autograd.grad(oeq.typed_linear(x, weight, types, leaves[0]), leaves[0], grad, create_graph=True)
+    cot = normal(torch.Generator().manual_seed(1), 4, 40)
+    back, = torch.autograd.grad(db, grad, cot)
+    known = (types >= 0) & (types < 4)
+    want = torch.where(known[:, None], cot[torch.where(known, types, 0)], 0.0)
+    assert torch.equal(back, want[:, None].expand(-1, 3, -1) if components else want)
