@@ -103,7 +103,7 @@ def _cast(*tensors):
     """Under autocast, as torch's own linear layers."""
     if torch.is_autocast_enabled("cuda"):
         to = torch.get_autocast_dtype("cuda")
-        return [t if t is None or t.dtype == torch.float64 else t.to(to) for t in tensors]
+        return [t.to(to) if t is not None and t.is_floating_point() and t.dtype != torch.float64 else t for t in tensors]
     return tensors
 
 

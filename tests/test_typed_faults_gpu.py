@@ -142,3 +142,13 @@ def test_a_bias_gradient_differentiated_alone_has_no_other_term(components):
     known = (types >= 0) & (types < 4)
     want = torch.where(known[:, None], cot[torch.where(known, types, 0)], 0.0)
     assert torch.equal(back, want[:, None].expand(-1, 3, -1) if components else want)
+
+
+def test_autocast_leaves_integers_alone():
+    """They are refused as without it, not computed with."""
+    x, weight, types, bias, grad = linear_case(10, 0, 3, 16, 24, True, torch.float32)
+    with torch.autocast("cuda", dtype=torch.bfloat16):
+        with pytest.raises(RuntimeError, match="float32, float16 or bfloat16"):
+            oeq.typed_linear(x.long(), weight, types)
+        with pytest.raises(RuntimeError, match="Dtype mismatch for tensor 'down'"):
+            oeq.adapter_linear(x, weight[0], weight[:, :8].int(), weight[:, :, :8], types)
