@@ -447,7 +447,8 @@ __global__ __launch_bounds__(64 * WM * WN) void row_products(Args g) {
             float down[TM];
             float up_by[X::kEach];
             if constexpr (std::is_same<T, _Float16>::value) {
-                // A power of two for each row: parts of 11 bits each, whatever the size of u.
+                // A power of two for each row, which brings its largest element near the end of float16's range: parts of 11 bits each
+                // whatever the size of u, and what is small beside the largest keeps 16 bits down to 2^-24 of it.
                 for (int r = tid; r < BM; r += 64 * WAVES) {
                     const int at = min(m0 + r, rows.hi - 1);
                     const float* u = g.thin + (int64_t)Place(g.order, at, 1, g.rows).row * width;
@@ -457,9 +458,9 @@ __global__ __launch_bounds__(64 * WM * WN) void row_products(Args g) {
 #pragma unroll
                         for (int j = 0; j < 4; ++j) most = fmaxf(most, fabsf(v[j]) < INFINITY ? fabsf(v[j]) : 0.0f);
                     }
-                    // the largest that is finite, most, times 2^-e is between 1 / 2 and 1; infinities and NaN stay what they are
-                    const int e = most > 0 ? __builtin_amdgcn_frexp_expf(most) : 0;
-                    lift[r] = __builtin_amdgcn_ldexpf(1.0f, max(-e, -126) < 127 ? max(-e, -126) : 126);
+                    // the largest that is finite, most, times 2^e is between 2^14 and 2^15; infinities and NaN stay what they are
+                    const int e = most > 0 ? 15 - __builtin_amdgcn_frexp_expf(most) : 0;
+                    lift[r] = __builtin_amdgcn_ldexpf(1.0f, min(e, 126));
                 }
                 __syncthreads();
 #pragma unroll

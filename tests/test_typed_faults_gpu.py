@@ -152,3 +152,23 @@ def test_autocast_leaves_integers_alone():
             oeq.typed_linear(x.long(), weight, types)
         with pytest.raises(RuntimeError, match="Dtype mismatch for tensor 'down'"):
             oeq.adapter_linear(x, weight[0], weight[:, :8].int(), weight[:, :, :8], types)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("ratio", [2.0 ** 8, 2.0 ** 14, 2.0 ** 20])
+@pytest.mark.parametrize("rows", [40, 300])
+def test_adapters_keep_what_is_small_beside_the_rest_of_a_row(rows, ratio, dtype):
+    """Between the thin products a row has an element 1 .. 2 and one `ratio` times larger; half of the columns take the small one alone."""
+    gen = torch.Generator().manual_seed(rows)
+    x, weight = torch.zeros(rows, 64, device="cuda", dtype=dtype), torch.zeros(72, 64, device="cuda", dtype=dtype)
+    down, up = torch.zeros(1, 8, 64, device="cuda", dtype=dtype), torch.zeros(1, 72, 8, device="cuda", dtype=dtype)
+    small = 1 + torch.rand(rows, generator=gen)
+    x[:, 0], x[:, 1], x[:, 2] = ratio ** 0.5, small.to(dtype).cuda(), (small * 2.0 ** -9).to(dtype).cuda()
+    down[0, 0, 0], down[0, 5, 1], down[0, 5, 2] = ratio ** 0.5, 1.0, 1.0
+    up[0, 36:, 0], up[0, :, 5] = 1.0, normal(gen, 72, dtype=dtype)
+    types, scale = torch.zeros(rows, dtype=torch.int64, device="cuda"), torch.ones(1, device="cuda")
+    val, err = O.adapters(x, weight, down, up, types, scale)
+    got = oeq.adapter_linear(x, weight, down, up, types, scale=scale)
+    O.check(got[:, :36], val["out"][:, :36], err["out"][:, :36], "columns that take the small one")
+    if ratio < 2.0 ** 16:  # (else past float16)
+        O.check(got, val["out"], err["out"], "out")
