@@ -458,7 +458,7 @@ int oeq_type_lookup(int type, int64_t rows, int64_t types, int64_t channels, con
                     int64_t table_row_stride, double scale, void* out, void* stream);
 
 /* out[t] = scale times the sum of x over the rows of type t and their parts, in the index's order; x: [rows, parts, channels],
- * rows and parts strided; out: [types, channels], contiguous. */
+ * rows and parts strided; out: [types, channels], contiguous. Up to 2^19 channels. */
 size_t oeq_type_sum_workspace_bytes(int64_t rows, int64_t types, int64_t channels);
 int oeq_type_sum(int type, int64_t rows, int64_t parts, int64_t types, int64_t channels, const int64_t* type_of_row,
                  const int32_t* order, const int32_t* ptr, const void* x, int64_t row_stride, int64_t part_stride, double scale,
@@ -493,7 +493,7 @@ int oeq_typed_thin_product(const oeq_typed_rows* a, const float* scale, float* o
 /* out[t] = sum over the rows of type t (and their parts) of a_i^T b_i: [types, a_columns, b_columns], contiguous. */
 typedef struct {
     int32_t type;            /* of a, b and out */
-    int32_t thin;            /* 1: a is float, 2: b is float (one part a row), else 0 */
+    int32_t thin;            /* 1: a is float, 2: b is float (either with one part a row), else 0 */
     int64_t rows, parts;
     int64_t types, a_columns, b_columns;
     int64_t a_row_stride, a_part_stride, b_row_stride, b_part_stride;

@@ -111,7 +111,7 @@ def type_embedding(types: Union[torch.Tensor, RowGroups], weight: torch.Tensor, 
     r"""``scale * weight[types]``. The gradient of the table sums the rows of each type in their order.
 
     :param types: ``[rows]``, int64, or their index.
-    :param weight: ``[types, channels]``.
+    :param weight: ``[types, channels]``; up to 2^19 channels have a gradient.
     """
     types, order, ptr = _index(types)
     return _type_embedding(types, weight, scale, order, ptr)
@@ -136,7 +136,10 @@ def typed_linear(x: torch.Tensor, weight: torch.Tensor, types: Union[torch.Tenso
 def adapter_linear(x: torch.Tensor, weight: torch.Tensor, down: torch.Tensor, up: torch.Tensor,
                    adapters: Union[torch.Tensor, RowGroups], *, scale: Optional[torch.Tensor] = None) -> torch.Tensor:
     r"""A projection that all rows share plus the low-rank one of each row's adapter ``a``:
-    ``x[i] @ weight.T + scale[a] * (x[i] @ down[a].T) @ up[a].T``. What lies between the two thin products stays in 32 bits.
+    ``x[i] @ weight.T + scale[a] * (x[i] @ down[a].T) @ up[a].T``. What lies between the two thin products is a float32 sum, kept as
+    such in memory. Next to operands of 16 bits it enters the second product as two of them together, 16 bits of it with bfloat16 and 22
+    with float16 (16 at least for an element down to 2^-24 of its row's largest). It is whole with float32, and in the form for few rows (up
+    to 128, of weights that are contiguous along the sum), so that 16-bit results of 128 and of 129 rows can differ in the last bit.
 
     :param x: ``[rows, in]``.
     :param weight: ``[out, in]``.
