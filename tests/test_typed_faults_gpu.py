@@ -172,3 +172,24 @@ def test_adapters_keep_what_is_small_beside_the_rest_of_a_row(rows, ratio, dtype
     O.check(got[:, :36], val["out"][:, :36], err["out"][:, :36], "columns that take the small one")
     if ratio < 2.0 ** 16:  # (else past float16)
         O.check(got, val["out"], err["out"], "out")
+
+
+@pytest.mark.parametrize("rows", [9, 300])
+def test_long_sums_of_floats_are_added_up_in_parts(rows):
+    """2^24 and 4 095 ones: a chain of additions in 32 bits loses every one of them (half a unit of the sum each). In parts of 512 terms at
+    most the first part's ones are lost, the other parts are even numbers, which the total holds."""
+    n, most = 4096, 514
+    want = 2.0 ** 24 + n - 1
+    x, w = torch.ones(rows, n, device="cuda"), torch.ones(1, 64, n, device="cuda")
+    x[:, 0] = 2.0 ** 24
+    types, leaf = torch.zeros(rows, dtype=torch.int64, device="cuda"), torch.zeros(rows, 64, device="cuda", requires_grad=True)
+    assert (oeq.typed_linear(x, w, types) - want).abs().max() <= most
+    dx, = torch.autograd.grad(oeq.typed_linear(leaf, w.transpose(1, 2).contiguous(), types), leaf, x)  # (n columns out, 64 in)
+    assert (dx - want).abs().max() <= most
+    out = oeq.adapter_linear(x, torch.zeros(64, n, device="cuda"), w[:, :4].contiguous(), torch.eye(64, 4, device="cuda")[None], types)
+    assert (out[:, :4] - want).abs().max() <= most
+    g, x = torch.ones(n, 64, device="cuda"), torch.ones(n, rows, device="cuda")
+    x[0] = 2.0 ** 24
+    w = torch.zeros(1, 64, rows, device="cuda", requires_grad=True)
+    dw, = torch.autograd.grad(oeq.typed_linear(x, w, torch.zeros(n, dtype=torch.int64, device="cuda")), w, g)
+    assert (dw - want).abs().max() <= most
